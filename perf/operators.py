@@ -90,7 +90,8 @@ def _logits(n, v, dtype, gen, like=None):
         b = min(n, a + step)
         if like is None:
             t = torch.randn(b - a, v, device="cuda", generator=gen).mul_(2.5).sub_(5.0)
-            hot = torch.randint(0, v, (b - a, 12), device="cuda", generator=gen)
+            part = v // 12  # distinct columns: what a scatter does with equal ones is not settled
+            hot = torch.arange(12, device="cuda") * part + torch.randint(0, part, (b - a, 12), device="cuda", generator=gen)
             t.scatter_(1, hot, torch.randn(b - a, 12, device="cuda", generator=gen).mul_(3.0).add_(10.0))
         else:
             t = like[a:b].float()
@@ -166,6 +167,7 @@ def _run_own(s):
     c = s["case"]
     op = c["op"]
     cap = c.get("cap") or None
+    smooth = 0.05 if c.get("kind") == "sigmoid" else 0.0
     if op == "top":
         values, ids, lse = O.top_logits(s["x"], c["k"], softcap=cap, temperature=c["temp"])
         return {"values": values, "ids": ids, "lse": lse}
@@ -183,10 +185,10 @@ def _run_own(s):
                               temperature=c["temp"])
         return {"loss": loss.detach(), "grad": torch.autograd.grad(loss.sum(), s["leaf"])[0]}
     if op == "pairs":
-        loss, rewards, grad = O.preference_loss_grad(s["logp"], s["ref"], s["cu"], beta=0.1, label_smoothing=0.05,
+        loss, rewards, grad = O.preference_loss_grad(s["logp"], s["ref"], s["cu"], beta=0.1, label_smoothing=smooth,
                                                      kind=c["kind"])
         return {"loss": loss, "rewards": rewards, "grad": grad}
-    loss, rewards, logp, grad = O.preference_logits_grad(s["x"], s["t"], s["ref"], s["cu"], beta=0.1, label_smoothing=0.05,
+    loss, rewards, logp, grad = O.preference_logits_grad(s["x"], s["t"], s["ref"], s["cu"], beta=0.1, label_smoothing=smooth,
                                                          kind=c["kind"], softcap=cap)
     return {"loss": loss, "rewards": rewards, "logp": logp, "grad": grad}
 
@@ -257,7 +259,7 @@ def _plain_distill(s):
 
 
 def _plain_pairs(logp, ref, cu, kind, beta=0.1, smooth=0.05):
-    """(loss of each pair, rewards, gradient of their mean in each token's log-probability)."""
+    """(loss of each pair, rewards, gradient of their mean in each token's log-probability); `smooth` of the sigmoid loss."""
     n, seqs = logp.numel(), cu.numel() - 1
     at = torch.arange(n, device=logp.device)
     seq = (at.unsqueeze(1) >= cu[1:].unsqueeze(0)).sum(1)  # the sequence of each token
