@@ -1,0 +1,59 @@
+// Launch functions of the vocabulary objectives (objectives.cu, top_logits.cu, preference.cu), called by
+// their PyTorch side (objectives_torch.cpp), which checks the arguments. Nothing here needs PyTorch.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace me {
+
+constexpr int64_t kIgnoreToken = -100;  // the target of an untrained token
+constexpr int kMaxTop = 256;            // most teacher entries / top logits of a row
+
+enum class LogitType : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
+
+// N rows of V raw logits, `stride` elements apart; cap <= 0: no softcap.
+struct Logits {
+  const void* data;
+  int64_t stride, N, V;
+  LogitType type;
+  float cap;
+};
+// Where their gradient goes (the logits' type; it may be the logits themselves).
+struct Gradient {
+  void* data;
+  int64_t stride;
+};
+
+// The teacher's records: k entries a row; lse and weight may be null.
+struct TeacherArgs {
+  const int64_t* ids;
+  const float* top;
+  const float* lse;
+  const float* weight;
+  int k;
+  float temp;
+};
+
+void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, float2* stats, cudaStream_t stream);
+void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
+                        cudaStream_t stream);
+void launch_distill_fwd(const Logits& x, const TeacherArgs& teacher, float* loss, float4* stats, cudaStream_t stream);
+// g: one coefficient a row, or null for 1
+void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const float4* stats, const float* g, Gradient out,
+                        cudaStream_t stream);
+void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,
+                       cudaStream_t stream);
+
+struct PairArgs {
+  const float *logp, *ref;  // ref may be null
+  const int64_t* target;    // or null: every token is trained
+  const void* cu;           // [2 pairs + 1], int32 or int64
+  bool cu64;
+  int64_t tokens, pairs;
+  int kind;  // 0 sigmoid, 1 hinge, 2 ipo
+  float beta, smooth, scale;
+};
+void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* grad, cudaStream_t stream);
+
+}  // namespace me

@@ -1,0 +1,196 @@
+// PyTorch side of the vocabulary objectives: argument checks, outputs, the current stream.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/types.h>
+
+#include "objectives.h"
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+namespace {
+
+me::Logits check_logits(const Tensor& x, double cap, const char* what) {
+  TORCH_CHECK(x.is_cuda(), what, ": a CUDA tensor is needed");
+  TORCH_CHECK(x.dim() == 2, what, ": [rows, vocabulary] is needed, got ", x.dim(), " dimensions");
+  TORCH_CHECK(x.size(1) > 0 && x.size(1) <= INT32_MAX, what, ": a vocabulary of 1 to 2^31 - 1 entries is needed, got ",
+              x.size(1));
+  TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, what, ": a row's logits have to be contiguous");
+  me::LogitType type = me::LogitType::kF32;
+  if (x.scalar_type() == torch::kBFloat16) type = me::LogitType::kBF16;
+  else if (x.scalar_type() == torch::kHalf) type = me::LogitType::kF16;
+  else TORCH_CHECK(x.scalar_type() == torch::kFloat32, what, ": bfloat16, float16 or float32 is needed, got ",
+                   x.scalar_type());
+  return {x.data_ptr(), x.stride(0), x.size(0), x.size(1), type, (float)cap};
+}
+
+// One value a row of x, as `type`.
+Tensor check_rows(const Tensor& t, const Tensor& x, torch::ScalarType type, const char* what) {
+  TORCH_CHECK(t.device() == x.device(), what, ": on another device than the logits");
+  TORCH_CHECK(t.dim() == 1 && t.size(0) == x.size(0), what, ": one value a row is needed (", x.size(0), ")");
+  return t.to(type).contiguous();
+}
+
+Tensor gradient_like(const Tensor& x, const OptTensor& out, const char* what) {
+  if (!out.has_value()) return torch::empty(x.sizes(), x.options());
+  const Tensor& o = *out;
+  TORCH_CHECK(o.sizes() == x.sizes() && o.scalar_type() == x.scalar_type() && o.device() == x.device(), what,
+              ": out has another shape, type or device than the logits");
+  TORCH_CHECK((o.size(1) == 1 || o.stride(1) == 1) && (o.size(0) <= 1 || o.stride(0) >= o.size(1)), what,
+              ": out's rows have to be contiguous and apart from one another");
+  return o;
+}
+
+me::Gradient gradient_of(const Tensor& o) { return {o.data_ptr(), o.stride(0)}; }
+
+struct Teacher {
+  Tensor ids, top, lse, weight;
+  me::TeacherArgs args;
+};
+
+Teacher check_teacher(const Tensor& x, const Tensor& ids, const Tensor& top, const OptTensor& lse,
+                      const OptTensor& weight, double temp) {
+  TORCH_CHECK(ids.device() == x.device() && top.device() == x.device(),
+              "distill_loss: the teacher's tensors are on another device than the logits");
+  TORCH_CHECK(ids.dim() == 2 && ids.sizes() == top.sizes() && ids.size(0) == x.size(0),
+              "distill_loss: teacher_ids and teacher_logits are [rows, k], got ", ids.sizes(), " and ", top.sizes());
+  TORCH_CHECK(ids.size(1) >= 1 && ids.size(1) <= me::kMaxTop, "distill_loss: 1 to ", me::kMaxTop,
+              " teacher entries a row, got ", ids.size(1));
+  TORCH_CHECK(ids.scalar_type() == torch::kLong || ids.scalar_type() == torch::kInt,
+              "distill_loss: teacher_ids are int64 or int32");
+  Teacher t;
+  t.ids = ids.to(torch::kLong).contiguous();
+  t.top = top.to(torch::kFloat32).contiguous();
+  if (lse.has_value()) t.lse = check_rows(*lse, x, torch::kFloat32, "distill_loss: teacher_lse");
+  if (weight.has_value()) t.weight = check_rows(*weight, x, torch::kFloat32, "distill_loss: weights");
+  t.args = {t.ids.data_ptr<int64_t>(),
+            t.top.data_ptr<float>(),
+            lse.has_value() ? t.lse.data_ptr<float>() : nullptr,
+            weight.has_value() ? t.weight.data_ptr<float>() : nullptr,
+            (int)t.ids.size(1),
+            (float)temp};
+  return t;
+}
+
+float2* as2(const Tensor& t) { return reinterpret_cast<float2*>(t.data_ptr<float>()); }
+float4* as4(const Tensor& t) { return reinterpret_cast<float4*>(t.data_ptr<float>()); }
+
+}  // namespace
+
+// (logp [N], stats [N, 2])
+std::vector<Tensor> token_logprobs_fwd(Tensor x, Tensor target, double cap) {
+  const auto in = check_logits(x, cap, "token_logprobs");
+  const at::cuda::CUDAGuard guard(x.device());
+  auto t = check_rows(target, x, torch::kLong, "token_logprobs: targets");
+  auto opts = x.options().dtype(torch::kFloat32);
+  auto logp = torch::empty({in.N}, opts), stats = torch::empty({in.N, 2}, opts);
+  if (in.N == 0) return {logp, stats};
+  me::launch_logprob_fwd(in, t.data_ptr<int64_t>(), logp.data_ptr<float>(), as2(stats),
+                         at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {logp, stats};
+}
+
+Tensor token_logprobs_bwd(Tensor x, Tensor target, double cap, Tensor stats, Tensor g, OptTensor out) {
+  const auto in = check_logits(x, cap, "token_logprobs");
+  const at::cuda::CUDAGuard guard(x.device());
+  auto t = check_rows(target, x, torch::kLong, "token_logprobs: targets");
+  auto gr = check_rows(g, x, torch::kFloat32, "token_logprobs: gradient");
+  auto o = gradient_like(x, out, "token_logprobs");
+  if (in.N == 0) return o;
+  me::launch_logprob_bwd(in, t.data_ptr<int64_t>(), as2(stats), gr.data_ptr<float>(), gradient_of(o),
+                         at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return o;
+}
+
+// (loss [N], stats [N, 4])
+std::vector<Tensor> distill_fwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap,
+                                double temp) {
+  const auto in = check_logits(x, cap, "distill_loss");
+  const at::cuda::CUDAGuard guard(x.device());
+  const auto te = check_teacher(x, ids, top, lse, weight, temp);
+  auto opts = x.options().dtype(torch::kFloat32);
+  auto loss = torch::empty({in.N}, opts), stats = torch::empty({in.N, 4}, opts);
+  if (in.N == 0) return {loss, stats};
+  me::launch_distill_fwd(in, te.args, loss.data_ptr<float>(), as4(stats), at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, stats};
+}
+
+Tensor distill_bwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap, double temp,
+                   Tensor stats, OptTensor g, OptTensor out) {
+  const auto in = check_logits(x, cap, "distill_loss");
+  const at::cuda::CUDAGuard guard(x.device());
+  const auto te = check_teacher(x, ids, top, lse, weight, temp);
+  Tensor gr;
+  if (g.has_value()) gr = check_rows(*g, x, torch::kFloat32, "distill_loss: gradient");
+  auto o = gradient_like(x, out, "distill_loss");
+  if (in.N == 0) return o;
+  me::launch_distill_bwd(in, te.args, as4(stats), g.has_value() ? gr.data_ptr<float>() : nullptr, gradient_of(o),
+                         at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return o;
+}
+
+// (loss [N], dL/dx [N, V])
+std::vector<Tensor> distill_grad(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap,
+                                 double temp, OptTensor out) {
+  auto f = distill_fwd(x, ids, top, lse, weight, cap, temp);
+  return {f[0], distill_bwd(x, ids, top, lse, weight, cap, temp, f[1], c10::nullopt, out)};
+}
+
+// (values [N, k] fp32, ids [N, k] int64, lse [N] fp32)
+std::vector<Tensor> top_logits(Tensor x, int64_t k, double cap, double temp) {
+  const auto in = check_logits(x, cap, "top_logits");
+  const at::cuda::CUDAGuard guard(x.device());
+  const int64_t most = std::min<int64_t>(in.V, me::kMaxTop);
+  TORCH_CHECK(k >= 1 && k <= most, "top_logits: k from 1 to ", most, ", got ", k);
+  auto opts = x.options().dtype(torch::kFloat32);
+  auto values = torch::empty({in.N, k}, opts), lse = torch::empty({in.N}, opts);
+  auto ids = torch::empty({in.N, k}, x.options().dtype(torch::kLong));
+  if (in.N == 0) return {values, ids, lse};
+  me::launch_top_logits(in, (int)k, (float)temp, values.data_ptr<float>(), ids.data_ptr<int64_t>(),
+                        lse.data_ptr<float>(), at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {values, ids, lse};
+}
+
+// (loss [P], rewards [P, 2], scale * d sum(loss) / d logp [T])
+std::vector<Tensor> preference_pairs(Tensor logp, OptTensor ref, Tensor cu, int64_t kind, double beta, double smooth,
+                                     double scale, OptTensor target) {
+  TORCH_CHECK(logp.is_cuda() && logp.dim() == 1, "preference_loss: log-probabilities [tokens] on a GPU are needed");
+  TORCH_CHECK(cu.device() == logp.device() && cu.dim() == 1 && cu.size(0) % 2 == 1,
+              "preference_loss: cu_seqlens [2 pairs + 1] on the log-probabilities' device is needed");
+  TORCH_CHECK(cu.scalar_type() == torch::kInt || cu.scalar_type() == torch::kLong,
+              "preference_loss: cu_seqlens is int32 or int64");
+  const at::cuda::CUDAGuard guard(logp.device());
+  const int64_t n = logp.size(0), pairs = cu.size(0) / 2;
+  TORCH_CHECK(pairs <= INT32_MAX, "preference_loss: 2^31 - 1 pairs at most");
+  auto lp = logp.to(torch::kFloat32).contiguous();
+  Tensor rf, tg;
+  if (ref.has_value()) rf = check_rows(*ref, logp, torch::kFloat32, "preference_loss: ref_logps");
+  if (target.has_value()) tg = check_rows(*target, logp, torch::kLong, "preference_loss: targets");
+  auto off = cu.contiguous();
+  auto opts = lp.options();
+  auto loss = torch::empty({pairs}, opts), rewards = torch::empty({pairs, 2}, opts);
+  if (pairs == 0) return {loss, rewards, torch::zeros({n}, opts)};
+  auto grad = torch::empty({n}, opts);
+  me::launch_preference({lp.data_ptr<float>(), ref.has_value() ? rf.data_ptr<float>() : nullptr,
+                         target.has_value() ? tg.data_ptr<int64_t>() : nullptr, off.data_ptr(),
+                         off.scalar_type() == torch::kLong, n, pairs, (int)kind, (float)beta, (float)smooth,
+                         (float)scale},
+                        loss.data_ptr<float>(), as2(rewards), grad.data_ptr<float>(),
+                        at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, rewards, grad};
+}
+
+// (loss [P], rewards [P, 2], logp [T], d (scale * sum(loss)) / d logits [T, V])
+std::vector<Tensor> preference_logits(Tensor x, Tensor target, OptTensor ref, Tensor cu, int64_t kind, double beta,
+                                      double smooth, double scale, double cap, OptTensor out) {
+  auto f = token_logprobs_fwd(x, target, cap);
+  auto p = preference_pairs(f[0], ref, cu, kind, beta, smooth, scale, target);
+  return {p[0], p[1], f[0], token_logprobs_bwd(x, target, cap, f[1], p[2], out)};
+}

@@ -1,0 +1,376 @@
+"""Vocabulary objectives on the sm_100a kernels: against the 64-bit definitions at the sizes, types,
+strides and masks where they can go wrong; edge rules as on the CPU; streams, repeatability, refusals."""
+import pytest
+import torch
+
+import objective_oracle as oracle
+from micro_engram_fork_b200.ops import objectives as O
+from test_objectives import refusals
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+BF, HF, FP = torch.bfloat16, torch.float16, torch.float32
+
+
+def _gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def _x(N, V, dtype, seed=0, pitch=0, shift=0):
+    """Rows of logits `pitch` elements longer than V apart, `shift` elements into their storage."""
+    g = _gen(seed)
+    whole = torch.zeros(shift + N * (V + pitch), dtype=dtype, device=DEV)
+    x = whole[shift:].view(N, V + pitch)[:, :V]
+    x.copy_(torch.randn(N, V, device=DEV, generator=g) * 4)
+    if V > 4:
+        hot = torch.randint(0, V, (N, 3), device=DEV, generator=g)
+        x.scatter_(1, hot, torch.full((N, 3), 14.0, device=DEV, dtype=dtype))
+    return x
+
+
+def _teacher(N, V, k, seed=0):
+    g = _gen(seed)
+    ids = torch.rand(N, V, device=DEV, generator=g).topk(k, dim=1)[1]
+    return ids, torch.randn(N, k, device=DEV, generator=g) * 3
+
+
+# vocabularies around the vector, block and slice sizes; row pitches and offsets off 16 bytes
+SHAPES = [(1, 1, 0, 0), (3, 2, 0, 0), (2, 7, 1, 0), (5, 8, 0, 0), (4, 9, 0, 3), (3, 255, 2, 1), (6, 4096, 0, 0),
+          (37, 5003, 0, 0), (9, 5003, 5, 1), (2, 32768, 8, 0), (3, 65537, 0, 0), (301, 12345, 3, 0), (2, 262144, 0, 0),
+          (2, 300001, 0, 0), (1, 600008, 0, 0)]
+
+
+@pytest.mark.parametrize("cap", [None, 30.0])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+@pytest.mark.parametrize("N,V,pitch,shift", SHAPES)
+def test_token_logprobs(N, V, pitch, shift, dtype, cap):
+    x = _x(N, V, dtype, N + V, pitch, shift)
+    g = _gen(1)
+    t = torch.randint(0, V, (N,), device=DEV, generator=g)
+    if N > 2:
+        t[1] = -100
+    t[-1] = V - 1
+    coef = torch.randn(N, device=DEV, generator=g)
+    leaf = x.detach().requires_grad_()
+    logp = O.token_logprobs(leaf, t, softcap=cap)
+    dx, = torch.autograd.grad(logp, leaf, coef)
+    want, grad, mass = oracle.logprobs(x, t, cap, coef)
+    oracle.close_logp(logp.detach(), want, x, cap)
+    oracle.close_grad(dx, grad, coef, mass, dtype)
+    if N > 2:
+        assert bool((dx[1] == 0).all()) and logp[1] == 0
+
+
+@pytest.mark.parametrize("tail", [False, True])
+@pytest.mark.parametrize("dtype,cap,temp", [(BF, 30.0, 1.0), (BF, None, 2.0), (HF, 30.0, 2.0), (FP, None, 1.0),
+                                            (FP, 30.0, 0.7)])
+@pytest.mark.parametrize("N,V,pitch,shift", SHAPES)
+def test_distill(N, V, pitch, shift, dtype, cap, temp, tail):
+    x = _x(N, V, dtype, N + V, pitch, shift)
+    k = min(V, {0: 33, 1: 256, 2: 1}[V % 3])
+    ids, top = _teacher(N, V, k, 5)
+    lse = torch.logsumexp(top / temp, 1) + 0.4 if tail else None
+    w = torch.rand(N, device=DEV, generator=_gen(6)) + 0.2
+    if N > 2:
+        w[1] = 0.0
+        ids[2, k // 2:] = -1
+    if N > 4:
+        ids[3] = -1
+        top[4, 0] = -float("inf")
+    args = (x, ids, top, lse, w)
+    n = min(N, 40)  # the oracle walks the rows
+    want, grad, mass = oracle.distill(x[:n], ids[:n], top[:n], None if lse is None else lse[:n], w[:n], cap, temp)
+    scale = float(temp) ** 2 * 8
+    loss, dx = O.distill_loss_grad(*args, softcap=cap, temperature=temp)
+    oracle.close_logp(loss[:n], want, x[:n], cap, temp, factor=scale)
+    oracle.close_grad(dx[:n], grad, w[:n] * temp, mass, dtype)
+    leaf = x.detach().requires_grad_()
+    loss2 = O.distill_loss(leaf, *args[1:], softcap=cap, temperature=temp)
+    oracle.close_logp(loss2.detach()[:n], want, x[:n], cap, temp, factor=scale)
+    g = torch.randn(N, device=DEV, generator=_gen(7))
+    dx2, = torch.autograd.grad(loss2, leaf, g)
+    oracle.close_grad(dx2[:n], grad * g[:n, None].double(), w[:n] * temp * g[:n], mass, dtype)
+    if N > n:  # the rest against the plain form
+        ref = O.distill_ref(x[n:], ids[n:], top[n:], None if lse is None else lse[n:], w[n:], cap or 0.0, temp)
+        assert torch.allclose(loss[n:], ref[0], rtol=1e-4, atol=1e-4)
+        assert torch.allclose(dx[n:].float(), ref[1].float(), rtol=2.0 ** -7, atol=1e-6)
+    inplace = _x(N, V, dtype, N + V, pitch, shift)  # the same alignment: the same order of sums
+    loss3, dx3 = O.distill_loss_grad(inplace, *args[1:], softcap=cap, temperature=temp, out=inplace)
+    assert dx3 is inplace and torch.equal(dx3, dx) and torch.equal(loss3, loss)
+
+
+def test_distill_repeated_and_foreign_ids():
+    x = _x(3, 4097, BF, 3)
+    ids = torch.tensor([[5, 5, 9, -1], [4096, 0, 4097, 1 << 40], [7, 7, 7, 7]], device=DEV)
+    top = torch.tensor([[1.0, 2.0, 3.0, 9.0], [0.0, 1.0, 50.0, 60.0], [1.0, 1.0, 1.0, 1.0]], device=DEV)
+    for lse in (None, torch.full((3,), 5.0, device=DEV)):
+        loss, dx = O.distill_loss_grad(x, ids, top, lse, softcap=30.0)
+        ref, dref = O.distill_ref(x.double(), ids, top.double(), lse, None, 30.0, 1.0)
+        assert torch.allclose(loss.double(), ref, rtol=1e-5, atol=1e-5)
+        assert torch.allclose(dx.double(), dref, rtol=2.0 ** -7, atol=1e-6)
+
+
+def test_distill_whole_vocabulary():
+    x = _x(4, 200, FP, 8)
+    ids = torch.arange(200, device=DEV).expand(4, 200)
+    top = torch.randn(4, 200, device=DEV, generator=_gen(2))
+    lse = torch.logsumexp(top, 1)
+    a, b = (O.distill_loss_grad(x, ids, top, t) for t in (None, lse))
+    assert torch.allclose(a[0], b[0], rtol=1e-5, atol=1e-5) and torch.allclose(a[1], b[1], rtol=1e-4, atol=1e-6)
+
+
+TOP = [(1, 1, 1), (2, 9, 9), (5, 300, 256), (3, 4096, 8), (2, 5003, 100), (300, 3001, 20), (1, 262144, 20), (4, 262144, 256),
+       (700, 20000, 64), (2, 600007, 33)]
+
+
+def _check_top(x, k, cap, temp):
+    values, ids, lse = O.top_logits(x, k, softcap=cap, temperature=temp)
+    want = torch.sort(x.double(), dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(ids, want)
+    z = oracle.z64(x, cap)
+    zt = z.gather(1, want)
+    assert torch.allclose(values.double(), zt, rtol=2.0 ** -20, atol=2.0 ** -20)
+    oracle.close_logp(lse, torch.logsumexp(z / temp, 1), x, cap, temp)
+
+
+@pytest.mark.parametrize("dtype,cap,temp", [(BF, 30.0, 1.0), (HF, None, 2.0), (FP, 30.0, 0.5)])
+@pytest.mark.parametrize("N,V,k", TOP)
+def test_top_logits(N, V, k, dtype, cap, temp):
+    _check_top(_x(N, V, dtype, N + V, V % 3, V % 2), k, cap, temp)
+
+
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_top_logits_orders(dtype):
+    """Rows that a filter by block maxima handles worst: equal values, sorted both ways, one block of
+    large ones, few finite ones, zeros of both signs, infinities."""
+    V, k = 70001, 200
+    j = torch.arange(V, device=DEV, dtype=torch.float32)
+    inf = float("inf")
+    rows = [torch.zeros(V, device=DEV), j / V, -j / V, torch.where(j < 5000, 1.0 + (j % 7), -1.0),
+            torch.where(j % 1000 == 999, j / V, -inf), torch.where(j % 2 == 0, 0.0, -0.0), torch.where(j > V - 300, inf, j % 3),
+            torch.full((V,), -inf, device=DEV), torch.where((j >= 33000) & (j < 34000), 2.0, 1.0), (j * 7919 % V) % 50]
+    x = torch.stack(rows).to(dtype)
+    values, ids, lse = O.top_logits(x, k)
+    want = torch.sort(x.double(), dim=1, descending=True, stable=True)[1][:, :k]
+    assert torch.equal(ids, want)
+    assert torch.equal(values.double(), x.double().gather(1, want))
+    lse64 = torch.logsumexp(x.double(), 1)
+    keep = [0, 1, 2, 3, 4, 5, 8, 9]
+    oracle.close_logp(lse[keep], lse64[keep], x[keep], None)
+    assert bool(lse[6].isnan()) and lse[7] == -inf
+
+
+def test_top_logits_nan():
+    x = _x(3, 9001, BF, 4)
+    x[1, [70, 8000]] = float("nan")
+    values, ids, lse = O.top_logits(x, 5)
+    assert ids[1, :2].tolist() == [70, 8000] and bool(values[1, :2].isnan().all()) and bool(lse[1].isnan())
+    keep = x[1].float().clone()
+    keep[[70, 8000]] = -float("inf")
+    assert torch.equal(ids[1, 2:], torch.sort(keep, descending=True, stable=True)[1][:3])
+    assert bool(lse[[0, 2]].isfinite().all())
+
+
+@pytest.mark.parametrize("cap", [None, 5.0])
+@pytest.mark.parametrize("dtype,V", [(BF, 4096), (FP, 5003), (BF, 262144), (HF, 12345)])
+def test_non_finite(dtype, V, cap):
+    nan, inf = float("nan"), float("inf")
+    x = _x(7, V, dtype, 1)
+    low = torch.finfo(dtype).min
+    x[0] = nan                                  # untrained: not read
+    x[1, V // 2] = nan
+    x[2, V - 1] = inf
+    x[3] = -inf
+    x[4, 10:] = -inf                            # ten tokens left
+    x[5, : V - 1] = low                         # one token left, the others at the type's lowest value
+    t = torch.tensor([-100, 0, 0, 0, 3, V - 1, V], device=DEV)
+    leaf = x.detach().requires_grad_()
+    logp = O.token_logprobs(leaf, t, softcap=cap)
+    dx, = torch.autograd.grad(logp.sum(), leaf)
+    ref, grad = O.token_logprobs_ref(x.double(), t, cap or 0.0)
+    assert torch.equal(logp.isnan(), ref.isnan()) and torch.equal(dx.isnan(), grad(torch.ones(7, device=DEV)).isnan())
+    ok = ~ref.isnan()
+    assert torch.allclose(logp[ok].double(), ref[ok], rtol=1e-5, atol=1e-5)
+    assert logp[0] == 0 and bool((dx[0] == 0).all()) and bool(logp[6].isnan()) and bool(dx[6].isnan().all())
+    ids, top = _teacher(7, V, 8, 3)
+    ids[4] = torch.arange(8, device=DEV)
+    ids[5, 0] = V - 1
+    ids[5, 1:] = -1
+    w = torch.tensor([0.0, 1, 1, 1, 1, 1, 1], device=DEV)
+    for lse in (None, torch.logsumexp(top, 1) + 0.3):
+        loss, dx = O.distill_loss_grad(x, ids, top, lse, w, softcap=cap)
+        ref, dref = O.distill_ref(x.double(), ids, top.double(), None if lse is None else lse.double(), w, cap or 0.0, 1.0)
+        assert torch.equal(loss.isnan(), ref.isnan()) and loss[0] == 0 and bool((dx[0] == 0).all())
+        finite = ref.isfinite()
+        assert torch.equal(loss.isfinite(), finite)
+        assert torch.allclose(loss[finite].double(), ref[finite], rtol=1e-4, atol=1e-5)
+        assert torch.equal(dx[finite].isnan(), dref[finite].isnan())
+
+
+@pytest.mark.parametrize("kind", O.KINDS)
+@pytest.mark.parametrize("cu_type", [torch.int32, torch.int64])
+def test_pairs(kind, cu_type):
+    T = 7001
+    cu = [0, 1, 1, 900, 2900, 2901, 2901, 6000, 6998]
+    g = _gen(2)
+    lp, ref = (-torch.rand(T, device=DEV, generator=g) * 3 for _ in range(2))
+    cut = torch.tensor(cu, dtype=cu_type, device=DEV)
+    smooth = 0.05 if kind == "sigmoid" else 0.0
+    for r in (ref, None):
+        loss, rewards, grad = O.preference_loss_grad(lp, r, cut, beta=0.02, label_smoothing=smooth, kind=kind)
+        want = oracle.pairs(lp, r, cu, kind, 0.02, smooth, 0.25)
+        # the sums run over up to 3,100 values of 3 at most: 2^-24 * 9300 * a few, times beta
+        size = float(want[1].abs().max()) / 0.02
+        assert torch.allclose(rewards.double(), want[1], rtol=1e-5, atol=1e-2 * 0.02)
+        if kind == "ipo":  # a square of a sum
+            assert torch.allclose(loss.double(), want[0], rtol=1e-4, atol=1e-5 * size * size)
+        else:
+            assert torch.allclose(loss.double(), want[0], rtol=1e-4, atol=2e-4)
+        assert torch.allclose(grad.double(), want[2], rtol=1e-3, atol=1e-5)
+        assert bool((grad[6998:] == 0).all())
+        leaf = lp.clone().requires_grad_()
+        l2, r2 = O.preference_loss(leaf, r, cut, 0.02, smooth, kind)
+        c = torch.rand(4, device=DEV, generator=g)
+        (l2 * c).sum().backward()
+        seq = torch.tensor(cu).diff().to(DEV)
+        per = torch.nn.functional.pad((c * 4).repeat_interleave(2).repeat_interleave(seq), (0, T - 6998))
+        assert torch.equal(l2.detach(), loss) and torch.allclose(leaf.grad, grad * per, rtol=1e-5, atol=1e-9)
+
+
+def test_pairs_many_and_malformed():
+    g = _gen(9)
+    P = 700
+    lens = torch.randint(0, 9, (2 * P,), generator=torch.Generator().manual_seed(1))
+    cu = [0] + lens.cumsum(0).tolist()
+    lp = torch.randn(cu[-1], device=DEV, generator=g)
+    loss, rewards, grad = O.preference_loss_grad(lp, None, torch.tensor(cu, device=DEV), beta=0.5)
+    want = oracle.pairs(lp, None, cu, "sigmoid", 0.5, 0.0, 1 / P)
+    for a, b in zip((loss, rewards, grad), want):
+        assert torch.allclose(a.double(), b, rtol=1e-5, atol=1e-5)
+    bad = torch.tensor([5, 3, 40, 20, 1 << 30, -7, 9], device=DEV)  # read as 5, 5, 40, 40, T, T, T
+    a = O.preference_loss_grad(lp, None, bad)
+    b = O.preference_ref(lp.cpu(), None, bad.cpu(), 0, 0.1, 0.0, 1 / 3)
+    for u, v in zip(a, b):
+        assert torch.allclose(u.cpu(), v, rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("T,V,dtype,kind", [(1, 4096, BF, "sigmoid"), (60, 5003, HF, "ipo"), (200, 32768, BF, "hinge"),
+                                            (64, 262144, BF, "sigmoid")])
+def test_preference_from_logits(T, V, dtype, kind):
+    x = _x(T, V, dtype, T)
+    g = _gen(4)
+    t = torch.randint(0, V, (T,), device=DEV, generator=g)
+    cu = [0, T // 5, T // 2, T // 2, T - T // 6]
+    t[: T // 9] = -100
+    ref = -torch.rand(T, device=DEV, generator=g) * 20
+    ref[: T // 9] = float("nan")
+    loss, rewards, logps, dx = O.preference_logits_grad(x, t, ref, torch.tensor(cu, device=DEV), kind=kind, softcap=30.0)
+    lp64, _, _ = oracle.logprobs(x, t, 30.0, torch.zeros(T, device=DEV))
+    oracle.close_logp(logps, lp64, x, 30.0)
+    l64, r64, g64 = oracle.pairs(lp64, torch.where(t == -100, 0.0, ref), cu, kind, 0.1, 0.0, 0.5)
+    _, grad, mass = oracle.logprobs(x, t, 30.0, g64)
+    assert torch.allclose(rewards.double(), r64, rtol=1e-4, atol=1e-4)
+    assert torch.allclose(loss.double(), l64, rtol=1e-3, atol=1e-3)
+    # the pair's coefficient itself carries up to 1e-4 of relative error
+    tol = (1.01 * oracle.UNIT[dtype] + 1e-4) * grad.abs() + (2.0 ** -16) * g64.abs()[:, None] * mass + oracle.TINY[dtype]
+    assert bool(((dx.double() - grad).abs() <= tol).all())
+    assert bool((dx[: T // 9] == 0).all()) and bool((dx[cu[-1]:] == 0).all())
+
+
+def test_expanded_rows_and_empty():
+    row = _x(1, 5003, BF, 2)
+    x = row.expand(6, 5003)
+    t = torch.arange(6, device=DEV)
+    leaf = x.detach().requires_grad_()
+    logp = O.token_logprobs(leaf, t)
+    dx, = torch.autograd.grad(logp.sum(), leaf)
+    want, grad, mass = oracle.logprobs(x, t, None, torch.ones(6, device=DEV))
+    oracle.close_logp(logp.detach(), want, x, None)
+    oracle.close_grad(dx, grad, torch.ones(6, device=DEV), mass, BF)
+    none = x[:0]
+    assert O.token_logprobs(none, t[:0]).shape == (0,)
+    v, i, lse = O.top_logits(none, 4)
+    assert v.shape == (0, 4) and lse.shape == (0,)
+    loss, d = O.distill_loss_grad(none, t[:0, None], torch.zeros(0, 1, device=DEV))
+    assert loss.shape == (0,) and d.shape == (0, 5003)
+    loss, _, grad = O.preference_loss_grad(torch.ones(3, device=DEV), None, torch.zeros(1, dtype=torch.int64, device=DEV))
+    assert loss.shape == (0,) and grad.tolist() == [0, 0, 0]
+
+
+def test_offsets_past_32_bits():
+    """More than 2^31 logits: the last rows, against the same rows alone."""
+    N, V = 8240, 262144
+    if torch.cuda.mem_get_info()[0] < 14 << 30:
+        pytest.skip("needs 14 GB of free memory")
+    x = torch.empty(N, V, dtype=BF, device=DEV)
+    x.normal_(generator=_gen(3))
+    t = torch.randint(0, V, (N,), device=DEV, generator=_gen(4))
+    ids, top = t[:, None], torch.zeros(N, 1, device=DEV)
+    values, at, lse = O.top_logits(x, 3)
+    logp = O.token_logprobs(x, t)
+    tail = x[-9:].clone()
+    assert all(torch.equal(a[-9:], b) for a, b in zip((values, at, lse), O.top_logits(tail, 3)))
+    assert torch.allclose(logp[-9:], O.token_logprobs(tail, t[-9:]), rtol=1e-6, atol=1e-6)
+    loss, dx = O.distill_loss_grad(x, ids, top, softcap=30.0, out=x)
+    loss2, dx2 = O.distill_loss_grad(tail, ids[-9:], top[-9:], softcap=30.0)
+    assert torch.allclose(loss[-9:], loss2, rtol=1e-5, atol=1e-5)
+    assert torch.allclose(dx[-9:].float(), dx2.float(), rtol=2.0 ** -7, atol=1e-9)
+
+
+def _every_call(x, t, ids, top, w, cu):
+    out = list(O.top_logits(x, 40, softcap=30.0))
+    leaf = x.detach().requires_grad_()
+    logp = O.token_logprobs(leaf, t, softcap=30.0)
+    out += [logp.detach(), torch.autograd.grad(logp.sum(), leaf)[0]]
+    out += list(O.distill_loss_grad(x, ids, top, None, w, softcap=30.0))
+    out += list(O.distill_loss_grad(x, ids, top, torch.logsumexp(top, 1), w, softcap=30.0))
+    out += list(O.preference_logits_grad(x, t, None, cu, softcap=30.0))
+    return out
+
+
+def test_streams_and_repeats():
+    """The same bits on every run, on another stream, and as a CUDA graph."""
+    x = _x(500, 50001, BF, 1)
+    t = torch.randint(0, 50001, (500,), device=DEV, generator=_gen(1))
+    ids, top = _teacher(500, 50001, 30, 2)
+    w = torch.rand(500, device=DEV, generator=_gen(3))
+    cu = torch.tensor([0, 100, 300, 301, 480], device=DEV)
+    first = _every_call(x, t, ids, top, w, cu)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        moved = x + 0  # made on this stream: a launch on another one would race with it
+        second = _every_call(moved, t, ids, top, w, cu)
+        graph = torch.cuda.CUDAGraph()
+    s.synchronize()
+    for a, b in zip(first, second):
+        assert torch.equal(a, b)
+    with torch.cuda.graph(graph, stream=s):
+        third = _every_call(x, t, ids, top, w, cu)
+    graph.replay()
+    torch.cuda.synchronize()
+    for a, b in zip(first, third):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("what", list(refusals("cpu")))
+def test_refusals(what):
+    with pytest.raises(ValueError):
+        refusals(DEV)[what]()
+
+
+def test_native_refusals():
+    x = _x(4, 64, BF)
+    t = torch.zeros(4, dtype=torch.int64, device=DEV)
+    with pytest.raises(RuntimeError, match="contiguous"):
+        O.token_logprobs(_x(64, 4, BF).t(), t)
+    with pytest.raises(RuntimeError, match="bfloat16, float16 or float32"):
+        O.top_logits(x.double(), 2)
+    with pytest.raises(RuntimeError, match="another device"):
+        O.token_logprobs(x, t.cpu())
+    with pytest.raises(RuntimeError, match="another device"):
+        O.distill_loss(x, t[:, None], torch.zeros(4, 1))
+    with pytest.raises(RuntimeError, match="device"):
+        O.preference_loss(torch.zeros(4, device=DEV), None, torch.tensor([0, 1, 4]))
+    with pytest.raises(RuntimeError, match="apart"):
+        O.distill_loss_grad(x, t[:, None], torch.zeros(4, 1, device=DEV), out=x[:1].expand(4, 64))
