@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "act.cuh"
 #include "common.cuh"
 #include "objectives.h"
@@ -23,13 +25,175 @@ union Vec16 {
   T h[16 / sizeof(T)];
 };
 
-// z = c tanh(x / c), or x without a cap (cap <= 0).
+// z = c tanh(x / c), or x without a cap (cap <= 0): the accurate form of single elements.
 ME_DEVICE float softcap(float x, float cap) { return cap > 0.f ? cap * tanhf(x / cap) : x; }
 // dz/dx, from z.
 ME_DEVICE float softcap_slope(float z, float cap) {
   if (cap <= 0.f) return 1.f;
   const float t = z / cap;
   return 1.f - t * t;
+}
+
+// ---------------------------------------------------------------- two fp32 numbers an instruction
+typedef unsigned long long f32x2;
+
+ME_DEVICE f32x2 pack2(float a, float b) {
+  f32x2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+ME_DEVICE f32x2 both2(float a) { return pack2(a, a); }
+ME_DEVICE float2 unpack2(f32x2 v) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(v));
+  return r;
+}
+ME_DEVICE f32x2 fma2(f32x2 a, f32x2 b, f32x2 c) {
+  f32x2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+ME_DEVICE f32x2 mul2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+ME_DEVICE f32x2 add2(f32x2 a, f32x2 b) {
+  f32x2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// A 16-byte vector of logits as pairs, and back (one rounding).
+template <typename T>
+ME_DEVICE void to_pairs(uint4 v, f32x2 (&p)[Vec16<T>::kN / 2]) {
+  if constexpr (sizeof(T) == 4) {
+    p[0] = pack2(__uint_as_float(v.x), __uint_as_float(v.y));
+    p[1] = pack2(__uint_as_float(v.z), __uint_as_float(v.w));
+  } else {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        p[i] = pack2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+      } else {
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+        p[i] = pack2(f.x, f.y);
+      }
+    }
+  }
+}
+template <typename T>
+ME_DEVICE uint4 from_pairs(const f32x2 (&p)[Vec16<T>::kN / 2]) {
+  uint32_t w[4];
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float2 f = unpack2(p[i]);
+      w[2 * i] = __float_as_uint(f.x);
+      w[2 * i + 1] = __float_as_uint(f.y);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const float2 f = unpack2(p[i]);
+      if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+        const __nv_bfloat162 h = __float22bfloat162_rn(f);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      } else {
+        const __half2 h = __float22half2_rn(f);
+        w[i] = *reinterpret_cast<const uint32_t*>(&h);
+      }
+    }
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// Largest element of a vector, or largest magnitude (a NaN beside numbers is passed over).
+template <typename T, bool kAbs>
+ME_DEVICE float vec_max(uint4 v) {
+  if constexpr (sizeof(T) == 4) {
+    float a = __uint_as_float(v.x), b = __uint_as_float(v.y), c = __uint_as_float(v.z), d = __uint_as_float(v.w);
+    if (kAbs) a = fabsf(a), b = fabsf(b), c = fabsf(c), d = fabsf(d);
+    return fmaxf(fmaxf(a, b), fmaxf(c, d));
+  } else {
+    using T2 = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162, __half2>;
+    T2 a = *reinterpret_cast<T2*>(&v.x), b = *reinterpret_cast<T2*>(&v.y), c = *reinterpret_cast<T2*>(&v.z),
+       d = *reinterpret_cast<T2*>(&v.w);
+    if (kAbs) a = __habs2(a), b = __habs2(b), c = __habs2(c), d = __habs2(d);
+    const T2 m = __hmax2(__hmax2(a, b), __hmax2(c, d));
+    return fmaxf(to_f<T>(m.x), to_f<T>(m.y));
+  }
+}
+
+// How raw logits become exponents: z = softcap(x), y = z / tau.
+struct Scale {
+  float cap, inv_c2, inv_temp;  // inv_c2 = 1 / c^2
+};
+
+// c tanh(x / c) for |x| <= c: x + x w Q(w), w = (x / c)^2, Q the minimax polynomial of (tanh(u) / u - 1) / u^2
+// in u^2 on [0, 1] (Remez exchange on tanh itself). Degree 6: relative error 5e-9, and x enters
+// unrounded, so the result is a correctly scaled sum with about half a unit of error; degree 4: 7e-7, for
+// gradients in 16 bits. On the FMA pipe: ex2 and rcp would cost two of the special function unit's 16
+// results a clock, which the exponential of the softmax needs.
+template <int kDeg>
+ME_DEVICE f32x2 softcap2(f32x2 x, f32x2 inv_c2) {
+  const f32x2 w = mul2(mul2(x, x), inv_c2);
+  f32x2 q;
+  if constexpr (kDeg == 6) {
+    q = fma2(both2(-0.000358452002f), w, both2(0.00230136459f));
+    q = fma2(q, w, both2(-0.00794610642f));
+    q = fma2(q, w, both2(0.0214866576f));
+    q = fma2(q, w, both2(-0.0538798027f));
+    q = fma2(q, w, both2(0.133323446f));
+    q = fma2(q, w, both2(-0.333332954f));
+  } else {
+    q = fma2(both2(-0.00312657789f), w, both2(0.0169064092f));
+    q = fma2(q, w, both2(-0.0517682859f));
+    q = fma2(q, w, both2(0.132884903f));
+    q = fma2(q, w, both2(-0.333302797f));
+  }
+  return fma2(mul2(x, w), q, x);
+}
+
+// z of a vector: the polynomial, or element by element where one is beyond the cap.
+template <typename T, bool kCap, int kDeg>
+ME_DEVICE void vec_softcap(uint4 v, const Scale& sc, f32x2 (&z)[Vec16<T>::kN / 2]) {
+  to_pairs<T>(v, z);
+  if constexpr (kCap) {
+    if (vec_max<T, true>(v) <= sc.cap) {
+#pragma unroll
+      for (int i = 0; i < Vec16<T>::kN / 2; ++i) z[i] = softcap2<kDeg>(z[i], both2(sc.inv_c2));
+    } else {
+#pragma unroll 1
+      for (int i = 0; i < Vec16<T>::kN / 2; ++i) {
+        // (a loop that is not unrolled would index the pairs in local memory: rotate them instead)
+        const float2 f = unpack2(z[0]);
+#pragma unroll
+        for (int o = 0; o + 1 < Vec16<T>::kN / 2; ++o) z[o] = z[o + 1];
+        z[Vec16<T>::kN / 2 - 1] = pack2(softcap(f.x, sc.cap), softcap(f.y, sc.cap));
+      }
+    }
+  }
+}
+
+// e^d of a pair, -87 <= d <= 88: d = n ln 2 + r with n whole (Cody and Waite's two-step reduction), 2^n
+// added to the exponent of 2^(r / ln 2). The reduction keeps the argument's rounding out of the result,
+// which a sum of many terms would otherwise carry (1e-7 mean error at d = -10 with ex2 alone).
+ME_DEVICE f32x2 exp_pair(f32x2 d) {
+  const float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number in the low bits
+  const f32x2 t = fma2(d, both2(kLog2e), both2(kMagic));
+  f32x2 f = fma2(d, both2(kLog2e), fma2(t, both2(-1.f), both2(kMagic)));  // d log2 e - n
+  f = fma2(d, both2(1.925963033500011e-8f), f);  // log2 e - its fp32 value
+  const float2 g = unpack2(f), m = unpack2(t);
+  return pack2(__uint_as_float(__float_as_uint(exp2_fast(g.x)) + (__float_as_uint(m.x) << 23)),
+               __uint_as_float(__float_as_uint(exp2_fast(g.y)) + (__float_as_uint(m.y) << 23)));
+}
+// max(a, b) that keeps a NaN
+ME_DEVICE float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
 }
 
 // A logits matrix and its rows' stride in elements.
@@ -40,75 +204,182 @@ struct Rows {
   ME_DEVICE T* row(int64_t r) const { return base + r * stride; }
 };
 
-// Calls f(j, x_j) for every column of a row of V logits, the block's threads in turn: single
-// elements up to the first 16-byte boundary and after the last one, 16-byte vectors between.
-template <typename T, typename F>
-ME_DEVICE void for_row(const T* row, int64_t V, F&& f) {
-  constexpr int kN = Vec16<T>::kN;
-  int64_t head = ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T);
-  if (head > V) head = V;
-  for (int64_t j = threadIdx.x; j < head; j += blockDim.x) f(j, to_f<T>(row[j]));
-  const int64_t nvec = (V - head) / kN;
-  const uint4* body = reinterpret_cast<const uint4*>(row + head);
-  for (int64_t i = threadIdx.x; i < nvec; i += blockDim.x) {
-    Vec16<T> v;
-    v.u = body[i];
-#pragma unroll
-    for (int e = 0; e < kN; ++e) f(head + i * kN + e, to_f<T>(v.h[e]));
+// A block's share of one row: 16-byte vectors [begin, end) from `body`, and for the row's first and
+// last block the elements ahead of the first 16-byte boundary and after the last one.
+template <typename T>
+struct Slice {
+  static constexpr int kN = Vec16<T>::kN;
+  const T* row;
+  int64_t head, body_end, V;  // columns [head, body_end) are vectors
+  int64_t begin, end;         // of them, this block's
+  bool first, last;
+
+  ME_DEVICE Slice(const T* row_, int64_t V_, int rank, int ranks) : row(row_), V(V_) {
+    head = ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T);
+    if (head > V) head = V;
+    const int64_t nvec = (V - head) / kN, per = (nvec + ranks - 1) / ranks;
+    body_end = head + nvec * kN;
+    begin = min(nvec, rank * per);
+    end = min(nvec, begin + per);
+    first = rank == 0;
+    last = rank == ranks - 1;
   }
-  for (int64_t j = head + nvec * kN + threadIdx.x; j < V; j += blockDim.x) f(j, to_f<T>(row[j]));
-}
+  ME_DEVICE const uint4* body() const { return reinterpret_cast<const uint4*>(row + head); }
+  ME_DEVICE int64_t column(int64_t vec) const { return head + vec * kN; }
+  // The block's single columns, one a thread: -1 for the threads that have none.
+  ME_DEVICE int64_t single() const {
+    const int64_t t = threadIdx.x;
+    if (first && t < head) return t;
+    if (last && t >= 16 && t - 16 < V - body_end) return body_end + t - 16;
+    return -1;
+  }
+  // Whether a column is this block's.
+  ME_DEVICE bool holds(int64_t j) const {
+    if (j < head) return first;
+    if (j >= body_end) return last;
+    const int64_t v = (j - head) / kN;
+    return v >= begin && v < end;
+  }
+};
 
 // Running (m, s): s = sum exp(y - m), m the largest y so far. A NaN or +inf makes s NaN.
 struct MaxSum {
   float m = -INFINITY, s = 0.f;
   ME_DEVICE void add(float y) {
     if (y > m) {
-      s = s * exp2_fast((m - y) * kLog2e) + exp2_fast(y - y);  // + 1, or NaN for y = inf
+      s = s * expf(m - y) + expf(y - y);  // + 1, or NaN for y = inf
       m = y;
     } else if (y != -INFINITY) {  // y NaN: s becomes NaN
-      s += exp2_fast((y - m) * kLog2e);
+      s += expf(y - m);
     }
   }
-  ME_DEVICE void merge(float m2, float s2) {
-    if (m2 == -INFINITY) {
-      s += s2;  // 0, or NaN
+  ME_DEVICE void merge(MaxSum o) {
+    if (o.m == -INFINITY) {
+      s += o.s;  // 0, or NaN
     } else if (m == -INFINITY) {
-      s += s2;
-      m = m2;
+      s += o.s;
+      m = o.m;
     } else {
-      const float mx = fmaxf(m, m2);
-      s = s * exp2_fast((m - mx) * kLog2e) + s2 * exp2_fast((m2 - mx) * kLog2e);
+      const float mx = fmaxf(m, o.m);
+      s = s * expf(m - mx) + o.s * expf(o.m - mx);
       m = mx;
     }
   }
 };
 
-// Over the whole block, the same for all threads; `scratch` holds 64 floats.
-ME_DEVICE MaxSum block_merge(MaxSum a, float* scratch) {
+// No column is left out.
+struct KeepAll {
+  ME_DEVICE uint32_t operator()(int64_t) const { return 0; }
+  ME_DEVICE bool column(int64_t) const { return false; }
+};
+
+constexpr int kBatch = 4;  // vectors that a thread has in flight
+
+// This thread's share of sum exp(y - m) over a slice. `drop(vec)`: a mask of the vector's elements
+// that are left out (`drop.column(j)` for a single column).
+//
+// One pass with a fixed reference: rho = the largest y of the thread's first vectors, so no running
+// maximum is carried. A share that this does not suit (a sum out of range, a first batch of -inf, a
+// NaN or +inf anywhere) is added again element by element with a running maximum.
+template <typename T, bool kCap, typename Drop>
+ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop) {
+  constexpr int kN = Vec16<T>::kN, kP = kN / 2;
+  const uint4* body = sl.body();
+  const int64_t step = blockDim.x;
+  MaxSum out;
+  int64_t i = sl.begin + threadIdx.x;
+  if (i < sl.end) {
+    uint4 v[kBatch];
+    float top = -INFINITY, big = -INFINITY;
+    f32x2 sum = both2(0.f);
+    float rho = 0.f;
+    auto add = [&](uint4 x, int64_t vec) {
+      if constexpr (!kCap) big = fmaxf(big, vec_max<T, false>(x));
+      f32x2 y[kP];
+      vec_softcap<T, kCap, 6>(x, sc, y);
+      const uint32_t out_mask = drop(vec);
+#pragma unroll
+      for (int p = 0; p < kP; ++p) {
+        const float2 d = unpack2(fma2(y[p], both2(sc.inv_temp), both2(-rho)));
+        float a = max_nan(d.x, -87.f), b = max_nan(d.y, -87.f);
+        if (!std::is_same_v<Drop, KeepAll>) {
+          if (out_mask >> (2 * p) & 1) a = -87.f;
+          if (out_mask >> (2 * p) & 2) b = -87.f;
+        }
+        sum = add2(sum, exp_pair(pack2(a, b)));
+      }
+    };
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u * step < sl.end) v[u] = body[i + u * step];
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u * step < sl.end) top = fmaxf(top, vec_max<T, false>(v[u]));
+    rho = softcap(top, sc.cap) * sc.inv_temp;
+#pragma unroll
+    for (int u = 0; u < kBatch; ++u)
+      if (i + u * step < sl.end) add(v[u], i + u * step);
+    i += kBatch * step;
+    for (; i + (kBatch - 1) * step < sl.end; i += kBatch * step) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) v[u] = body[i + u * step];
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) add(v[u], i + u * step);
+    }
+    for (; i < sl.end; i += step) add(body[i], i);
+    const float2 s2 = unpack2(sum);
+    const float s = s2.x + s2.y;
+    const float far = kCap ? sc.cap * sc.inv_temp - rho : big * sc.inv_temp - rho;  // the largest exponent
+    if (s > 1e-30f && s < 1e37f && far < 80.f) {
+      out.m = rho;
+      out.s = s;
+    } else {
+      for (i = sl.begin + threadIdx.x; i < sl.end; i += step) {
+        const uint32_t out_mask = drop(i);
+        for (int e = 0; e < kN; ++e)
+          if (!(out_mask >> e & 1)) out.add(softcap(to_f<T>(sl.row[sl.column(i) + e]), sc.cap) * sc.inv_temp);
+      }
+    }
+  }
+  const int64_t j = sl.single();
+  if (j >= 0 && !drop.column(j)) out.add(softcap(to_f<T>(sl.row[j]), sc.cap) * sc.inv_temp);
+  return out;
+}
+
+// Block-wide largest and sum; `scratch` holds 32 floats and is free again after the next barrier.
+ME_DEVICE float block_max(float v, float* scratch) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, a.m, o), s2 = __shfl_xor_sync(0xffffffffu, a.s, o);
-    a.merge(m2, s2);
-  }
+  v = warp_max(v);
   __syncthreads();
-  if (lane == 0) {
-    scratch[wid] = a.m;
-    scratch[32 + wid] = a.s;
-  }
+  if (lane == 0) scratch[wid] = v;
   __syncthreads();
+  return warp_max(lane < nw ? scratch[lane] : -INFINITY);
+}
+
+// The block's (m, s), the same for all threads: one exponential a thread.
+ME_DEVICE MaxSum block_merge(MaxSum a, float* scratch) {
   MaxSum r;
-  if (lane < nw) {
-    r.m = scratch[lane];
-    r.s = scratch[32 + lane];
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    const float m2 = __shfl_xor_sync(0xffffffffu, r.m, o), s2 = __shfl_xor_sync(0xffffffffu, r.s, o);
-    r.merge(m2, s2);
-  }
+  r.m = block_max(a.m, scratch);
+  // a.m = -inf: a.s is 0 or NaN
+  r.s = block_sum(a.m == -INFINITY ? a.s : a.s * expf(a.m - r.m), scratch);
   return r;
+}
+
+// ---------------------------------------------------------------- thread-block clusters
+ME_DEVICE uint32_t cluster_rank() {
+  uint32_t r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+ME_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+ME_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// A float in the shared memory of the cluster's block `rank`, at the place that `p` has in this one.
+ME_DEVICE float cluster_load(const float* p, uint32_t rank) {
+  uint32_t a = (uint32_t)__cvta_generic_to_shared(p), b;
+  float v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(rank));
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(b) : "memory");
+  return v;
 }
 
 // SMs of the current device (one kind of GPU is built for).
@@ -120,6 +391,23 @@ inline int objective_sms() {
     return c;
   }();
   return n;
+}
+
+// Launches `kernel` on grid blocks in clusters of `cluster`.
+template <typename... Params, typename... Args>
+cudaError_t launch_cluster(void (*kernel)(Params...), int64_t grid, int threads, int cluster, cudaStream_t stream,
+                           Args... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)grid);
+  cfg.blockDim = dim3(threads);
+  cfg.stream = stream;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = cluster;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
 template <typename T>

@@ -39,7 +39,8 @@ void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, flo
 void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
                         cudaStream_t stream);
 void launch_distill_fwd(const Logits& x, const TeacherArgs& teacher, float* loss, float4* stats, cudaStream_t stream);
-// g: one coefficient a row, or null for 1
+// value and gradient of sum(loss) in one launch
+void launch_distill_grad(const Logits& x, const TeacherArgs& teacher, float* loss, Gradient out, cudaStream_t stream);
 void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const float4* stats, const float* g, Gradient out,
                         cudaStream_t stream);
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,

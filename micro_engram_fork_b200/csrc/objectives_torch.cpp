@@ -16,6 +16,7 @@ me::Logits check_logits(const Tensor& x, double cap, const char* what) {
   TORCH_CHECK(x.dim() == 2, what, ": [rows, vocabulary] is needed, got ", x.dim(), " dimensions");
   TORCH_CHECK(x.size(1) > 0 && x.size(1) <= INT32_MAX, what, ": a vocabulary of 1 to 2^31 - 1 entries is needed, got ",
               x.size(1));
+  TORCH_CHECK(x.size(0) < (1 << 28), what, ": 2^28 - 1 rows at most, got ", x.size(0));
   TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, what, ": a row's logits have to be contiguous");
   me::LogitType type = me::LogitType::kF32;
   if (x.scalar_type() == torch::kBFloat16) type = me::LogitType::kBF16;
@@ -120,15 +121,14 @@ std::vector<Tensor> distill_fwd(Tensor x, Tensor ids, Tensor top, OptTensor lse,
 }
 
 Tensor distill_bwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap, double temp,
-                   Tensor stats, OptTensor g, OptTensor out) {
+                   Tensor stats, Tensor g, OptTensor out) {
   const auto in = check_logits(x, cap, "distill_loss");
   const at::cuda::CUDAGuard guard(x.device());
   const auto te = check_teacher(x, ids, top, lse, weight, temp);
-  Tensor gr;
-  if (g.has_value()) gr = check_rows(*g, x, torch::kFloat32, "distill_loss: gradient");
+  auto gr = check_rows(g, x, torch::kFloat32, "distill_loss: gradient");
   auto o = gradient_like(x, out, "distill_loss");
   if (in.N == 0) return o;
-  me::launch_distill_bwd(in, te.args, as4(stats), g.has_value() ? gr.data_ptr<float>() : nullptr, gradient_of(o),
+  me::launch_distill_bwd(in, te.args, as4(stats), gr.data_ptr<float>(), gradient_of(o),
                          at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
@@ -137,8 +137,15 @@ Tensor distill_bwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor we
 // (loss [N], dL/dx [N, V])
 std::vector<Tensor> distill_grad(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap,
                                  double temp, OptTensor out) {
-  auto f = distill_fwd(x, ids, top, lse, weight, cap, temp);
-  return {f[0], distill_bwd(x, ids, top, lse, weight, cap, temp, f[1], c10::nullopt, out)};
+  const auto in = check_logits(x, cap, "distill_loss");
+  const at::cuda::CUDAGuard guard(x.device());
+  const auto te = check_teacher(x, ids, top, lse, weight, temp);
+  auto o = gradient_like(x, out, "distill_loss");
+  auto loss = torch::empty({in.N}, x.options().dtype(torch::kFloat32));
+  if (in.N == 0) return {loss, o};
+  me::launch_distill_grad(in, te.args, loss.data_ptr<float>(), gradient_of(o), at::cuda::getCurrentCUDAStream());
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {loss, o};
 }
 
 // (values [N, k] fp32, ids [N, k] int64, lse [N] fp32)

@@ -19,6 +19,10 @@ ME_DEVICE uint32_t order_key(float x) {
   const uint32_t b = __float_as_uint(x + 0.f);
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+template <typename T, typename F>
+ME_DEVICE void for_row(const T* row, int64_t V, F&& f) {
+  for (int64_t j = threadIdx.x; j < V; j += blockDim.x) f(j, to_f<T>(row[j]));
+}
 // Radix selection, eight bits of the key a pass over the row: the exact k-th largest key, then every
 // larger one and the lowest ids among its equals, ranked by counting.
 template <typename T>
