@@ -74,12 +74,12 @@ ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m,
   const bool aligned = (reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0;
   auto one = [&](uint4 x, int64_t vec) {
     f32x2 z[kP];
-    vec_softcap<T, kCap, sizeof(T) == 4 ? 6 : 4>(x, sc, z);
+    vec_softcap<T, kCap>(x, sc, z);
 #pragma unroll
     for (int p = 0; p < kP; ++p) {
       const float2 a = unpack2(mul2(fma2(z[p], both2(sc.inv_temp), both2(-m)), both2(kLog2e)));
       const f32x2 e = mul2(pack2(exp2_fast(a.x), exp2_fast(a.y)), both2(coef));
-      if constexpr (kCap) z[p] = mul2(e, fma2(mul2(z[p], both2(-sc.inv_c2)), z[p], both2(1.f)));
+      if constexpr (kCap) z[p] = mul2(e, fma2(mul2(z[p], both2(sc.slope)), z[p], both2(1.f)));
       else z[p] = e;
     }
     Vec16<T> r;
@@ -397,10 +397,6 @@ int ranks_for_two_passes(const Logits& x) {
   return ranks_for(x.N, x.V, c);
 }
 
-Scale scale_of(const Logits& x, float temp) {
-  return {x.cap, x.cap > 0.f ? (float)(1.0 / ((double)x.cap * x.cap)) : 0.f, (float)(1.0 / (double)temp)};
-}
-
 }  // namespace
 
 namespace me {
@@ -418,7 +414,7 @@ void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, flo
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, launch_cluster(logprob_fwd_kernel<T, kCap>, x.N * ranks, kThreads,
                                                                    ranks, stream, rows_in<T>(x), x.V, ranks, target,
-                                                                   scale_of(x, 1.f), logp, stats)));
+                                                                   make_scale(x.cap, 1.f), logp, stats)));
 }
 
 void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
@@ -426,7 +422,7 @@ void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* st
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, logprob_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
-                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, target, scale_of(x, 1.f),
+                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, target, make_scale(x.cap, 1.f),
                                          stats, g)));
 }
 
@@ -435,7 +431,7 @@ void launch_distill_fwd(const Logits& x, const TeacherArgs& te, float* loss, flo
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, false> : distill_kernel<T, kCap, false, false>;
     launch_cluster(kernel, x.N * ranks, kThreads, ranks, stream, rows_in<T>(x), Rows<T>{}, x.V, ranks, te,
-                   scale_of(x, te.temp), loss, stats);
+                   make_scale(x.cap, te.temp), loss, stats);
   }));
 }
 
@@ -444,7 +440,7 @@ void launch_distill_grad(const Logits& x, const TeacherArgs& te, float* loss, Gr
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, true> : distill_kernel<T, kCap, false, true>;
     launch_cluster(kernel, x.N * ranks, kThreads, ranks, stream, rows_in<T>(x), rows_out<T>(out), x.V, ranks, te,
-                   scale_of(x, te.temp), loss, (float4*)nullptr);
+                   make_scale(x.cap, te.temp), loss, (float4*)nullptr);
   }));
 }
 
@@ -453,7 +449,7 @@ void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const float4* st
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, distill_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
-                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, te, scale_of(x, te.temp),
+                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, te, make_scale(x.cap, te.temp),
                                          stats, g)));
 }
 

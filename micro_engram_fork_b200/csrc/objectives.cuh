@@ -4,6 +4,8 @@
 
 #include <cuda_fp16.h>
 
+#include <string.h>
+
 #include <type_traits>
 
 #include "act.cuh"
@@ -126,44 +128,54 @@ ME_DEVICE float vec_max(uint4 v) {
   }
 }
 
-// How raw logits become exponents: z = softcap(x), y = z / tau.
+// How raw logits become exponents: z = softcap(x), y = z / tau. `limit`: the largest |x| that softcap2
+// may be given (negative: none).
 struct Scale {
-  float cap, inv_c2, inv_temp;  // inv_c2 = 1 / c^2
+  float cap, limit, inv_temp, slope;  // slope = -1 / c^2
+  f32x2 q[7];                         // softcap2's coefficients, each one twice
 };
 
-// c tanh(x / c) for |x| <= c: x + x w Q(w), w = (x / c)^2, Q the minimax polynomial of (tanh(u) / u - 1) / u^2
-// in u^2 on [0, 1] (Remez exchange on tanh itself). Degree 6: relative error 5e-9, and x enters
-// unrounded, so the result is a correctly scaled sum with about half a unit of error; degree 4: 7e-7, for
-// gradients in 16 bits. On the FMA pipe: ex2 and rcp would cost two of the special function unit's 16
-// results a clock, which the exponential of the softmax needs.
-template <int kDeg>
-ME_DEVICE f32x2 softcap2(f32x2 x, f32x2 inv_c2) {
-  const f32x2 w = mul2(mul2(x, x), inv_c2);
-  f32x2 q;
-  if constexpr (kDeg == 6) {
-    q = fma2(both2(-0.000358452002f), w, both2(0.00230136459f));
-    q = fma2(q, w, both2(-0.00794610642f));
-    q = fma2(q, w, both2(0.0214866576f));
-    q = fma2(q, w, both2(-0.0538798027f));
-    q = fma2(q, w, both2(0.133323446f));
-    q = fma2(q, w, both2(-0.333332954f));
-  } else {
-    q = fma2(both2(-0.00312657789f), w, both2(0.0169064092f));
-    q = fma2(q, w, both2(-0.0517682859f));
-    q = fma2(q, w, both2(0.132884903f));
-    q = fma2(q, w, both2(-0.333302797f));
+// c tanh(x / c) for |x| <= c: x + x v Q(v), v = x^2, Q the minimax polynomial of (tanh(u) / u - 1) / u^2 in
+// u^2 on [0, 1] (Remez exchange on tanh itself; its coefficients carry the powers of 1 / c^2).
+// Relative error 5e-9, and x enters unrounded: half a unit of error, in nine operations of the FMA
+// pipe. By exponential and reciprocal it would be two results of the special function unit, which gives
+// 16 a clock on an SM and has the softmax's exponential to do.
+ME_DEVICE f32x2 softcap2(f32x2 x, const Scale& sc) {
+  const f32x2 v = mul2(x, x);
+  f32x2 q = fma2(sc.q[6], v, sc.q[5]);
+#pragma unroll
+  for (int i = 4; i >= 0; --i) q = fma2(q, v, sc.q[i]);
+  return fma2(mul2(x, v), q, x);
+}
+
+inline Scale make_scale(float cap, float temp) {
+  static const double kQ[7] = {-0.333332954, 0.133323446, -0.0538798027, 0.0214866576, -0.00794610642,
+                               0.00230136459, -0.000358452002};
+  Scale s = {cap, 0.f, (float)(1.0 / (double)temp), 0.f, {}};
+  if (cap > 0.f) {
+    const double r = 1.0 / ((double)cap * cap);
+    s.slope = (float)-r;
+    // (c^14 has to be an fp32 number; other caps take the element's form)
+    s.limit = cap > 4e-3f && cap < 400.f ? cap : -1.f;
+    double p = r;
+    for (int i = 0; i < 7; ++i, p *= r) {
+      const float q = (float)(s.limit > 0.f ? kQ[i] * p : 0.0);
+      uint32_t bits;
+      memcpy(&bits, &q, 4);
+      s.q[i] = (unsigned long long)bits << 32 | bits;
+    }
   }
-  return fma2(mul2(x, w), q, x);
+  return s;
 }
 
 // z of a vector: the polynomial, or element by element where one is beyond the cap.
-template <typename T, bool kCap, int kDeg>
+template <typename T, bool kCap>
 ME_DEVICE void vec_softcap(uint4 v, const Scale& sc, f32x2 (&z)[Vec16<T>::kN / 2]) {
   to_pairs<T>(v, z);
   if constexpr (kCap) {
-    if (vec_max<T, true>(v) <= sc.cap) {
+    if (vec_max<T, true>(v) <= sc.limit) {
 #pragma unroll
-      for (int i = 0; i < Vec16<T>::kN / 2; ++i) z[i] = softcap2<kDeg>(z[i], both2(sc.inv_c2));
+      for (int i = 0; i < Vec16<T>::kN / 2; ++i) z[i] = softcap2(z[i], sc);
     } else {
 #pragma unroll 1
       for (int i = 0; i < Vec16<T>::kN / 2; ++i) {
@@ -278,9 +290,13 @@ constexpr int kBatch = 4;  // vectors that a thread has in flight
 // This thread's share of sum exp(y - m) over a slice. `drop(vec)`: a mask of the vector's elements
 // that are left out (`drop.column(j)` for a single column).
 //
-// One pass with a fixed reference: rho = the largest y of the thread's first vectors, so no running
-// maximum is carried. A share that this does not suit (a sum out of range, a first batch of -inf, a
-// NaN or +inf anywhere) is added again element by element with a running maximum.
+// One pass with a fixed reference: the largest z of the thread's first vectors, so no running maximum
+// is carried. A share that this does not suit (a sum out of range, a first batch of -inf, a NaN or
+// +inf anywhere) is added again element by element with a running maximum.
+//
+// With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
+// moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
+// form, since nothing else is rounded then.
 template <typename T, bool kCap, typename Drop>
 ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
@@ -291,22 +307,38 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
   if (i < sl.end) {
     uint4 v[kBatch];
     float top = -INFINITY, big = -INFINITY;
-    f32x2 sum = both2(0.f);
-    float rho = 0.f;
+    float sum0 = 0.f, sum1 = 0.f;
+    float ref = 0.f;  // with a softcap of z, else of y
+    const float k = sc.inv_temp * kLog2e;
     auto add = [&](uint4 x, int64_t vec) {
       if constexpr (!kCap) big = fmaxf(big, vec_max<T, false>(x));
       f32x2 y[kP];
-      vec_softcap<T, kCap, 6>(x, sc, y);
+      vec_softcap<T, kCap>(x, sc, y);
       const uint32_t out_mask = drop(vec);
 #pragma unroll
       for (int p = 0; p < kP; ++p) {
-        const float2 d = unpack2(fma2(y[p], both2(sc.inv_temp), both2(-rho)));
-        float a = max_nan(d.x, -87.f), b = max_nan(d.y, -87.f);
-        if (!std::is_same_v<Drop, KeepAll>) {
-          if (out_mask >> (2 * p) & 1) a = -87.f;
-          if (out_mask >> (2 * p) & 2) b = -87.f;
+        float2 d;
+        if constexpr (kCap) {
+          d = unpack2(add2(y[p], both2(-ref)));
+          d.x *= k;
+          d.y *= k;
+        } else {
+          d = unpack2(fma2(y[p], both2(sc.inv_temp), both2(-ref)));
+          d.x = max_nan(d.x, -87.f);
+          d.y = max_nan(d.y, -87.f);
         }
-        sum = add2(sum, exp_pair(pack2(a, b)));
+        if (!std::is_same_v<Drop, KeepAll>) {
+          if (out_mask >> (2 * p) & 1) d.x = -126.f * (kCap ? 2.f : 0.69f);
+          if (out_mask >> (2 * p) & 2) d.y = -126.f * (kCap ? 2.f : 0.69f);
+        }
+        if constexpr (kCap) {
+          d.x = exp2_fast(d.x);
+          d.y = exp2_fast(d.y);
+        } else {
+          d = unpack2(exp_pair(pack2(d.x, d.y)));
+        }
+        sum0 += d.x;
+        sum1 += d.y;
       }
     };
 #pragma unroll
@@ -315,7 +347,7 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
       if (i + u * step < sl.end) top = fmaxf(top, vec_max<T, false>(v[u]));
-    rho = softcap(top, sc.cap) * sc.inv_temp;
+    ref = kCap ? softcap(top, sc.cap) : top * sc.inv_temp;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u)
       if (i + u * step < sl.end) add(v[u], i + u * step);
@@ -327,11 +359,10 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
       for (int u = 0; u < kBatch; ++u) add(v[u], i + u * step);
     }
     for (; i < sl.end; i += step) add(body[i], i);
-    const float2 s2 = unpack2(sum);
-    const float s = s2.x + s2.y;
-    const float far = kCap ? sc.cap * sc.inv_temp - rho : big * sc.inv_temp - rho;  // the largest exponent
+    const float s = sum0 + sum1;
+    const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big * sc.inv_temp - ref;  // the largest exponent
     if (s > 1e-30f && s < 1e37f && far < 80.f) {
-      out.m = rho;
+      out.m = kCap ? ref * sc.inv_temp : ref;
       out.s = s;
     } else {
       for (i = sl.begin + threadIdx.x; i < sl.end; i += step) {
