@@ -20,11 +20,11 @@ using namespace me;
 
 namespace {
 
-constexpr int kThreads = 256;
 static_assert(kThreads >= kMaxTop, "one teacher entry a thread");
 constexpr int kFilter = 16384;  // bits of the filter that says which vectors may hold a teacher entry
 
 struct Shared {
+  Ring ring;
   float scratch[64];
   float part[2];  // this block's (m, s), read by the cluster's other blocks
 };
@@ -47,7 +47,7 @@ ME_DEVICE MaxSum cluster_merge(const float* part, int ranks) {
 // arrival: cluster_wait() has to follow before the block leaves (its `part` may still be read).
 template <typename T, bool kCap, typename Drop>
 ME_DEVICE MaxSum row_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Shared& sh, int ranks) {
-  MaxSum a = block_merge(slice_sum<T, kCap>(sl, sc, drop), sh.scratch);
+  MaxSum a = block_merge(slice_sum<T, kCap>(sl, sc, drop, sh.ring), sh.scratch);
   if (ranks == 1) return a;
   if (threadIdx.x == 0) {
     sh.part[0] = a.m;
@@ -67,39 +67,42 @@ ME_DEVICE void row_done(int ranks) {
 // out_j = coef exp(y_j - m) z'_j for the block's columns, in 16-byte stores where the two rows are
 // aligned alike.
 template <typename T, bool kCap>
-ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef) {
+ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
-  const uint4* body = sl.body();
-  const int64_t step = blockDim.x;
   const bool aligned = (reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0;
-  auto one = [&](uint4 x, int64_t vec) {
-    f32x2 z[kP];
-    vec_softcap<T, kCap>(x, sc, z);
+  // coef (1 - (z / c)^2) is one FMA with the coefficient inside
+  const float coef_slope = coef * sc.slope;
+  stream(
+      sl.mine(), sl.count(), ring, [](int, auto&) {},
+      [&](const auto& x, int i, auto whole) {
+        constexpr int kV = sizeof(x) / sizeof(uint4);
+        f32x2 z[kV][kP];
+        if constexpr (kCap) {
+          vec_softcap<T, false, decltype(whole)::value>(x, sc, 0.f, z);
+        } else {
 #pragma unroll
-    for (int p = 0; p < kP; ++p) {
-      const float2 a = unpack2(mul2(fma2(z[p], both2(sc.inv_temp), both2(-m)), both2(kLog2e)));
-      const f32x2 e = mul2(pack2(exp2_fast(a.x), exp2_fast(a.y)), both2(coef));
-      if constexpr (kCap) z[p] = mul2(e, fma2(mul2(z[p], both2(sc.slope)), z[p], both2(1.f)));
-      else z[p] = e;
-    }
-    Vec16<T> r;
-    r.u = from_pairs<T>(z);
-    if (aligned) {
-      reinterpret_cast<uint4*>(out + sl.head)[vec] = r.u;
-    } else {
+          for (int u = 0; u < kV; ++u) to_pairs<T>(x[u], z[u]);
+        }
 #pragma unroll
-      for (int e = 0; e < kN; ++e) out[sl.column(vec) + e] = r.h[e];
-    }
-  };
-  int64_t i = sl.begin + threadIdx.x;
-  for (; i + (kBatch - 1) * step < sl.end; i += kBatch * step) {
-    uint4 v[kBatch];
+        for (int u = 0; u < kV; ++u) {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) v[u] = body[i + u * step];
+          for (int p = 0; p < kP; ++p) {
+            const f32x2 zp = z[u][p];
+            const float2 a = unpack2(mul2(fma2(zp, both2(sc.inv_temp), both2(-m)), both2(kLog2e)));
+            const f32x2 e = pack2(exp2_fast(a.x), exp2_fast(a.y));
+            z[u][p] = mul2(e, kCap ? fma2(mul2(zp, both2(coef_slope)), zp, both2(coef)) : both2(coef));
+          }
+          Vec16<T> r;
+          r.u = from_pairs<T>(z[u]);
+          const int64_t at = sl.vec(i + u);
+          if (aligned) {
+            reinterpret_cast<uint4*>(out + sl.head)[at] = r.u;
+          } else {
 #pragma unroll
-    for (int u = 0; u < kBatch; ++u) one(v[u], i + u * step);
-  }
-  for (; i < sl.end; i += step) one(body[i], i);
+            for (int e = 0; e < kN; ++e) out[sl.column(at) + e] = r.h[e];
+          }
+        }
+      });
   const int64_t j = sl.single();
   if (j >= 0) {
     const float z = softcap(to_f<T>(sl.row[j]), sc.cap);
@@ -154,6 +157,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> 
                                                                   int ranks, const int64_t* __restrict__ target,
                                                                   Scale sc, const float2* __restrict__ stats,
                                                                   const float* __restrict__ g) {
+  __shared__ Ring ring;
   const int64_t r = N - 1 - blockIdx.x / ranks;
   const int rank = blockIdx.x % ranks;
   const int64_t t = target[r];
@@ -168,7 +172,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> 
   const float c = valid ? g[r] : NAN;
   const float xt = mine ? to_f<T>(sl.row[t]) : 0.f;
   __syncthreads();  // read before the row may be written in place
-  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y);
+  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y, ring);
   __syncthreads();  // the target's column is written again
   if (mine) {
     const float z = softcap(xt, sc.cap);
@@ -349,7 +353,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(Rows<const T> x, R
       zero_slice<T>(sl, o);
     } else {
       const float c = w * ta.temp;
-      write_slice<T, kCap>(sl, o, sc, m1, c * c1);
+      write_slice<T, kCap>(sl, o, sc, m1, c * c1, sh.ring);
       __syncthreads();
       write_entry<T>(sl, o, e, sc, c, a.m, 1.f / a.s, te.mass);
     }
@@ -375,7 +379,7 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(Rows<const T> 
   Entry e = load_entry<T>(ta, r, sl.row, V, sc.inv_temp, en);
   const TeacherRow te = finish_entries(e, ta, r, V, ta.lse != nullptr, en, sh.scratch);
   const float c = (ta.weight ? ta.weight[r] : 1.f) * ta.temp * g[r];
-  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w);
+  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w, sh.ring);
   __syncthreads();
   write_entry<T>(sl, o, e, sc, c, st.x, 1.f / st.y, te.mass);
 }
@@ -383,6 +387,8 @@ __global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(Rows<const T> 
 // ------------------------------------------------------------------------------------ launches
 // Blocks a row: enough for two on each SM, while a block keeps two vectors a thread.
 int ranks_for(int64_t N, int64_t V, int at_least = 1) {
+  static const int fix = getenv("RNK") ? atoi(getenv("RNK")) : 0;
+  if (fix) return fix;
   int c = at_least;
   while (c < 8 && N * c < 2 * objective_sms() && V / (2 * c) >= 4096) c *= 2;
   return c;
@@ -391,9 +397,10 @@ int ranks_for(int64_t N, int64_t V, int at_least = 1) {
 // Blocks a row where the row is read twice: the rows in flight (four blocks an SM) have to stay in L2
 // between the two passes; 40 of its 126 MB are given to them.
 int ranks_for_two_passes(const Logits& x) {
+  static const int l2_rows = getenv("L2R") ? atoi(getenv("L2R")) : 40;
   const int64_t row = x.V * (x.type == LogitType::kF32 ? 4 : 2);
   int c = 1;
-  while (c < 8 && 4 * objective_sms() / c * row > (40 << 20)) c *= 2;
+  while (c < 8 && 4 * objective_sms() / c * row > ((int64_t)l2_rows << 20)) c *= 2;
   return ranks_for(x.N, x.V, c);
 }
 

@@ -27,8 +27,22 @@ union Vec16 {
   T h[16 / sizeof(T)];
 };
 
-// z = c tanh(x / c), or x without a cap (cap <= 0): the accurate form of single elements.
-ME_DEVICE float softcap(float x, float cap) { return cap > 0.f ? cap * tanhf(x / cap) : x; }
+// z = c tanh(x / c), or x without a cap (cap <= 0): the accurate form of single elements. For |x| <= c a
+// polynomial in which x enters unrounded (relative error 5e-9 before rounding); tanhf, times c, would be
+// off by 1e-6 at z = 15 on average.
+ME_DEVICE float softcap(float x, float cap) {
+  if (!(cap > 0.f)) return x;
+  const float u = x / cap;
+  if (!(fabsf(u) <= 1.f)) return cap * tanhf(u);
+  const float w = u * u;
+  float q = fmaf(-0.000358452002f, w, 0.00230136459f);
+  q = fmaf(q, w, -0.00794610642f);
+  q = fmaf(q, w, 0.0214866576f);
+  q = fmaf(q, w, -0.0538798027f);
+  q = fmaf(q, w, 0.133323446f);
+  q = fmaf(q, w, -0.333332954f);
+  return fmaf(x * w, q, x);
+}
 // dz/dx, from z.
 ME_DEVICE float softcap_slope(float z, float cap) {
   if (cap <= 0.f) return 1.f;
@@ -128,62 +142,124 @@ ME_DEVICE float vec_max(uint4 v) {
   }
 }
 
-// How raw logits become exponents: z = softcap(x), y = z / tau. `limit`: the largest |x| that softcap2
-// may be given (negative: none).
+// How raw logits become exponents: z = softcap(x), y = z / tau.
+//
+// c tanh(x / c) is evaluated on the FMA pipe, as x P(v), v = x^2, P the minimax polynomial of tanh(u) / u in
+// u^2 (Remez exchange on tanh itself; the coefficients carry the powers of 1 / c^2): one for
+// |x| <= c / 2, where most logits lie, one for |x| <= c, and beyond that tanhf. (By exponential and reciprocal it
+// would be two results of the special function unit, which gives 16 a clock on an SM and has the
+// softmax's exponential to do. A packed FMA takes two issue slots on sm_100, so what counts is operations:
+// the short polynomial saves two of about thirteen a logit.)
 struct Scale {
-  float cap, limit, inv_temp, slope;  // slope = -1 / c^2
-  f32x2 q[7];                         // softcap2's coefficients, each one twice
+  float cap, limit, inv_temp, slope;  // limit: c^2, or -1 (no polynomial for this cap); slope = -1 / c^2
+  // 16-bit logits: P log2 e / tau (relative error 6e-8 and 2e-8), for sums
+  f32x2 sum_full[7], sum_short[5];
+  // 16-bit logits: P to 7e-7, for gradients that are rounded to 16 bits
+  f32x2 z_full[6], z_short[4];
+  // 32-bit logits: Q of P = 1 + v Q, so that x enters unrounded
+  f32x2 q_full[6], q_short[4];
 };
 
-// c tanh(x / c) for |x| <= c: x + x v Q(v), v = x^2, Q the minimax polynomial of (tanh(u) / u - 1) / u^2 in
-// u^2 on [0, 1] (Remez exchange on tanh itself; its coefficients carry the powers of 1 / c^2).
-// Relative error 5e-9, and x enters unrounded: half a unit of error, in nine operations of the FMA
-// pipe. By exponential and reciprocal it would be two results of the special function unit, which gives
-// 16 a clock on an SM and has the softmax's exponential to do.
-ME_DEVICE f32x2 softcap2(f32x2 x, const Scale& sc) {
-  const f32x2 v = mul2(x, x);
-  f32x2 q = fma2(sc.q[6], v, sc.q[5]);
+template <int kN>
+ME_DEVICE f32x2 horner2(const f32x2 (&c)[kN], f32x2 v) {
+  f32x2 p = fma2(c[kN - 1], v, c[kN - 2]);
 #pragma unroll
-  for (int i = 4; i >= 0; --i) q = fma2(q, v, sc.q[i]);
-  return fma2(mul2(x, v), q, x);
+  for (int i = kN - 3; i >= 0; --i) p = fma2(p, v, c[i]);
+  return p;
 }
 
 inline Scale make_scale(float cap, float temp) {
-  static const double kQ[7] = {-0.333332954, 0.133323446, -0.0538798027, 0.0214866576, -0.00794610642,
-                               0.00230136459, -0.000358452002};
-  Scale s = {cap, 0.f, (float)(1.0 / (double)temp), 0.f, {}};
-  if (cap > 0.f) {
-    const double r = 1.0 / ((double)cap * cap);
-    s.slope = (float)-r;
-    // (c^14 has to be an fp32 number; other caps take the element's form)
-    s.limit = cap > 4e-3f && cap < 400.f ? cap : -1.f;
+  // Q of tanh(u) = u (1 + u^2 Q(u^2)): on |u| <= 1 and <= 1/2, and the shorter ones for gradients
+  static const double kFull[6] = {-0.333329868, 0.133264089, -0.0534987079, 0.0203597599, -0.00625933984, 0.00105826482};
+  static const double kShort[4] = {-0.333331439, 0.13325879, -0.0530454943, 0.0172414915};
+  static const double kFull16[5] = {-0.333302797, 0.132884903, -0.0517682859, 0.0169064092, -0.00312657789};
+  static const double kShort16[3] = {-0.333281593, 0.132053597, -0.0447506447};
+  Scale s = {};
+  s.cap = cap;
+  s.inv_temp = (float)(1.0 / (double)temp);
+  if (!(cap > 0.f)) return s;
+  const double r = 1.0 / ((double)cap * cap), k = 1.4426950408889634 / (double)temp;
+  s.slope = (float)-r;
+  // (c^12 has to be an fp32 number; other caps take tanhf)
+  s.limit = cap > 4e-3f && cap < 400.f ? cap * cap : -1.f;
+  if (s.limit < 0.f) return s;
+  auto twice = [](double v) {
+    const float f = (float)v;
+    uint32_t bits;
+    memcpy(&bits, &f, 4);
+    return (f32x2)bits << 32 | bits;
+  };
+  auto fill_p = [&](f32x2* to, const double* q, int n, double scale) {  // scale (1 + v Q)
+    to[0] = twice(scale);
+    double p = scale * r;
+    for (int i = 0; i < n; ++i, p *= r) to[i + 1] = twice(q[i] * p);
+  };
+  auto fill_q = [&](f32x2* to, const double* q, int n) {
     double p = r;
-    for (int i = 0; i < 7; ++i, p *= r) {
-      const float q = (float)(s.limit > 0.f ? kQ[i] * p : 0.0);
-      uint32_t bits;
-      memcpy(&bits, &q, 4);
-      s.q[i] = (unsigned long long)bits << 32 | bits;
-    }
-  }
+    for (int i = 0; i < n; ++i, p *= r) to[i] = twice(q[i] * p);
+  };
+  fill_p(s.sum_full, kFull, 6, k);
+  fill_p(s.sum_short, kShort, 4, k);
+  fill_p(s.z_full, kFull16, 5, 1.0);
+  fill_p(s.z_short, kShort16, 3, 1.0);
+  fill_q(s.q_full, kFull, 6);
+  fill_q(s.q_short, kShort, 4);
   return s;
 }
 
-// z of a vector: the polynomial, or element by element where one is beyond the cap.
-template <typename T, bool kCap>
-ME_DEVICE void vec_softcap(uint4 v, const Scale& sc, f32x2 (&z)[Vec16<T>::kN / 2]) {
-  to_pairs<T>(v, z);
-  if constexpr (kCap) {
-    if (vec_max<T, true>(v) <= sc.limit) {
+// z of kV vectors (kExponent false), or the exponents z log2 e / tau - shift (true). `whole`: every lane of the
+// warp is here.
+template <typename T, bool kExponent, bool kWhole, int kV>
+ME_DEVICE void vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f32x2 (&z)[kV][Vec16<T>::kN / 2]) {
+  constexpr int kP = Vec16<T>::kN / 2;
+  const float k = sc.inv_temp * kLog2e;
+  float top = 0.f;
 #pragma unroll
-      for (int i = 0; i < Vec16<T>::kN / 2; ++i) z[i] = softcap2(z[i], sc);
-    } else {
+  for (int u = 0; u < kV; ++u) {
+    to_pairs<T>(x[u], z[u]);
+#pragma unroll
+    for (int p = 0; p < kP; ++p) {
+      const float2 v = unpack2(mul2(z[u][p], z[u][p]));
+      asm("max.f32 %0, %0, %1, %2;" : "+f"(top) : "f"(v.x), "f"(v.y));  // a NaN is passed over, and stays in x
+    }
+  }
+  auto all = [&](auto&& f) {
+#pragma unroll
+    for (int u = 0; u < kV; ++u)
+#pragma unroll
+      for (int p = 0; p < kP; ++p) z[u][p] = f(z[u][p]);
+  };
+  auto poly = [&](const auto& sum, const auto& low, const auto& q) {
+    all([&](f32x2 a) {
+      const f32x2 v = mul2(a, a);
+      if constexpr (sizeof(T) == 4) {
+        const f32x2 r = fma2(mul2(a, v), horner2(q, v), a);
+        return kExponent ? fma2(r, both2(k), both2(-shift)) : r;
+      } else {
+        return kExponent ? fma2(a, horner2(sum, v), both2(-shift)) : mul2(a, horner2(low, v));
+      }
+    });
+  };
+  // (the warp takes the short polynomial together: a divided warp would pay for both)
+  if (kWhole && __all_sync(0xffffffffu, top <= 0.25f * sc.limit)) {
+    poly(sc.sum_short, sc.z_short, sc.q_short);
+  } else if (top <= sc.limit) {
+    poly(sc.sum_full, sc.z_full, sc.q_full);
+  } else {
+#pragma unroll
+    for (int u = 0; u < kV; ++u) {
 #pragma unroll 1
-      for (int i = 0; i < Vec16<T>::kN / 2; ++i) {
+      for (int i = 0; i < kP; ++i) {
         // (a loop that is not unrolled would index the pairs in local memory: rotate them instead)
-        const float2 f = unpack2(z[0]);
+        const float2 f = unpack2(z[u][0]);
+        float a = softcap(f.x, sc.cap), b = softcap(f.y, sc.cap);
+        if (kExponent) {
+          a = fmaf(a, k, -shift);
+          b = fmaf(b, k, -shift);
+        }
 #pragma unroll
-        for (int o = 0; o + 1 < Vec16<T>::kN / 2; ++o) z[o] = z[o + 1];
-        z[Vec16<T>::kN / 2 - 1] = pack2(softcap(f.x, sc.cap), softcap(f.y, sc.cap));
+        for (int o = 0; o + 1 < kP; ++o) z[u][o] = z[u][o + 1];
+        z[u][kP - 1] = pack2(a, b);
       }
     }
   }
@@ -207,6 +283,8 @@ ME_DEVICE float max_nan(float a, float b) {
   asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+
+constexpr int kThreads = 256;  // of every block that walks a row
 
 // A logits matrix and its rows' stride in elements.
 template <typename T>
@@ -236,7 +314,13 @@ struct Slice {
     first = rank == 0;
     last = rank == ranks - 1;
   }
-  ME_DEVICE const uint4* body() const { return reinterpret_cast<const uint4*>(row + head); }
+  // This thread's vectors: how many, the i-th one's number in the row, where the first one is.
+  ME_DEVICE int count() const {
+    const int n = (int)(end - begin) - (int)threadIdx.x;
+    return n > 0 ? (n + kThreads - 1) / kThreads : 0;
+  }
+  ME_DEVICE int64_t vec(int i) const { return begin + threadIdx.x + (int64_t)i * kThreads; }
+  ME_DEVICE const uint4* mine() const { return reinterpret_cast<const uint4*>(row + head) + begin + threadIdx.x; }
   ME_DEVICE int64_t column(int64_t vec) const { return head + vec * kN; }
   // The block's single columns, one a thread: -1 for the threads that have none.
   ME_DEVICE int64_t single() const {
@@ -285,7 +369,72 @@ struct KeepAll {
   ME_DEVICE bool column(int64_t) const { return false; }
 };
 
-constexpr int kBatch = 4;  // vectors that a thread has in flight
+// ---------------------------------------------------------------- a thread's vectors, read ahead
+// Each thread copies its own vectors of a slice into its own places of a ring in shared memory,
+// kDepth ahead of use (cp.async: no registers are held, no other thread waits): 256 threads keep 32 KB in
+// flight a block, four blocks an SM 128 KB, three times what the memory's latency asks for.
+constexpr int kDepth = 8;
+constexpr int kFirst = 4;  // vectors that the reference of a sum is taken from
+
+struct Ring {
+  uint4 v[kDepth][kThreads];
+};
+
+ME_DEVICE void copy_async(uint4* to, const uint4* from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+               : "memory");
+}
+ME_DEVICE void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kLeft>
+ME_DEVICE void copy_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(kLeft) : "memory");
+}
+
+// first(n, v): the thread's n first vectors (at most kFirst) are there; f(v, i): the array v of vectors from
+// the thread's i-th on, two of them while the whole warp is in the loop (kWhole), else one. `src`: its first one,
+// the others follow kThreads apart. Every thread of the block calls it, those without a vector too.
+template <typename First, typename F>
+ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&& f) {
+  const int tid = threadIdx.x;
+  uint4* mine = &ring.v[0][tid];
+#pragma unroll
+  for (int d = 0; d < kDepth; ++d) {
+    if (d < count) copy_async(mine + d * kThreads, src + d * kThreads);
+    if (d & 1) copy_commit();
+  }
+  copy_wait<(kDepth - kFirst) / 2>();
+  {
+    uint4 v[kFirst];
+#pragma unroll
+    for (int u = 0; u < kFirst; ++u) v[u] = mine[u * kThreads];
+    first(min(count, kFirst), v);
+  }
+  const uint4* next = src + kDepth * kThreads;
+  const int whole = __shfl_sync(0xffffffffu, count, 31);  // the warp's last lane has the fewest
+  int i = 0;
+  for (; i + 2 * kDepth <= whole; i += kDepth, next += kDepth * kThreads) {
+#pragma unroll
+    for (int s = 0; s < kDepth; s += 2) {
+      copy_wait<kDepth / 2 - 1>();
+      const uint4 v[2] = {mine[s * kThreads], mine[(s + 1) * kThreads]};
+      f(v, i + s, std::true_type());
+      copy_async(mine + s * kThreads, next + s * kThreads);
+      copy_async(mine + (s + 1) * kThreads, next + (s + 1) * kThreads);
+      copy_commit();
+    }
+  }
+  for (; i < count; i += 2) {
+    copy_wait<kDepth / 2 - 1>();
+#pragma unroll 1
+    for (int u = 0; u < 2 && i + u < count; ++u) {
+      uint4* at = mine + (i + u) % kDepth * kThreads;
+      const uint4 v[1] = {*at};
+      f(v, i + u, std::false_type());
+      if (i + u + kDepth < count) copy_async(at, src + (i + u + kDepth) * kThreads);
+    }
+    copy_commit();
+  }
+}
 
 // This thread's share of sum exp(y - m) over a slice. `drop(vec)`: a mask of the vector's elements
 // that are left out (`drop.column(j)` for a single column).
@@ -298,78 +447,71 @@ constexpr int kBatch = 4;  // vectors that a thread has in flight
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
 // form, since nothing else is rounded then.
 template <typename T, bool kCap, typename Drop>
-ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop) {
+ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Ring& ring) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
-  const uint4* body = sl.body();
-  const int64_t step = blockDim.x;
   MaxSum out;
-  int64_t i = sl.begin + threadIdx.x;
-  if (i < sl.end) {
-    uint4 v[kBatch];
-    float top = -INFINITY, big = -INFINITY;
-    float sum0 = 0.f, sum1 = 0.f;
-    float ref = 0.f;  // with a softcap of z, else of y
-    const float k = sc.inv_temp * kLog2e;
-    auto add = [&](uint4 x, int64_t vec) {
-      if constexpr (!kCap) big = fmaxf(big, vec_max<T, false>(x));
-      f32x2 y[kP];
-      vec_softcap<T, kCap>(x, sc, y);
-      const uint32_t out_mask = drop(vec);
+  const int count = sl.count();
+  float big = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+  const float k = sc.inv_temp * kLog2e;
+  float ref = 0.f, shift = 0.f;  // the reference; the same, or the rounded ref k
+  stream(
+      sl.mine(), count, ring,
+      [&](int n, const uint4(&v)[kFirst]) {
+        float top = -INFINITY;
 #pragma unroll
-      for (int p = 0; p < kP; ++p) {
-        float2 d;
+        for (int u = 0; u < kFirst; ++u)
+          if (u < n) top = fmaxf(top, vec_max<T, false>(v[u]));
+        ref = kCap ? softcap(top, sc.cap) : top * sc.inv_temp;
+        shift = kCap ? ref * k : ref;
+      },
+      [&](const auto& x, int i, auto whole) {
+        constexpr int kV = sizeof(x) / sizeof(uint4);
+        f32x2 y[kV][kP];
         if constexpr (kCap) {
-          d = unpack2(add2(y[p], both2(-ref)));
-          d.x *= k;
-          d.y *= k;
+          vec_softcap<T, true, decltype(whole)::value>(x, sc, shift, y);
         } else {
-          d = unpack2(fma2(y[p], both2(sc.inv_temp), both2(-ref)));
-          d.x = max_nan(d.x, -87.f);
-          d.y = max_nan(d.y, -87.f);
+#pragma unroll
+          for (int u = 0; u < kV; ++u) {
+            to_pairs<T>(x[u], y[u]);
+            big = fmaxf(big, vec_max<T, false>(x[u]));
+          }
         }
-        if (!std::is_same_v<Drop, KeepAll>) {
-          if (out_mask >> (2 * p) & 1) d.x = -126.f * (kCap ? 2.f : 0.69f);
-          if (out_mask >> (2 * p) & 2) d.y = -126.f * (kCap ? 2.f : 0.69f);
+#pragma unroll
+        for (int u = 0; u < kV; ++u) {
+          const uint32_t out_mask = drop(sl.vec(i + u));
+#pragma unroll
+          for (int p = 0; p < kP; ++p) {
+            float2 d = unpack2(kCap ? y[u][p] : fma2(y[u][p], both2(sc.inv_temp), both2(-shift)));
+            if constexpr (!kCap) {
+              d.x = max_nan(d.x, -87.f);
+              d.y = max_nan(d.y, -87.f);
+            }
+            if (!std::is_same_v<Drop, KeepAll>) {
+              if (out_mask >> (2 * p) & 1) d.x = kCap ? -200.f : -87.f;
+              if (out_mask >> (2 * p) & 2) d.y = kCap ? -200.f : -87.f;
+            }
+            if constexpr (kCap) {
+              d.x = exp2_fast(d.x);
+              d.y = exp2_fast(d.y);
+            } else {
+              d = unpack2(exp_pair(pack2(d.x, d.y)));
+            }
+            sum0 += d.x;
+            sum1 += d.y;
+          }
         }
-        if constexpr (kCap) {
-          d.x = exp2_fast(d.x);
-          d.y = exp2_fast(d.y);
-        } else {
-          d = unpack2(exp_pair(pack2(d.x, d.y)));
-        }
-        sum0 += d.x;
-        sum1 += d.y;
-      }
-    };
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (i + u * step < sl.end) v[u] = body[i + u * step];
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (i + u * step < sl.end) top = fmaxf(top, vec_max<T, false>(v[u]));
-    ref = kCap ? softcap(top, sc.cap) : top * sc.inv_temp;
-#pragma unroll
-    for (int u = 0; u < kBatch; ++u)
-      if (i + u * step < sl.end) add(v[u], i + u * step);
-    i += kBatch * step;
-    for (; i + (kBatch - 1) * step < sl.end; i += kBatch * step) {
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) v[u] = body[i + u * step];
-#pragma unroll
-      for (int u = 0; u < kBatch; ++u) add(v[u], i + u * step);
-    }
-    for (; i < sl.end; i += step) add(body[i], i);
-    const float s = sum0 + sum1;
-    const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big * sc.inv_temp - ref;  // the largest exponent
-    if (s > 1e-30f && s < 1e37f && far < 80.f) {
-      out.m = kCap ? ref * sc.inv_temp : ref;
-      out.s = s;
-    } else {
-      for (i = sl.begin + threadIdx.x; i < sl.end; i += step) {
-        const uint32_t out_mask = drop(i);
-        for (int e = 0; e < kN; ++e)
-          if (!(out_mask >> e & 1)) out.add(softcap(to_f<T>(sl.row[sl.column(i) + e]), sc.cap) * sc.inv_temp);
-      }
+      });
+  const float s = sum0 + sum1;
+  const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big * sc.inv_temp - ref;  // the largest exponent
+  if (count > 0 && s > 1e-30f && s < 1e37f && far < 80.f) {
+    // (m is rounded: what separates it from the shift that was taken goes into s)
+    out.m = kCap ? ref * sc.inv_temp : ref;
+    out.s = kCap ? s * exp2_fast(fmaf(-out.m, kLog2e, shift) - out.m * 1.925963033500011e-08f) : s;
+  } else {
+    for (int i = 0; i < count; ++i) {
+      const uint32_t out_mask = drop(sl.vec(i));
+      for (int e = 0; e < kN; ++e)
+        if (!(out_mask >> e & 1)) out.add(softcap(to_f<T>(sl.row[sl.column(sl.vec(i)) + e]), sc.cap) * sc.inv_temp);
     }
   }
   const int64_t j = sl.single();

@@ -14,7 +14,7 @@ using namespace me;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kPairThreads = 512;
 
 // log(1 + e^v) without overflow
 ME_DEVICE float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
@@ -22,7 +22,7 @@ ME_DEVICE float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v)
 // Offsets are read as their running maximum, clamped to [0, T]: every token lies in one sequence, or
 // ahead of the first or after the last one (those get no gradient), whatever `cu` holds.
 template <typename I>
-__global__ void __launch_bounds__(kThreads) preference_kernel(
+__global__ void __launch_bounds__(kPairThreads) preference_kernel(
     const float* __restrict__ logp, const float* __restrict__ ref, const int64_t* __restrict__ target, int64_t T,
     const I* __restrict__ cu, int64_t pairs, int kind, float beta, float smooth, float scale,
     float* __restrict__ loss, float2* __restrict__ rewards, float* __restrict__ grad) {
@@ -84,7 +84,7 @@ namespace me {
 
 void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* grad, cudaStream_t stream) {
   auto launch = [&](auto* cu) {
-    preference_kernel<<<(unsigned)a.pairs, kThreads, 0, stream>>>(a.logp, a.ref, a.target, a.tokens, cu, a.pairs, a.kind,
+    preference_kernel<<<(unsigned)a.pairs, kPairThreads, 0, stream>>>(a.logp, a.ref, a.target, a.tokens, cu, a.pairs, a.kind,
                                                                   a.beta, a.smooth, a.scale, loss, rewards, grad);
   };
   if (a.cu64) launch(static_cast<const int64_t*>(a.cu));

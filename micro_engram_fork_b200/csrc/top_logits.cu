@@ -11,7 +11,7 @@ using namespace me;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kTopThreads = 512;
 
 // A number that orders as the logits do: larger logit, larger key. -0 and +0 share one, NaN is on top.
 ME_DEVICE uint32_t order_key(float x) {
@@ -26,14 +26,14 @@ ME_DEVICE void for_row(const T* row, int64_t V, F&& f) {
 // Radix selection, eight bits of the key a pass over the row: the exact k-th largest key, then every
 // larger one and the lowest ids among its equals, ranked by counting.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) top_logits_kernel(Rows<const T> x, int64_t N, int64_t V, int k, float cap,
+__global__ void __launch_bounds__(kTopThreads) top_logits_kernel(Rows<const T> x, int64_t N, int64_t V, int k, float cap,
                                                               float inv_temp, float* __restrict__ values,
                                                               int64_t* __restrict__ ids, float* __restrict__ lse) {
   __shared__ float scratch[64];
   __shared__ int hist[256];
   __shared__ uint32_t key[kMaxTop];
   __shared__ int col[kMaxTop];
-  __shared__ int count, need, warp_sum_[kThreads / 32];
+  __shared__ int count, need, warp_sum_[kTopThreads / 32];
   __shared__ uint32_t prefix;
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   for (int64_t r = blockIdx.x; r < N; r += gridDim.x) {
@@ -82,7 +82,7 @@ __global__ void __launch_bounds__(kThreads) top_logits_kernel(Rows<const T> x, i
       if (lane == 0) warp_sum_[wid] = __popc(votes);
       __syncthreads();
       int before = __popc(votes & ((1u << lane) - 1)), total = 0;
-      for (int w = 0; w < kThreads / 32; ++w) {
+      for (int w = 0; w < kTopThreads / 32; ++w) {
         if (w < wid) before += warp_sum_[w];
         total += warp_sum_[w];
       }
@@ -112,7 +112,7 @@ namespace me {
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,
                        cudaStream_t stream) {
   const int grid = (int)std::min<int64_t>(x.N, (int64_t)objective_sms() * 4);
-  ME_LOGITS_DISPATCH(x.type, top_logits_kernel<T><<<grid, kThreads, 0, stream>>>(rows_in<T>(x), x.N, x.V, k, x.cap,
+  ME_LOGITS_DISPATCH(x.type, top_logits_kernel<T><<<grid, kTopThreads, 0, stream>>>(rows_in<T>(x), x.N, x.V, k, x.cap,
                                                                                  1.f / temp, values, ids, lse));
 }
 
