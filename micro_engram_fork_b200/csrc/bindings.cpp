@@ -81,9 +81,8 @@ torch::Tensor token_logprobs_bwd(torch::Tensor x, torch::Tensor target, double c
 std::vector<torch::Tensor> distill_fwd(torch::Tensor x, torch::Tensor ids, torch::Tensor top,
                                        c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> weight,
                                        double cap, double temp);
-torch::Tensor distill_bwd(torch::Tensor x, torch::Tensor ids, torch::Tensor top, c10::optional<torch::Tensor> lse,
-                          c10::optional<torch::Tensor> weight, double cap, double temp, torch::Tensor stats,
-                          torch::Tensor g, c10::optional<torch::Tensor> out);
+torch::Tensor distill_bwd(torch::Tensor x, torch::Tensor rows, c10::optional<torch::Tensor> weight, double cap,
+                          double temp, torch::Tensor stats, torch::Tensor g, c10::optional<torch::Tensor> out);
 std::vector<torch::Tensor> distill_grad(torch::Tensor x, torch::Tensor ids, torch::Tensor top,
                                         c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> weight,
                                         double cap, double temp, c10::optional<torch::Tensor> out);

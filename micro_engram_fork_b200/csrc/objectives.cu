@@ -20,60 +20,16 @@ using namespace me;
 
 namespace {
 
-static_assert(kThreads >= kMaxTop, "one teacher entry a thread");
-constexpr int kFilter = 16384;  // bits of the filter that says which vectors may hold a teacher entry
-
-struct Shared {
-  Ring ring;
-  float scratch[64];
-  float part[2];  // this block's (m, s), read by the cluster's other blocks
-};
-
-// The row's (m, s) from its blocks' (all threads of all blocks get the same); `s` may be NaN.
-ME_DEVICE MaxSum cluster_merge(const float* part, int ranks) {
-  const int lane = threadIdx.x & 31;
-  MaxSum a;
-  if (lane < ranks) {
-    a.m = cluster_load(part, lane);
-    a.s = cluster_load(part + 1, lane);
-  }
-  MaxSum r;
-  r.m = warp_max(a.m);
-  r.s = warp_sum(a.m == -INFINITY ? a.s : a.s * expf(a.m - r.m));
-  return r;
-}
-
-// Adds a row's exponentials over its cluster, the same result for every thread. Ends after a cluster
-// arrival: cluster_wait() has to follow before the block leaves (its `part` may still be read).
-template <typename T, bool kCap, typename Drop>
-ME_DEVICE MaxSum row_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Shared& sh, int ranks) {
-  MaxSum a = block_merge(slice_sum<T, kCap>(sl, sc, drop, sh.ring), sh.scratch);
-  if (ranks == 1) return a;
-  if (threadIdx.x == 0) {
-    sh.part[0] = a.m;
-    sh.part[1] = a.s;
-  }
-  cluster_arrive();
-  cluster_wait();
-  a = cluster_merge(sh.part, ranks);
-  cluster_arrive();
-  return a;
-}
-ME_DEVICE void row_done(int ranks) {
-  if (ranks > 1) cluster_wait();
-}
-
 // ------------------------------------------------------------------------------------ gradient of a slice
 // out_j = coef exp(y_j - m) z'_j for the block's columns, in 16-byte stores where the two rows are
 // aligned alike.
-template <typename T, bool kCap>
-ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
+template <typename T, bool kCap, typename Walk>
+ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Walk&& walk) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   const bool aligned = (reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0;
   // coef (1 - (z / c)^2) is one FMA with the coefficient inside
   const float coef_slope = coef * sc.slope;
-  stream(
-      sl.mine(), sl.count(), ring, [](int, auto&) {},
+  walk(
       [&](const auto& x, int i, auto whole) {
         constexpr int kV = sizeof(x) / sizeof(uint4);
         f32x2 z[kV][kP];
@@ -94,7 +50,7 @@ ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m,
           }
           Vec16<T> r;
           r.u = from_pairs<T>(z[u]);
-          const int64_t at = sl.vec(i + u);
+          const int at = sl.vec(i + u);
           if (aligned) {
             reinterpret_cast<uint4*>(out + sl.head)[at] = r.u;
           } else {
@@ -103,7 +59,7 @@ ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m,
           }
         }
       });
-  const int64_t j = sl.single();
+  const int j = sl.single();
   if (j >= 0) {
     const float z = softcap(to_f<T>(sl.row[j]), sc.cap);
     out[j] = from_f<T>(coef * exp2_fast((z * sc.inv_temp - m) * kLog2e) * softcap_slope(z, sc.cap));
@@ -114,25 +70,26 @@ template <typename T>
 ME_DEVICE void zero_slice(const Slice<T>& sl, T* out) {
   const int64_t head = ((16 - (reinterpret_cast<uintptr_t>(out) & 15)) & 15) / sizeof(T);
   if (head == sl.head || sl.begin >= sl.end) {
-    for (int64_t i = sl.begin + threadIdx.x; i < sl.end; i += blockDim.x)
+    for (int i = sl.begin + threadIdx.x; i < sl.end; i += kThreads)
       reinterpret_cast<uint4*>(out + sl.head)[i] = make_uint4(0, 0, 0, 0);
   } else {
-    for (int64_t j = sl.column(sl.begin) + threadIdx.x; j < sl.column(sl.end); j += blockDim.x)
+    for (int j = sl.column(sl.begin) + threadIdx.x; j < sl.column(sl.end); j += kThreads)
       out[j] = from_f<T>(0.f);
   }
-  const int64_t j = sl.single();
+  const int j = sl.single();
   if (j >= 0) out[j] = from_f<T>(0.f);
 }
 
 // ------------------------------------------------------------------------------------ log-probabilities
 template <typename T, bool kCap>
-__global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> x, int64_t V, int ranks,
+__global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> x, int V, int lg_ranks,
                                                                   const int64_t* __restrict__ target, Scale sc,
                                                                   float* __restrict__ logp,
                                                                   float2* __restrict__ stats) {
-  __shared__ Shared sh;
-  const int64_t r = blockIdx.x / ranks;
-  const int rank = blockIdx.x % ranks;
+  __shared__ Ring ring;
+  __shared__ float2 part[kWarps];
+  const int64_t r = (blockIdx.x >> lg_ranks);
+  const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
   const int64_t t = target[r];
   if (t == kIgnoreToken) {
     if (threadIdx.x == 0 && rank == 0) {
@@ -141,38 +98,42 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> 
     }
     return;
   }
-  const Slice<T> sl(x.row(r), V, rank, ranks);
+  const Slice<T> sl(x.row(r), V, rank, lg_ranks);
   const float xt = t >= 0 && t < V ? to_f<T>(sl.row[t]) : NAN;
-  const MaxSum a = row_sum<T, kCap>(sl, sc, KeepAll(), sh, ranks);
+  const MaxSum a = row_merge(
+      slice_sum<T, kCap>(sl, sc, KeepAll(),
+                         [&](auto&& first, auto&& f) { stream(sl.mine(), sl.count(), ring, first, f); }),
+      part, lg_ranks);
   if (threadIdx.x == 0 && rank == 0) {
     logp[r] = softcap(xt, sc.cap) - a.m - logf(a.s);
     stats[r] = make_float2(a.m, a.s);
   }
-  row_done(ranks);
+  row_done(lg_ranks);
 }
 
 // Rows are taken last to first: where the forward pass just went over them, the last ones are in L2.
 template <typename T, bool kCap>
-__global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int64_t V,
-                                                                  int ranks, const int64_t* __restrict__ target,
+__global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int V,
+                                                                  int lg_ranks, const int64_t* __restrict__ target,
                                                                   Scale sc, const float2* __restrict__ stats,
                                                                   const float* __restrict__ g) {
   __shared__ Ring ring;
-  const int64_t r = N - 1 - blockIdx.x / ranks;
-  const int rank = blockIdx.x % ranks;
+  const int64_t r = N - 1 - (blockIdx.x >> lg_ranks);
+  const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
   const int64_t t = target[r];
-  const Slice<T> sl(x.row(r), V, rank, ranks);
+  const Slice<T> sl(x.row(r), V, rank, lg_ranks);
   T* o = out.row(r);
   if (t == kIgnoreToken) {
     zero_slice<T>(sl, o);
     return;
   }
-  const bool valid = t >= 0 && t < V, mine = valid && sl.holds(t) && threadIdx.x == 0;
+  const bool valid = t >= 0 && t < V, mine = valid && sl.holds((int)t) && threadIdx.x == 0;
   const float2 ms = stats[r];
   const float c = valid ? g[r] : NAN;
   const float xt = mine ? to_f<T>(sl.row[t]) : 0.f;
   __syncthreads();  // read before the row may be written in place
-  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y, ring);
+  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y,
+                       [&](auto&& f) { stream(sl.mine(), sl.count(), ring, [](int, auto&) {}, f); });
   __syncthreads();  // the target's column is written again
   if (mine) {
     const float z = softcap(xt, sc.cap);
@@ -181,123 +142,228 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> 
 }
 
 // ------------------------------------------------------------------------------------ distillation
-struct Entries {
-  int id[kMaxTop];    // < 0: an unused entry
-  float q[kMaxTop];   // probability
-};
-
-// A thread's entry of the row's teacher.
+// A teacher's entry, and what the student's side of its column needs.
 struct Entry {
-  int id = -1;
-  float t = -INFINITY;  // t_k / tau
-  float x = 0.f;        // the student's raw logit
-  float q = 0.f;        // probability; log q = (t - m) - log_s
-  bool first = false;   // no earlier entry has this id
-  float q_id = 0.f;     // sum of q over the entries with this id
+  int id;       // -1: unused, or an earlier entry has the same id
+  float q;      // the probability of all entries with this id
+  float y;      // the student's y
+  float slope;  // z'
 };
+static_assert(sizeof(Entry) == sizeof(float4));
+
+// What a row's loss needs of the teacher.
 struct TeacherRow {
-  float m, log_s;
-  float mass;    // sum of q, and of the rest's
-  float q_rest;  // the rest's probability
-  bool any;      // an entry with q != 0
+  float b;       // sum q [log q - (y - y_ref)]: with it the divergence is b + sum q [log s + (m - y_ref)]
+  float sum_q;
+  float q_rest;  // with a rest: its probability
+  float mass;    // sum of q and q_rest
+  float y_ref;   // the entries' largest y
+  float s;       // sum exp(y - y_ref) over the entries (each id once)
+  float any;     // 1: an entry has q != 0
+  float pad;
 };
+static_assert(sizeof(TeacherRow) == kTeacherRowBytes && sizeof(Entry) == kEntryBytes);
 
+constexpr int kFilter = 8192;  // bits of a filter over a row's entries
+
+// One warp a row of the teacher's records: probabilities, repeated ids, the student's logits there. It
+// runs ahead of the kernels that walk the logits, which then wait for nothing but the logits (with this
+// in their blocks, eight to a row, the chain ids -> logits -> sums took half of a block's time).
 template <typename T>
-ME_DEVICE Entry load_entry(const TeacherArgs& a, int64_t r, const T* row, int64_t V, float inv_temp, Entries& en) {
-  Entry e;
-  if (threadIdx.x < a.k) {
-    const int64_t id = a.ids[r * a.k + threadIdx.x];
-    if (id >= 0 && id < V) {
-      e.id = (int)id;
-      e.t = a.top[r * a.k + threadIdx.x] * inv_temp;
-      e.x = to_f<T>(row[id]);
+__global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int64_t N, int V, TeacherArgs a, Scale sc,
+                                                           Entry* __restrict__ entries, TeacherRow* __restrict__ rows) {
+  __shared__ __align__(16) int ids[kWarps][kMaxTop];
+  __shared__ float qs[kWarps][kMaxTop];
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  const int64_t r = (int64_t)blockIdx.x * kWarps + wid;
+  if (r >= N || (a.weight && a.weight[r] == 0.f)) return;
+  const bool tail = a.lse != nullptr;
+  const T* row = x.row(r);
+  int* id = ids[wid];
+  float* qr = qs[wid];
+  float t[kMaxTop / 32], y[kMaxTop / 32], slope[kMaxTop / 32];
+  float m = -INFINITY, y_ref = -INFINITY, used = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxTop / 32; ++i) {
+    const int k = lane + 32 * i;
+    t[i] = -INFINITY;
+    y[i] = slope[i] = 0.f;
+    if (k >= a.k) continue;
+    const int64_t j = a.ids[r * a.k + k];
+    const bool there = j >= 0 && j < V;  // other ids are unused entries
+    id[k] = there ? (int)j : -1;
+    if (!there) continue;
+    t[i] = a.top[r * a.k + k] * sc.inv_temp;
+    const float z = softcap(to_f<T>(row[j]), sc.cap);
+    y[i] = z * sc.inv_temp;
+    slope[i] = softcap_slope(z, sc.cap);
+    m = fmaxf(m, t[i]);
+    y_ref = fmaxf(y_ref, y[i]);
+    used += 1.f;
+  }
+  m = tail ? a.lse[r] : warp_max(m);
+  y_ref = warp_max(y_ref);
+  if (y_ref == -INFINITY) y_ref = 0.f;
+  float q[kMaxTop / 32];
+  float sum = 0.f;
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < kMaxTop / 32; ++i) {
+    q[i] = t[i] == -INFINITY ? 0.f : expf(t[i] - m);
+    sum += q[i];
+    any = any || q[i] != 0.f;
+  }
+  sum = warp_sum(sum);
+  used = warp_sum(used);
+  any = __any_sync(0xffffffffu, any);
+  const float inv = tail || !any ? 1.f : 1.f / sum, log_s = tail ? 0.f : logf(sum);
+  float b = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxTop / 32; ++i) {
+    const int k = lane + 32 * i;
+    q[i] *= inv;
+    if (k < a.k) qr[k] = q[i];
+    if (q[i] == 0.f) continue;
+    // maxima first: what is left to round is of the size of the difference
+    b += y[i] == -INFINITY ? INFINITY : q[i] * (((t[i] - m) - (y[i] - y_ref)) - log_s);
+  }
+  b = warp_sum(b);
+  if (!tail && any) sum = 1.f;
+  if (lane < 3 && a.k + lane < (a.k + 3) / 4 * 4) id[a.k + lane] = -2;  // (the list is read by fours)
+  __syncwarp();
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < kMaxTop / 32; ++i) {
+    const int k = lane + 32 * i;
+    if (32 * i >= a.k) break;
+    const int mine = k < a.k ? id[k] : -1;
+    bool first = mine >= 0;
+    float q_id = q[i];
+    // Repeated ids: each is found once by itself; more often, the list is gone over again.
+    int found = 0;
+    for (int o = 0; o < a.k; o += 4) {
+      const int4 v = *reinterpret_cast<const int4*>(id + o);
+      found += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
+    }
+    if (first && found > 1) {
+      for (int o = 0; o < a.k; ++o) {
+        if (id[o] != mine || o == k) continue;
+        first = first && o > k;
+        q_id += qr[o];
+      }
+    }
+    if (first) s += y[i] == -INFINITY ? 0.f : expf(y[i] - y_ref);
+    if (k < a.k) {
+      Entry e = {first ? mine : -1, q_id, y[i], slope[i]};
+      reinterpret_cast<float4*>(entries)[r * a.k + k] = *reinterpret_cast<float4*>(&e);
     }
   }
-  en.id[threadIdx.x] = e.id;
-  return e;
-}
-
-// Probabilities of the entries; `tail`: all other tokens are one more class.
-ME_DEVICE TeacherRow finish_entries(Entry& e, const TeacherArgs& a, int64_t r, int64_t V, bool tail, Entries& en,
-                                    float* scratch) {
-  TeacherRow te;
-  te.m = tail ? a.lse[r] : block_max(e.t, scratch);
-  e.q = e.t == -INFINITY ? 0.f : expf(e.t - te.m);
-  if (!tail) {
-    const float s = block_sum(e.q, scratch);
-    e.q = e.q == 0.f ? 0.f : e.q / s;
-    te.log_s = logf(s);
-  } else {
-    te.log_s = 0.f;
+  s = warp_sum(s);
+  if (lane == 0) {
+    // no rest where the entries are the whole vocabulary: 1 - sum is rounding then
+    const float q_rest = tail && used < (float)V ? fmaxf(0.f, 1.f - sum) : 0.f;
+    rows[r] = {b, sum, q_rest, tail ? sum + q_rest : 1.f, y_ref, s, any ? 1.f : 0.f, 0.f};
   }
-  en.q[threadIdx.x] = e.q;
-  const float2 sums = block_sum2(e.q, e.id >= 0 ? 1.f : 0.f, scratch);  // (its barriers publish en)
-  te.any = __syncthreads_or(e.q != 0.f);
-  // no rest where the entries are the whole vocabulary: 1 - sum is rounding then
-  te.q_rest = tail && sums.y < (float)V ? fmaxf(0.f, 1.f - sums.x) : 0.f;
-  te.mass = tail ? sums.x + te.q_rest : 1.f;
-  if (e.id >= 0) {
-    e.first = true;
-    for (int i = 0; i < a.k; ++i) {
-      if (en.id[i] != e.id) continue;
-      e.first = e.first && i >= (int)threadIdx.x;
-      e.q_id += en.q[i];
-    }
-  }
-  return te;
 }
 
 // Leaves the teacher's entries out of a sum. A bit of the filter is set for each vector that holds
-// one (and stands for every 16384th vector); such a vector is compared with the list.
+// one (and stands for every 8192nd vector); such a vector is compared with the list.
 template <typename T>
 struct DropEntries {
   const uint32_t* filter;
-  const Entries* en;
-  int k;
-  int64_t head;
-  ME_DEVICE uint32_t operator()(int64_t vec) const {
+  const int* id;
+  int k, head;
+  ME_DEVICE uint32_t operator()(int vec) const {
     constexpr int kN = Vec16<T>::kN;
     const uint32_t b = (uint32_t)vec & (kFilter - 1);
     if (!(filter[b >> 5] >> (b & 31) & 1)) return 0;
-    const int j0 = (int)(head + vec * kN);
+    const int j0 = head + vec * kN;
     uint32_t mask = 0;
     for (int i = 0; i < k; ++i) {
-      const uint32_t d = (uint32_t)(en->id[i] - j0);
-      if (d < (uint32_t)kN) mask |= 1u << d;  // an unused entry is negative: never within
+      const uint32_t d = (uint32_t)(id[i] - j0);
+      if (id[i] >= 0 && d < (uint32_t)kN) mask |= 1u << d;
     }
     return mask;
   }
-  ME_DEVICE bool column(int64_t j) const {
+  ME_DEVICE bool column(int j) const {
     for (int i = 0; i < k; ++i)
-      if (en->id[i] == (int)j) return true;
+      if (id[i] == j) return true;
     return false;
   }
 };
 
-// The entries' own columns, after the slice was written without them.
-template <typename T>
-ME_DEVICE void write_entry(const Slice<T>& sl, T* out, const Entry& e, const Scale& sc, float c, float m, float inv_s,
-                           float mass) {
-  if (!e.first || !sl.holds(e.id)) return;
-  const float z = softcap(e.x, sc.cap);
-  out[e.id] = from_f<T>(c * (expf(z * sc.inv_temp - m) * inv_s * mass - e.q_id) * softcap_slope(z, sc.cap));
+// The student's side of a row, from the sum over its columns (with a rest: over those that are no entry).
+struct Student {
+  MaxSum all;
+  float log_s;
+  float m1, c1;      // p_j rho_j = c1 exp(y_j - m1) for the columns that are no entry
+  float log_p_rest;
+};
+template <bool kTail>
+ME_DEVICE Student finish_student(MaxSum a, const TeacherRow& te) {
+  Student st;
+  const MaxSum rest = a;
+  if (kTail) {
+    MaxSum own;
+    own.m = te.s == 0.f ? -INFINITY : te.y_ref;
+    own.s = te.s;
+    a.merge(own);
+  }
+  st.all = a;
+  st.log_s = logf(a.s);
+  st.m1 = a.m;
+  st.c1 = 1.f / a.s;
+  st.log_p_rest = 0.f;
+  if (kTail) {
+    const bool some = rest.m != -INFINITY;
+    const float share = some ? expf(rest.m - a.m) : 0.f, p_rest = share * (rest.s / a.s);
+    // (a rest that fp32 cannot hold: by its logarithm)
+    st.log_p_rest = p_rest > 1e-30f ? logf(p_rest) : some ? rest.m - a.m + (logf(rest.s) - st.log_s) : -INFINITY;
+    st.m1 = some ? rest.m : 0.f;
+    st.c1 = some ? te.mass * (share / a.s) - te.q_rest / rest.s : 0.f * st.log_s;
+  }
+  return st;
 }
 
-// One cluster a row. Value (and the statistics that the backward pass starts from: m, s (-1: a row
-// without gradient), m', c'; without a rest m' = m, c' = 1 / s), or with kGrad value and gradient:
-// the slice is read again, from L2, once the cluster has the row's sum.
+// The row's divergence.
+ME_DEVICE float divergence(const TeacherRow& te, const Student& st) {
+  float kl = te.b + te.sum_q * (st.log_s + (st.all.m - te.y_ref));
+  if (te.q_rest > 0.f) kl += te.q_rest * (logf(te.q_rest) - st.log_p_rest);
+  return kl;
+}
+
+// A thread's entry of the row (k is at most a block's threads).
+static_assert(kThreads >= kMaxTop);
+ME_DEVICE Entry load_entry(const Entry* entries, int64_t r, int k) {
+  Entry e = {-1, 0.f, 0.f, 0.f};
+  if (threadIdx.x < k) *reinterpret_cast<float4*>(&e) = reinterpret_cast<const float4*>(entries)[r * k + threadIdx.x];
+  return e;
+}
+// The entries' own columns, after the slice was written without them.
+template <typename T>
+ME_DEVICE void write_entry(const Slice<T>& sl, T* out, const Entry& e, float c, float m, float inv_s, float mass) {
+  if (e.id >= 0 && sl.holds(e.id)) out[e.id] = from_f<T>(c * (expf(e.y - m) * inv_s * mass - e.q) * e.slope);
+}
+
+// One cluster a row. With kGrad value and gradient: each block keeps its slice of the row in shared
+// memory (`depth` vectors a thread) until the cluster has the row's sum, so a logit is read once from
+// memory. Without, the value and the statistics that the backward pass starts from: m, s (-1: a row
+// without gradient), m', c'.
 template <typename T, bool kCap, bool kTail, bool kGrad>
-__global__ void __launch_bounds__(kThreads, 4) distill_kernel(Rows<const T> x, Rows<T> out, int64_t V, int ranks,
-                                                              TeacherArgs ta, Scale sc, float* __restrict__ loss,
-                                                              float4* __restrict__ stats) {
-  __shared__ Shared sh;
-  __shared__ Entries en;
+__global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
+    distill_kernel(Rows<const T> x, Rows<T> out, int V, int lg_ranks, int depth, int k,
+                   const float* __restrict__ weight, float temp, const Entry* __restrict__ entries,
+                   const TeacherRow* __restrict__ rows, Scale sc, float* __restrict__ loss,
+                   float4* __restrict__ stats) {
+  extern __shared__ uint4 dynamic[];  // the slice, or the ring
+  __shared__ float2 part[kWarps];
   __shared__ uint32_t filter[kTail ? kFilter / 32 : 1];
-  const int64_t r = blockIdx.x / ranks;
-  const int rank = blockIdx.x % ranks;
-  const Slice<T> sl(x.row(r), V, rank, ranks);
+  __shared__ int ids[kTail ? kMaxTop : 1];
+  const int64_t r = blockIdx.x >> lg_ranks;
+  const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
+  const Slice<T> sl(x.row(r), V, rank, lg_ranks);
   T* o = kGrad ? out.row(r) : nullptr;
-  const float w = ta.weight ? ta.weight[r] : 1.f;
+  const float w = weight ? weight[r] : 1.f;
   const bool writer = threadIdx.x == 0 && rank == 0;
   if (w == 0.f) {
     if (writer) loss[r] = 0.f;
@@ -305,86 +371,89 @@ __global__ void __launch_bounds__(kThreads, 4) distill_kernel(Rows<const T> x, R
     if (kGrad) zero_slice<T>(sl, o);
     return;
   }
-  Entry e = load_entry<T>(ta, r, sl.row, V, sc.inv_temp, en);
+  if (kGrad) hold_issue(sl.mine(), sl.count(), depth, dynamic);
+  const Entry e = kGrad || kTail ? load_entry(entries, r, k) : Entry{};
+  const TeacherRow te = rows[r];
+  auto walk = [&](auto&& first, auto&& f) {
+    if constexpr (kGrad) {
+      // (the reference comes from the first group: at most kFirst vectors of it)
+      copy_wait<kGroups - 1>();
+      uint4 v[kFirst];
+      const int n = min(min(sl.count(), kFirst), hold_group(depth));
+#pragma unroll
+      for (int u = 0; u < kFirst; ++u)
+        if (u < n) v[u] = dynamic[u * kThreads + threadIdx.x];
+      first(n, v);
+      hold_walk<true>(sl.count(), depth, dynamic, f);
+    } else {
+      stream(sl.mine(), sl.count(), *reinterpret_cast<Ring*>(dynamic), first, f);
+    }
+  };
   MaxSum a;
   if constexpr (kTail) {
     for (int i = threadIdx.x; i < kFilter / 32; i += kThreads) filter[i] = 0;
+    if (threadIdx.x < k) ids[threadIdx.x] = e.id;
     __syncthreads();
     if (e.id >= sl.head && e.id < sl.body_end) {
       const uint32_t b = (uint32_t)((e.id - sl.head) / Vec16<T>::kN) & (kFilter - 1);
       atomicOr(&filter[b >> 5], 1u << (b & 31));
     }
     __syncthreads();
-    a = row_sum<T, kCap>(sl, sc, DropEntries<T>{filter, &en, ta.k, sl.head}, sh, ranks);
+    a = slice_sum<T, kCap>(sl, sc, DropEntries<T>{filter, ids, k, sl.head}, walk);
   } else {
-    a = row_sum<T, kCap>(sl, sc, KeepAll(), sh, ranks);
+    a = slice_sum<T, kCap>(sl, sc, KeepAll(), walk);
   }
-  const TeacherRow te = finish_entries(e, ta, r, V, kTail, en, sh.scratch);
-  const float y = softcap(e.x, sc.cap) * sc.inv_temp;
-  const MaxSum rest = a;
-  if constexpr (kTail) {
-    MaxSum own;
-    own.m = block_max(e.first ? y : -INFINITY, sh.scratch);
-    own.s = block_sum(e.first && y != -INFINITY ? expf(y - own.m) : 0.f, sh.scratch);
-    a.merge(own);
-  }
-  const float log_s = logf(a.s);
-  float kl = 0.f;
-  // maxima first: what is left to round is of the size of the difference
-  if (e.q != 0.f) kl = e.q * (((e.t - te.m) - (y - a.m)) + (log_s - te.log_s));
-  kl = block_sum(kl, sh.scratch);
-  float m1 = a.m, c1 = 1.f / a.s;
-  if constexpr (kTail) {
-    const bool some = rest.m != -INFINITY;
-    const float share = some ? expf(rest.m - a.m) : 0.f, p_rest = share * (rest.s / a.s);
-    // (a rest that fp32 cannot hold: by its logarithm)
-    const float log_rest = p_rest > 1e-30f ? logf(p_rest) : some ? rest.m - a.m + (logf(rest.s) - log_s) : -INFINITY;
-    if (te.q_rest > 0.f) kl += te.q_rest * (logf(te.q_rest) - log_rest);
-    m1 = some ? rest.m : 0.f;
-    c1 = some ? te.mass * (share / a.s) - te.q_rest / rest.s : 0.f * log_s;
-  }
-  const bool nothing = !kTail && !te.any;  // no entry: nothing to match
+  a = row_merge(a, part, lg_ranks);
+  const Student st = finish_student<kTail>(a, te);
+  const bool nothing = !kTail && te.any == 0.f;  // no entry: nothing to match
   if (writer) {
-    loss[r] = nothing ? 0.f : w * ta.temp * ta.temp * kl;
-    if (!kGrad) stats[r] = make_float4(a.m, nothing ? -1.f : a.s, m1, c1);
+    loss[r] = nothing ? 0.f : w * temp * temp * divergence(te, st);
+    if (!kGrad) stats[r] = make_float4(st.all.m, nothing ? -1.f : st.all.s, st.m1, st.c1);
   }
   if constexpr (kGrad) {
     if (nothing) {
       zero_slice<T>(sl, o);
     } else {
-      const float c = w * ta.temp;
-      write_slice<T, kCap>(sl, o, sc, m1, c * c1, sh.ring);
+      const float c = w * temp;
+      write_slice<T, kCap>(sl, o, sc, st.m1, c * st.c1,
+                           [&](auto&& f) { hold_walk<false>(sl.count(), depth, dynamic, f); });
       __syncthreads();
-      write_entry<T>(sl, o, e, sc, c, a.m, 1.f / a.s, te.mass);
+      write_entry<T>(sl, o, e, c, st.all.m, 1.f / st.all.s, te.mass);
     }
   }
-  row_done(ranks);
+  row_done(lg_ranks);
 }
 
 template <typename T, bool kCap>
-__global__ void __launch_bounds__(kThreads, 4) distill_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int64_t V,
-                                                                  int ranks, TeacherArgs ta, Scale sc,
-                                                                  const float4* __restrict__ stats,
-                                                                  const float* __restrict__ g) {
-  __shared__ Shared sh;
-  __shared__ Entries en;
-  const int64_t r = N - 1 - blockIdx.x / ranks;  // last to first, as above
-  const Slice<T> sl(x.row(r), V, blockIdx.x % ranks, ranks);
+__global__ void __launch_bounds__(kThreads, 4)
+    distill_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int V, int lg_ranks, int k,
+                       const float* __restrict__ weight, float temp, const Entry* __restrict__ entries,
+                       const TeacherRow* __restrict__ rows, Scale sc, const float4* __restrict__ stats,
+                       const float* __restrict__ g) {
+  __shared__ Ring ring;
+  const int64_t r = N - 1 - (blockIdx.x >> lg_ranks);  // last to first, as above
+  const Slice<T> sl(x.row(r), V, blockIdx.x & ((1 << lg_ranks) - 1), lg_ranks);
   T* o = out.row(r);
   const float4 st = stats[r];
   if (st.y == -1.f) {
     zero_slice<T>(sl, o);
     return;
   }
-  Entry e = load_entry<T>(ta, r, sl.row, V, sc.inv_temp, en);
-  const TeacherRow te = finish_entries(e, ta, r, V, ta.lse != nullptr, en, sh.scratch);
-  const float c = (ta.weight ? ta.weight[r] : 1.f) * ta.temp * g[r];
-  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w, sh.ring);
+  const Entry e = load_entry(entries, r, k);
+  const float c = (weight ? weight[r] : 1.f) * temp * (g ? g[r] : 1.f);
+  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w,
+                       [&](auto&& f) { stream(sl.mine(), sl.count(), ring, [](int, auto&) {}, f); });
   __syncthreads();
-  write_entry<T>(sl, o, e, sc, c, st.x, 1.f / st.y, te.mass);
+  write_entry<T>(sl, o, e, c, st.x, 1.f / st.y, rows[r].mass);
 }
 
 // ------------------------------------------------------------------------------------ launches
+int ilog2(int c) {
+  int l = 0;
+  while (1 << l < c) ++l;
+  return l;
+}
+
 // Blocks a row: enough for two on each SM, while a block keeps two vectors a thread.
 int ranks_for(int64_t N, int64_t V, int at_least = 1) {
   static const int fix = getenv("RNK") ? atoi(getenv("RNK")) : 0;
@@ -394,14 +463,27 @@ int ranks_for(int64_t N, int64_t V, int at_least = 1) {
   return c;
 }
 
-// Blocks a row where the row is read twice: the rows in flight (four blocks an SM) have to stay in L2
-// between the two passes; 40 of its 126 MB are given to them.
-int ranks_for_two_passes(const Logits& x) {
-  static const int l2_rows = getenv("L2R") ? atoi(getenv("L2R")) : 40;
-  const int64_t row = x.V * (x.type == LogitType::kF32 ? 4 : 2);
+// Value and gradient at once: blocks a row, and vectors that a thread keeps. 16 (64 KB a block) let three
+// blocks share an SM, so that one's copies run under another's arithmetic.
+struct HoldPlan {
+  int ranks, depth;
+  bool fits;
+};
+HoldPlan hold_plan(const Logits& x) {
+  const int64_t vecs = (x.V * (x.type == LogitType::kF32 ? 4 : 2) + 15) / 16;
+  static const int most = getenv("DPT") ? atoi(getenv("DPT")) : 16;
+  auto depth = [&](int c) { return ((vecs + c - 1) / c + kThreads - 1) / kThreads; };
   int c = 1;
-  while (c < 8 && 4 * objective_sms() / c * row > ((int64_t)l2_rows << 20)) c *= 2;
-  return ranks_for(x.N, x.V, c);
+  while (c < 8 && depth(c) > most) c *= 2;
+  c = ranks_for(x.N, x.V, c);
+  const int64_t d = depth(c);
+  return {c, (int)d, d <= 48};
+}
+
+// Lets a kernel have more than 48 KB of shared memory.
+template <typename K>
+void allow_smem(K* kernel, int bytes) {
+  if (bytes > (32 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 }  // namespace
@@ -419,8 +501,8 @@ namespace me {
 
 void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, float2* stats, cudaStream_t stream) {
   const int ranks = ranks_for(x.N, x.V);
-  ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, launch_cluster(logprob_fwd_kernel<T, kCap>, x.N * ranks, kThreads,
-                                                                   ranks, stream, rows_in<T>(x), x.V, ranks, target,
+  ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, launch_cluster(logprob_fwd_kernel<T, kCap>, x.N * ranks, ranks, 0,
+                                                                   stream, rows_in<T>(x), x.V, ilog2(ranks), target,
                                                                    make_scale(x.cap, 1.f), logp, stats)));
 }
 
@@ -429,35 +511,50 @@ void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* st
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, logprob_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
-                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, target, make_scale(x.cap, 1.f),
-                                         stats, g)));
+                                         rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), target,
+                                         make_scale(x.cap, 1.f), stats, g)));
 }
 
-void launch_distill_fwd(const Logits& x, const TeacherArgs& te, float* loss, float4* stats, cudaStream_t stream) {
+void launch_teacher(const Logits& x, const TeacherArgs& te, void* entries, void* rows, cudaStream_t stream) {
+  ME_LOGITS_DISPATCH(x.type, teacher_kernel<T><<<(unsigned)((x.N + kWarps - 1) / kWarps), kThreads, 0, stream>>>(
+                                 rows_in<T>(x), x.N, (int)x.V, te, make_scale(x.cap, te.temp),
+                                 static_cast<Entry*>(entries), static_cast<TeacherRow*>(rows)));
+}
+
+void launch_distill_fwd(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows, float* loss,
+                        float4* stats, cudaStream_t stream) {
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, false> : distill_kernel<T, kCap, false, false>;
-    launch_cluster(kernel, x.N * ranks, kThreads, ranks, stream, rows_in<T>(x), Rows<T>{}, x.V, ranks, te,
+    launch_cluster(kernel, x.N * ranks, ranks, sizeof(Ring), stream, rows_in<T>(x), Rows<T>{}, x.V, ilog2(ranks), 0, te.k,
+                   te.weight, te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
                    make_scale(x.cap, te.temp), loss, stats);
   }));
 }
 
-void launch_distill_grad(const Logits& x, const TeacherArgs& te, float* loss, Gradient out, cudaStream_t stream) {
-  const int ranks = ranks_for_two_passes(x);
+bool launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows, float* loss,
+                         Gradient out, cudaStream_t stream) {
+  const HoldPlan plan = hold_plan(x);
+  if (!plan.fits) return false;
+  const int smem = plan.depth * kThreads * 16;
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, true> : distill_kernel<T, kCap, false, true>;
-    launch_cluster(kernel, x.N * ranks, kThreads, ranks, stream, rows_in<T>(x), rows_out<T>(out), x.V, ranks, te,
-                   make_scale(x.cap, te.temp), loss, (float4*)nullptr);
+    allow_smem(kernel, smem);
+    launch_cluster(kernel, x.N * plan.ranks, plan.ranks, smem, stream, rows_in<T>(x), rows_out<T>(out), x.V,
+                   ilog2(plan.ranks), plan.depth, te.k, te.weight, te.temp, static_cast<const Entry*>(entries),
+                   static_cast<const TeacherRow*>(rows), make_scale(x.cap, te.temp), loss, (float4*)nullptr);
   }));
+  return true;
 }
 
-void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const float4* stats, const float* g, Gradient out,
-                        cudaStream_t stream) {
+void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows,
+                        const float4* stats, const float* g, Gradient out, cudaStream_t stream) {
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, distill_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
-                                         rows_in<T>(x), rows_out<T>(out), x.N, x.V, ranks, te, make_scale(x.cap, te.temp),
-                                         stats, g)));
+                                         rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), te.k, te.weight,
+                                         te.temp, static_cast<const Entry*>(entries),
+                                         static_cast<const TeacherRow*>(rows), make_scale(x.cap, te.temp), stats, g)));
 }
 
 }  // namespace me

@@ -294,46 +294,44 @@ struct Rows {
   ME_DEVICE T* row(int64_t r) const { return base + r * stride; }
 };
 
-// A block's share of one row: 16-byte vectors [begin, end) from `body`, and for the row's first and
-// last block the elements ahead of the first 16-byte boundary and after the last one.
+// A block's share of one row: 16-byte vectors [begin, end) from `head` on, and for the row's first and
+// last block the elements ahead of the first 16-byte boundary and after the last one. (V is below 2^31.)
 template <typename T>
 struct Slice {
   static constexpr int kN = Vec16<T>::kN;
   const T* row;
-  int64_t head, body_end, V;  // columns [head, body_end) are vectors
-  int64_t begin, end;         // of them, this block's
+  int V, head, body_end;  // columns [head, body_end) are vectors
+  int begin, end;         // of them, this block's
   bool first, last;
 
-  ME_DEVICE Slice(const T* row_, int64_t V_, int rank, int ranks) : row(row_), V(V_) {
-    head = ((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / sizeof(T);
-    if (head > V) head = V;
-    const int64_t nvec = (V - head) / kN, per = (nvec + ranks - 1) / ranks;
+  // the row's blocks are 2^lg_ranks
+  ME_DEVICE Slice(const T* row_, int V_, int rank, int lg_ranks) : row(row_), V(V_) {
+    head = (int)((16 - (reinterpret_cast<uintptr_t>(row) & 15)) & 15) / (int)sizeof(T);
+    head = min(head, V);
+    const int nvec = (V - head) / kN, per = (nvec + (1 << lg_ranks) - 1) >> lg_ranks;
     body_end = head + nvec * kN;
-    begin = min(nvec, rank * per);
-    end = min(nvec, begin + per);
+    begin = (int)min((long long)nvec, (long long)rank * per);
+    end = min(nvec - begin, per) + begin;
     first = rank == 0;
-    last = rank == ranks - 1;
+    last = rank == (1 << lg_ranks) - 1;
   }
   // This thread's vectors: how many, the i-th one's number in the row, where the first one is.
-  ME_DEVICE int count() const {
-    const int n = (int)(end - begin) - (int)threadIdx.x;
-    return n > 0 ? (n + kThreads - 1) / kThreads : 0;
-  }
-  ME_DEVICE int64_t vec(int i) const { return begin + threadIdx.x + (int64_t)i * kThreads; }
+  ME_DEVICE int count() const { return (end - begin + kThreads - 1 - (int)threadIdx.x) / kThreads; }
+  ME_DEVICE int vec(int i) const { return begin + threadIdx.x + i * kThreads; }
   ME_DEVICE const uint4* mine() const { return reinterpret_cast<const uint4*>(row + head) + begin + threadIdx.x; }
-  ME_DEVICE int64_t column(int64_t vec) const { return head + vec * kN; }
+  ME_DEVICE int column(int v) const { return head + v * kN; }
   // The block's single columns, one a thread: -1 for the threads that have none.
-  ME_DEVICE int64_t single() const {
-    const int64_t t = threadIdx.x;
+  ME_DEVICE int single() const {
+    const int t = threadIdx.x;
     if (first && t < head) return t;
     if (last && t >= 16 && t - 16 < V - body_end) return body_end + t - 16;
     return -1;
   }
   // Whether a column is this block's.
-  ME_DEVICE bool holds(int64_t j) const {
+  ME_DEVICE bool holds(int j) const {
     if (j < head) return first;
     if (j >= body_end) return last;
-    const int64_t v = (j - head) / kN;
+    const int v = (j - head) / kN;
     return v >= begin && v < end;
   }
 };
@@ -365,8 +363,8 @@ struct MaxSum {
 
 // No column is left out.
 struct KeepAll {
-  ME_DEVICE uint32_t operator()(int64_t) const { return 0; }
-  ME_DEVICE bool column(int64_t) const { return false; }
+  ME_DEVICE uint32_t operator()(int) const { return 0; }
+  ME_DEVICE bool column(int) const { return false; }
 };
 
 // ---------------------------------------------------------------- a thread's vectors, read ahead
@@ -436,6 +434,44 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
   }
 }
 
+// The same vectors, all kept: `hold` has place for each of the block's vectors ([i][thread]), and the
+// slice can be walked again without a second read. Copies are issued in eight groups of two vectors or more.
+constexpr int kGroups = 8;
+ME_DEVICE int hold_group(int depth) { return max(2, (depth + kGroups - 1) / kGroups); }
+ME_DEVICE void hold_issue(const uint4* src, int count, int depth, uint4* hold) {
+  uint4* mine = hold + threadIdx.x;
+  const int group = hold_group(depth);
+#pragma unroll 1
+  for (int g = 0; g < kGroups; ++g) {
+    for (int d = g * group; d < min(count, (g + 1) * group); ++d) copy_async(mine + d * kThreads, src + d * kThreads);
+    copy_commit();
+  }
+}
+// f as in stream(). kWait: the first walk, in which the i-th group is waited for with i empty ones behind it.
+template <bool kWait, typename F>
+ME_DEVICE void hold_walk(int count, int depth, const uint4* hold, F&& f) {
+  const uint4* mine = hold + threadIdx.x;
+  const int whole = __shfl_sync(0xffffffffu, count, 31);
+  const int group = kWait ? hold_group(depth) : depth;
+#pragma unroll 1
+  for (int g = 0; g < (kWait ? kGroups : 1); ++g) {
+    if (kWait) copy_wait<kGroups - 1>();
+    const int end = (g + 1) * group;
+    int i = g * group;
+#pragma unroll 1
+    for (; i + 2 <= min(whole, end); i += 2) {
+      const uint4 v[2] = {mine[i * kThreads], mine[(i + 1) * kThreads]};
+      f(v, i, std::true_type());
+    }
+#pragma unroll 1
+    for (; i < min(count, end); ++i) {
+      const uint4 v[1] = {mine[i * kThreads]};
+      f(v, i, std::false_type());
+    }
+    if (kWait) copy_commit();
+  }
+}
+
 // This thread's share of sum exp(y - m) over a slice. `drop(vec)`: a mask of the vector's elements
 // that are left out (`drop.column(j)` for a single column).
 //
@@ -446,16 +482,16 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
 // form, since nothing else is rounded then.
-template <typename T, bool kCap, typename Drop>
-ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Ring& ring) {
+// walk(first, f): how the slice is gone over (stream() or hold_walk()).
+template <typename T, bool kCap, typename Drop, typename Walk>
+ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Walk&& walk) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   MaxSum out;
   const int count = sl.count();
   float big = -INFINITY, sum0 = 0.f, sum1 = 0.f;
   const float k = sc.inv_temp * kLog2e;
   float ref = 0.f, shift = 0.f;  // the reference; the same, or the rounded ref k
-  stream(
-      sl.mine(), count, ring,
+  walk(
       [&](int n, const uint4(&v)[kFirst]) {
         float top = -INFINITY;
 #pragma unroll
@@ -514,45 +550,64 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
         if (!(out_mask >> e & 1)) out.add(softcap(to_f<T>(sl.row[sl.column(sl.vec(i)) + e]), sc.cap) * sc.inv_temp);
     }
   }
-  const int64_t j = sl.single();
+  const int j = sl.single();
   if (j >= 0 && !drop.column(j)) out.add(softcap(to_f<T>(sl.row[j]), sc.cap) * sc.inv_temp);
   return out;
 }
 
-// Block-wide largest and sum; `scratch` holds 32 floats and is free again after the next barrier.
-ME_DEVICE float block_max(float v, float* scratch) {
-  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
-  v = warp_max(v);
-  __syncthreads();
-  if (lane == 0) scratch[wid] = v;
-  __syncthreads();
-  return warp_max(lane < nw ? scratch[lane] : -INFINITY);
-}
-
-// The block's (m, s), the same for all threads: one exponential a thread.
-ME_DEVICE MaxSum block_merge(MaxSum a, float* scratch) {
+// The warp's (m, s), the same for every lane: one exponential a lane.
+ME_DEVICE MaxSum warp_merge(MaxSum a) {
   MaxSum r;
-  r.m = block_max(a.m, scratch);
-  // a.m = -inf: a.s is 0 or NaN
-  r.s = block_sum(a.m == -INFINITY ? a.s : a.s * expf(a.m - r.m), scratch);
+  r.m = warp_max(a.m);
+  // (m = -inf: s is 0 or NaN)
+  r.s = warp_sum(a.m == -INFINITY ? a.s : a.s * expf(a.m - r.m));
   return r;
 }
 
 // ---------------------------------------------------------------- thread-block clusters
-ME_DEVICE uint32_t cluster_rank() {
-  uint32_t r;
-  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
-  return r;
-}
 ME_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 ME_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
-// A float in the shared memory of the cluster's block `rank`, at the place that `p` has in this one.
-ME_DEVICE float cluster_load(const float* p, uint32_t rank) {
+// A pair in the shared memory of the cluster's block `rank`, at the place that `p` has in this one.
+ME_DEVICE float2 cluster_load(const float2* p, uint32_t rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), b;
-  float v;
+  float2 v;
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(a), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(b) : "memory");
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(b) : "memory");
   return v;
+}
+
+constexpr int kWarps = kThreads / 32;
+
+// A row's (m, s) from its threads', the same bits for every thread of the cluster: the warps' pairs are
+// exchanged behind one barrier. Where there is more than one block, row_done() has to follow before
+// the block leaves (others may still read its pairs).
+ME_DEVICE MaxSum row_merge(MaxSum a, float2* part, int lg_ranks) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
+  a = warp_merge(a);
+  if (lane == 0) part[wid] = make_float2(a.m, a.s);
+  MaxSum r;
+  if (lg_ranks == 0) {
+    __syncthreads();
+    if (lane < kWarps) {
+      r.m = part[lane].x;
+      r.s = part[lane].y;
+    }
+  } else {
+    cluster_arrive();
+    cluster_wait();
+    for (int i = lane; i < kWarps << lg_ranks; i += 32) {
+      const float2 o = cluster_load(part + i % kWarps, i / kWarps);
+      MaxSum b;
+      b.m = o.x;
+      b.s = o.y;
+      r.merge(b);
+    }
+    cluster_arrive();
+  }
+  return warp_merge(r);
+}
+ME_DEVICE void row_done(int lg_ranks) {
+  if (lg_ranks > 0) cluster_wait();
 }
 
 // SMs of the current device (one kind of GPU is built for).
@@ -566,13 +621,14 @@ inline int objective_sms() {
   return n;
 }
 
-// Launches `kernel` on grid blocks in clusters of `cluster`.
+// Launches `kernel` on `grid` blocks of kThreads in clusters of `cluster`.
 template <typename... Params, typename... Args>
-cudaError_t launch_cluster(void (*kernel)(Params...), int64_t grid, int threads, int cluster, cudaStream_t stream,
+cudaError_t launch_cluster(void (*kernel)(Params...), int64_t grid, int cluster, int smem, cudaStream_t stream,
                            Args... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)grid);
-  cfg.blockDim = dim3(threads);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;

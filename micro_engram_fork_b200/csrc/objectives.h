@@ -38,11 +38,17 @@ struct TeacherArgs {
 void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, float2* stats, cudaStream_t stream);
 void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
                         cudaStream_t stream);
-void launch_distill_fwd(const Logits& x, const TeacherArgs& teacher, float* loss, float4* stats, cudaStream_t stream);
-// value and gradient of sum(loss) in one launch
-void launch_distill_grad(const Logits& x, const TeacherArgs& teacher, float* loss, Gradient out, cudaStream_t stream);
-void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const float4* stats, const float* g, Gradient out,
-                        cudaStream_t stream);
+// What launch_teacher() leaves for the other three: N k entries and N rows, 16-byte aligned.
+constexpr int kEntryBytes = 16, kTeacherRowBytes = 32;
+void launch_teacher(const Logits& x, const TeacherArgs& teacher, void* entries, void* rows, cudaStream_t stream);
+void launch_distill_fwd(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows, float* loss,
+                        float4* stats, cudaStream_t stream);
+// Value and gradient of sum(loss) in one launch. False: a row is too long for it (take the two others).
+bool launch_distill_grad(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows, float* loss,
+                         Gradient out, cudaStream_t stream);
+// g: one coefficient a row, or null for 1
+void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows,
+                        const float4* stats, const float* g, Gradient out, cudaStream_t stream);
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,
                        cudaStream_t stream);
 

@@ -106,7 +106,23 @@ Tensor token_logprobs_bwd(Tensor x, Tensor target, double cap, Tensor stats, Ten
   return o;
 }
 
-// (loss [N], stats [N, 4])
+namespace {
+// The kernels' view of the teacher's rows: k entries of 4 and one of 8 floats a row.
+struct TeacherRows {
+  Tensor buffer;
+  float* entries;
+  float* rows;
+};
+TeacherRows teacher_rows(const Tensor& x, int64_t k) {
+  TeacherRows t;
+  t.buffer = torch::empty({x.size(0), k + 2, me::kEntryBytes / 4}, x.options().dtype(torch::kFloat32));
+  t.entries = t.buffer.data_ptr<float>();
+  t.rows = t.entries + x.size(0) * k * (me::kEntryBytes / 4);
+  return t;
+}
+}  // namespace
+
+// (loss [N], stats [N, 4], the teacher's rows, which distill_bwd takes)
 std::vector<Tensor> distill_fwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap,
                                 double temp) {
   const auto in = check_logits(x, cap, "distill_loss");
@@ -114,22 +130,31 @@ std::vector<Tensor> distill_fwd(Tensor x, Tensor ids, Tensor top, OptTensor lse,
   const auto te = check_teacher(x, ids, top, lse, weight, temp);
   auto opts = x.options().dtype(torch::kFloat32);
   auto loss = torch::empty({in.N}, opts), stats = torch::empty({in.N, 4}, opts);
-  if (in.N == 0) return {loss, stats};
-  me::launch_distill_fwd(in, te.args, loss.data_ptr<float>(), as4(stats), at::cuda::getCurrentCUDAStream());
+  const auto rows = teacher_rows(x, te.args.k);
+  if (in.N == 0) return {loss, stats, rows.buffer};
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  me::launch_teacher(in, te.args, rows.entries, rows.rows, stream);
+  me::launch_distill_fwd(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), as4(stats), stream);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {loss, stats};
+  return {loss, stats, rows.buffer};
 }
 
-Tensor distill_bwd(Tensor x, Tensor ids, Tensor top, OptTensor lse, OptTensor weight, double cap, double temp,
-                   Tensor stats, Tensor g, OptTensor out) {
+Tensor distill_bwd(Tensor x, Tensor rows, OptTensor weight, double cap, double temp, Tensor stats, Tensor g,
+                   OptTensor out) {
   const auto in = check_logits(x, cap, "distill_loss");
   const at::cuda::CUDAGuard guard(x.device());
-  const auto te = check_teacher(x, ids, top, lse, weight, temp);
   auto gr = check_rows(g, x, torch::kFloat32, "distill_loss: gradient");
+  Tensor w;
+  if (weight.has_value()) w = check_rows(*weight, x, torch::kFloat32, "distill_loss: weights");
   auto o = gradient_like(x, out, "distill_loss");
   if (in.N == 0) return o;
-  me::launch_distill_bwd(in, te.args, as4(stats), gr.data_ptr<float>(), gradient_of(o),
-                         at::cuda::getCurrentCUDAStream());
+  me::TeacherArgs te = {};
+  te.k = (int)rows.size(1) - 2;
+  te.weight = weight.has_value() ? w.data_ptr<float>() : nullptr;
+  te.temp = (float)temp;
+  const float* entries = rows.data_ptr<float>();
+  me::launch_distill_bwd(in, te, entries, entries + in.N * te.k * (me::kEntryBytes / 4), as4(stats),
+                         gr.data_ptr<float>(), gradient_of(o), at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
 }
@@ -143,7 +168,14 @@ std::vector<Tensor> distill_grad(Tensor x, Tensor ids, Tensor top, OptTensor lse
   auto o = gradient_like(x, out, "distill_loss");
   auto loss = torch::empty({in.N}, x.options().dtype(torch::kFloat32));
   if (in.N == 0) return {loss, o};
-  me::launch_distill_grad(in, te.args, loss.data_ptr<float>(), gradient_of(o), at::cuda::getCurrentCUDAStream());
+  const auto rows = teacher_rows(x, te.args.k);
+  const auto stream = at::cuda::getCurrentCUDAStream();
+  me::launch_teacher(in, te.args, rows.entries, rows.rows, stream);
+  if (!me::launch_distill_grad(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), gradient_of(o), stream)) {
+    auto stats = torch::empty({in.N, 4}, loss.options());
+    me::launch_distill_fwd(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), as4(stats), stream);
+    me::launch_distill_bwd(in, te.args, rows.entries, rows.rows, as4(stats), nullptr, gradient_of(o), stream);
+  }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {loss, o};
 }

@@ -23,6 +23,16 @@ template <typename T, typename F>
 ME_DEVICE void for_row(const T* row, int64_t V, F&& f) {
   for (int64_t j = threadIdx.x; j < V; j += blockDim.x) f(j, to_f<T>(row[j]));
 }
+ME_DEVICE MaxSum block_merge(MaxSum a, float* scratch) {
+  const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5, nw = blockDim.x >> 5;
+  a = warp_merge(a);
+  __syncthreads();
+  if (lane == 0) scratch[wid] = a.m, scratch[32 + wid] = a.s;
+  __syncthreads();
+  MaxSum r;
+  if (lane < nw) r.m = scratch[lane], r.s = scratch[32 + lane];
+  return warp_merge(r);
+}
 // Radix selection, eight bits of the key a pass over the row: the exact k-th largest key, then every
 // larger one and the lowest ids among its equals, ranked by counting.
 template <typename T>

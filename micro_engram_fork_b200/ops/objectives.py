@@ -271,20 +271,22 @@ class _Distill(torch.autograd.Function):
         ctx.args = cap, temperature
         ctx.native = use_native(x)
         if ctx.native:
-            loss, stats = native().distill_fwd(x, ids, top, lse, weights, cap, temperature)
+            loss, stats, rows = native().distill_fwd(x, ids, top, lse, weights, cap, temperature)
+            ctx.save_for_backward(x, weights, stats, rows)
         else:
-            loss, stats = distill_ref(x, ids, top, lse, weights, cap, temperature)[0], None
-        ctx.save_for_backward(x, ids, top, lse, weights, stats)
+            loss = distill_ref(x, ids, top, lse, weights, cap, temperature)[0]
+            ctx.save_for_backward(x, ids, top, lse, weights)
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        x, ids, top, lse, weights, stats = ctx.saved_tensors
         cap, temperature = ctx.args
         if ctx.native:
-            dx = native().distill_bwd(x, ids, top, lse, weights, cap, temperature, stats, g, None)
+            x, weights, stats, rows = ctx.saved_tensors
+            dx = native().distill_bwd(x, rows, weights, cap, temperature, stats, g, None)
         else:
+            x, ids, top, lse, weights = ctx.saved_tensors
             w = g if weights is None else torch.where(weights != 0, weights * g, 0.0)
             dx = distill_ref(x, ids, top, lse, w, cap, temperature)[1]
         return dx, None, None, None, None, None, None
