@@ -448,21 +448,6 @@ __global__ void __launch_bounds__(kThreads, 4)
 }
 
 // ------------------------------------------------------------------------------------ launches
-int ilog2(int c) {
-  int l = 0;
-  while (1 << l < c) ++l;
-  return l;
-}
-
-// Blocks a row: enough for two on each SM, while a block keeps two vectors a thread.
-int ranks_for(int64_t N, int64_t V, int at_least = 1) {
-  static const int fix = getenv("RNK") ? atoi(getenv("RNK")) : 0;
-  if (fix) return fix;
-  int c = at_least;
-  while (c < 8 && N * c < 2 * objective_sms() && V / (2 * c) >= 4096) c *= 2;
-  return c;
-}
-
 // Value and gradient at once: blocks a row, and vectors that a thread keeps. 16 (64 KB a block) let three
 // blocks share an SM, so that one's copies run under another's arithmetic.
 struct HoldPlan {
@@ -480,24 +465,9 @@ HoldPlan hold_plan(const Logits& x) {
   return {c, (int)d, d <= 48};
 }
 
-// Lets a kernel have more than 48 KB of shared memory.
-template <typename K>
-void allow_smem(K* kernel, int bytes) {
-  if (bytes > (32 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
-}
-
 }  // namespace
 
 namespace me {
-
-#define ME_CAP_DISPATCH(CAP, ...)        \
-  if ((CAP) > 0.f) {                     \
-    constexpr bool kCap = true;          \
-    __VA_ARGS__;                         \
-  } else {                               \
-    constexpr bool kCap = false;         \
-    __VA_ARGS__;                         \
-  }
 
 void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, float2* stats, cudaStream_t stream) {
   const int ranks = ranks_for(x.N, x.V);

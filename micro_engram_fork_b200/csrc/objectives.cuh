@@ -482,9 +482,13 @@ ME_DEVICE void hold_walk(int count, int depth, const uint4* hold, F&& f) {
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
 // form, since nothing else is rounded then.
-// walk(first, f): how the slice is gone over (stream() or hold_walk()).
-template <typename T, bool kCap, typename Drop, typename Walk>
-ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Walk&& walk) {
+// walk(first, f): how the slice is gone over (stream() or hold_walk()). watch(x, i): sees each of the thread's
+// vectors, in order.
+struct WatchNothing {
+  ME_DEVICE void operator()(uint4, int) const {}
+};
+template <typename T, bool kCap, typename Drop, typename Walk, typename Watch = WatchNothing>
+ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Walk&& walk, Watch&& watch = Watch()) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   MaxSum out;
   const int count = sl.count();
@@ -514,6 +518,7 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
         }
 #pragma unroll
         for (int u = 0; u < kV; ++u) {
+          watch(x[u], i + u);
           const uint32_t out_mask = drop(sl.vec(i + u));
 #pragma unroll
           for (int p = 0; p < kP; ++p) {
@@ -639,6 +644,27 @@ cudaError_t launch_cluster(void (*kernel)(Params...), int64_t grid, int cluster,
   return cudaLaunchKernelEx(&cfg, kernel, Params(args)...);
 }
 
+inline int ilog2(int c) {
+  int l = 0;
+  while (1 << l < c) ++l;
+  return l;
+}
+
+// Blocks a row: enough for two on each SM, while a block keeps two vectors a thread.
+inline int ranks_for(int64_t N, int64_t V, int at_least = 1) {
+  static const int fix = getenv("RNK") ? atoi(getenv("RNK")) : 0;
+  if (fix) return fix;
+  int c = at_least;
+  while (c < 8 && N * c < 2 * objective_sms() && V / (2 * c) >= 4096) c *= 2;
+  return c;
+}
+
+// Lets a kernel have more than 48 KB of shared memory.
+template <typename K>
+void allow_smem(K* kernel, int bytes) {
+  if (bytes > (32 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+}
+
 template <typename T>
 Rows<const T> rows_in(const Logits& x) {
   return {static_cast<const T*>(x.data), x.stride};
@@ -658,6 +684,15 @@ Rows<T> rows_out(const Gradient& g) {
   } else {                                 \
     using T = float;                       \
     __VA_ARGS__;                           \
+  }
+
+#define ME_CAP_DISPATCH(CAP, ...)        \
+  if ((CAP) > 0.f) {                     \
+    constexpr bool kCap = true;          \
+    __VA_ARGS__;                         \
+  } else {                               \
+    constexpr bool kCap = false;         \
+    __VA_ARGS__;                         \
   }
 
 }  // namespace me

@@ -309,7 +309,10 @@ def test_offsets_past_32_bits():
     values, at, lse = O.top_logits(x, 3)
     logp = O.token_logprobs(x, t)
     tail = x[-9:].clone()
-    assert all(torch.equal(a[-9:], b) for a, b in zip((values, at, lse), O.top_logits(tail, 3)))
+    few = O.top_logits(tail, 3)
+    assert torch.equal(values[-9:], few[0]) and torch.equal(at[-9:], few[1])
+    # (sums: a row of a small batch is split over more blocks, in another order)
+    assert torch.allclose(lse[-9:], few[2], rtol=1e-6, atol=1e-6)
     assert torch.allclose(logp[-9:], O.token_logprobs(tail, t[-9:]), rtol=1e-6, atol=1e-6)
     loss, dx = O.distill_loss_grad(x, ids, top, softcap=30.0, out=x)
     loss2, dx2 = O.distill_loss_grad(tail, ids[-9:], top[-9:], softcap=30.0)
