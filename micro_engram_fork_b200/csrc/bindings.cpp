@@ -75,24 +75,22 @@ std::vector<torch::Tensor> ce_fwd(torch::Tensor z, torch::Tensor labels, int64_t
 void ce_bwd_inplace(torch::Tensor z, torch::Tensor labels, int64_t start, double softcap, torch::Tensor lse,
                     torch::Tensor w_row);
 // objectives_torch.cpp (objectives.cu, top_logits.cu, preference.cu)
-std::vector<torch::Tensor> token_logprobs_fwd(torch::Tensor x, torch::Tensor target, double cap);
-torch::Tensor token_logprobs_bwd(torch::Tensor x, torch::Tensor target, double cap, torch::Tensor stats,
-                                 torch::Tensor g, c10::optional<torch::Tensor> out);
-std::vector<torch::Tensor> distill_fwd(torch::Tensor x, torch::Tensor ids, torch::Tensor top,
-                                       c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> weight,
-                                       double cap, double temp);
-torch::Tensor distill_bwd(torch::Tensor x, torch::Tensor rows, c10::optional<torch::Tensor> weight, double cap,
-                          double temp, torch::Tensor stats, torch::Tensor g, c10::optional<torch::Tensor> out);
+torch::Tensor token_logprobs(torch::Tensor x, torch::Tensor target, c10::optional<double> cap);
+torch::Tensor distill_loss(torch::Tensor x, torch::Tensor ids, torch::Tensor top, c10::optional<torch::Tensor> lse,
+                           c10::optional<torch::Tensor> weight, c10::optional<double> cap, double temp);
 std::vector<torch::Tensor> distill_grad(torch::Tensor x, torch::Tensor ids, torch::Tensor top,
                                         c10::optional<torch::Tensor> lse, c10::optional<torch::Tensor> weight,
-                                        double cap, double temp, c10::optional<torch::Tensor> out);
-std::vector<torch::Tensor> top_logits(torch::Tensor x, int64_t k, double cap, double temp);
+                                        c10::optional<double> cap, double temp, c10::optional<torch::Tensor> out);
+std::vector<torch::Tensor> top_logits(torch::Tensor x, int64_t k, c10::optional<double> cap, double temp);
+std::vector<torch::Tensor> preference_loss(torch::Tensor logp, c10::optional<torch::Tensor> ref, torch::Tensor cu,
+                                           int64_t kind, double beta, double smooth);
 std::vector<torch::Tensor> preference_pairs(torch::Tensor logp, c10::optional<torch::Tensor> ref, torch::Tensor cu,
-                                            int64_t kind, double beta, double smooth, double scale,
+                                            int64_t kind, double beta, double smooth, c10::optional<double> scale,
                                             c10::optional<torch::Tensor> target);
 std::vector<torch::Tensor> preference_logits(torch::Tensor x, torch::Tensor target, c10::optional<torch::Tensor> ref,
-                                             torch::Tensor cu, int64_t kind, double beta, double smooth, double scale,
-                                             double cap, c10::optional<torch::Tensor> out);
+                                             torch::Tensor cu, int64_t kind, double beta, double smooth,
+                                             c10::optional<double> scale, c10::optional<double> cap,
+                                             c10::optional<torch::Tensor> out);
 // attention.cu
 std::vector<torch::Tensor> attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor doc_start,
                                     int64_t window, double scale);
@@ -175,12 +173,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("geglu_bwd", &geglu_bwd);
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd_inplace", &ce_bwd_inplace);
-  m.def("token_logprobs_fwd", &token_logprobs_fwd);
-  m.def("token_logprobs_bwd", &token_logprobs_bwd);
-  m.def("distill_fwd", &distill_fwd);
-  m.def("distill_bwd", &distill_bwd);
+  m.def("token_logprobs", &token_logprobs);
+  m.def("distill_loss", &distill_loss);
   m.def("distill_grad", &distill_grad);
   m.def("top_logits", &top_logits);
+  m.def("preference_loss", &preference_loss);
   m.def("preference_pairs", &preference_pairs);
   m.def("preference_logits", &preference_logits);
   m.def("attn_fwd", &attn_fwd);

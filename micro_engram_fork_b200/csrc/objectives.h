@@ -62,5 +62,8 @@ struct PairArgs {
   float beta, smooth, scale;
 };
 void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* grad, cudaStream_t stream);
+// out_t = grad_t * g of the token's pair
+void launch_preference_scale(const float* grad, const float* g, const void* cu, bool cu64, int64_t tokens, int64_t pairs,
+                             float* out, cudaStream_t stream);
 
 }  // namespace me

@@ -19,16 +19,14 @@ constexpr int kPairThreads = 512;
 // log(1 + e^v) without overflow
 ME_DEVICE float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
 
-// Offsets are read as their running maximum, clamped to [0, T]: every token lies in one sequence, or
-// ahead of the first or after the last one (those get no gradient), whatever `cu` holds.
+// A pair's offsets [a, b) and [b, c): `cu` is read as its running maximum, clamped to [0, T], so every token lies
+// in one sequence, or ahead of the first or after the last one (those get no gradient), whatever it holds.
+struct Bounds {
+  int64_t a, b, c;
+};
 template <typename I>
-__global__ void __launch_bounds__(kPairThreads) preference_kernel(
-    const float* __restrict__ logp, const float* __restrict__ ref, const int64_t* __restrict__ target, int64_t T,
-    const I* __restrict__ cu, int64_t pairs, int kind, float beta, float smooth, float scale,
-    float* __restrict__ loss, float2* __restrict__ rewards, float* __restrict__ grad) {
-  __shared__ float scratch[64];
+ME_DEVICE Bounds pair_bounds(const I* cu, int64_t p, int64_t T) {
   __shared__ long long bound[4];  // the running maximum ahead of this pair, its three offsets
-  const int64_t p = blockIdx.x;
   long long top = 0;
   for (int64_t i = threadIdx.x; i < 2 * p; i += blockDim.x) top = max(top, (long long)cu[i]);
   if (threadIdx.x < 4) bound[threadIdx.x] = 0;
@@ -43,7 +41,33 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(
     }
   }
   __syncthreads();
-  const int64_t a = bound[1], b = bound[2], c = bound[3];
+  return {bound[1], bound[2], bound[3]};
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kPairThreads) preference_scale_kernel(const float* __restrict__ grad,
+                                                                        const float* __restrict__ g,
+                                                                        const I* __restrict__ cu, int64_t T,
+                                                                        int64_t pairs, float* __restrict__ out) {
+  const int64_t p = blockIdx.x;
+  const Bounds s = pair_bounds(cu, p, T);
+  const float c = g[p];
+  for (int64_t t = s.a + threadIdx.x; t < s.c; t += blockDim.x) out[t] = grad[t] * c;
+  if (p == 0)
+    for (int64_t t = threadIdx.x; t < s.a; t += blockDim.x) out[t] = 0.f;
+  if (p == pairs - 1)
+    for (int64_t t = s.c + threadIdx.x; t < T; t += blockDim.x) out[t] = 0.f;
+}
+
+template <typename I>
+__global__ void __launch_bounds__(kPairThreads) preference_kernel(
+    const float* __restrict__ logp, const float* __restrict__ ref, const int64_t* __restrict__ target, int64_t T,
+    const I* __restrict__ cu, int64_t pairs, int kind, float beta, float smooth, float scale,
+    float* __restrict__ loss, float2* __restrict__ rewards, float* __restrict__ grad) {
+  __shared__ float scratch[64];
+  const int64_t p = blockIdx.x;
+  const Bounds s = pair_bounds(cu, p, T);
+  const int64_t a = s.a, b = s.b, c = s.c;
   auto ratio = [&](int64_t t) {
     if (target && target[t] == kIgnoreToken) return 0.f;
     return logp[t] - (ref ? ref[t] : 0.f);
@@ -89,6 +113,15 @@ void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* g
   };
   if (a.cu64) launch(static_cast<const int64_t*>(a.cu));
   else launch(static_cast<const int*>(a.cu));
+}
+
+void launch_preference_scale(const float* grad, const float* g, const void* cu, bool cu64, int64_t tokens, int64_t pairs,
+                             float* out, cudaStream_t stream) {
+  auto launch = [&](auto* offsets) {
+    preference_scale_kernel<<<(unsigned)pairs, kPairThreads, 0, stream>>>(grad, g, offsets, tokens, pairs, out);
+  };
+  if (cu64) launch(static_cast<const int64_t*>(cu));
+  else launch(static_cast<const int*>(cu));
 }
 
 }  // namespace me

@@ -37,6 +37,18 @@ KINDS = ("sigmoid", "hinge", "ipo")
 
 
 # ------------------------------------------------------------------------- argument checks
+# (of the plain forms; the kernels' entry points check the same in C++, where it costs a call next to nothing)
+def _kernel(name, *args):
+    """A kernel's entry point; its complaints about an argument's value are ValueErrors."""
+    try:
+        return getattr(native(), name)(*args)
+    except RuntimeError as e:
+        head, mark, text = str(e).partition("value: ")
+        if head or not mark:
+            raise
+        raise ValueError(text.split("\nException raised from", 1)[0]) from None
+
+
 def _cap(softcap):
     cap = 0.0 if softcap is None else float(softcap)
     if not 0.0 <= cap < float("inf"):
@@ -97,19 +109,22 @@ def _teacher(ids, logits, lead):
     return ids.reshape(-1, ids.shape[-1]), logits.reshape(-1, ids.shape[-1])
 
 
-def _pair_args(cu_seqlens, beta, label_smoothing, kind):
+def _pair_args(beta, label_smoothing, kind):
     if kind not in KINDS:
         raise ValueError(f"kind: one of {', '.join(KINDS)}, got {kind!r}")
-    if not 0.0 < float(beta) < float("inf"):
+    if not 0.0 < beta < float("inf"):
         raise ValueError(f"beta: a positive number, got {beta}")
-    if not 0.0 <= float(label_smoothing) <= 0.5 or (label_smoothing and kind != "sigmoid"):
+    if not 0.0 <= label_smoothing <= 0.5 or (label_smoothing and kind != "sigmoid"):
         raise ValueError(f"label_smoothing: 0 to 0.5, of the sigmoid loss only, got {label_smoothing} with {kind}")
+    return KINDS.index(kind), float(beta), float(label_smoothing)
+
+
+def _check_offsets(cu_seqlens):
     if cu_seqlens.dim() != 1 or cu_seqlens.numel() % 2 != 1:
         raise ValueError("cu_seqlens: offsets [2 pairs + 1] of packed sequences (chosen, rejected, chosen, ...) are "
                          f"needed, got shape {tuple(cu_seqlens.shape)}")
     if cu_seqlens.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"cu_seqlens: int64 or int32 is needed, got {cu_seqlens.dtype}")
-    return KINDS.index(kind), float(beta), float(label_smoothing)
 
 
 # ------------------------------------------------------------------------- plain PyTorch forms
@@ -218,85 +233,74 @@ def preference_ref(logps, ref_logps, cu_seqlens, kind=0, beta=0.1, smooth=0.0, s
 
 
 # ------------------------------------------------------------------------- teacher's top logits
-@torch.no_grad()
 def top_logits(logits, k, softcap=None, temperature=1.0):
     """The k largest logits of each row, after the softcap, in descending order (equal logits by the
     lower id; NaN above +inf): (values [..., k] fp32, ids [..., k] int64, lse [...] fp32), lse the
     log-sum-exp of the whole row at `temperature`, which distill_loss takes as teacher_lse. k is at
     most 256. No gradient."""
+    if logits.dim() != 2:
+        lead = logits.shape[:-1]
+        values, ids, lse = top_logits(_rows(logits), k, softcap, temperature)
+        return values.view(*lead, k), ids.view(*lead, k), lse.view(lead)
+    if use_native(logits):
+        return tuple(_kernel("top_logits", logits, k, softcap, temperature))
     x, cap, temperature = _rows(logits), _cap(softcap), _temperature(temperature)
-    k, lead = int(k), logits.shape[:-1]
     if not 1 <= k <= min(x.shape[1], MAX_TOP):
         raise ValueError(f"k: 1 to {min(x.shape[1], MAX_TOP)}, got {k}")
-    f = native().top_logits if use_native(x) else top_logits_ref
-    values, ids, lse = f(x, k, cap, temperature)
-    return values.view(*lead, k), ids.view(*lead, k), lse.view(lead)
+    with torch.no_grad():
+        return top_logits_ref(x, k, cap, temperature)
 
 
 # ------------------------------------------------------------------------- token log-probabilities
-class _TokenLogprobs(torch.autograd.Function):
+class _TokenLogprobsRef(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, targets, cap):
         ctx.cap = cap
-        ctx.native = use_native(x)
-        if ctx.native:
-            logp, stats = native().token_logprobs_fwd(x, targets, cap)
-            ctx.save_for_backward(x, targets, stats)
-        else:
-            logp, _ = token_logprobs_ref(x, targets, cap)
-            ctx.save_for_backward(x, targets)
-        return logp
+        ctx.save_for_backward(x, targets)
+        return token_logprobs_ref(x, targets, cap)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        if ctx.native:
-            x, targets, stats = ctx.saved_tensors
-            return native().token_logprobs_bwd(x, targets, ctx.cap, stats, g, None), None, None
         x, targets = ctx.saved_tensors
         return token_logprobs_ref(x, targets, ctx.cap)[1](g), None, None
 
 
 def token_logprobs(logits, targets, softcap=None):
     """log softmax(z)[target] of each row, fp32 [...]; targets [...] with -100 untrained (0)."""
-    x, cap = _rows(logits), _cap(softcap)
-    t = _targets(targets, logits.shape[:-1])
-    return _TokenLogprobs.apply(x, t, cap).view(logits.shape[:-1])
+    if logits.dim() != 2:
+        lead = logits.shape[:-1]
+        return token_logprobs(_rows(logits), _per_row(targets, lead, "targets"), softcap).view(lead)
+    if use_native(logits):
+        return _kernel("token_logprobs", logits, targets, softcap)
+    return _TokenLogprobsRef.apply(_rows(logits), _targets(targets, logits.shape[:1]), _cap(softcap))
 
 
 # ------------------------------------------------------------------------- distillation
-class _Distill(torch.autograd.Function):
+class _DistillRef(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, ids, top, lse, weights, cap, temperature):
         ctx.args = cap, temperature
-        ctx.native = use_native(x)
-        if ctx.native:
-            loss, stats, rows = native().distill_fwd(x, ids, top, lse, weights, cap, temperature)
-            ctx.save_for_backward(x, weights, stats, rows)
-        else:
-            loss = distill_ref(x, ids, top, lse, weights, cap, temperature)[0]
-            ctx.save_for_backward(x, ids, top, lse, weights)
-        return loss
+        ctx.save_for_backward(x, ids, top, lse, weights)
+        return distill_ref(x, ids, top, lse, weights, cap, temperature)[0]
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        cap, temperature = ctx.args
-        if ctx.native:
-            x, weights, stats, rows = ctx.saved_tensors
-            dx = native().distill_bwd(x, rows, weights, cap, temperature, stats, g, None)
-        else:
-            x, ids, top, lse, weights = ctx.saved_tensors
-            w = g if weights is None else torch.where(weights != 0, weights * g, 0.0)
-            dx = distill_ref(x, ids, top, lse, w, cap, temperature)[1]
-        return dx, None, None, None, None, None, None
+        x, ids, top, lse, weights = ctx.saved_tensors
+        w = g if weights is None else torch.where(weights != 0, weights * g, 0.0)
+        return distill_ref(x, ids, top, lse, w, *ctx.args)[1], None, None, None, None, None, None
 
 
-def _distill_args(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature):
-    x, lead = _rows(logits), logits.shape[:-1]
-    ids, top = _teacher(teacher_ids, teacher_logits, lead)
-    return (x, ids, top, _per_row(teacher_lse, lead, "teacher_lse"), _per_row(weights, lead, "weights"), _cap(softcap),
-            _temperature(temperature))
+def _flat_teacher(logits, ids, top, lse, weights):
+    """The arguments of logits with other than two dimensions, by rows."""
+    lead = logits.shape[:-1]
+    ids, top = _teacher(ids, top, lead)
+    return _rows(logits), ids, top, _per_row(lse, lead, "teacher_lse"), _per_row(weights, lead, "weights")
+
+
+def _checked_teacher(logits, ids, top, lse, weights, softcap, temperature):
+    return (*_flat_teacher(logits, ids, top, lse, weights), _cap(softcap), _temperature(temperature))
 
 
 def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None, softcap=None, temperature=1.0):
@@ -306,31 +310,39 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
     k at most 256. Without teacher_lse the teacher's distribution is the softmax of its entries; with
     teacher_lse [...] (top_logits' lse at the same temperature) the entries keep their probabilities
     and all other tokens together form one more class. The gradient goes to `logits` alone."""
-    args = _distill_args(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
-    return _Distill.apply(*args).view(logits.shape[:-1])
+    if logits.dim() != 2:
+        flat = _flat_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights)
+        return distill_loss(*flat, softcap, temperature).view(logits.shape[:-1])
+    if use_native(logits):
+        return _kernel("distill_loss", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
+    return _DistillRef.apply(*_checked_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap,
+                                               temperature))
 
 
-@torch.no_grad()
 def distill_loss_grad(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None, softcap=None,
                       temperature=1.0, out=None):
     """(distill_loss [...], gradient of its sum [..., V]) in one call. `out` takes the gradient; it may
     be `logits` itself, and must not overlap it otherwise."""
-    args = _distill_args(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
-    o = _out_rows(out, logits)
-    if use_native(args[0]):
-        loss, dx = native().distill_grad(*args, o)
-    else:
+    if logits.dim() != 2:
+        flat = _flat_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights)
+        loss, dx = distill_loss_grad(*flat, softcap, temperature, _out_rows(out, logits))
+        return loss.view(logits.shape[:-1]), dx.view(logits.shape) if out is None else out
+    if use_native(logits):
+        loss, dx = _kernel("distill_grad", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature,
+                                         out)
+        return loss, dx if out is None else out
+    args = _checked_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
+    _out_rows(out, logits)
+    with torch.no_grad():
         loss, dx = distill_ref(*args)
-        dx = dx if o is None else o.copy_(dx)
-    return loss.view(logits.shape[:-1]), dx.view(logits.shape) if out is None else out
+        return loss, dx if out is None else out.copy_(dx)
 
 
 # ------------------------------------------------------------------------- preference pairs
-class _Preference(torch.autograd.Function):
+class _PreferenceRef(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logps, ref, cu, kind, beta, smooth):
-        f = native().preference_pairs if use_native(logps) else preference_ref
-        loss, rewards, grad = f(logps, ref, cu, kind, beta, smooth, 1.0, None)
+        loss, rewards, grad = preference_ref(logps, ref, cu, kind, beta, smooth)
         ctx.save_for_backward(grad, cu)
         ctx.dtype = logps.dtype
         ctx.mark_non_differentiable(rewards)
@@ -360,42 +372,50 @@ def preference_loss(logps, ref_logps, cu_seqlens, beta=0.1, label_smoothing=0.0,
     offsets, chosen and rejected in turn, non-decreasing from 0 to T at most; an empty sequence sums to 0.
     rewards: beta times each sequence's summed log ratio (chosen, rejected), without a gradient.
     kind: "sigmoid" (with label_smoothing, the share of wrong labels), "hinge" or "ipo"."""
+    kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
+    if use_native(logps):
+        return tuple(_kernel("preference_loss", logps, ref_logps, cu_seqlens, kind, beta, smooth))
     _check_tokens(logps, ref_logps)
-    kind, beta, smooth = _pair_args(cu_seqlens, beta, label_smoothing, kind)
-    return _Preference.apply(logps, ref_logps, cu_seqlens, kind, beta, smooth)
+    _check_offsets(cu_seqlens)
+    return _PreferenceRef.apply(logps, ref_logps, cu_seqlens, kind, beta, smooth)
 
 
-@torch.no_grad()
+def _mean_scale(scale, cu_seqlens):
+    return 1.0 / max(1, cu_seqlens.numel() // 2) if scale is None else float(scale)
+
+
 def preference_loss_grad(logps, ref_logps, cu_seqlens, beta=0.1, label_smoothing=0.0, kind="sigmoid", scale=None):
     """(loss [P], rewards [P, 2], scale * gradient of sum(loss) in logps [T]); scale None is 1 / P, the
     mean over the pairs."""
+    kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
+    if use_native(logps):
+        return tuple(_kernel("preference_pairs", logps, ref_logps, cu_seqlens, kind, beta, smooth, scale, None))
     _check_tokens(logps, ref_logps)
-    kind, beta, smooth = _pair_args(cu_seqlens, beta, label_smoothing, kind)
-    scale = 1.0 / max(1, cu_seqlens.numel() // 2) if scale is None else float(scale)
-    f = native().preference_pairs if use_native(logps) else preference_ref
-    return tuple(f(logps, ref_logps, cu_seqlens, kind, beta, smooth, scale, None))
+    _check_offsets(cu_seqlens)
+    with torch.no_grad():
+        return preference_ref(logps, ref_logps, cu_seqlens, kind, beta, smooth, _mean_scale(scale, cu_seqlens))
 
 
-@torch.no_grad()
 def preference_logits_grad(logits, targets, ref_logps, cu_seqlens, beta=0.1, label_smoothing=0.0, kind="sigmoid",
                            scale=None, softcap=None, out=None):
     """From the logits [T, V] of packed sequences (see preference_loss) and their targets [T] (-100
     untrained, the reference's value there is not read) to (loss [P], rewards [P, 2], logps [T],
     scale * gradient of sum(loss) in the logits [T, V]). `out` as in distill_loss_grad."""
+    kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
+    if use_native(logits):
+        loss, rewards, logps, dx = _kernel("preference_logits", logits, targets, ref_logps, cu_seqlens, kind, beta, smooth,
+                                                              scale, softcap, out)
+        return loss, rewards, logps, dx if out is None else out
     if logits.dim() != 2:
         raise ValueError(f"logits [tokens, V] are needed, got shape {tuple(logits.shape)}")
     x, cap = _rows(logits), _cap(softcap)
     t = _targets(targets, x.shape[:1])
     _per_row(ref_logps, x.shape[:1], "ref_logps")
-    o = _out_rows(out, logits)
-    kind, beta, smooth = _pair_args(cu_seqlens, beta, label_smoothing, kind)
-    scale = 1.0 / max(1, cu_seqlens.numel() // 2) if scale is None else float(scale)
-    if use_native(x):
-        loss, rewards, logps, dx = native().preference_logits(x, t, ref_logps, cu_seqlens, kind, beta, smooth, scale,
-                                                              cap, o)
-    else:
+    _out_rows(out, logits)
+    _check_offsets(cu_seqlens)
+    with torch.no_grad():
         logps, grad = token_logprobs_ref(x, t, cap)
-        loss, rewards, g = preference_ref(logps, ref_logps, cu_seqlens, kind, beta, smooth, scale, t)
+        loss, rewards, g = preference_ref(logps, ref_logps, cu_seqlens, kind, beta, smooth,
+                                          _mean_scale(scale, cu_seqlens), t)
         dx = grad(g)
-        dx = dx if o is None else o.copy_(dx)
-    return loss, rewards, logps, dx
+        return loss, rewards, logps, dx if out is None else out.copy_(dx)
