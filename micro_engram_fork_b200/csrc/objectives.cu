@@ -23,13 +23,14 @@ namespace {
 // ------------------------------------------------------------------------------------ gradient of a slice
 // out_j = coef exp(y_j - m) z'_j for the block's columns, in 16-byte stores where the two rows are
 // aligned alike.
-template <typename T, bool kCap, typename Walk>
-ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Walk&& walk) {
+template <typename T, bool kCap, bool kAligned>
+ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
-  const bool aligned = (reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0;
   // coef (1 - (z / c)^2) is one FMA with the coefficient inside
-  const float coef_slope = coef * sc.slope;
-  walk(
+  const float coef_slope = coef * sc.slope, k = sc.inv_temp * kLog2e, shift = m * kLog2e;
+  T* mine = out + sl.column(sl.vec(0));
+  stream(
+      sl.mine(), sl.count(), ring, [](int, auto&) {},
       [&](const auto& x, int i, auto whole) {
         constexpr int kV = sizeof(x) / sizeof(uint4);
         f32x2 z[kV][kP];
@@ -44,21 +45,28 @@ ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m,
 #pragma unroll
           for (int p = 0; p < kP; ++p) {
             const f32x2 zp = z[u][p];
-            const float2 a = unpack2(mul2(fma2(zp, both2(sc.inv_temp), both2(-m)), both2(kLog2e)));
+            // (a 16-bit result is rounded at 2^-9 or 2^-12: the exponent's rounding, 2e-6, may stay)
+            const float2 a = unpack2(sizeof(T) == 4 ? mul2(fma2(zp, both2(sc.inv_temp), both2(-m)), both2(kLog2e))
+                                                    : fma2(zp, both2(k), both2(-shift)));
             const f32x2 e = pack2(exp2_fast(a.x), exp2_fast(a.y));
             z[u][p] = mul2(e, kCap ? fma2(mul2(zp, both2(coef_slope)), zp, both2(coef)) : both2(coef));
           }
           Vec16<T> r;
           r.u = from_pairs<T>(z[u]);
-          const int at = sl.vec(i + u);
-          if (aligned) {
-            reinterpret_cast<uint4*>(out + sl.head)[at] = r.u;
+          T* at = mine + (i + u) * (kThreads * kN);
+          if constexpr (kAligned) {
+            *reinterpret_cast<uint4*>(at) = r.u;
           } else {
 #pragma unroll
-            for (int e = 0; e < kN; ++e) out[sl.column(at) + e] = r.h[e];
+            for (int e = 0; e < kN; ++e) at[e] = r.h[e];
           }
         }
       });
+}
+template <typename T, bool kCap>
+ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
+  if ((reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0) write_vectors<T, kCap, true>(sl, out, sc, m, coef, ring);
+  else write_vectors<T, kCap, false>(sl, out, sc, m, coef, ring);
   const int j = sl.single();
   if (j >= 0) {
     const float z = softcap(to_f<T>(sl.row[j]), sc.cap);
@@ -101,9 +109,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> 
   const Slice<T> sl(x.row(r), V, rank, lg_ranks);
   const float xt = t >= 0 && t < V ? to_f<T>(sl.row[t]) : NAN;
   const MaxSum a = row_merge(
-      slice_sum<T, kCap>(sl, sc, KeepAll(),
-                         [&](auto&& first, auto&& f) { stream(sl.mine(), sl.count(), ring, first, f); }),
-      part, lg_ranks);
+      slice_sum<T, kCap>(sl, sc, KeepAll(), ring), part, lg_ranks);
   if (threadIdx.x == 0 && rank == 0) {
     logp[r] = softcap(xt, sc.cap) - a.m - logf(a.s);
     stats[r] = make_float2(a.m, a.s);
@@ -132,8 +138,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> 
   const float c = valid ? g[r] : NAN;
   const float xt = mine ? to_f<T>(sl.row[t]) : 0.f;
   __syncthreads();  // read before the row may be written in place
-  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y,
-                       [&](auto&& f) { stream(sl.mine(), sl.count(), ring, [](int, auto&) {}, f); });
+  write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y, ring);
   __syncthreads();  // the target's column is written again
   if (mine) {
     const float z = softcap(xt, sc.cap);
@@ -345,17 +350,15 @@ ME_DEVICE void write_entry(const Slice<T>& sl, T* out, const Entry& e, float c, 
   if (e.id >= 0 && sl.holds(e.id)) out[e.id] = from_f<T>(c * (expf(e.y - m) * inv_s * mass - e.q) * e.slope);
 }
 
-// One cluster a row. With kGrad value and gradient: each block keeps its slice of the row in shared
-// memory (`depth` vectors a thread) until the cluster has the row's sum, so a logit is read once from
-// memory. Without, the value and the statistics that the backward pass starts from: m, s (-1: a row
-// without gradient), m', c'.
+// One cluster a row. Value, and the statistics that the backward pass starts from: m, s (-1: a row without
+// gradient), m', c'; or with kGrad value and gradient: the slice is read again once the cluster has the
+// row's sum, from L2 where the rows in flight fit there.
 template <typename T, bool kCap, bool kTail, bool kGrad>
-__global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
-    distill_kernel(Rows<const T> x, Rows<T> out, int V, int lg_ranks, int depth, int k,
-                   const float* __restrict__ weight, float temp, const Entry* __restrict__ entries,
-                   const TeacherRow* __restrict__ rows, Scale sc, float* __restrict__ loss,
-                   float4* __restrict__ stats) {
-  extern __shared__ uint4 dynamic[];  // the slice, or the ring
+__global__ void __launch_bounds__(kThreads, 4)
+    distill_kernel(Rows<const T> x, Rows<T> out, int V, int lg_ranks, int k, const float* __restrict__ weight,
+                   float temp, const Entry* __restrict__ entries, const TeacherRow* __restrict__ rows, Scale sc,
+                   float* __restrict__ loss, float4* __restrict__ stats) {
+  __shared__ Ring ring;
   __shared__ float2 part[kWarps];
   __shared__ uint32_t filter[kTail ? kFilter / 32 : 1];
   __shared__ int ids[kTail ? kMaxTop : 1];
@@ -371,26 +374,9 @@ __global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
     if (kGrad) zero_slice<T>(sl, o);
     return;
   }
-  if (kGrad) hold_issue(sl.mine(), sl.count(), depth, dynamic);
-  const Entry e = kGrad || kTail ? load_entry(entries, r, k) : Entry{};
-  const TeacherRow te = rows[r];
-  auto walk = [&](auto&& first, auto&& f) {
-    if constexpr (kGrad) {
-      // (the reference comes from the first group: at most kFirst vectors of it)
-      copy_wait<kGroups - 1>();
-      uint4 v[kFirst];
-      const int n = min(min(sl.count(), kFirst), hold_group(depth));
-#pragma unroll
-      for (int u = 0; u < kFirst; ++u)
-        if (u < n) v[u] = dynamic[u * kThreads + threadIdx.x];
-      first(n, v);
-      hold_walk<true>(sl.count(), depth, dynamic, f);
-    } else {
-      stream(sl.mine(), sl.count(), *reinterpret_cast<Ring*>(dynamic), first, f);
-    }
-  };
   MaxSum a;
   if constexpr (kTail) {
+    const Entry e = load_entry(entries, r, k);
     for (int i = threadIdx.x; i < kFilter / 32; i += kThreads) filter[i] = 0;
     if (threadIdx.x < k) ids[threadIdx.x] = e.id;
     __syncthreads();
@@ -399,12 +385,12 @@ __global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
       atomicOr(&filter[b >> 5], 1u << (b & 31));
     }
     __syncthreads();
-    a = slice_sum<T, kCap>(sl, sc, DropEntries<T>{filter, ids, k, sl.head}, walk);
+    a = slice_sum<T, kCap>(sl, sc, DropEntries<T>{filter, ids, k, sl.head}, ring);
   } else {
-    a = slice_sum<T, kCap>(sl, sc, KeepAll(), walk);
+    a = slice_sum<T, kCap>(sl, sc, KeepAll(), ring);
   }
-  a = row_merge(a, part, lg_ranks);
-  const Student st = finish_student<kTail>(a, te);
+  const TeacherRow te = rows[r];
+  const Student st = finish_student<kTail>(row_merge(a, part, lg_ranks), te);
   const bool nothing = !kTail && te.any == 0.f;  // no entry: nothing to match
   if (writer) {
     loss[r] = nothing ? 0.f : w * temp * temp * divergence(te, st);
@@ -415,10 +401,9 @@ __global__ void __launch_bounds__(kThreads, kGrad ? 3 : 4)
       zero_slice<T>(sl, o);
     } else {
       const float c = w * temp;
-      write_slice<T, kCap>(sl, o, sc, st.m1, c * st.c1,
-                           [&](auto&& f) { hold_walk<false>(sl.count(), depth, dynamic, f); });
+      write_slice<T, kCap>(sl, o, sc, st.m1, c * st.c1, ring);
       __syncthreads();
-      write_entry<T>(sl, o, e, c, st.all.m, 1.f / st.all.s, te.mass);
+      write_entry<T>(sl, o, load_entry(entries, r, k), c, st.all.m, 1.f / st.all.s, te.mass);
     }
   }
   row_done(lg_ranks);
@@ -440,31 +425,13 @@ __global__ void __launch_bounds__(kThreads, 4)
     return;
   }
   const Entry e = load_entry(entries, r, k);
-  const float c = (weight ? weight[r] : 1.f) * temp * (g ? g[r] : 1.f);
-  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w,
-                       [&](auto&& f) { stream(sl.mine(), sl.count(), ring, [](int, auto&) {}, f); });
+  const float c = (weight ? weight[r] : 1.f) * temp * g[r];
+  write_slice<T, kCap>(sl, o, sc, st.z, c * st.w, ring);
   __syncthreads();
   write_entry<T>(sl, o, e, c, st.x, 1.f / st.y, rows[r].mass);
 }
 
 // ------------------------------------------------------------------------------------ launches
-// Value and gradient at once: blocks a row, and vectors that a thread keeps. 16 (64 KB a block) let three
-// blocks share an SM, so that one's copies run under another's arithmetic.
-struct HoldPlan {
-  int ranks, depth;
-  bool fits;
-};
-HoldPlan hold_plan(const Logits& x) {
-  const int64_t vecs = (x.V * (x.type == LogitType::kF32 ? 4 : 2) + 15) / 16;
-  static const int most = getenv("DPT") ? atoi(getenv("DPT")) : 16;
-  auto depth = [&](int c) { return ((vecs + c - 1) / c + kThreads - 1) / kThreads; };
-  int c = 1;
-  while (c < 8 && depth(c) > most) c *= 2;
-  c = ranks_for(x.N, x.V, c);
-  const int64_t d = depth(c);
-  return {c, (int)d, d <= 48};
-}
-
 }  // namespace
 
 namespace me {
@@ -496,25 +463,21 @@ void launch_distill_fwd(const Logits& x, const TeacherArgs& te, const void* entr
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, false> : distill_kernel<T, kCap, false, false>;
-    launch_cluster(kernel, x.N * ranks, ranks, sizeof(Ring), stream, rows_in<T>(x), Rows<T>{}, x.V, ilog2(ranks), 0, te.k,
-                   te.weight, te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
+    launch_cluster(kernel, x.N * ranks, ranks, 0, stream, rows_in<T>(x), Rows<T>{}, x.V, ilog2(ranks), te.k, te.weight,
+                   te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
                    make_scale(x.cap, te.temp), loss, stats);
   }));
 }
 
-bool launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows, float* loss,
+void launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows, float* loss,
                          Gradient out, cudaStream_t stream) {
-  const HoldPlan plan = hold_plan(x);
-  if (!plan.fits) return false;
-  const int smem = plan.depth * kThreads * 16;
+  const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, true> : distill_kernel<T, kCap, false, true>;
-    allow_smem(kernel, smem);
-    launch_cluster(kernel, x.N * plan.ranks, plan.ranks, smem, stream, rows_in<T>(x), rows_out<T>(out), x.V,
-                   ilog2(plan.ranks), plan.depth, te.k, te.weight, te.temp, static_cast<const Entry*>(entries),
-                   static_cast<const TeacherRow*>(rows), make_scale(x.cap, te.temp), loss, (float4*)nullptr);
+    launch_cluster(kernel, x.N * ranks, ranks, 0, stream, rows_in<T>(x), rows_out<T>(out), x.V, ilog2(ranks), te.k,
+                   te.weight, te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
+                   make_scale(x.cap, te.temp), loss, (float4*)nullptr);
   }));
-  return true;
 }
 
 void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows,

@@ -434,44 +434,6 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
   }
 }
 
-// The same vectors, all kept: `hold` has place for each of the block's vectors ([i][thread]), and the
-// slice can be walked again without a second read. Copies are issued in eight groups of two vectors or more.
-constexpr int kGroups = 8;
-ME_DEVICE int hold_group(int depth) { return max(2, (depth + kGroups - 1) / kGroups); }
-ME_DEVICE void hold_issue(const uint4* src, int count, int depth, uint4* hold) {
-  uint4* mine = hold + threadIdx.x;
-  const int group = hold_group(depth);
-#pragma unroll 1
-  for (int g = 0; g < kGroups; ++g) {
-    for (int d = g * group; d < min(count, (g + 1) * group); ++d) copy_async(mine + d * kThreads, src + d * kThreads);
-    copy_commit();
-  }
-}
-// f as in stream(). kWait: the first walk, in which the i-th group is waited for with i empty ones behind it.
-template <bool kWait, typename F>
-ME_DEVICE void hold_walk(int count, int depth, const uint4* hold, F&& f) {
-  const uint4* mine = hold + threadIdx.x;
-  const int whole = __shfl_sync(0xffffffffu, count, 31);
-  const int group = kWait ? hold_group(depth) : depth;
-#pragma unroll 1
-  for (int g = 0; g < (kWait ? kGroups : 1); ++g) {
-    if (kWait) copy_wait<kGroups - 1>();
-    const int end = (g + 1) * group;
-    int i = g * group;
-#pragma unroll 1
-    for (; i + 2 <= min(whole, end); i += 2) {
-      const uint4 v[2] = {mine[i * kThreads], mine[(i + 1) * kThreads]};
-      f(v, i, std::true_type());
-    }
-#pragma unroll 1
-    for (; i < min(count, end); ++i) {
-      const uint4 v[1] = {mine[i * kThreads]};
-      f(v, i, std::false_type());
-    }
-    if (kWait) copy_commit();
-  }
-}
-
 // This thread's share of sum exp(y - m) over a slice. `drop(vec)`: a mask of the vector's elements
 // that are left out (`drop.column(j)` for a single column).
 //
@@ -482,20 +444,20 @@ ME_DEVICE void hold_walk(int count, int depth, const uint4* hold, F&& f) {
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
 // form, since nothing else is rounded then.
-// walk(first, f): how the slice is gone over (stream() or hold_walk()). watch(x, i): sees each of the thread's
-// vectors, in order.
+// watch(x, i): sees each of the thread's vectors, in order.
 struct WatchNothing {
   ME_DEVICE void operator()(uint4, int) const {}
 };
-template <typename T, bool kCap, typename Drop, typename Walk, typename Watch = WatchNothing>
-ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Walk&& walk, Watch&& watch = Watch()) {
+template <typename T, bool kCap, typename Drop, typename Watch = WatchNothing>
+ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Ring& ring, Watch&& watch = Watch()) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   MaxSum out;
   const int count = sl.count();
   float big = -INFINITY, sum0 = 0.f, sum1 = 0.f;
   const float k = sc.inv_temp * kLog2e;
   float ref = 0.f, shift = 0.f;  // the reference; the same, or the rounded ref k
-  walk(
+  stream(
+      sl.mine(), count, ring,
       [&](int n, const uint4(&v)[kFirst]) {
         float top = -INFINITY;
 #pragma unroll

@@ -43,10 +43,10 @@ constexpr int kEntryBytes = 16, kTeacherRowBytes = 32;
 void launch_teacher(const Logits& x, const TeacherArgs& teacher, void* entries, void* rows, cudaStream_t stream);
 void launch_distill_fwd(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows, float* loss,
                         float4* stats, cudaStream_t stream);
-// Value and gradient of sum(loss) in one launch. False: a row is too long for it (take the two others).
-bool launch_distill_grad(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows, float* loss,
+// value and gradient of sum(loss) in one launch
+void launch_distill_grad(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows, float* loss,
                          Gradient out, cudaStream_t stream);
-// g: one coefficient a row, or null for 1
+// g: one coefficient a row
 void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows,
                         const float4* stats, const float* g, Gradient out, cudaStream_t stream);
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,

@@ -72,7 +72,13 @@ Tensor check_whole(const Tensor& t, const Tensor& x, const char* what) {
 }
 
 Tensor gradient_like(const Tensor& x, const OptTensor& out, const char* what) {
-  if (!out.has_value()) return torch::empty(x.sizes(), x.options());
+  if (!out.has_value()) {
+    const auto opts = x.options().requires_grad(false);
+    // rows a little apart (a padded vocabulary): the gradient's too, so that both are aligned alike
+    if (x.size(0) > 1 && x.stride(0) > x.size(1) && x.stride(0) <= x.size(1) + 64)
+      return torch::empty_strided(x.sizes(), {x.stride(0), 1}, opts);
+    return torch::empty(x.sizes(), opts);
+  }
   const Tensor& o = *out;
   ME_CHECK_VALUE(o.sizes() == x.sizes() && o.scalar_type() == x.scalar_type() && o.device() == x.device(), what,
                     ": out has another shape, type or device than the logits");
@@ -210,11 +216,7 @@ std::vector<Tensor> distill_grad(Tensor x, Tensor ids, Tensor top, OptTensor lse
   const auto rows = teacher_rows(x, te.args.k);
   const auto stream = at::cuda::getCurrentCUDAStream();
   me::launch_teacher(in, te.args, rows.entries, rows.rows, stream);
-  if (!me::launch_distill_grad(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), gradient_of(o), stream)) {
-    auto stats = torch::empty({in.N, 4}, loss.options());
-    me::launch_distill_fwd(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), as4(stats), stream);
-    me::launch_distill_bwd(in, te.args, rows.entries, rows.rows, as4(stats), nullptr, gradient_of(o), stream);
-  }
+  me::launch_distill_grad(in, te.args, rows.entries, rows.rows, loss.data_ptr<float>(), gradient_of(o), stream);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {loss, o};
 }

@@ -193,7 +193,7 @@ __global__ void __launch_bounds__(kThreads, 4)
   float best = -INFINITY;
   const int group = 1 << lg_group, count = sl.count();
   MaxSum a = slice_sum<T, kCap>(
-      sl, sc, KeepAll(), [&](auto&& first, auto&& f) { stream(sl.mine(), count, work.ring, first, f); },
+      sl, sc, KeepAll(), work.ring,
       [&](uint4 v, int i) {
         best = fmaxf(best, vec_max<T, false>(v));
         if ((i + 1 & group - 1) == 0) {
