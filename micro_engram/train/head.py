@@ -13,6 +13,10 @@ Each rank keeps row_range(V) of the tied embedding / output head (outside the ba
          token's rows on its owner's GPU; every exchange between ranks goes through peer
          memory (micro_engram_fork_b200/parallel/vocab_comm.py), none through NCCL.
 
+  other  distill / token_logprobs / top_logits: the other objectives over the vocabulary
+         (micro_engram_fork_b200/ops/objectives.py) on the same chunks of logits, for a head that is whole
+         on this GPU (world 1; a head is 1-3 GB, so every rank of a data-parallel run can hold one).
+
 Every rank runs the same chunk count: the chunk size comes from ceil(V/world), never from
 this rank's own row count (micro_engram/train/head.py:38-42 of the reference). Loss terms
 are sums; the trainer divides by the step's trained-token count.
@@ -20,7 +24,7 @@ are sums; the trainer divides by the step's trained-token count.
 import torch
 import torch.distributed as dist
 
-from micro_engram_fork_b200.ops import use_native
+from micro_engram_fork_b200.ops import objectives, use_native
 
 from ..rows import _group, _RowLookup, row_range
 
@@ -121,6 +125,86 @@ class VocabShard:
         else:
             total = _VocabParallelCE.apply(hidden, labels, self)
         return total, count
+
+    # ------------------------------------------------------------------ other objectives
+    def _whole(self, hidden):
+        if self.world != 1:
+            raise ValueError("this objective needs the whole head on one GPU: VocabShard(weight, rank=0, world=1)")
+        if hidden.dim() != 2 or hidden.shape[1] != self.d:
+            raise ValueError(f"hidden states [tokens, {self.d}] are needed, got {tuple(hidden.shape)}")
+        return _chunks(hidden.shape[0], self.chunk_bf16 if use_native(hidden) else self.chunk)
+
+    def _logits(self, hidden):
+        """(raw logits [n, V], the same with the padding columns that the GEMMs want)."""
+        h = hidden.detach().to(self.weight.dtype).contiguous()
+        if use_native(h):
+            from micro_engram_fork_b200 import native
+
+            z = native().gemm(h, self.gemm_weight, True, None)
+            return z[:, :self.rows], z
+        z = h @ self.weight.t()
+        return z, z
+
+    @torch.no_grad()
+    def top_logits(self, hidden, k, temperature=1.0):
+        """(values, ids, lse) of each token's k largest softcapped logits: what this model records as a
+        teacher. hidden [N, d]; see ops.objectives.top_logits."""
+        parts = [objectives.top_logits(self._logits(hidden[a:b])[0], k, self.softcap, temperature)
+                 for a, b in self._whole(hidden)]
+        if not parts:
+            parts = [objectives.top_logits(self._logits(hidden)[0], k, self.softcap, temperature)]
+        return tuple(torch.cat(p) for p in zip(*parts))
+
+    def token_logprobs(self, hidden, labels):
+        """log p(label) of each token, fp32 [N] (0 where the label is -100), differentiable in hidden."""
+        def chunk(z, a, b, out):
+            if out is None:
+                return objectives.token_logprobs(z, labels[a:b], self.softcap)
+            return objectives.token_logprobs_grad(z, labels[a:b], None, self.softcap, out)[0]
+
+        return _HeadObjective.apply(hidden, self, chunk, torch.is_grad_enabled() and hidden.requires_grad)
+
+    def distill(self, hidden, teacher_ids, teacher_logits, teacher_lse=None, weights=None, temperature=1.0):
+        """The weighted divergence from a teacher's top logits of each token, fp32 [N], differentiable in
+        hidden; see ops.objectives.distill_loss."""
+        def chunk(z, a, b, out):
+            args = (z, teacher_ids[a:b], teacher_logits[a:b], None if teacher_lse is None else teacher_lse[a:b],
+                    None if weights is None else weights[a:b], self.softcap, temperature)
+            return objectives.distill_loss(*args) if out is None else objectives.distill_loss_grad(*args, out=out)[0]
+
+        return _HeadObjective.apply(hidden, self, chunk, torch.is_grad_enabled() and hidden.requires_grad)
+
+
+class _HeadObjective(torch.autograd.Function):
+    """Per-token values of an objective over the vocabulary. Per chunk of tokens: the logits GEMM, the
+    objective's kernels (which overwrite the logits with each token's gradient), the dH GEMM. A token's value
+    depends on its own row alone, so the backward pass scales the rows of dH: the logits are computed
+    once and never kept, and a loss over the values (a preference loss over sequences) needs no second
+    pass over the vocabulary."""
+
+    @staticmethod
+    def forward(ctx, hidden, shard, chunk, need_grad):
+        w = shard.gemm_weight
+        values = torch.zeros(hidden.shape[0], dtype=torch.float32, device=hidden.device)
+        dh = torch.empty(hidden.shape[0], shard.d, dtype=torch.float32, device=hidden.device) if need_grad else None
+        for a, b in shard._whole(hidden):
+            z, padded = shard._logits(hidden[a:b])
+            values[a:b] = chunk(z, a, b, z if need_grad else None)
+            if need_grad:
+                if use_native(padded):
+                    from micro_engram_fork_b200 import native
+
+                    dh[a:b] = native().gemm_f32(padded, w)
+                else:
+                    dh[a:b] = (z @ shard.weight).float()
+            del z, padded
+        ctx.dh, ctx.hdtype = dh, hidden.dtype
+        return values
+
+    @staticmethod
+    def backward(ctx, g):
+        dh, ctx.dh = ctx.dh, None
+        return (dh * g.float().unsqueeze(1)).to(ctx.hdtype), None, None, None
 
 
 def _gather(x, group, world):

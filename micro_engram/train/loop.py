@@ -36,6 +36,7 @@ from . import model as M
 from .checkpoint import Checkpoints
 from .data import EpochPlan, collate, prepare
 from .faults import FaultHook
+from .objectives import NextToken
 from .offload import ActivationOffload
 from .report import Reporter, to_host
 
@@ -75,6 +76,7 @@ class Trainer:
     def __init__(self, cfg):
         self.cfg = cfg
         self.rank, self.world, self.local, self.device = setup_dist()
+        self.objective = NextToken()            # what a step minimises (train/objectives.py)
         self.ctx = {"ids": None, "pos": None}   # the micro-batch's ids/positions, read by the engram hooks
         self.global_step = self.epoch = self.step_in_epoch = 0
         self.timers = PhaseTimers(enabled=os.environ.get("MICRO_ENGRAM_PHASE_TIMES") == "1", device=self.device)
@@ -293,10 +295,20 @@ class Trainer:
         batch = collate(self.samples, bins, self.cfg.sequence_len, self.pad_id, pin=self.device.type == "cuda")
         return {k: v.to(self.device, non_blocking=True) for k, v in batch.items()}
 
+    def hidden(self, batch):
+        """Final hidden states [tokens, d] of one micro-batch."""
+        ids, pos = (batch[k].reshape(1, -1) for k in ("input_ids", "position_ids"))  # one row
+        self.ctx["ids"], self.ctx["pos"] = ids, pos
+        try:
+            h = self.text(self.vocab.embed(ids), pos)
+        finally:
+            self.ctx["ids"] = self.ctx["pos"] = None
+        return h.reshape(-1, h.shape[-1])
+
     def forward_loss(self, batch, scale):
-        """Sum of this GPU's token losses of one micro-batch (a device scalar); runs the
-        backward of loss * scale."""
-        ids, pos, labels = (batch[k].reshape(1, -1) for k in ("input_ids", "position_ids", "labels"))  # one row
+        """Sum of this GPU's losses of one micro-batch (a device scalar); runs the backward of
+        loss * scale."""
+        ids, pos = (batch[k].reshape(1, -1) for k in ("input_ids", "position_ids"))  # one row
         self.ctx["ids"], self.ctx["pos"] = ids, pos
         with self.timers.phase("embed"):
             emb = self.vocab.embed(ids)
@@ -305,7 +317,7 @@ class Trainer:
                                                                       self.cfg.no_grad_prefix):
             h = self.text(emb, pos)
         with self.timers.phase("loss"):
-            total, _ = self.vocab.loss_sum(h.reshape(-1, h.shape[-1]), labels.reshape(-1))
+            total = self.objective(self.vocab, h.reshape(-1, h.shape[-1]), batch)
         with self.timers.phase("backward"):
             (total * scale).backward()
         if self.offload:
@@ -320,11 +332,11 @@ class Trainer:
         reads them at logging steps only)."""
         if batches is None:
             batches = [self._micro_batch(b) for b in micro]
-        tokens = torch.stack([(b["labels"] != -100).sum() for b in batches]).sum()
+        tokens = torch.stack([self.objective.terms(b) for b in batches]).sum()
         if self.world > 1:
             dist.all_reduce(tokens)
         count = tokens.clamp_min(1).float()
-        scale = self.world / count   # per-token mean over every micro-batch and rank (loss * world / N)
+        scale = self.world / count   # mean over every micro-batch's and rank's terms (trained tokens; loss * world / N)
         loss = torch.zeros((), device=self.device)
         for b in batches:
             loss += self.forward_loss(b, scale)

@@ -76,6 +76,8 @@ void ce_bwd_inplace(torch::Tensor z, torch::Tensor labels, int64_t start, double
                     torch::Tensor w_row);
 // objectives_torch.cpp (objectives.cu, top_logits.cu, preference.cu)
 torch::Tensor token_logprobs(torch::Tensor x, torch::Tensor target, c10::optional<double> cap);
+std::vector<torch::Tensor> token_logprobs_grad(torch::Tensor x, torch::Tensor target, c10::optional<torch::Tensor> coef,
+                                               c10::optional<double> cap, c10::optional<torch::Tensor> out);
 torch::Tensor distill_loss(torch::Tensor x, torch::Tensor ids, torch::Tensor top, c10::optional<torch::Tensor> lse,
                            c10::optional<torch::Tensor> weight, c10::optional<double> cap, double temp);
 std::vector<torch::Tensor> distill_grad(torch::Tensor x, torch::Tensor ids, torch::Tensor top,
@@ -174,6 +176,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("ce_fwd", &ce_fwd);
   m.def("ce_bwd_inplace", &ce_bwd_inplace);
   m.def("token_logprobs", &token_logprobs);
+  m.def("token_logprobs_grad", &token_logprobs_grad);
   m.def("distill_loss", &distill_loss);
   m.def("distill_grad", &distill_grad);
   m.def("top_logits", &top_logits);

@@ -151,6 +151,15 @@ Tensor token_logprobs_bwd(Tensor x, Tensor target, OptDouble cap, Tensor stats, 
   return o;
 }
 
+// (logp [N], gradient of sum(coef * logp) in the logits [N, V]); coef: 1 unless given
+std::vector<Tensor> token_logprobs_grad(Tensor x, Tensor target, OptTensor coef, OptDouble cap, OptTensor out) {
+  auto t = check_whole(target, x, "targets");
+  Tensor g = coef.has_value() ? check_rows(*coef, x, torch::kFloat32, "coefficients")
+                              : torch::ones({x.size(0)}, x.options().dtype(torch::kFloat32).requires_grad(false));
+  auto f = token_logprobs_fwd(x, t, cap);
+  return {f[0], token_logprobs_bwd(x, t, cap, f[1], g, out)};
+}
+
 namespace {
 // The kernels' view of the teacher's rows: k entries of 4 and one of 8 floats a row.
 struct TeacherRows {

@@ -9,6 +9,7 @@ z = c tanh(x / c) itself. Gradients are those in the raw logits, in their type, 
   distill_loss            weighted KL(teacher || student) of each token (autograd)
   distill_loss_grad       the same with its gradient in one call, optionally in place of the logits
   token_logprobs          log softmax(z)[target] of each token (autograd)
+  token_logprobs_grad     the same with its gradient for given coefficients in one call
   preference_loss         paired log-ratio loss of packed chosen / rejected sequences, on token
                           log-probabilities (autograd)
   preference_loss_grad    the same with its gradient in the log-probabilities in one call
@@ -274,6 +275,26 @@ def token_logprobs(logits, targets, softcap=None):
     if use_native(logits):
         return _kernel("token_logprobs", logits, targets, softcap)
     return _TokenLogprobsRef.apply(_rows(logits), _targets(targets, logits.shape[:1]), _cap(softcap))
+
+
+def token_logprobs_grad(logits, targets, coefficients=None, softcap=None, out=None):
+    """(token_logprobs [...], gradient of sum(coefficients * token_logprobs) [..., V]) in one call;
+    coefficients [...] are 1 unless given. `out` as in distill_loss_grad."""
+    if logits.dim() != 2:
+        lead = logits.shape[:-1]
+        logp, dx = token_logprobs_grad(_rows(logits), _per_row(targets, lead, "targets"),
+                                       _per_row(coefficients, lead, "coefficients"), softcap, _out_rows(out, logits))
+        return logp.view(lead), dx.view(logits.shape) if out is None else out
+    if use_native(logits):
+        logp, dx = _kernel("token_logprobs_grad", logits, targets, coefficients, softcap, out)
+        return logp, dx if out is None else out
+    x, lead = _rows(logits), logits.shape[:1]
+    t, g = _targets(targets, lead), _per_row(coefficients, lead, "coefficients")
+    _out_rows(out, logits)
+    with torch.no_grad():
+        logp, grad = token_logprobs_ref(x, t, _cap(softcap))
+        dx = grad(torch.ones_like(logp) if g is None else g)
+        return logp, dx if out is None else out.copy_(dx)
 
 
 # ------------------------------------------------------------------------- distillation

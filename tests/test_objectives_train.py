@@ -1,0 +1,103 @@
+"""The objectives in the trainer and its head: per-token values and their gradients in the hidden states
+against the objectives on the whole logits, the refusal of a split head, and the example (distillation and
+preference training of a small random base), on CPU tensors and on the sm_100a kernels."""
+import os
+import sys
+
+import pytest
+import torch
+
+import objective_oracle as oracle
+from micro_engram_fork_b200.ops import objectives as O
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+DEVICES = ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)]
+
+
+def _shard(dev, V=1003, d=64, chunk=16, softcap=30.0):
+    from micro_engram.train.head import VocabShard
+
+    torch.manual_seed(0)
+    W = (torch.randn(V, d) * 0.3).to(torch.bfloat16)
+    return VocabShard(W, 0, 1, softcap=softcap, chunk_tokens=chunk, device=dev), W.to(dev)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_head(dev):
+    """Chunks of 16 tokens (the last one short), a vocabulary that is padded for the GEMMs."""
+    shard, W = _shard(dev)
+    N, k = 53, 12
+    h = torch.randn(N, 64, device=dev).to(torch.bfloat16)
+    z = (h @ W.t()).detach()  # the same bf16 logits up to one rounding
+    z64 = oracle.z64(z, 30.0)
+    values, ids, lse = shard.top_logits(h, k, temperature=1.5)
+    want = z64.topk(k, dim=1)[0]
+    # a bf16 logit of up to 32 is rounded at 2^-4: the two products may differ by a unit
+    assert torch.allclose(values.double(), want, atol=0.13) and values.shape == ids.shape == (N, k)
+    assert torch.allclose(lse.double(), torch.logsumexp(z64 / 1.5, 1), atol=0.02)
+    assert ids.max() < W.shape[0]
+
+    labels = torch.randint(0, W.shape[0], (N,), device=dev)
+    labels[::5] = -100
+    coef = torch.randn(N, device=dev)
+    w = torch.rand(N, device=dev)
+    w[3] = 0.0
+    teacher = torch.randn(N, k, device=dev) * 3
+    t_lse = torch.logsumexp(teacher, 1) + 0.2
+    h64 = h.double().requires_grad_()
+    x64 = h64 @ W.double().t()
+    cases = {
+        "logprobs": (lambda v: shard.token_logprobs(v, labels), O.token_logprobs_ref(x64.detach(), labels, 30.0)[0],
+                     O.token_logprobs_ref(x64.detach(), labels, 30.0)[1](coef.double())),
+        "distill": (lambda v: shard.distill(v, ids, teacher, t_lse, w, 1.5),
+                    O.distill_ref(x64.detach(), ids, teacher.double(), t_lse, w, 30.0, 1.5)[0],
+                    O.distill_ref(x64.detach(), ids, teacher.double(), t_lse, w, 30.0, 1.5)[1] * coef.double()[:, None]),
+    }
+    for name, (call, value, dx) in cases.items():
+        leaf = h.clone().requires_grad_()
+        got = call(leaf)
+        assert got.shape == (N,) and got.dtype == torch.float32
+        # logits rounded to bf16 (2^-9 of up to 16): a few hundredths in a value
+        assert torch.allclose(got.detach().double(), value, atol=0.15), name
+        (got * coef).sum().backward()
+        dh = dx @ W.double()
+        err = (leaf.grad.double() - dh).abs().max().item()
+        assert err <= 3e-2 * dh.abs().max().item(), (name, err)
+        with torch.no_grad():
+            assert torch.allclose(call(h), got.detach(), rtol=1e-5, atol=1e-5), name
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_head_edges(dev):
+    shard, W = _shard(dev)
+    none = torch.zeros(0, 64, device=dev, dtype=torch.bfloat16)
+    assert shard.token_logprobs(none, torch.zeros(0, dtype=torch.int64, device=dev)).shape == (0,)
+    assert shard.top_logits(none, 3)[0].shape == (0, 3)
+    with pytest.raises(ValueError):
+        shard.top_logits(torch.zeros(2, 65, device=dev), 3)
+
+
+def test_split_head_is_refused():
+    from micro_engram.train.head import VocabShard
+
+    shard = VocabShard(torch.randn(64, 8), 0, 2)
+    with pytest.raises(ValueError):
+        shard.top_logits(torch.randn(3, 8), 2)
+    with pytest.raises(ValueError):
+        shard.token_logprobs(torch.randn(3, 8), torch.zeros(3, dtype=torch.int64))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_example(dev, monkeypatch, dist_env):
+    if dev == "cpu":
+        monkeypatch.setenv("MICRO_ENGRAM_CPU", "1")
+    monkeypatch.syspath_prepend(os.path.join(ROOT, "examples"))
+    import distill_and_prefer
+
+    out = distill_and_prefer.main(steps=12, seq=96 if dev == "cpu" else 512)
+    assert out["device"].startswith(dev)
+    first, last = out["distill_loss"]
+    assert first > 0 and last < 0.7 * first
+    first, last = out["preference_loss"]
+    assert abs(first - 0.6931) < 1e-2 and last < 0.5 * first and min(out["margins"]) > 0
+    sys.modules.pop("distill_and_prefer", None)
