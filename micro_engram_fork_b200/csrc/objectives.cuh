@@ -125,22 +125,33 @@ ME_DEVICE uint4 from_pairs(const f32x2 (&p)[Vec16<T>::kN / 2]) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// Largest element of a vector, or largest magnitude (a NaN beside numbers is passed over).
-template <typename T, bool kAbs>
-ME_DEVICE float vec_max(uint4 v) {
-  if constexpr (sizeof(T) == 4) {
-    float a = __uint_as_float(v.x), b = __uint_as_float(v.y), c = __uint_as_float(v.z), d = __uint_as_float(v.w);
-    if (kAbs) a = fabsf(a), b = fabsf(b), c = fabsf(c), d = fabsf(d);
-    return fmaxf(fmaxf(a, b), fmaxf(c, d));
-  } else {
-    using T2 = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162, __half2>;
-    T2 a = *reinterpret_cast<T2*>(&v.x), b = *reinterpret_cast<T2*>(&v.y), c = *reinterpret_cast<T2*>(&v.z),
-       d = *reinterpret_cast<T2*>(&v.w);
-    if (kAbs) a = __habs2(a), b = __habs2(b), c = __habs2(c), d = __habs2(d);
-    const T2 m = __hmax2(__hmax2(a, b), __hmax2(c, d));
-    return fmaxf(to_f<T>(m.x), to_f<T>(m.y));
+// The running largest of a thread's logits (a NaN beside numbers is passed over). 16-bit types: two lanes in one
+// register.
+template <typename T>
+struct MaxOf {
+  using T2 = std::conditional_t<std::is_same_v<T, __nv_bfloat16>, __nv_bfloat162,
+                                std::conditional_t<std::is_same_v<T, __half>, __half2, float>>;
+  T2 m;
+  ME_DEVICE MaxOf() { clear(); }
+  ME_DEVICE void clear() {
+    if constexpr (sizeof(T) == 4) m = -INFINITY;
+    else m = T2(from_f<T>(-INFINITY), from_f<T>(-INFINITY));
   }
-}
+  ME_DEVICE void add(uint4 v) {
+    if constexpr (sizeof(T) == 4) {
+      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(v.x), __uint_as_float(v.y)),
+                         fmaxf(__uint_as_float(v.z), __uint_as_float(v.w))));
+    } else {
+      const T2 a = *reinterpret_cast<T2*>(&v.x), b = *reinterpret_cast<T2*>(&v.y), c = *reinterpret_cast<T2*>(&v.z),
+               d = *reinterpret_cast<T2*>(&v.w);
+      m = __hmax2(m, __hmax2(__hmax2(a, b), __hmax2(c, d)));
+    }
+  }
+  ME_DEVICE float value() const {
+    if constexpr (sizeof(T) == 4) return m;
+    else return fmaxf(to_f<T>(m.x), to_f<T>(m.y));
+  }
+};
 
 // How raw logits become exponents: z = softcap(x), y = z / tau.
 //
@@ -455,43 +466,45 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
 // form, since nothing else is rounded then.
-// watch(x, i): sees each of the thread's vectors, in order.
+// watch(x, i): sees the thread's vectors from the i-th on, one or two at a time, in order.
 struct WatchNothing {
-  ME_DEVICE void operator()(uint4, int) const {}
+  template <typename X>
+  ME_DEVICE void operator()(const X&, int) const {}
 };
 template <typename T, bool kCap, typename Drop, typename Watch = WatchNothing>
 ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop, Ring& ring, Watch&& watch = Watch()) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   MaxSum out;
   const int count = sl.count();
-  float big = -INFINITY, sum0 = 0.f, sum1 = 0.f;
+  MaxOf<T> big;
+  float sum0 = 0.f, sum1 = 0.f;
   const float k = sc.inv_temp * kLog2e;
   float ref = 0.f, shift = 0.f;  // the reference; the same, or the rounded ref k
   stream(
       sl.mine(), count, ring,
       [&](int n, const uint4(&v)[kFirst]) {
-        float top = -INFINITY;
+        MaxOf<T> top;
 #pragma unroll
         for (int u = 0; u < kFirst; ++u)
-          if (u < n) top = fmaxf(top, vec_max<T, false>(v[u]));
-        ref = kCap ? softcap(top, sc.cap) : top * sc.inv_temp;
+          if (u < n) top.add(v[u]);
+        ref = kCap ? softcap(top.value(), sc.cap) : top.value() * sc.inv_temp;
         shift = kCap ? ref * k : ref;
       },
       [&](const auto& x, int i, auto whole) {
         constexpr int kV = sizeof(x) / sizeof(uint4);
         f32x2 y[kV][kP];
+        watch(x, i);
         if constexpr (kCap) {
           vec_softcap<T, true, decltype(whole)::value>(x, sc, shift, y);
         } else {
 #pragma unroll
           for (int u = 0; u < kV; ++u) {
             to_pairs<T>(x[u], y[u]);
-            big = fmaxf(big, vec_max<T, false>(x[u]));
+            big.add(x[u]);
           }
         }
 #pragma unroll
         for (int u = 0; u < kV; ++u) {
-          watch(x[u], i + u);
           const uint32_t out_mask = drop(sl.vec(i + u));
 #pragma unroll
           for (int p = 0; p < kP; ++p) {
@@ -516,7 +529,7 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
         }
       });
   const float s = sum0 + sum1;
-  const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big * sc.inv_temp - ref;  // the largest exponent
+  const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big.value() * sc.inv_temp - ref;  // the largest exponent
   if (count > 0 && s > 1e-30f && s < 1e37f && far < 80.f) {
     // (m is rounded: what separates it from the shift that was taken goes into s)
     out.m = kCap ? ref * sc.inv_temp : ref;

@@ -141,38 +141,73 @@ ME_DEVICE void push(Work& work, int* count, uint64_t c) {
     asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(cluster_at(&work.pick.found[at], 0)), "l"(c) : "memory");
 }
 
-// The largest v (its low 16 bits 0) that at least k of the keys reach, 0 if there are fewer: two bits a step.
-ME_DEVICE uint32_t kth_bound(const uint32_t (&keys)[kMaxGroups], int n, int k, uint32_t (*counts)[kWarps][2]) {
+// A lower bound of the k-th largest of the row's group maxima: at least k of them reach it, and few more than that
+// (2 k + 64, or as many as are equal). Each thread brings the largest of its groups; 256 threads reach the smallest of
+// those, so the k-th largest lies between it and the largest key. A histogram of 256 steps over that range tells the
+// step that it is in, a second one over that step where too many lie there.
+struct Bound {
+  uint32_t ends[kWarps][2];
+  int hist[256];
+  int bin, above, count;
+};
+static_assert(kMaxTop <= kThreads);
+ME_DEVICE uint32_t kth_bound(const uint32_t (&keys)[kMaxGroups], int n, int k, Bound& w) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
-  uint32_t bound = 0;
-#pragma unroll 1
-  for (int bit = 30, turn = 0; bit >= 16; bit -= 2, turn ^= 1) {
-    const uint32_t v1 = bound | 1u << bit, v2 = bound | 2u << bit, v3 = bound | 3u << bit;
-    uint32_t c12 = 0, c3 = 0;  // (a count is 4096 at most)
+  uint32_t high = 0;
 #pragma unroll
-    for (int i = 0; i < kMaxGroups; ++i) {
-      if (i >= n) break;
-      c12 += (keys[i] >= v1 ? 1u : 0u) + (keys[i] >= v2 ? 1u << 16 : 0u);
-      c3 += keys[i] >= v3 ? 1u : 0u;
-    }
-    c12 = __reduce_add_sync(0xffffffffu, c12);
-    c3 = __reduce_add_sync(0xffffffffu, c3);
-    if (lane == 0) {
-      counts[turn][wid][0] = c12;
-      counts[turn][wid][1] = c3;
+  for (int i = 0; i < kMaxGroups; ++i) high = max(high, keys[i]);  // (those past n are 0)
+  uint32_t low = __reduce_min_sync(0xffffffffu, high);
+  high = __reduce_max_sync(0xffffffffu, high);
+  if (lane == 0) {
+    w.ends[wid][0] = low;
+    w.ends[wid][1] = high;
+  }
+  w.hist[threadIdx.x] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarps; ++i) {
+    low = min(low, w.ends[i][0]);
+    high = max(high, w.ends[i][1]);
+  }
+  for (int left = k;;) {
+    const int shift = max(24 - __clz(high - low | 1u), 0);  // (high - low) >> shift <= 255
+#pragma unroll
+    for (int i = 0; i < kMaxGroups; ++i)
+      if (i < n && keys[i] >= low && keys[i] <= high) atomicAdd(&w.hist[keys[i] - low >> shift], 1);
+    __syncthreads();
+    if (wid == 0) {
+      int mine[8], sum = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sum += mine[i] = w.hist[lane * 8 + i];
+      int from = sum;  // of this lane's steps and the higher lanes'
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_down_sync(0xffffffffu, from, o);
+        if (lane + o < 32) from += v;
+      }
+      const uint32_t enough = __ballot_sync(0xffffffffu, from >= left);
+      if (lane == 31 - __clz(enough | 1u)) {
+        int above = from - sum, bin = 7;
+        while (bin > 0 && above + mine[7] < left) {  // (the steps from the top; rotated, not indexed)
+          above += mine[7];
+#pragma unroll
+          for (int i = 7; i > 0; --i) mine[i] = mine[i - 1];
+          --bin;
+        }
+        w.bin = lane * 8 + bin;
+        w.above = above;
+        w.count = mine[7];
+      }
     }
     __syncthreads();
-    c12 = c3 = 0;
-#pragma unroll
-    for (int i = 0; i < kWarps; ++i) {
-      c12 += counts[turn][i][0];
-      c3 += counts[turn][i][1];
-    }
-    if (c3 >= (uint32_t)k) bound = v3;
-    else if (c12 >> 16 >= (uint32_t)k) bound = v2;
-    else if ((c12 & 0xffff) >= (uint32_t)k) bound = v1;
+    low += (uint32_t)w.bin << shift;
+    if (shift == 0 || k - left + w.above + w.count <= 2 * k + 64) return low;
+    left -= w.above;
+    high = min(high, low + (1u << shift) - 1);
+    __syncthreads();
+    w.hist[threadIdx.x] = 0;
+    __syncthreads();
   }
-  return bound;
 }
 
 // One cluster a row. A thread's groups are 2^lg_group of its vectors each.
@@ -182,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 4)
                float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   extern __shared__ uint4 dynamic[];
   __shared__ float2 part[kWarps];
-  __shared__ uint32_t counts[2][kWarps][2];
+  __shared__ Bound select;
   __shared__ int found, hits;
   Work& work = *reinterpret_cast<Work*>(dynamic);
   uint32_t* top = reinterpret_cast<uint32_t*>(dynamic + sizeof(Work) / sizeof(uint4));  // [groups][thread]
@@ -190,18 +225,18 @@ __global__ void __launch_bounds__(kThreads, 4)
   const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
   const Slice<T> sl(x.row(r), V, rank, lg_ranks);
   if (threadIdx.x == 0) found = hits = 0;
-  float best = -INFINITY;
+  MaxOf<T> best;
   const int group = 1 << lg_group, count = sl.count();
-  MaxSum a = slice_sum<T, kCap>(
-      sl, sc, KeepAll(), work.ring,
-      [&](uint4 v, int i) {
-        best = fmaxf(best, vec_max<T, false>(v));
-        if ((i + 1 & group - 1) == 0) {
-          top[(i >> lg_group) * kThreads + threadIdx.x] = order_key(best);
-          best = -INFINITY;
-        }
-      });
-  if (count & group - 1) top[(count >> lg_group) * kThreads + threadIdx.x] = order_key(best);
+  MaxSum a = slice_sum<T, kCap>(sl, sc, KeepAll(), work.ring, [&](const auto& v, int i) {
+    constexpr int kV = sizeof(v) / sizeof(uint4);
+#pragma unroll
+    for (int u = 0; u < kV; ++u) best.add(v[u]);
+    if ((i + kV & group - 1) == 0) {
+      top[(i >> lg_group) * kThreads + threadIdx.x] = order_key(best.value());
+      best.clear();
+    }
+  });
+  if (count & group - 1) top[(count >> lg_group) * kThreads + threadIdx.x] = order_key(best.value());
   for (int g = (count + group - 1) >> lg_group; g < groups; ++g) top[g * kThreads + threadIdx.x] = 0;
   a = row_merge(a, part, lg_ranks);  // (behind its barrier the blocks' groups are there)
   const bool lead = rank == 0;
@@ -226,7 +261,8 @@ __global__ void __launch_bounds__(kThreads, 4)
       asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(keys[i]) : "r"(cluster_at(mine, i & ((1 << lg_ranks) - 1))));
     }
   }
-  const uint32_t bound = kth_bound(keys, n, k, counts);
+  const uint32_t bound = kth_bound(keys, n, k, select);
+  const float least = key_value(bound);  // (a NaN where there are too few groups: no candidates then)
   for (int g = 0; g < groups; ++g) {
     if (top[g * kThreads + threadIdx.x] < bound || g << lg_group >= count) continue;
     const int at = atomicAdd(&hits, 1);
@@ -243,14 +279,14 @@ __global__ void __launch_bounds__(kThreads, 4)
       v.u = *reinterpret_cast<const uint4*>(sl.row + sl.column(vec));
 #pragma unroll
       for (int e = 0; e < Vec16<T>::kN; ++e) {
-        const uint32_t q = order_key(to_f<T>(v.h[e]));
-        if (q >= bound) push(work, &found, candidate(q, sl.column(vec) + e));
+        const float f = to_f<T>(v.h[e]);
+        if (f >= least) push(work, &found, candidate(order_key(f), sl.column(vec) + e));
       }
     }
     const int j = sl.single();
     if (j >= 0) {
-      const uint32_t q = order_key(to_f<T>(sl.row[j]));
-      if (q >= bound) push(work, &found, candidate(q, j));
+      const float f = to_f<T>(sl.row[j]);
+      if (f >= least) push(work, &found, candidate(order_key(f), j));
     }
   } else if (threadIdx.x == 0) {  // too many: more candidates than there is room for
     asm volatile("red.shared::cluster.add.u32 [%0], %1;" ::"r"(cluster_at(&found, 0)), "r"(kFound + 1) : "memory");
@@ -274,11 +310,11 @@ namespace me {
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,
                        cudaStream_t stream) {
   const int ranks = ranks_for(x.N, x.V), lg_ranks = ilog2(ranks);
-  // Groups of up to eight vectors, as long as there are eight times as many of them as logits asked
-  // for (then about 1.07 k logits reach the bound); more vectors where a thread would have too many groups.
+  // Groups of two to eight vectors (they are seen by twos), eight as long as there are eight times as many of them
+  // as logits asked for (then about 1.07 k logits reach the bound); more where a thread would have too many groups.
   const int64_t vecs = (x.V * (x.type == LogitType::kF32 ? 4 : 2) + 15) / 16;
   const int per_thread = (int)(((vecs + ranks - 1) / ranks + kThreads - 1) / kThreads);
-  int lg_group = 0;
+  int lg_group = 1;
   while (lg_group < 3 && vecs >> (lg_group + 1) >= 8 * k) ++lg_group;
   while (((per_thread + (1 << lg_group) - 1) >> lg_group) << lg_ranks > kMaxGroups) ++lg_group;
   const int groups = (per_thread + (1 << lg_group) - 1) >> lg_group;
