@@ -122,7 +122,7 @@ template <typename T, bool kCap>
 __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int V,
                                                                   int lg_ranks, const int64_t* __restrict__ target,
                                                                   Scale sc, const float2* __restrict__ stats,
-                                                                  const float* __restrict__ g) {
+                                                                  const float* __restrict__ g, int64_t g_step) {
   __shared__ Ring ring;
   const int64_t r = N - 1 - (blockIdx.x >> lg_ranks);
   const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
@@ -135,7 +135,7 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> 
   }
   const bool valid = t >= 0 && t < V, mine = valid && sl.holds((int)t) && threadIdx.x == 0;
   const float2 ms = stats[r];
-  const float c = valid ? g[r] : NAN;
+  const float c = valid ? g[r * g_step] : NAN;
   const float xt = mine ? to_f<T>(sl.row[t]) : 0.f;
   __syncthreads();  // read before the row may be written in place
   write_slice<T, kCap>(sl, o, sc, ms.x, -c / ms.y, ring);
@@ -414,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     distill_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int V, int lg_ranks, int k,
                        const float* __restrict__ weight, float temp, const Entry* __restrict__ entries,
                        const TeacherRow* __restrict__ rows, Scale sc, const float4* __restrict__ stats,
-                       const float* __restrict__ g) {
+                       const float* __restrict__ g, int64_t g_step) {
   __shared__ Ring ring;
   const int64_t r = N - 1 - (blockIdx.x >> lg_ranks);  // last to first, as above
   const Slice<T> sl(x.row(r), V, blockIdx.x & ((1 << lg_ranks) - 1), lg_ranks);
@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kThreads, 4)
     return;
   }
   const Entry e = load_entry(entries, r, k);
-  const float c = (weight ? weight[r] : 1.f) * temp * g[r];
+  const float c = (weight ? weight[r] : 1.f) * temp * g[r * g_step];
   write_slice<T, kCap>(sl, o, sc, st.z, c * st.w, ring);
   __syncthreads();
   write_entry<T>(sl, o, e, c, st.x, 1.f / st.y, rows[r].mass);
@@ -443,13 +443,13 @@ void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, flo
                                                                    make_scale(x.cap, 1.f), logp, stats)));
 }
 
-void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
+void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, RowValues g, Gradient out,
                         cudaStream_t stream) {
   const int ranks = ranks_for_gradient(x);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, logprob_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
                                          rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), target,
-                                         make_scale(x.cap, 1.f), stats, g)));
+                                         make_scale(x.cap, 1.f), stats, g.data, g.step)));
 }
 
 void launch_teacher(const Logits& x, const TeacherArgs& te, void* entries, void* rows, cudaStream_t stream) {
@@ -481,13 +481,13 @@ void launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* ent
 }
 
 void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows,
-                        const float4* stats, const float* g, Gradient out, cudaStream_t stream) {
+                        const float4* stats, RowValues g, Gradient out, cudaStream_t stream) {
   const int ranks = ranks_for_gradient(x);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, distill_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
                                          rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), te.k, te.weight,
                                          te.temp, static_cast<const Entry*>(entries),
-                                         static_cast<const TeacherRow*>(rows), make_scale(x.cap, te.temp), stats, g)));
+                                         static_cast<const TeacherRow*>(rows), make_scale(x.cap, te.temp), stats, g.data, g.step)));
 }
 
 }  // namespace me

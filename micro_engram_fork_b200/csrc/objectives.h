@@ -25,6 +25,12 @@ struct Gradient {
   int64_t stride;
 };
 
+// One number a row, `step` apart (0: one for all).
+struct RowValues {
+  const float* data;
+  int64_t step;
+};
+
 // The teacher's records: k entries a row; lse and weight may be null.
 struct TeacherArgs {
   const int64_t* ids;
@@ -36,7 +42,7 @@ struct TeacherArgs {
 };
 
 void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, float2* stats, cudaStream_t stream);
-void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, const float* g, Gradient out,
+void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, RowValues g, Gradient out,
                         cudaStream_t stream);
 // What launch_teacher() leaves for the other three: N k entries and N rows, 16-byte aligned.
 constexpr int kEntryBytes = 16, kTeacherRowBytes = 32;
@@ -48,7 +54,7 @@ void launch_distill_grad(const Logits& x, const TeacherArgs& teacher, const void
                          Gradient out, cudaStream_t stream);
 // g: one coefficient a row
 void launch_distill_bwd(const Logits& x, const TeacherArgs& teacher, const void* entries, const void* rows,
-                        const float4* stats, const float* g, Gradient out, cudaStream_t stream);
+                        const float4* stats, RowValues g, Gradient out, cudaStream_t stream);
 void launch_top_logits(const Logits& x, int k, float temp, float* values, int64_t* ids, float* lse,
                        cudaStream_t stream);
 

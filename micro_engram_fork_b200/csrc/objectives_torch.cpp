@@ -65,6 +65,14 @@ Tensor check_rows(const Tensor& t, const Tensor& x, torch::ScalarType type, cons
   TORCH_CHECK(t.device() == x.device(), what, ": on another device than the logits");
   return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous();
 }
+// A gradient's coefficient for each row of x, as it comes (autograd's are often one number expanded). `hold` keeps it.
+me::RowValues check_coefficients(const Tensor& g, const Tensor& x, Tensor& hold) {
+  ME_CHECK_VALUE(g.dim() == 1 && g.size(0) == x.size(0), "coefficients: one value a row of logits is needed (",
+                 text(x.size(0)), "), got shape ", shape(g));
+  TORCH_CHECK(g.device() == x.device(), "coefficients: on another device than the logits");
+  hold = g.scalar_type() == torch::kFloat32 ? g : g.to(torch::kFloat32);
+  return {hold.data_ptr<float>(), hold.size(0) > 1 ? hold.stride(0) : 0};
+}
 Tensor check_whole(const Tensor& t, const Tensor& x, const char* what) {
   ME_CHECK_VALUE(t.scalar_type() == torch::kLong || t.scalar_type() == torch::kInt, what,
                     ": int64 or int32 is needed, got ", t.scalar_type());
@@ -142,10 +150,11 @@ Tensor token_logprobs_bwd(Tensor x, Tensor target, OptDouble cap, Tensor stats, 
   const auto in = check_logits(x, cap, "token_logprobs");
   const at::cuda::CUDAGuard guard(x.device());
   auto t = check_whole(target, x, "targets");
-  auto gr = check_rows(g, x, torch::kFloat32, "token_logprobs: gradient");
+  Tensor hold;
+  const auto gr = check_coefficients(g, x, hold);
   auto o = gradient_like(x, out, "token_logprobs");
   if (in.N == 0) return o;
-  me::launch_logprob_bwd(in, t.data_ptr<int64_t>(), as2(stats), gr.data_ptr<float>(), gradient_of(o),
+  me::launch_logprob_bwd(in, t.data_ptr<int64_t>(), as2(stats), gr, gradient_of(o),
                          at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
@@ -154,8 +163,7 @@ Tensor token_logprobs_bwd(Tensor x, Tensor target, OptDouble cap, Tensor stats, 
 // (logp [N], gradient of sum(coef * logp) in the logits [N, V]); coef: 1 unless given
 std::vector<Tensor> token_logprobs_grad(Tensor x, Tensor target, OptTensor coef, OptDouble cap, OptTensor out) {
   auto t = check_whole(target, x, "targets");
-  Tensor g = coef.has_value() ? check_rows(*coef, x, torch::kFloat32, "coefficients")
-                              : torch::ones({x.size(0)}, x.options().dtype(torch::kFloat32).requires_grad(false));
+  Tensor g = coef.has_value() ? *coef : torch::ones({1}, x.options().dtype(torch::kFloat32).requires_grad(false)).expand(x.size(0));
   auto f = token_logprobs_fwd(x, t, cap);
   return {f[0], token_logprobs_bwd(x, t, cap, f[1], g, out)};
 }
@@ -197,7 +205,8 @@ Tensor distill_bwd(Tensor x, Tensor rows, OptTensor weight, OptDouble cap, doubl
                    OptTensor out) {
   const auto in = check_logits(x, cap, "distill_loss");
   const at::cuda::CUDAGuard guard(x.device());
-  auto gr = check_rows(g, x, torch::kFloat32, "distill_loss: gradient");
+  Tensor hold;
+  const auto gr = check_coefficients(g, x, hold);
   Tensor w;
   if (weight.has_value()) w = check_rows(*weight, x, torch::kFloat32, "weights");
   auto o = gradient_like(x, out, "distill_loss");
@@ -208,7 +217,7 @@ Tensor distill_bwd(Tensor x, Tensor rows, OptTensor weight, OptDouble cap, doubl
   te.temp = (float)temp;
   const float* entries = rows.data_ptr<float>();
   me::launch_distill_bwd(in, te, entries, entries + in.N * te.k * (me::kEntryBytes / 4), as4(stats),
-                         gr.data_ptr<float>(), gradient_of(o), at::cuda::getCurrentCUDAStream());
+                         gr, gradient_of(o), at::cuda::getCurrentCUDAStream());
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return o;
 }

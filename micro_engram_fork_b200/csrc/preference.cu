@@ -14,7 +14,7 @@ using namespace me;
 
 namespace {
 
-constexpr int kPairThreads = 512;
+constexpr int kPairThreads = 1024;  // at most: a block has 256 for short sequences
 
 // log(1 + e^v) without overflow
 ME_DEVICE float softplus(float v) { return fmaxf(v, 0.f) + log1pf(expf(-fabsf(v))); }
@@ -73,7 +73,9 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(
     return logp[t] - (ref ? ref[t] : 0.f);
   };
   float rc = 0.f, rr = 0.f;
+#pragma unroll 8
   for (int64_t t = a + threadIdx.x; t < b; t += blockDim.x) rc += ratio(t);
+#pragma unroll 8
   for (int64_t t = b + threadIdx.x; t < c; t += blockDim.x) rr += ratio(t);
   const float2 sums = block_sum2(rc, rr, scratch);
   const float h = sums.x - sums.y, u = beta * h;
@@ -102,13 +104,17 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(
     for (int64_t t = c + threadIdx.x; t < T; t += blockDim.x) grad[t] = 0.f;
 }
 
+// Threads of a pair's block: all of them where a thread would have more than four tokens.
+int pair_threads(int64_t tokens, int64_t pairs) { return tokens / pairs > 4 * 256 ? kPairThreads : 256; }
+
 }  // namespace
 
 namespace me {
 
 void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* grad, cudaStream_t stream) {
+  const int threads = pair_threads(a.tokens, a.pairs);
   auto launch = [&](auto* cu) {
-    preference_kernel<<<(unsigned)a.pairs, kPairThreads, 0, stream>>>(a.logp, a.ref, a.target, a.tokens, cu, a.pairs, a.kind,
+    preference_kernel<<<(unsigned)a.pairs, threads, 0, stream>>>(a.logp, a.ref, a.target, a.tokens, cu, a.pairs, a.kind,
                                                                   a.beta, a.smooth, a.scale, loss, rewards, grad);
   };
   if (a.cu64) launch(static_cast<const int64_t*>(a.cu));
@@ -118,7 +124,7 @@ void launch_preference(const PairArgs& a, float* loss, float2* rewards, float* g
 void launch_preference_scale(const float* grad, const float* g, const void* cu, bool cu64, int64_t tokens, int64_t pairs,
                              float* out, cudaStream_t stream) {
   auto launch = [&](auto* offsets) {
-    preference_scale_kernel<<<(unsigned)pairs, kPairThreads, 0, stream>>>(grad, g, offsets, tokens, pairs, out);
+    preference_scale_kernel<<<(unsigned)pairs, pair_threads(tokens, pairs), 0, stream>>>(grad, g, offsets, tokens, pairs, out);
   };
   if (cu64) launch(static_cast<const int64_t*>(cu));
   else launch(static_cast<const int*>(cu));
