@@ -3,7 +3,7 @@
 Layout:
   ops/       autograd ops backed by the hand-written sm_100a kernels in csrc/ (engram
              hash/gather/gate/row-grad/Adam, RMSNorm, q/k/v norm + RoPE, GeGLU, softcapped
-             CE, attention, tcgen05 GEMM), each with a plain PyTorch reference used on CPU
+             CE, the other objectives over the vocabulary, attention, tcgen05 GEMM), each with a plain PyTorch reference used on CPU
              and as the test oracle
   parallel/  symmetric peer memory over NVLink (CUDA IPC), the row store of the
              row-sharded engram tables, P2P collectives

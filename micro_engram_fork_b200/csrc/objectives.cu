@@ -22,15 +22,16 @@ namespace {
 
 // ------------------------------------------------------------------------------------ gradient of a slice
 // out_j = coef exp(y_j - m) z'_j for the block's columns, in 16-byte stores where the two rows are
-// aligned alike.
+// aligned alike. The slice is walked from its end: what a sum has just read last is in L2.
 template <typename T, bool kCap, bool kAligned>
 ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
   constexpr int kN = Vec16<T>::kN, kP = kN / 2;
   // coef (1 - (z / c)^2) is one FMA with the coefficient inside
   const float coef_slope = coef * sc.slope, k = sc.inv_temp * kLog2e, shift = m * kLog2e;
-  T* mine = out + sl.column(sl.vec(0));
-  stream(
-      sl.mine(), sl.count(), ring, [](int, auto&) {},
+  const int last = max(sl.count() - 1, 0);
+  T* mine = out + sl.column(sl.vec(last));
+  stream<-kThreads>(
+      sl.mine() + last * kThreads, sl.count(), ring, [](int, auto&) {},
       [&](const auto& x, int i, auto whole) {
         constexpr int kV = sizeof(x) / sizeof(uint4);
         f32x2 z[kV][kP];
@@ -53,7 +54,7 @@ ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float 
           }
           Vec16<T> r;
           r.u = from_pairs<T>(z[u]);
-          T* at = mine + (i + u) * (kThreads * kN);
+          T* at = mine - (i + u) * (kThreads * kN);
           if constexpr (kAligned) {
             *reinterpret_cast<uint4*>(at) = r.u;
           } else {

@@ -401,14 +401,14 @@ ME_DEVICE void copy_wait() {
 
 // first(n, v): the thread's n first vectors (at most kFirst) are there; f(v, i): the array v of vectors from
 // the thread's i-th on, two of them while the whole warp is in the loop (kWhole), else one. `src`: its first one,
-// the others follow kThreads apart. Every thread of the block calls it, those without a vector too.
-template <typename First, typename F>
+// the others follow kStep (+-kThreads) apart. Every thread of the block calls it, those without a vector too.
+template <int kStep = kThreads, typename First, typename F>
 ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&& f) {
   const int tid = threadIdx.x;
   uint4* mine = &ring.v[0][tid];
 #pragma unroll
   for (int d = 0; d < kDepth; ++d) {
-    if (d < count) copy_async(mine + d * kThreads, src + d * kThreads);
+    if (d < count) copy_async(mine + d * kThreads, src + d * kStep);
     if (d & 1) copy_commit();
   }
   copy_wait<(kDepth - kFirst) / 2>();
@@ -418,17 +418,17 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
     for (int u = 0; u < kFirst; ++u) v[u] = mine[u * kThreads];
     first(min(count, kFirst), v);
   }
-  const uint4* next = src + kDepth * kThreads;
+  const uint4* next = src + kDepth * kStep;
   const int whole = __shfl_sync(0xffffffffu, count, 31);  // the warp's last lane has the fewest
   int i = 0;
-  for (; i + 2 * kDepth <= whole; i += kDepth, next += kDepth * kThreads) {
+  for (; i + 2 * kDepth <= whole; i += kDepth, next += kDepth * kStep) {
 #pragma unroll
     for (int s = 0; s < kDepth; s += 2) {
       copy_wait<kDepth / 2 - 1>();
       const uint4 v[2] = {mine[s * kThreads], mine[(s + 1) * kThreads]};
       f(v, i + s, std::true_type());
-      copy_async(mine + s * kThreads, next + s * kThreads);
-      copy_async(mine + (s + 1) * kThreads, next + (s + 1) * kThreads);
+      copy_async(mine + s * kThreads, next + s * kStep);
+      copy_async(mine + (s + 1) * kThreads, next + (s + 1) * kStep);
       copy_commit();
     }
   }
@@ -441,7 +441,7 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
     f(v, i, std::true_type());
 #pragma unroll
     for (int u = 0; u < 2; ++u)
-      if (i + u + kDepth < count) copy_async(at + u * kThreads, src + (i + u + kDepth) * kThreads);
+      if (i + u + kDepth < count) copy_async(at + u * kThreads, src + (i + u + kDepth) * kStep);
     copy_commit();
   }
 #pragma unroll 1

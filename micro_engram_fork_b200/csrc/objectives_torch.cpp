@@ -305,6 +305,11 @@ namespace {
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// The gradients are not differentiable themselves (create_graph would make a graph without them).
+void check_once() {
+  TORCH_CHECK(!at::GradMode::is_enabled(), "the gradient of this objective cannot be differentiated (create_graph)");
+}
+
 OptTensor optional(const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
 
 struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
@@ -315,6 +320,7 @@ struct TokenLogprobs : torch::autograd::Function<TokenLogprobs> {
     return f[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
     const auto s = ctx->get_saved_variables();
     return {token_logprobs_bwd(s[0], s[1], ctx->saved_data["cap"].toDouble(), s[2], g[0], OptTensor()), Tensor(),
             Tensor()};
@@ -331,6 +337,7 @@ struct Distill : torch::autograd::Function<Distill> {
     return f[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
     const auto s = ctx->get_saved_variables();
     auto dx = distill_bwd(s[0], s[3], optional(s[1]), ctx->saved_data["cap"].toDouble(),
                           ctx->saved_data["temp"].toDouble(), s[2], g[0], OptTensor());
@@ -347,6 +354,7 @@ struct Preference : torch::autograd::Function<Preference> {
     return {p[0], p[1]};
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once();
     const auto s = ctx->get_saved_variables();
     const at::cuda::CUDAGuard guard(s[0].device());
     auto gp = g[0].to(torch::kFloat32).contiguous(), out = torch::empty_like(s[0]), off = s[1].contiguous();

@@ -4,7 +4,7 @@ events (warm-up, synchronize on both sides) and reported against the measured ro
 figures otherwise). Also the workload that the committed ncu summaries in profiles/ capture.
 
   python -m micro_engram_fork_b200.utils.kernel_bench [--case all|gemm|attn_fwd|attn_bwd|gate|ce|qkv|geglu|rows|
-                                                       norms|ce_bwd|nf4|ce_gemm|tp] [--iters N] [--small]
+                                                       norms|ce_bwd|nf4|ce_gemm|tp|objectives] [--iters N] [--small]
 """
 import argparse
 import json
@@ -393,9 +393,33 @@ def case_tp(C, dev, it, pk):
     return r
 
 
+def case_objectives(C, dev, it, pk):
+    """The objectives over the vocabulary on one chunk of 2048 x 262144 bf16 logits, softcap 30, every token
+    trained: bytes are the logits read once and, where there is a gradient, written once."""
+    from ..ops import objectives as O
+
+    N, V, k = 2048, 262144, 64
+    z = (torch.randn(N, V, device=dev) * 2.5 - 5.0).to(torch.bfloat16)
+    grad = torch.empty_like(z)
+    t = torch.randint(0, V, (N,), device=dev)
+    values, ids, lse = O.top_logits(z, k, softcap=30.0)
+    cu = torch.arange(0, N + 1, N // 8, device=dev)
+    one, two = z.numel() * 2, z.numel() * 4
+    r = {}
+    for name, nbytes, fn in (
+            ("top_logits k 64", one, lambda: O.top_logits(z, k, softcap=30.0)),
+            ("token_logprobs", one, lambda: O.token_logprobs(z, t, softcap=30.0)),
+            ("distill_loss_grad k 64", two, lambda: O.distill_loss_grad(z, ids, values, softcap=30.0, out=grad)),
+            ("distill_loss_grad k 64, rest", two, lambda: O.distill_loss_grad(z, ids, values, lse, softcap=30.0, out=grad)),
+            ("preference_logits_grad, 4 pairs", two, lambda: O.preference_logits_grad(z, t, None, cu, softcap=30.0,
+                                                                                     out=grad))):
+        r.update(_hbm(f"{name} {N}x{V}", nbytes, _time(fn, it), pk))
+    return r
+
+
 CASES = {"gemm": case_gemm, "attn_fwd": case_attn_fwd, "attn_bwd": case_attn_bwd, "gate": case_gate, "ce": case_ce,
          "qkv": case_qkv, "geglu": case_geglu, "rows": case_rows, "norms": case_norms, "ce_bwd": case_ce_bwd,
-         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp}
+         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp, "objectives": case_objectives}
 
 
 def main(argv=None):
