@@ -644,12 +644,16 @@ inline int ranks_for(int64_t N, int64_t V, int per_sm = 4) {
   while (c < 8 && N * c < per_sm * objective_sms() && V / (2 * c) >= 4096) c *= 2;
   return c;
 }
-// The same where a gradient is written: two for long rows (a thread keeps 32 vectors or more), whose blocks end
-// more evenly (distillation of 2048 x 262144 by 1 / 2 / 4 / 8: 435 / 424 / 445 / 445 us).
-inline int ranks_for_gradient(const Logits& x) {
+// The same for the kernels that write a gradient. Where a row's blocks wait for one another, two for long rows (a
+// thread keeps 32 vectors or more; distillation of 2048 x 262144 by 1 / 2 / 4 / 8: 430 / 417 / 418 / 438 us);
+// where they do not, as many as leave a thread 16 vectors (the preference step's backward pass, 1024 of 2048 rows
+// trained, by 1 / 2 / 4 / 8: the step takes 397 / 385 / 372 / 366 us).
+inline int ranks_for_gradient(const Logits& x, bool alone) {
   const int64_t vecs = x.V * (x.type == LogitType::kF32 ? 4 : 2) / 16;
-  const int c = ranks_for(x.N, x.V);
-  return c == 1 && vecs / 2 >= 32 * kThreads ? 2 : c;
+  const int most = alone ? 8 : 2, least = alone ? 16 : 32;
+  int c = ranks_for(x.N, x.V);
+  while (c < most && vecs / (2 * c) >= least * kThreads) c *= 2;
+  return c;
 }
 
 // Lets a kernel have more than 48 KB of shared memory.
