@@ -170,8 +170,6 @@ struct TeacherRow {
 };
 static_assert(sizeof(TeacherRow) == kTeacherRowBytes && sizeof(Entry) == kEntryBytes);
 
-constexpr int kFilter = 8192;  // bits of a filter over a row's entries
-
 // One warp a row of the teacher's records: probabilities, repeated ids, the student's logits there. It
 // runs ahead of the kernels that walk the logits, which then wait for nothing but the logits (with this
 // in their blocks, eight to a row, the chain ids -> logits -> sums took half of a block's time).
@@ -272,24 +270,27 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
   }
 }
 
-// Leaves the teacher's entries out of a sum. A bit of the filter is set for each vector that holds
-// one (and stands for every 8192nd vector); such a vector is compared with the list.
+// Leaves the teacher's entries out of a sum: a byte for each of the block's vectors says which of its elements are
+// entries. (A filter with one bit for several vectors and a look at the list made the sum take 2.3 times as long.)
+// A slice of more vectors than there are bytes shares them, and looks at the list behind a byte that is set.
+constexpr int kMostMasks = 32768;
 template <typename T>
 struct DropEntries {
-  const uint32_t* filter;
+  const uint8_t* mask;
   const int* id;
-  int k, head;
+  int k, head, begin;
+  bool exact;
   ME_DEVICE uint32_t operator()(int vec) const {
     constexpr int kN = Vec16<T>::kN;
-    const uint32_t b = (uint32_t)vec & (kFilter - 1);
-    if (!(filter[b >> 5] >> (b & 31) & 1)) return 0;
+    uint32_t m = mask[vec - begin & kMostMasks - 1];
+    if (m == 0 || exact) return m;
+    m = 0;
     const int j0 = head + vec * kN;
-    uint32_t mask = 0;
     for (int i = 0; i < k; ++i) {
       const uint32_t d = (uint32_t)(id[i] - j0);
-      if (id[i] >= 0 && d < (uint32_t)kN) mask |= 1u << d;
+      if (id[i] >= 0 && d < (uint32_t)kN) m |= 1u << d;
     }
-    return mask;
+    return m;
   }
   ME_DEVICE bool column(int j) const {
     for (int i = 0; i < k; ++i)
@@ -297,6 +298,8 @@ struct DropEntries {
     return false;
   }
 };
+// Its bytes, for a slice of n vectors.
+ME_HOST_DEVICE int mask_bytes(int n) { return ((n < kMostMasks ? n : kMostMasks) + 15) / 16 * 16; }
 
 // The student's side of a row, from the sum over its columns (with a rest: over those that are no entry).
 struct Student {
@@ -361,8 +364,8 @@ __global__ void __launch_bounds__(kThreads, 4)
                    float* __restrict__ loss, float4* __restrict__ stats) {
   __shared__ Ring ring;
   __shared__ float2 part[kWarps];
-  __shared__ uint32_t filter[kTail ? kFilter / 32 : 1];
   __shared__ int ids[kTail ? kMaxTop : 1];
+  extern __shared__ uint4 masks[];  // with a rest
   const int64_t r = blockIdx.x >> lg_ranks;
   const int rank = blockIdx.x & ((1 << lg_ranks) - 1);
   const Slice<T> sl(x.row(r), V, rank, lg_ranks);
@@ -378,15 +381,19 @@ __global__ void __launch_bounds__(kThreads, 4)
   MaxSum a;
   if constexpr (kTail) {
     const Entry e = load_entry(entries, r, k);
-    for (int i = threadIdx.x; i < kFilter / 32; i += kThreads) filter[i] = 0;
+    const int vecs = sl.end - sl.begin;
+    for (int i = threadIdx.x; i < mask_bytes(vecs) / 16; i += kThreads) masks[i] = make_uint4(0, 0, 0, 0);
     if (threadIdx.x < k) ids[threadIdx.x] = e.id;
     __syncthreads();
     if (e.id >= sl.head && e.id < sl.body_end) {
-      const uint32_t b = (uint32_t)((e.id - sl.head) / Vec16<T>::kN) & (kFilter - 1);
-      atomicOr(&filter[b >> 5], 1u << (b & 31));
+      constexpr int kN = Vec16<T>::kN;
+      const int v = (e.id - sl.head) / kN - sl.begin, at = v & kMostMasks - 1;
+      if (v >= 0 && v < vecs)
+        atomicOr(reinterpret_cast<uint32_t*>(masks) + at / 4, 1u << (at % 4 * 8 + (e.id - sl.head) % kN));
     }
     __syncthreads();
-    a = slice_sum<T, kCap>(sl, sc, DropEntries<T>{filter, ids, k, sl.head}, ring);
+    const DropEntries<T> drop = {reinterpret_cast<const uint8_t*>(masks), ids, k, sl.head, sl.begin, vecs <= kMostMasks};
+    a = slice_sum<T, kCap>(sl, sc, drop, ring);
   } else {
     a = slice_sum<T, kCap>(sl, sc, KeepAll(), ring);
   }
@@ -433,6 +440,13 @@ __global__ void __launch_bounds__(kThreads, 4)
 }
 
 // ------------------------------------------------------------------------------------ launches
+// Dynamic shared memory of distill_kernel: DropEntries' bytes.
+int masks_for(const Logits& x, const TeacherArgs& te, int ranks) {
+  if (!te.lse) return 0;
+  const int64_t vecs = x.V * (x.type == LogitType::kF32 ? 4 : 2) / 16;
+  return mask_bytes((int)((vecs + ranks - 1) / ranks));
+}
+
 }  // namespace
 
 namespace me {
@@ -464,7 +478,9 @@ void launch_distill_fwd(const Logits& x, const TeacherArgs& te, const void* entr
   const int ranks = ranks_for(x.N, x.V);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, false> : distill_kernel<T, kCap, false, false>;
-    launch_cluster(kernel, x.N * ranks, ranks, 0, stream, rows_in<T>(x), Rows<T>{}, x.V, ilog2(ranks), te.k, te.weight,
+    const int smem = masks_for(x, te, ranks);
+    allow_smem(kernel, smem);
+    launch_cluster(kernel, x.N * ranks, ranks, smem, stream, rows_in<T>(x), Rows<T>{}, x.V, ilog2(ranks), te.k, te.weight,
                    te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
                    make_scale(x.cap, te.temp), loss, stats);
   }));
@@ -475,7 +491,9 @@ void launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* ent
   const int ranks = ranks_for_gradient(x, false);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, true> : distill_kernel<T, kCap, false, true>;
-    launch_cluster(kernel, x.N * ranks, ranks, 0, stream, rows_in<T>(x), rows_out<T>(out), x.V, ilog2(ranks), te.k,
+    const int smem = masks_for(x, te, ranks);
+    allow_smem(kernel, smem);
+    launch_cluster(kernel, x.N * ranks, ranks, smem, stream, rows_in<T>(x), rows_out<T>(out), x.V, ilog2(ranks), te.k,
                    te.weight, te.temp, static_cast<const Entry*>(entries), static_cast<const TeacherRow*>(rows),
                    make_scale(x.cap, te.temp), loss, (float4*)nullptr);
   }));

@@ -505,17 +505,25 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
         }
 #pragma unroll
         for (int u = 0; u < kV; ++u) {
-          const uint32_t out_mask = drop(sl.vec(i + u));
+          if (!std::is_same_v<Drop, KeepAll>) {
+            const uint32_t out_mask = drop(sl.vec(i + u));
+            if (out_mask) {
+              const float gone = kCap ? -200.f : -INFINITY;
+#pragma unroll
+              for (int p = 0; p < kP; ++p) {
+                float2 f = unpack2(y[u][p]);
+                if (out_mask >> (2 * p) & 1) f.x = gone;
+                if (out_mask >> (2 * p) & 2) f.y = gone;
+                y[u][p] = pack2(f.x, f.y);
+              }
+            }
+          }
 #pragma unroll
           for (int p = 0; p < kP; ++p) {
             float2 d = unpack2(kCap ? y[u][p] : fma2(y[u][p], both2(sc.inv_temp), both2(-shift)));
             if constexpr (!kCap) {
               d.x = max_nan(d.x, -87.f);
               d.y = max_nan(d.y, -87.f);
-            }
-            if (!std::is_same_v<Drop, KeepAll>) {
-              if (out_mask >> (2 * p) & 1) d.x = kCap ? -200.f : -87.f;
-              if (out_mask >> (2 * p) & 2) d.y = kCap ? -200.f : -87.f;
             }
             if constexpr (kCap) {
               d.x = exp2_fast(d.x);
@@ -656,10 +664,10 @@ inline int ranks_for_gradient(const Logits& x, bool alone) {
   return c;
 }
 
-// Lets a kernel have more than 48 KB of shared memory.
+// Lets a kernel have more than 48 KB of shared memory, the ring and `bytes` at the launch.
 template <typename K>
 void allow_smem(K* kernel, int bytes) {
-  if (bytes > (32 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (bytes > (8 << 10)) cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
 }
 
 template <typename T>
