@@ -176,8 +176,10 @@ static_assert(sizeof(TeacherRow) == kTeacherRowBytes && sizeof(Entry) == kEntryB
 template <typename T>
 __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int64_t N, int V, TeacherArgs a, Scale sc,
                                                            Entry* __restrict__ entries, TeacherRow* __restrict__ rows) {
-  __shared__ __align__(16) int ids[kWarps][kMaxTop];
-  __shared__ float qs[kWarps][kMaxTop];
+  constexpr int kSeen = 8192;  // bits
+  __shared__ int ids[kWarps][kMaxTop], firsts[kWarps][kMaxTop];
+  __shared__ float qs[kWarps][kMaxTop], sums[kWarps][kMaxTop];
+  __shared__ uint32_t seen_bits[kWarps][kSeen / 32];
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   const int64_t r = (int64_t)blockIdx.x * kWarps + wid;
   if (r >= N || (a.weight && a.weight[r] == 0.f)) return;
@@ -233,34 +235,54 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
   }
   b = warp_sum(b);
   if (!tail && any) sum = 1.f;
-  if (lane < 3 && a.k + lane < (a.k + 3) / 4 * 4) id[a.k + lane] = -2;  // (the list is read by fours)
+  // Repeated ids: a bit that is set already (by one of 8192 ids, so seldom by another id) asks for a look at the
+  // list; the first entry with an id stands for all of them.
+  uint32_t* seen = seen_bits[wid];
+  int* first = firsts[wid];
+  float* q_id = sums[wid];
+  for (int i = lane; i < kSeen / 32; i += 32) seen[i] = 0;
+#pragma unroll
+  for (int i = 0; i < kMaxTop / 32; ++i) {
+    const int k = lane + 32 * i;
+    if (k < a.k) {
+      first[k] = id[k];
+      q_id[k] = q[i];
+    }
+  }
+  __syncwarp();
+  for (int k0 = 0; k0 < a.k; k0 += 32) {
+    const int k = k0 + lane;
+    bool again = false;
+    if (k < a.k && id[k] >= 0) {
+      const int bit = id[k] & (kSeen - 1);
+      again = atomicOr(&seen[bit >> 5], 1u << (bit & 31)) >> (bit & 31) & 1;
+    }
+    for (uint32_t look = __ballot_sync(0xffffffffu, again); look; look &= look - 1) {
+      const int same = id[k0 + __ffs(look) - 1];
+      int one = a.k;
+      float total = 0.f;
+      for (int o = lane; o < a.k; o += 32) {
+        if (id[o] != same) continue;
+        one = min(one, o);
+        total += qr[o];
+      }
+      one = __reduce_min_sync(0xffffffffu, one);
+      total = warp_sum(total);
+      for (int o = lane; o < a.k; o += 32)
+        if (id[o] == same && o != one) first[o] = -1;
+      if (lane == 0) q_id[one] = total;
+      __syncwarp();
+    }
+  }
   __syncwarp();
   float s = 0.f;
 #pragma unroll
   for (int i = 0; i < kMaxTop / 32; ++i) {
     const int k = lane + 32 * i;
-    if (32 * i >= a.k) break;
-    const int mine = k < a.k ? id[k] : -1;
-    bool first = mine >= 0;
-    float q_id = q[i];
-    // Repeated ids: each is found once by itself; more often, the list is gone over again.
-    int found = 0;
-    for (int o = 0; o < a.k; o += 4) {
-      const int4 v = *reinterpret_cast<const int4*>(id + o);
-      found += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
-    }
-    if (first && found > 1) {
-      for (int o = 0; o < a.k; ++o) {
-        if (id[o] != mine || o == k) continue;
-        first = first && o > k;
-        q_id += qr[o];
-      }
-    }
-    if (first) s += y[i] == -INFINITY ? 0.f : expf(y[i] - y_ref);
-    if (k < a.k) {
-      Entry e = {first ? mine : -1, q_id, y[i], slope[i]};
-      reinterpret_cast<float4*>(entries)[r * a.k + k] = *reinterpret_cast<float4*>(&e);
-    }
+    if (k >= a.k) continue;
+    if (first[k] >= 0) s += y[i] == -INFINITY ? 0.f : expf(y[i] - y_ref);
+    Entry e = {first[k], q_id[k], y[i], slope[i]};
+    reinterpret_cast<float4*>(entries)[r * a.k + k] = *reinterpret_cast<float4*>(&e);
   }
   s = warp_sum(s);
   if (lane == 0) {

@@ -157,17 +157,18 @@ struct MaxOf {
 //
 // c tanh(x / c) is evaluated on the FMA pipe, as x P(v), v = x^2, P the minimax polynomial of tanh(u) / u in
 // u^2 (Remez exchange on tanh itself; the coefficients carry the powers of 1 / c^2): one for
-// |x| <= c / 2, where most logits lie, one for |x| <= c, and beyond that tanhf. (By exponential and reciprocal it
+// |x| <= c / 2, where most logits lie, one for |x| <= c. (By exponential and reciprocal it
 // would be two results of the special function unit, which gives 16 a clock on an SM and has the
 // softmax's exponential to do. A packed FMA takes two issue slots on sm_100, so what counts is operations:
 // the short polynomial saves two of about thirteen a logit.)
 struct Scale {
   float cap, limit, inv_temp, slope;  // limit: c^2, or -1 (no polynomial for this cap); slope = -1 / c^2
+  float twice;                        // 2 log2 e / c
   // 16-bit logits: P log2 e / tau (relative error 6e-8 and 2e-8), for sums
   f32x2 sum_full[7], sum_short[5];
   // 16-bit logits: P to 7e-7, for gradients that are rounded to 16 bits
   f32x2 z_full[6], z_short[4];
-  // 32-bit logits: Q of P = 1 + v Q, so that x enters unrounded
+  // 32-bit logits, and vectors with a logit beyond the cap: Q of P = 1 + v Q, so that x enters unrounded
   f32x2 q_full[6], q_short[4];
 };
 
@@ -191,6 +192,7 @@ inline Scale make_scale(float cap, float temp) {
   if (!(cap > 0.f)) return s;
   const double r = 1.0 / ((double)cap * cap), k = 1.4426950408889634 / (double)temp;
   s.slope = (float)-r;
+  s.twice = (float)(2.0 * 1.4426950408889634 / (double)cap);
   // (c^12 has to be an fp32 number; other caps take tanhf)
   s.limit = cap > 4e-3f && cap < 400.f ? cap * cap : -1.f;
   if (s.limit < 0.f) return s;
@@ -256,6 +258,22 @@ ME_DEVICE void vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f
     poly(sc.sum_short, sc.z_short, sc.q_short);
   } else if (top <= sc.limit) {
     poly(sc.sum_full, sc.z_full, sc.q_full);
+  } else if (sc.limit > 0.f) {
+    // Some logit is beyond the cap: there c (1 - 2 / (e^(2 |u|) + 1)) by the special function unit, whose error the
+    // small second term scales down (to 2e-6 at c = 30); the polynomial for the others.
+    all([&](f32x2 a) {
+      const f32x2 v = mul2(a, a);
+      const float2 f = unpack2(a), near = unpack2(fma2(mul2(a, v), horner2(sc.q_full, v), a));
+      float r[2] = {near.x, near.y};
+#pragma unroll
+      for (int l = 0; l < 2; ++l) {
+        const float x = l ? f.y : f.x, size = fabsf(x);
+        const float t = fmaf(-2.f, rcp_fast(exp2_fast(size * sc.twice) + 1.f), 1.f);
+        if (size > sc.cap) r[l] = copysignf(sc.cap * t, x);
+      }
+      const f32x2 z2 = pack2(r[0], r[1]);
+      return kExponent ? fma2(z2, both2(k), both2(-shift)) : z2;
+    });
   } else {
 #pragma unroll
     for (int u = 0; u < kV; ++u) {

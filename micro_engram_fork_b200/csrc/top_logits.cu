@@ -210,9 +210,10 @@ ME_DEVICE uint32_t kth_bound(const uint32_t (&keys)[kMaxGroups], int n, int k, B
   }
 }
 
-// One cluster a row. A thread's groups are 2^lg_group of its vectors each.
+// One cluster a row. A thread's groups are 2^lg_group of its vectors each. (Three blocks an SM where the softcap's
+// polynomial on 16-bit vectors wants more than 64 registers: 263 instead of 292 us for 2048 x 262144.)
 template <typename T, bool kCap>
-__global__ void __launch_bounds__(kThreads, 4)
+__global__ void __launch_bounds__(kThreads, kCap && sizeof(T) == 2 ? 3 : 4)
     top_kernel(Rows<const T> x, int V, int lg_ranks, int k, int lg_group, int groups, Scale sc,
                float* __restrict__ values, int64_t* __restrict__ ids, float* __restrict__ lse) {
   extern __shared__ uint4 dynamic[];
