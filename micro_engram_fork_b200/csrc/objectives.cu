@@ -482,7 +482,7 @@ void launch_logprob_fwd(const Logits& x, const int64_t* target, float* logp, flo
 
 void launch_logprob_bwd(const Logits& x, const int64_t* target, const float2* stats, RowValues g, Gradient out,
                         cudaStream_t stream) {
-  const int ranks = ranks_for_gradient(x, true);
+  const int ranks = ranks_for_gradient(x);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, logprob_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
                                          rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), target,
@@ -510,7 +510,7 @@ void launch_distill_fwd(const Logits& x, const TeacherArgs& te, const void* entr
 
 void launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows, float* loss,
                          Gradient out, cudaStream_t stream) {
-  const int ranks = ranks_for_gradient(x, false);
+  const int ranks = ranks_for_both(x);
   ME_LOGITS_DISPATCH(x.type, ME_CAP_DISPATCH(x.cap, {
     auto* kernel = te.lse ? distill_kernel<T, kCap, true, true> : distill_kernel<T, kCap, false, true>;
     const int smem = masks_for(x, te, ranks);
@@ -523,7 +523,7 @@ void launch_distill_grad(const Logits& x, const TeacherArgs& te, const void* ent
 
 void launch_distill_bwd(const Logits& x, const TeacherArgs& te, const void* entries, const void* rows,
                         const float4* stats, RowValues g, Gradient out, cudaStream_t stream) {
-  const int ranks = ranks_for_gradient(x, true);
+  const int ranks = ranks_for_gradient(x);
   ME_LOGITS_DISPATCH(
       x.type, ME_CAP_DISPATCH(x.cap, distill_bwd_kernel<T, kCap><<<(unsigned)(x.N * ranks), kThreads, 0, stream>>>(
                                          rows_in<T>(x), rows_out<T>(out), x.N, (int)x.V, ilog2(ranks), te.k, te.weight,

@@ -670,15 +670,26 @@ inline int ranks_for(int64_t N, int64_t V, int per_sm = 4) {
   while (c < 8 && N * c < per_sm * objective_sms() && V / (2 * c) >= 4096) c *= 2;
   return c;
 }
-// The same for the kernels that write a gradient. Where a row's blocks wait for one another, two for long rows (a
-// thread keeps 32 vectors or more; distillation of 2048 x 262144 by 1 / 2 / 4 / 8: 430 / 417 / 418 / 438 us);
-// where they do not, as many as leave a thread 16 vectors (the preference step's backward pass, 1024 of 2048 rows
-// trained, by 1 / 2 / 4 / 8: the step takes 397 / 385 / 372 / 366 us).
-inline int ranks_for_gradient(const Logits& x, bool alone) {
+// The same for the backward pass alone, whose blocks do not wait for one another: as many as leave a thread 16
+// vectors (the preference step with 1024 of 2048 rows of 262144 trained, by 1 / 2 / 4 / 8: 397 / 385 / 372 / 366 us).
+inline int ranks_for_gradient(const Logits& x) {
   const int64_t vecs = x.V * (x.type == LogitType::kF32 ? 4 : 2) / 16;
-  const int most = alone ? 8 : 2, least = alone ? 16 : 32;
   int c = ranks_for(x.N, x.V);
-  while (c < most && vecs / (2 * c) >= least * kThreads) c *= 2;
+  while (c < 8 && vecs / (2 * c) >= 16 * kThreads) c *= 2;
+  return c;
+}
+
+// And for value and gradient in one kernel, which reads a row twice. More blocks a row: fewer rows in flight, so that the
+// second read finds them in L2; but what a block does once a row counts for more. 16-bit logits with a softcap are
+// bound by arithmetic: two where a thread keeps 32 vectors then (1024 x 262144 by 1 / 2 / 4 / 8: 277 / 262 / 264 /
+// 298 us; 100000: 116 / 118 / 145 / 185). The others by memory: until the rows in flight take 64 MB, while a thread
+// keeps 16 vectors (bf16 without a cap, 262144: 258 / 254 / 238 / 219, 100000: 103 / 95 / 113 / 150; fp32, 262144:
+// 505 / 503 / 488 / 460, 100000: 204 / 197 / 178 / 226).
+inline int ranks_for_both(const Logits& x) {
+  const int64_t row = x.V * (x.type == LogitType::kF32 ? 4 : 2), vecs = row / 16;
+  int c = ranks_for(x.N, x.V);
+  if (x.cap > 0.f && x.type != LogitType::kF32) return c == 1 && vecs / 2 >= 32 * kThreads ? 2 : c;
+  while (c < 8 && 4 * objective_sms() / c * row > (64 << 20) && vecs / (2 * c) >= 16 * kThreads) c *= 2;
   return c;
 }
 
