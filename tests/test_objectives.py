@@ -143,6 +143,20 @@ def test_leading_dimensions_and_out():
     assert dx2 is y and torch.equal(dx, y) and torch.equal(loss, loss2) and loss.shape == (2, 3)
 
 
+def test_one_call_forms():
+    x = torch.randn(6, 40)
+    t = torch.tensor([0, 39, -100, 5, 6, 7])
+    coef = torch.randn(6)
+    leaf = x.clone().requires_grad_()
+    logp = O.token_logprobs(leaf, t, softcap=4.0)
+    logp.backward(coef)
+    got, dx = O.token_logprobs_grad(x, t, coef, softcap=4.0)
+    assert torch.equal(got, logp.detach()) and torch.equal(dx, leaf.grad)
+    got, dx = O.token_logprobs_grad(x.view(2, 3, 40), t.view(2, 3), softcap=4.0)
+    assert got.shape == (2, 3) and dx.shape == (2, 3, 40)
+    assert torch.equal(dx.view(6, 40), O.token_logprobs_grad(x, t, torch.ones(6), softcap=4.0)[1])
+
+
 def refusals(dev):
     """(what is refused, the call) on `dev`; shared with the GPU tests."""
     x = torch.randn(4, 9, device=dev)
@@ -159,6 +173,7 @@ def refusals(dev):
         "empty vocabulary": lambda: O.token_logprobs(x[:, :0], t),
         "targets' shape": lambda: O.token_logprobs(x, t[:3]),
         "targets' type": lambda: O.token_logprobs(x, t.float()),
+        "coefficients": lambda: O.token_logprobs_grad(x, t, torch.ones(3, device=dev)),
         "teacher's shapes": lambda: O.distill_loss(x, ids, top[:, :1]),
         "teacher's rows": lambda: O.distill_loss(x, ids[:3], top[:3]),
         "teacher's ids": lambda: O.distill_loss(x, ids.float(), top),

@@ -99,6 +99,59 @@ def test_distill(N, V, pitch, shift, dtype, cap, temp, tail):
     assert dx3 is inplace and torch.equal(dx3, dx) and torch.equal(loss3, loss)
 
 
+@pytest.mark.parametrize("dtype,cap", [(BF, 30.0), (HF, 12.0), (FP, 30.0), (BF, 1e-3), (FP, 1000.0)])
+def test_beyond_the_cap(dtype, cap):
+    """Logits on both sides of the cap in the same vectors, and caps for which there is no polynomial."""
+    N, V = 9, 20011
+    x = (torch.randn(N, V, device=DEV, generator=_gen(1)) * 25).to(dtype)
+    x[:, 5] = float("inf")
+    x[:, 6] = -float("inf")
+    t = torch.randint(0, V, (N,), device=DEV, generator=_gen(2))
+    t[0] = 5
+    coef = torch.randn(N, device=DEV, generator=_gen(3))
+    logp, dx = O.token_logprobs_grad(x, t, coef, softcap=cap)
+    finite = x.clamp(-3e4, 3e4)  # the same z, and derivatives that the oracle can take
+    want, grad, mass = oracle.logprobs(finite, t, cap, coef)
+    oracle.close_logp(logp, want, finite, cap)
+    oracle.close_grad(dx, grad, coef, mass, dtype)
+    leaf = x.detach().requires_grad_()
+    logp2 = O.token_logprobs(leaf, t, softcap=cap)
+    assert torch.equal(logp2.detach(), logp)
+    assert torch.equal(torch.autograd.grad(logp2, leaf, coef)[0], dx)
+
+
+def test_rows_longer_than_the_masks():
+    """More vectors in a block's slice than there are bytes for the teacher's entries (they are shared then)."""
+    N, V, k = 2, 2300011, 200
+    x = _x(N, V, BF, 5)
+    ids, top = _teacher(N, V, k, 6)
+    ids[0, :3] = torch.tensor([17, 17 + 32768 * 8, V - 1], device=DEV)
+    lse = torch.logsumexp(top, 1) + 0.5
+    w = torch.ones(N, device=DEV)
+    loss, dx = O.distill_loss_grad(x, ids, top, lse, w, softcap=30.0)
+    want, grad, mass = oracle.distill(x, ids, top, lse, w, 30.0, 1.0)
+    oracle.close_logp(loss, want, x, 30.0, factor=8)
+    oracle.close_grad(dx, grad, w, mass, BF)
+    _check_top(x, 100, 30.0, 1.0)
+
+
+def test_padded_rows_keep_their_pitch():
+    x = _x(40, 5003, BF, 3, pitch=5)
+    t = torch.randint(0, 5003, (40,), device=DEV, generator=_gen(1))
+    leaf = x.detach().requires_grad_()
+    dx, = torch.autograd.grad(O.token_logprobs(leaf, t, softcap=30.0).sum(), leaf)
+    _, same = O.token_logprobs_grad(x.contiguous(), t, None, softcap=30.0)
+    assert dx.shape == x.shape and torch.allclose(dx.float(), same.float(), rtol=2.0 ** -7, atol=1e-9)
+    _, wide = O.token_logprobs_grad(x, t, None, softcap=30.0, out=torch.empty(40, 5003, dtype=BF, device=DEV))
+    assert torch.equal(wide, dx)
+
+
+def test_gradients_are_not_differentiated():
+    x = _x(3, 64, FP).requires_grad_()
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(O.token_logprobs(x, torch.zeros(3, dtype=torch.int64, device=DEV)).sum(), x, create_graph=True)
+
+
 def test_distill_repeated_and_foreign_ids():
     x = _x(3, 4097, BF, 3)
     ids = torch.tensor([[5, 5, 9, -1], [4096, 0, 4097, 1 << 40], [7, 7, 7, 7]], device=DEV)
