@@ -478,8 +478,7 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
 // that are left out (`drop.column(j)` for a single column).
 //
 // One pass with a fixed reference: the largest z of the thread's first vectors, so no running maximum
-// is carried. A share that this does not suit (a sum out of range, a first batch of -inf, a NaN or
-// +inf anywhere) is added again element by element with a running maximum.
+// is carried. A share that this does not suit (a sum out of range, a NaN or +inf anywhere) is added again element by element with a running maximum.
 //
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
 // moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
@@ -505,7 +504,9 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
 #pragma unroll
         for (int u = 0; u < kFirst; ++u)
           if (u < n) top.add(v[u]);
-        ref = kCap ? softcap(top.value(), sc.cap) : top.value() * sc.inv_temp;
+        // (masked columns only, -inf or the type's lowest: 0 suits the others as well as any)
+        const float lowest = std::is_same_v<T, __half> ? -65504.f : -1e38f;
+        ref = kCap ? softcap(top.value(), sc.cap) : top.value() > lowest ? top.value() * sc.inv_temp : 0.f;
         shift = kCap ? ref * k : ref;
       },
       [&](const auto& x, int i, auto whole) {
@@ -556,7 +557,7 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
       });
   const float s = sum0 + sum1;
   const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big.value() * sc.inv_temp - ref;  // the largest exponent
-  if (count > 0 && s > 1e-30f && s < 1e37f && far < 80.f) {
+  if (count > 0 && s > 1e-20f && s < 1e37f && far < 80.f) {  // (masked columns add 2e-38 each)
     // (m is rounded: what separates it from the shift that was taken goes into s)
     out.m = kCap ? ref * sc.inv_temp : ref;
     out.s = kCap ? s * exp2_fast(fmaf(-out.m, kLog2e, shift) - out.m * 1.925963033500011e-08f) : s;
@@ -602,6 +603,7 @@ ME_DEVICE MaxSum row_merge(MaxSum a, float2* part, int lg_ranks) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   a = warp_merge(a);
   if (lane == 0) part[wid] = make_float2(a.m, a.s);
+  __syncwarp();
   MaxSum r;
   if (lg_ranks == 0) {
     __syncthreads();
@@ -624,6 +626,7 @@ ME_DEVICE MaxSum row_merge(MaxSum a, float2* part, int lg_ranks) {
   return warp_merge(r);
 }
 ME_DEVICE void row_done(int lg_ranks) {
+  __syncwarp();
   if (lg_ranks > 0) cluster_wait();
 }
 

@@ -260,6 +260,42 @@ def test_non_finite(dtype, V, cap):
         assert torch.equal(dx[finite].isnan(), dref[finite].isnan())
 
 
+@pytest.mark.parametrize("low", [-float("inf"), None])
+@pytest.mark.parametrize("dtype", [BF, HF, FP])
+def test_masked_columns(dtype, low):
+    """Most columns masked (-inf, or the type's lowest value), ahead of the others or between them."""
+    N, V, k = 6, 30011, 16
+    x = _x(N, V, dtype, 3)
+    low = torch.finfo(dtype).min if low is None else low
+    x[:3, : V - 700] = low
+    x[3:, (torch.arange(V, device=DEV) % 50) != 7] = low
+    x[2] -= 900 if dtype != HF else 200
+    keep = [torch.arange(V - 700, V, device=DEV)] * 3 + [torch.arange(7, V, 50, device=DEV)] * 3
+    g = _gen(5)
+    t = torch.stack([c[torch.randint(0, c.numel(), (1,), device=DEV, generator=g)][0] for c in keep])
+    ids = torch.stack([c[torch.randperm(c.numel(), device=DEV, generator=g)[:k]] for c in keep])
+    top = torch.randn(N, k, device=DEV, generator=g) * 3
+    coef = torch.randn(N, device=DEV, generator=g)
+    logp, dx = O.token_logprobs_grad(x, t, coef)
+    z = torch.where(x.double() <= torch.finfo(dtype).min, -float("inf"), x.double())  # the lowest value has p = 0 too
+    want, grad, mass = oracle.logprobs(z, t, None, coef)
+    oracle.close_logp(logp, want, torch.where(z.isinf(), 0.0, z), None)
+    oracle.close_grad(dx, torch.where(z.isinf(), 0.0, grad), coef, mass, dtype)
+    w = torch.ones(N, device=DEV)
+    for lse in (None, torch.logsumexp(top, 1) + 0.5):
+        loss, dx = O.distill_loss_grad(x, ids, top, lse, w)
+        for r in range(N):  # the kept columns alone are the same problem
+            at = torch.searchsorted(keep[r], ids[r])[None]
+            want, grad, mass = oracle.distill(x[r:r + 1, keep[r]], at, top[r:r + 1], None if lse is None else lse[r:r + 1],
+                                              w[:1], None, 1.0)
+            oracle.close_logp(loss[r:r + 1], want, x[r:r + 1, keep[r]], None, factor=8)
+            oracle.close_grad(dx[r:r + 1, keep[r]], grad, w[:1], mass, dtype)
+        assert int((dx != 0).sum()) <= sum(c.numel() for c in keep)
+    values, at, lse = O.top_logits(x, k)
+    assert torch.equal(at, torch.sort(x.double(), dim=1, descending=True, stable=True)[1][:, :k])
+    oracle.close_logp(lse, torch.logsumexp(z, 1), torch.where(z.isinf(), 0.0, z), None)
+
+
 @pytest.mark.parametrize("kind", O.KINDS)
 @pytest.mark.parametrize("cu_type", [torch.int32, torch.int64])
 def test_pairs(kind, cu_type):
