@@ -90,6 +90,8 @@ ME_DEVICE void zero_slice(const Slice<T>& sl, T* out) {
 }
 
 // ------------------------------------------------------------------------------------ log-probabilities
+// One cluster a row, one walk. Bound by issue slots under a softcap (97 for 8 logits a thread): 2048 x 262144 bf16,
+// softcap 30, 198 us, 0.82 of the copy rate with every row counted; fp32 without one runs at the copy rate.
 template <typename T, bool kCap>
 __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> x, int V, int lg_ranks,
                                                                   const int64_t* __restrict__ target, Scale sc,
@@ -118,7 +120,8 @@ __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> 
   row_done(lg_ranks);
 }
 
-// Rows are taken last to first: where the forward pass just went over them, the last ones are in L2.
+// Rows are taken last to first: where the forward pass just went over them, the last ones are in L2. Bound by memory, one
+// read and one write of a logit: 0.75 of the DRAM's peak for 1184 x 262144 bf16 with half of the rows trained.
 template <typename T, bool kCap>
 __global__ void __launch_bounds__(kThreads, 4) logprob_bwd_kernel(Rows<const T> x, Rows<T> out, int64_t N, int V,
                                                                   int lg_ranks, const int64_t* __restrict__ target,
@@ -378,7 +381,8 @@ ME_DEVICE void write_entry(const Slice<T>& sl, T* out, const Entry& e, float c, 
 
 // One cluster a row. Value, and the statistics that the backward pass starts from: m, s (-1: a row without
 // gradient), m', c'; or with kGrad value and gradient: the slice is read again once the cluster has the
-// row's sum, from L2 where the rows in flight fit there.
+// row's sum, from L2 where the rows in flight fit there (1024 x 262144 bf16: 262 us with a softcap, where they do not,
+// for 164 us of one read and one write; 219 us without one).
 template <typename T, bool kCap, bool kTail, bool kGrad>
 __global__ void __launch_bounds__(kThreads, 4)
     distill_kernel(Rows<const T> x, Rows<T> out, int V, int lg_ranks, int k, const float* __restrict__ weight,
