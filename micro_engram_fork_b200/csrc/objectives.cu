@@ -35,9 +35,8 @@ ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float 
       [&](const auto& x, int i, auto whole) {
         constexpr int kV = sizeof(x) / sizeof(uint4);
         f32x2 z[kV][kP];
-        [[maybe_unused]] bool beyond = false;
         if constexpr (kCap) {
-          beyond = vec_softcap<T, false, decltype(whole)::value>(x, sc, 0.f, z);
+          vec_softcap<T, false, decltype(whole)::value>(x, sc, 0.f, z);
         } else {
 #pragma unroll
           for (int u = 0; u < kV; ++u) to_pairs<T>(x[u], z[u]);
@@ -51,16 +50,7 @@ ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float 
             const float2 a = unpack2(sizeof(T) == 4 ? mul2(fma2(zp, both2(sc.inv_temp), both2(-m)), both2(kLog2e))
                                                     : fma2(zp, both2(k), both2(-shift)));
             const f32x2 e = pack2(exp2_fast(a.x), exp2_fast(a.y));
-            f32x2 slope = both2(coef);
-            if constexpr (kCap) {
-              if (beyond) {  // (1 - t^2 of t itself: exactly 0 where the cap is reached)
-                const f32x2 t = mul2(zp, both2(sc.inv_cap));
-                slope = mul2(slope, fma2(mul2(t, both2(-1.f)), t, both2(1.f)));
-              } else {
-                slope = fma2(mul2(zp, both2(coef_slope)), zp, both2(coef));
-              }
-            }
-            z[u][p] = mul2(e, slope);
+            z[u][p] = mul2(e, kCap ? fma2(mul2(zp, both2(coef_slope)), zp, both2(coef)) : both2(coef));
           }
           Vec16<T> r;
           r.u = from_pairs<T>(z[u]);

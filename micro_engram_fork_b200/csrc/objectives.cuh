@@ -163,7 +163,7 @@ struct MaxOf {
 // the short polynomial saves two of about thirteen a logit.)
 struct Scale {
   float cap, limit, inv_temp, slope;  // limit: c^2, or -1 (no polynomial for this cap); slope = -1 / c^2
-  float twice, inv_cap;               // 2 log2 e / c, 1 / c
+  float twice;                        // 2 log2 e / c
   // 16-bit logits: P log2 e / tau (relative error 6e-8 and 2e-8), for sums
   f32x2 sum_full[7], sum_short[5];
   // 16-bit logits: P to 7e-7, for gradients that are rounded to 16 bits
@@ -193,7 +193,6 @@ inline Scale make_scale(float cap, float temp) {
   const double r = 1.0 / ((double)cap * cap), k = 1.4426950408889634 / (double)temp;
   s.slope = (float)-r;
   s.twice = (float)(2.0 * 1.4426950408889634 / (double)cap);
-  s.inv_cap = (float)(1.0 / (double)cap);
   // (c^12 has to be an fp32 number; other caps take tanhf)
   s.limit = cap > 4e-3f && cap < 400.f ? cap * cap : -1.f;
   if (s.limit < 0.f) return s;
@@ -221,10 +220,10 @@ inline Scale make_scale(float cap, float temp) {
   return s;
 }
 
-// z of kV vectors (kExponent false), or the exponents z log2 e / tau - shift (true). kWhole: every lane of the
-// warp is here. Returns whether some logit is beyond the cap.
+// z of kV vectors (kExponent false), or the exponents z log2 e / tau - shift (true). `whole`: every lane of the
+// warp is here.
 template <typename T, bool kExponent, bool kWhole, int kV>
-ME_DEVICE bool vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f32x2 (&z)[kV][Vec16<T>::kN / 2]) {
+ME_DEVICE void vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f32x2 (&z)[kV][Vec16<T>::kN / 2]) {
   constexpr int kP = Vec16<T>::kN / 2;
   const float k = sc.inv_temp * kLog2e;
   float top = 0.f;
@@ -257,10 +256,8 @@ ME_DEVICE bool vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f
   // (the warp takes the short polynomial together: a divided warp would pay for both)
   if (kWhole && __all_sync(0xffffffffu, top <= 0.25f * sc.limit)) {
     poly(sc.sum_short, sc.z_short, sc.q_short);
-    return false;
   } else if (top <= sc.limit) {
     poly(sc.sum_full, sc.z_full, sc.q_full);
-    return false;
   } else if (sc.limit > 0.f) {
     // Some logit is beyond the cap: there c (1 - 2 / (e^(2 |u|) + 1)) by the special function unit, whose error the
     // small second term scales down (to 2e-6 at c = 30); the polynomial for the others.
@@ -295,7 +292,6 @@ ME_DEVICE bool vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f
       }
     }
   }
-  return true;
 }
 
 // e^d of a pair, -87 <= d <= 88: d = n ln 2 + r with n whole (Cody and Waite's two-step reduction), 2^n
