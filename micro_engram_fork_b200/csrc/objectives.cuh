@@ -294,17 +294,20 @@ ME_DEVICE void vec_softcap(const uint4 (&x)[kV], const Scale& sc, float shift, f
   }
 }
 
-// e^d of a pair, -87 <= d <= 88: d = n ln 2 + r with n whole (Cody and Waite's two-step reduction), 2^n
-// added to the exponent of 2^(r / ln 2). The reduction keeps the argument's rounding out of the result,
-// which a sum of many terms would otherwise carry (1e-7 mean error at d = -10 with ex2 alone).
+// e^d of a pair, -87 <= d <= 88: the argument is reduced as in Cody and Waite, "Software Manual for the Elementary
+// Functions" (1980), chapter 6: n = d / ln 2 rounded to a whole number, r = d - n ln 2, e^d = 2^n e^r. An FMA forms
+// d - n ln 2 with one rounding, at the size of r, so the first of their two constants is enough: what fp32 leaves out
+// of ln 2 (1.9e-9) moves e^d by 3e-8 at d = -10. e^r is ex2 of r log2 e, |r| <= 0.35, and 2^n goes onto the exponent.
+// (ex2 of d log2 e itself carries that product's rounding, up to 5e-7 at d = -10, into a sum of many terms.) A NaN gives
+// a NaN or 3e38: either way the sum that it enters is out of range.
 ME_DEVICE f32x2 exp_pair(f32x2 d) {
-  const float kMagic = 12582912.f;  // 1.5 * 2^23: adding it rounds to a whole number in the low bits
-  const f32x2 t = fma2(d, both2(kLog2e), both2(kMagic));
-  f32x2 f = fma2(d, both2(kLog2e), fma2(t, both2(-1.f), both2(kMagic)));  // d log2 e - n
-  f = fma2(d, both2(1.925963033500011e-8f), f);  // log2 e - its fp32 value
-  const float2 g = unpack2(f), m = unpack2(t);
-  return pack2(__uint_as_float(__float_as_uint(exp2_fast(g.x)) + (__float_as_uint(m.x) << 23)),
-               __uint_as_float(__float_as_uint(exp2_fast(g.y)) + (__float_as_uint(m.y) << 23)));
+  const float kWhole = 12582912.f;  // 1.5 * 2^23: the fp32 numbers around it are the whole ones
+  const float kLn2 = 0.693147180559945309f;
+  const f32x2 t = fma2(d, both2(kLog2e), both2(kWhole));  // n + 1.5 * 2^23: n stands in the low bits
+  const f32x2 r = fma2(add2(t, both2(-kWhole)), both2(-kLn2), d);
+  const float2 g = unpack2(mul2(r, both2(kLog2e))), n = unpack2(t);
+  return pack2(__uint_as_float(__float_as_uint(exp2_fast(g.x)) + (__float_as_uint(n.x) << 23)),
+               __uint_as_float(__float_as_uint(exp2_fast(g.y)) + (__float_as_uint(n.y) << 23)));
 }
 // max(a, b) that keeps a NaN
 ME_DEVICE float max_nan(float a, float b) {
@@ -481,8 +484,8 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
 // is carried. A share that this does not suit (a sum out of range, a NaN or +inf anywhere) is added again element by element with a running maximum.
 //
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
-// moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one the two-step
-// form, since nothing else is rounded then.
+// moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one exp_pair(),
+// since nothing else is rounded then.
 // watch(x, i): sees the thread's vectors from the i-th on, one or two at a time, in order.
 struct WatchNothing {
   template <typename X>
@@ -560,7 +563,7 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
   if (count > 0 && s > 1e-20f && s < 1e37f && far < 80.f) {  // (masked columns add 2e-38 each)
     // (m is rounded: what separates it from the shift that was taken goes into s)
     out.m = kCap ? ref * sc.inv_temp : ref;
-    out.s = kCap ? s * exp2_fast(fmaf(-out.m, kLog2e, shift) - out.m * 1.925963033500011e-08f) : s;
+    out.s = kCap ? s * exp2_fast((float)(shift - 1.4426950408889634 * out.m)) : s;
   } else {
     for (int i = 0; i < count; ++i) {
       const uint32_t out_mask = drop(sl.vec(i));

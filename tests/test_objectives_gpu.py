@@ -1,5 +1,7 @@
 """Vocabulary objectives on the sm_100a kernels: against the 64-bit definitions at the sizes, types,
 strides and masks where they can go wrong; edge rules as on the CPU; streams, repeatability, refusals."""
+import math
+
 import pytest
 import torch
 
@@ -466,3 +468,21 @@ def test_native_refusals():
         O.preference_loss(torch.zeros(4, device=DEV), None, torch.tensor([0, 1, 4]))
     with pytest.raises(RuntimeError, match="apart"):
         O.distill_loss_grad(x, t[:, None], torch.zeros(4, 1, device=DEV), out=x[:1].expand(4, 64))
+
+
+def test_exponential_alone():
+    """Rows whose sum is 2^q equal terms e^d with d close to -q ln 2, so that its logarithm is close to 0 and nothing but
+    the exponential rounds: a thread's first four vectors are masked (its sum's reference is 0 then), its others hold
+    two terms at most in each of two partial sums, and the sums of threads are powers of two times one term."""
+    V, per = 8188, 64
+    i = torch.arange(1024, device=DEV)
+    place = 4096 + 4 * (i % 256) + i // 256 % 2 + 1024 * (i // 512)
+    delta = torch.linspace(-0.345, 0.345, per, dtype=torch.float64, device=DEV)
+    q = torch.arange(11, device=DEV).repeat_interleave(per)
+    d = (delta.repeat(11) - q * math.log(2)).float()
+    x = torch.where(i < (1 << q).unsqueeze(1), d.unsqueeze(1), -float("inf"))
+    whole = torch.full((q.numel(), V), -float("inf"), device=DEV)
+    whole[:, place] = x
+    want = d.double() + q * math.log(2)
+    # ex2's 2^-22; ln 2 and log2 e in fp32, the roundings of r and of its product: 6e-8; the logarithm's two units
+    assert float((O.top_logits(whole, 1)[2].double() - want).abs().max()) <= 3 * 2.0 ** -23
