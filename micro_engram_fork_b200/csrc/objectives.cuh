@@ -586,8 +586,15 @@ ME_DEVICE MaxSum warp_merge(MaxSum a) {
 }
 
 // ---------------------------------------------------------------- thread-block clusters
-ME_DEVICE void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
-ME_DEVICE void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+// (.aligned: the lanes of a warp have to execute them together, whatever divergent code came before)
+ME_DEVICE void cluster_arrive() {
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+ME_DEVICE void cluster_wait() {
+  __syncwarp();
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
 // A pair in the shared memory of the cluster's block `rank`, at the place that `p` has in this one.
 ME_DEVICE float2 cluster_load(const float2* p, uint32_t rank) {
   uint32_t a = (uint32_t)__cvta_generic_to_shared(p), b;
@@ -606,7 +613,6 @@ ME_DEVICE MaxSum row_merge(MaxSum a, float2* part, int lg_ranks) {
   const int lane = threadIdx.x & 31, wid = threadIdx.x >> 5;
   a = warp_merge(a);
   if (lane == 0) part[wid] = make_float2(a.m, a.s);
-  __syncwarp();
   MaxSum r;
   if (lg_ranks == 0) {
     __syncthreads();
@@ -629,7 +635,6 @@ ME_DEVICE MaxSum row_merge(MaxSum a, float2* part, int lg_ranks) {
   return warp_merge(r);
 }
 ME_DEVICE void row_done(int lg_ranks) {
-  __syncwarp();
   if (lg_ranks > 0) cluster_wait();
 }
 

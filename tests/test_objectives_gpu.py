@@ -486,3 +486,42 @@ def test_exponential_alone():
     want = d.double() + q * math.log(2)
     # ex2's 2^-22; ln 2 and log2 e in fp32, the roundings of r and of its product: 6e-8; the logarithm's two units
     assert float((O.top_logits(whole, 1)[2].double() - want).abs().max()) <= 3 * 2.0 ** -23
+
+
+@pytest.mark.parametrize("V", [8200, 12005, 16301])
+@pytest.mark.parametrize("dtype", [BF, FP])
+def test_two_blocks_a_row(dtype, V):
+    """Half a warp merges the shares of two blocks, and each lane by its own branch: shares of masked columns alone, of
+    NaN and of numbers side by side; the same bits again and again."""
+    inf, nan = float("inf"), float("nan")
+    x = _x(9, V, dtype, V)
+    x[0, : V // 2 + 64] = -inf      # nothing in the first block
+    x[1, V // 2 - 64:] = -inf       # nothing in the second one
+    x[2, V - 1000] = nan
+    x[3, 1000] = inf
+    x[4, (torch.arange(V, device=DEV) // 256) % 2 == 0] = -inf  # nothing for some of the warps
+    x[5] = -inf
+    x[6, : V - 1] = -inf
+    x[7, :2100] = -inf
+    t = torch.full((9,), V - 1, device=DEV)
+    t[1] = 5
+    want, grad = O.token_logprobs_ref(x.double(), t)
+    dref = grad(torch.ones(9, device=DEV))
+    ids, top = t[:, None], torch.zeros(9, 1, device=DEV)
+    loss64, _ = O.distill_ref(x.double(), ids, top.double(), torch.ones(9, device=DEV))
+    first = None
+    for _ in range(20):
+        logp, dx = O.token_logprobs_grad(x, t)
+        loss, dd = O.distill_loss_grad(x, ids, top, torch.ones(9, device=DEV))
+        lse = O.top_logits(x, 3)[2]
+        out = [logp, dx, loss, dd, lse]
+        first = first or out
+        for a, b in zip(out, first):
+            assert torch.equal(a.nan_to_num(7.0), b.nan_to_num(7.0)) and torch.equal(a.isnan(), b.isnan())
+    assert torch.equal(logp.isnan(), want.isnan()) and want.isnan().tolist() == [False] * 2 + [True] * 2 + [False, True] + [False] * 3
+    ok = ~want.isnan()
+    assert torch.allclose(logp[ok].double(), want[ok], rtol=1e-5, atol=1e-5)
+    oracle.close_grad(dx[ok], dref[ok], torch.ones(int(ok.sum()), device=DEV), torch.ones_like(dref[ok]), dtype)
+    assert torch.equal(loss.isfinite(), loss64.isfinite())
+    some = loss64.isfinite()
+    assert torch.allclose(loss[some].double(), loss64[some], rtol=1e-4, atol=1e-5)
