@@ -248,8 +248,10 @@ ME_DEVICE uint32_t mapa_shared(uint32_t saddr, uint32_t rank) {
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
   return r;
 }
-// All threads of every CTA in the cluster (release/acquire at cluster scope).
+// All threads of every CTA in the cluster (release/acquire at cluster scope). The barrier is an aligned one: the lanes
+// of a warp that left each other (one of them sets up barriers) come together first.
 ME_DEVICE void cluster_sync() {
+  __syncwarp();
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // Arrive (release, cluster scope) on an mbarrier given by its shared::cluster address.
