@@ -327,7 +327,7 @@ struct Rows {
 };
 
 // A block's share of one row: 16-byte vectors [begin, end) from `head` on, and for the row's first and
-// last block the elements ahead of the first 16-byte boundary and after the last one. (V is below 2^31.)
+// last block the elements ahead of the first 16-byte boundary and after the last one. (V is at most kMaxColumns.)
 template <typename T>
 struct Slice {
   static constexpr int kN = Vec16<T>::kN;

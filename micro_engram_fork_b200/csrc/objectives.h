@@ -9,6 +9,9 @@ namespace me {
 
 constexpr int64_t kIgnoreToken = -100;  // the target of an untrained token
 constexpr int kMaxTop = 256;            // most teacher entries / top logits of a row
+// Most columns of a row. The kernels count them in 32 bits, and a loop that steps by a block's threads (or by their
+// vectors: 256 times 8 columns) ends up to 2048 past the row's end.
+constexpr int64_t kMaxColumns = INT32_MAX - 4096;
 
 enum class LogitType : int { kBF16 = 0, kF16 = 1, kF32 = 2 };
 

@@ -46,8 +46,8 @@ me::Logits check_logits(const Tensor& x, const OptDouble& cap, const char* what)
   TORCH_CHECK(x.is_cuda(), what, ": a CUDA tensor is needed");
   ME_CHECK_VALUE(x.dim() == 2 && x.is_floating_point(), what, ": logits [rows, V] of a floating type are needed, got ",
                     x.scalar_type(), " of shape ", shape(x));
-  ME_CHECK_VALUE(x.size(1) > 0 && x.size(1) <= INT32_MAX, what, ": a vocabulary of 1 to 2^31 - 1 entries is needed, got ",
-                    text(x.size(1)));
+  ME_CHECK_VALUE(x.size(1) > 0 && x.size(1) <= me::kMaxColumns, what, ": a vocabulary of 1 to ", text(me::kMaxColumns),
+                    " entries is needed, got ", text(x.size(1)));
   TORCH_CHECK(x.size(0) < (1 << 28), what, ": 2^28 - 1 rows at most, got ", text(x.size(0)));
   TORCH_CHECK(x.size(1) == 1 || x.stride(1) == 1, what, ": a row's logits have to be contiguous");
   me::LogitType type = me::LogitType::kF32;

@@ -21,6 +21,7 @@ and are the tests' second opinion. Rules that hold for both:
 
   targets       -100 is an untrained token: log-probability 0, gradient 0, its logits are not read.
                 Any other target outside [0, V) gives NaN.
+  logits        V is at most 2^31 - 4097 for the kernels, k (teacher's entries, top logits) at most 256
   teacher_ids   an id outside [0, V) is an unused entry; ids of one row are distinct (a repeated id
                 counts as the sum of its probabilities)
   weights       0 is an untrained token: loss 0, gradient 0, whatever its logits hold

@@ -525,3 +525,15 @@ def test_two_blocks_a_row(dtype, V):
     assert torch.equal(loss.isfinite(), loss64.isfinite())
     some = loss64.isfinite()
     assert torch.allclose(loss[some].double(), loss64[some], rtol=1e-4, atol=1e-5)
+
+
+@pytest.mark.parametrize("V", [2 ** 31 - 100, 2 ** 31 - 4096, 2 ** 31 + 5])
+def test_too_many_columns(V):
+    """Rows whose column numbers would pass 32 bits within a loop are refused (nothing is read: one element, expanded)."""
+    x = torch.zeros(1, 1, device=DEV, dtype=BF).expand(2, V)
+    t = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for call in (lambda: O.top_logits(x, 1), lambda: O.token_logprobs(x, t), lambda: O.token_logprobs_grad(x, t),
+                 lambda: O.distill_loss_grad(x, t[:, None], torch.zeros(2, 1, device=DEV)),
+                 lambda: O.preference_logits_grad(x, t, None, torch.tensor([0, 1, 2], device=DEV))):
+        with pytest.raises(ValueError, match="vocabulary"):
+            call()
