@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
   int* id = ids[wid];
   float* qr = qs[wid];
   float t[kMaxTop / 32], y[kMaxTop / 32], slope[kMaxTop / 32];
-  float m = -INFINITY, y_ref = -INFINITY, used = 0.f;
+  float m = -INFINITY, y_ref = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kMaxTop / 32; ++i) {
     const int k = lane + 32 * i;
@@ -208,7 +208,6 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
     slope[i] = softcap_slope(z, sc.cap);
     m = fmaxf(m, t[i]);
     y_ref = fmaxf(y_ref, y[i]);
-    used += 1.f;
   }
   m = tail ? a.lse[r] : warp_max(m);
   y_ref = warp_max(y_ref);
@@ -223,20 +222,14 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
     any = any || q[i] != 0.f;
   }
   sum = warp_sum(sum);
-  used = warp_sum(used);
   any = __any_sync(0xffffffffu, any);
   const float inv = tail || !any ? 1.f : 1.f / sum, log_s = tail ? 0.f : logf(sum);
-  float b = 0.f;
 #pragma unroll
   for (int i = 0; i < kMaxTop / 32; ++i) {
     const int k = lane + 32 * i;
     q[i] *= inv;
     if (k < a.k) qr[k] = q[i];
-    if (q[i] == 0.f) continue;
-    // maxima first: what is left to round is of the size of the difference
-    b += y[i] == -INFINITY ? INFINITY : q[i] * (((t[i] - m) - (y[i] - y_ref)) - log_s);
   }
-  b = warp_sum(b);
   if (!tail && any) sum = 1.f;
   // Repeated ids: a bit that is set already (by one of 8192 ids, so seldom by another id) asks for a look at the
   // list; the first entry with an id stands for all of them.
@@ -278,16 +271,26 @@ __global__ void __launch_bounds__(kThreads) teacher_kernel(Rows<const T> x, int6
     }
   }
   __syncwarp();
-  float s = 0.f;
+  // what the loss needs, by ids: q log q of an id's whole probability
+  float b = 0.f, s = 0.f, used = 0.f;
 #pragma unroll
   for (int i = 0; i < kMaxTop / 32; ++i) {
     const int k = lane + 32 * i;
     if (k >= a.k) continue;
-    if (first[k] >= 0) s += y[i] == -INFINITY ? 0.f : expf(y[i] - y_ref);
-    Entry e = {first[k], q_id[k], y[i], slope[i]};
+    const float q_all = q_id[k];
+    Entry e = {first[k], q_all, y[i], slope[i]};
     reinterpret_cast<float4*>(entries)[r * a.k + k] = *reinterpret_cast<float4*>(&e);
+    if (first[k] < 0) continue;
+    s += y[i] == -INFINITY ? 0.f : expf(y[i] - y_ref);
+    used += 1.f;
+    if (q_all == 0.f) continue;
+    // maxima first: what is left to round is of the size of the difference
+    const float log_q = q_all == q[i] ? (t[i] - m) - log_s : logf(q_all);
+    b += y[i] == -INFINITY ? INFINITY : q_all * (log_q - (y[i] - y_ref));
   }
+  b = warp_sum(b);
   s = warp_sum(s);
+  used = warp_sum(used);
   if (lane == 0) {
     // no rest where the entries are the whole vocabulary: 1 - sum is rounding then
     const float q_rest = tail && used < (float)V ? fmaxf(0.f, 1.f - sum) : 0.f;

@@ -173,6 +173,21 @@ def token_logprobs_ref(x, targets, cap=0.0):
     return logp, grad
 
 
+def _merge_repeats(ids, used, t):
+    """(used, t) with repeated ids merged: an id's first entry has the log of its entries' summed exponentials, the
+    others are unused."""
+    at = torch.where(used, ids, -1).sort(dim=1)[0]
+    rows = ((at[:, 1:] == at[:, :-1]) & (at[:, 1:] >= 0)).any(dim=1).nonzero().squeeze(1)
+    if rows.numel() == 0:
+        return used, t
+    mine, use = ids[rows], used[rows]
+    same = (mine.unsqueeze(2) == mine.unsqueeze(1)) & use.unsqueeze(1) & use.unsqueeze(2)
+    first = use & ~same.tril(-1).any(dim=2)
+    sums = torch.where(same, t[rows].unsqueeze(1), float("-inf")).logsumexp(dim=2)
+    one = torch.where(same.sum(dim=2) > 1, sums, t[rows])
+    return used.index_copy(0, rows, first), t.index_copy(0, rows, torch.where(first, one, float("-inf")))
+
+
 def distill_ref(x, ids, top, lse=None, weights=None, cap=0.0, temperature=1.0):
     """(loss [N], gradient of sum(loss) [N, V])."""
     z, slope = _softcapped(x, cap)
@@ -181,7 +196,7 @@ def distill_ref(x, ids, top, lse=None, weights=None, cap=0.0, temperature=1.0):
     ids = ids.long()
     used = (ids >= 0) & (ids < V)
     col = ids.clamp(0, V - 1)
-    t = torch.where(used, top.to(z.dtype) / temperature, float("-inf"))
+    used, t = _merge_repeats(ids, used, torch.where(used, top.to(z.dtype) / temperature, float("-inf")))
     log_p = y - _log_sum_exp(y).unsqueeze(1)
     p = log_p.exp()
     some = t.amax(dim=1, keepdim=True) != float("-inf")

@@ -88,3 +88,45 @@ def close_grad(got, want, coef, mass, dtype):
     err = (got.double() - want).abs()
     assert torch.equal(got.isnan(), want.isnan())
     assert bool(((err <= tol) | want.isnan()).all()), float((err - tol).max())
+
+
+def merged(ids, top, temp):
+    """The same teacher with one entry an id: the first one has the sum of the probabilities, the others are unused."""
+    ids, top = ids.clone(), top.double() / temp
+    for r in range(ids.shape[0]):
+        for j in ids[r].unique().tolist():
+            at = (ids[r] == j).nonzero().squeeze(1)
+            top[r, at[0]] = torch.logsumexp(top[r, at], 0)
+            ids[r, at[1:]] = -1
+    return ids, top * temp
+
+
+def rest_mass(x, ids, top, lse, cap, temp):
+    """What the teacher's rest puts on each column that is no entry (its probability times the column's share of the
+    student's rest): with the probabilities and the entries' own, all that a gradient with a rest is a sum of."""
+    lp = torch.log_softmax(z64(x, cap) / temp, 1)
+    out = torch.zeros_like(lp)
+    for r in range(x.shape[0] if lse is not None else 0):
+        used = ids[r] >= 0
+        keep = torch.ones(x.shape[1], dtype=torch.bool, device=x.device)
+        keep[ids[r][used]] = False
+        q_rest = (1 - (top[r][used].double() / temp - lse[r].double()).exp().sum()).clamp_min(0)
+        if bool(keep.any()):
+            out[r, keep] = q_rest * (lp[r, keep] - torch.logsumexp(lp[r, keep], 0)).exp()
+    return out
+
+
+def repeated_cases(dev):
+    """(V, ids, top, lse or None): repeated ids, among them rows whose entries are the whole vocabulary only if repeats
+    are counted, or are it with repeats."""
+    g = torch.Generator(device=dev).manual_seed(11)
+    for V, k, N in ((2, 2, 3), (2, 3, 4), (4, 4, 6), (37, 12, 8), (5003, 256, 5), (9001, 40, 6)):
+        ids = torch.randint(0, min(V, max(2, k // 3)), (N, k), device=dev, generator=g)
+        ids[0] = ids[0, 0]                      # one token, k times
+        ids[1] = torch.arange(k, device=dev) % V  # every token as long as there are some
+        if k > 3:
+            ids[2, k // 2:] = -1
+        top = torch.randn(N, k, device=dev, generator=g) * 3
+        top[N - 1, 0] = -float("inf")
+        for lse in (None, torch.logsumexp(top / 1.5, 1) + 0.3, torch.logsumexp(top / 1.5, 1)):
+            yield V, ids, top, lse

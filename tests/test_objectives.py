@@ -199,3 +199,32 @@ def refusals(dev):
 def test_refusals(what):
     with pytest.raises(ValueError):
         refusals("cpu")[what]()
+
+
+@pytest.mark.parametrize("cap", [None, 30.0])
+def test_repeated_ids(cap):
+    """A repeated id is one entry with the sum of its probabilities: value, gradient, and whether there is a rest."""
+    for V, ids, top, lse in oracle.repeated_cases("cpu"):
+        N = ids.shape[0]
+        x = torch.randn(N, V, generator=torch.Generator().manual_seed(V)) * 4
+        w = torch.ones(N)
+        one_ids, one_top = oracle.merged(ids, top, 1.5)
+        want, grad, mass = oracle.distill(x, one_ids, one_top, lse, w, cap, 1.5)
+        mass = mass + oracle.rest_mass(x, one_ids, one_top, lse, cap, 1.5)
+        for loss, dx in (O.distill_loss_grad(x, ids, top, lse, w, softcap=cap, temperature=1.5),
+                         O.distill_loss_grad(x, one_ids, one_top, lse, w, softcap=cap, temperature=1.5)):
+            oracle.close_logp(loss, want, x, cap, 1.5, factor=8)
+            oracle.close_grad(dx, grad, 1.5 * w, mass, torch.float32)
+
+
+def test_repeated_ids_by_hand():
+    """A student that is certain of the teacher's only token has nothing to learn, however often that token is named."""
+    x = torch.full((1, 9), -200.0)
+    x[0, 5] = 0.0
+    loss, dx = O.distill_loss_grad(x, torch.tensor([[5, 5]]), torch.zeros(1, 2))
+    assert abs(float(loss)) < 1e-6 and float(dx.abs().max()) < 1e-6
+    x = torch.tensor([[0.3, -0.2]])
+    lse = torch.tensor([1.5])
+    a = O.distill_loss_grad(x, torch.tensor([[0, 0]]), torch.tensor([[0.0, 0.0]]), lse)
+    b = O.distill_loss_grad(x, torch.tensor([[0]]), torch.tensor([[2.0]]).log(), lse)
+    assert torch.allclose(a[0], b[0], atol=1e-6) and torch.allclose(a[1], b[1], atol=1e-6)

@@ -537,3 +537,19 @@ def test_too_many_columns(V):
                  lambda: O.preference_logits_grad(x, t, None, torch.tensor([0, 1, 2], device=DEV))):
         with pytest.raises(ValueError, match="vocabulary"):
             call()
+
+
+@pytest.mark.parametrize("dtype,cap", [(BF, 30.0), (HF, None), (FP, None), (FP, 30.0)])
+def test_repeated_ids(dtype, cap):
+    for V, ids, top, lse in oracle.repeated_cases(DEV):
+        x = _x(ids.shape[0], V, dtype, V)
+        w = torch.ones(ids.shape[0], device=DEV)
+        one = oracle.merged(ids, top, 1.5)
+        want, grad, mass = oracle.distill(x, *one, lse, w, cap, 1.5)
+        mass = mass + oracle.rest_mass(x, *one, lse, cap, 1.5)
+        leaf = x.detach().requires_grad_()
+        auto = O.distill_loss(leaf, ids, top, lse, w, softcap=cap, temperature=1.5)
+        auto = auto.detach(), torch.autograd.grad(auto.sum(), leaf)[0]
+        for loss, dx in (O.distill_loss_grad(x, ids, top, lse, w, softcap=cap, temperature=1.5), auto):
+            oracle.close_logp(loss, want, x, cap, 1.5, factor=8)
+            oracle.close_grad(dx, grad, 1.5 * w, mass, dtype)
