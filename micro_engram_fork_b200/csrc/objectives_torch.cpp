@@ -92,6 +92,9 @@ Tensor gradient_like(const Tensor& x, const OptTensor& out, const char* what) {
                     ": out has another shape, type or device than the logits");
   TORCH_CHECK((o.size(1) == 1 || o.stride(1) == 1) && (o.size(0) <= 1 || o.stride(0) >= o.size(1)), what,
               ": out's rows have to be contiguous and apart from one another");
+  // The kernels write through the pointer: a graph that has saved these values (an earlier objective's, of the same
+  // logits) learns of it by the version.
+  o.unsafeGetTensorImpl()->bump_version();
   return o;
 }
 

@@ -359,7 +359,8 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
 def distill_loss_grad(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=None, softcap=None,
                       temperature=1.0, out=None):
     """(distill_loss [...], gradient of its sum [..., V]) in one call. `out` takes the gradient; it may
-    be `logits` itself, and must not overlap it otherwise."""
+    be `logits` itself, and must not overlap it otherwise (a graph that has saved the overwritten values
+    refuses its backward pass, as after any PyTorch operator in place)."""
     if logits.dim() != 2:
         flat = _flat_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights)
         loss, dx = distill_loss_grad(*flat, softcap, temperature, _out_rows(out, logits))

@@ -228,3 +228,32 @@ def test_repeated_ids_by_hand():
     a = O.distill_loss_grad(x, torch.tensor([[0, 0]]), torch.tensor([[0.0, 0.0]]), lse)
     b = O.distill_loss_grad(x, torch.tensor([[0]]), torch.tensor([[2.0]]).log(), lse)
     assert torch.allclose(a[0], b[0], atol=1e-6) and torch.allclose(a[1], b[1], atol=1e-6)
+
+
+def overwritten(dev):
+    """An earlier graph on the logits, and a call that overwrites them: the graph's backward has to refuse."""
+    cu = torch.tensor([0, 2, 4], device=dev)
+    t = torch.tensor([1, 2, 3, 4], device=dev)
+    ids, top = t[:, None], torch.zeros(4, 1, device=dev)
+    graphs = {"logprobs": lambda x: O.token_logprobs(x, t), "distill": lambda x: O.distill_loss(x, ids, top)}
+    writes = {"logprobs": lambda z: O.token_logprobs_grad(z, t, out=z), "distill": lambda z: O.distill_loss_grad(z, ids, top, out=z),
+              "preference": lambda z: O.preference_logits_grad(z, t, None, cu, out=z)}
+    for graph in graphs.values():
+        for write in writes.values():
+            x = torch.randn(4, 9, device=dev, requires_grad=True)
+            y = graph(x)
+            version = x._version
+            write(x.detach())
+            assert x._version > version
+            yield y
+    x = torch.randn(2, 2, 9, device=dev, requires_grad=True)  # by way of flattened rows
+    y = O.token_logprobs(x, t.view(2, 2))
+    z = x.detach()
+    O.distill_loss_grad(z, ids.view(2, 2, 1), top.view(2, 2, 1), out=z)
+    yield y
+
+
+def test_overwritten_logits():
+    for y in overwritten("cpu"):
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()

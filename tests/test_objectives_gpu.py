@@ -7,7 +7,7 @@ import torch
 
 import objective_oracle as oracle
 from micro_engram_fork_b200.ops import objectives as O
-from test_objectives import refusals
+from test_objectives import overwritten, refusals
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -553,3 +553,18 @@ def test_repeated_ids(dtype, cap):
         for loss, dx in (O.distill_loss_grad(x, ids, top, lse, w, softcap=cap, temperature=1.5), auto):
             oracle.close_logp(loss, want, x, cap, 1.5, factor=8)
             oracle.close_grad(dx, grad, 1.5 * w, mass, dtype)
+
+
+def test_overwritten_logits():
+    for y in overwritten(DEV):
+        with pytest.raises(RuntimeError, match="inplace"):
+            y.sum().backward()
+
+
+def test_overwritten_logits_of_inference():
+    with torch.inference_mode():
+        x = _x(4, 300, BF, 1)
+        t = torch.arange(4, device=DEV)
+        logp, dx = O.token_logprobs_grad(x.clone(), t)
+        logp2, dx2 = O.token_logprobs_grad(x, t, out=x)
+    assert dx2 is x and torch.equal(dx, x) and torch.equal(logp, logp2)
