@@ -5,7 +5,8 @@ An objective is given to the trainer before its steps (``trainer.objective = Dis
 final hidden states of a micro-batch and the batch's tensors, and returns the sum of its terms:
 
   NextToken     labels
-  Distillation  teacher_ids, teacher_logits [tokens, k] (and teacher_lse [tokens]): record_teacher()
+  Distillation  teacher_ids, teacher_logits [tokens, k] (and teacher_lse [tokens] with the temperature that it is of,
+                teacher_temperature): record_teacher()
   Preference    ref_logps [tokens] (record_reference()) and cu_seqlens [2 pairs + 1]; one micro-batch
                 holds whole pairs
 
@@ -37,13 +38,20 @@ class NextToken:
 
 class Distillation(NextToken):
     """Summed divergence from the teacher over the trained tokens; with_rest: the teacher's mass outside its
-    entries is a class of its own (teacher_lse, recorded at the same temperature)."""
+    entries is a class of its own (teacher_lse, recorded at the same temperature: a batch that says another one, in
+    teacher_temperature, is refused)."""
 
     def __init__(self, temperature=1.0, with_rest=False):
         self.temperature, self.with_rest = float(temperature), with_rest
 
     def __call__(self, vocab, hidden, batch):
-        lse = _flat(batch, "teacher_lse") if self.with_rest else None
+        lse = None
+        if self.with_rest:
+            lse = _flat(batch, "teacher_lse")
+            recorded = float(batch.get("teacher_temperature", self.temperature))
+            if recorded != self.temperature:
+                raise ValueError(f"teacher_lse was recorded at temperature {recorded:g}, the distillation with the rest "
+                                 f"is at {self.temperature:g}: record_teacher(..., temperature={self.temperature:g})")
         k = batch["teacher_ids"].shape[-1]
         weights = (_flat(batch, "labels") != IGNORE).float()
         return vocab.distill(hidden, batch["teacher_ids"].reshape(-1, k), batch["teacher_logits"].reshape(-1, k), lse,
@@ -67,10 +75,12 @@ class Preference:
 
 
 def record_teacher(trainer, batch, k, temperature=1.0):
-    """The batch with this trainer's model's top logits on it: teacher_ids, teacher_logits, teacher_lse."""
+    """The batch with this trainer's model's top logits on it: teacher_ids, teacher_logits, teacher_lse and
+    teacher_temperature (one number, on the host)."""
     with torch.no_grad():
         values, ids, lse = trainer.vocab.top_logits(trainer.hidden(batch), k, temperature)
-    return {**batch, "teacher_ids": ids, "teacher_logits": values, "teacher_lse": lse}
+    return {**batch, "teacher_ids": ids, "teacher_logits": values, "teacher_lse": lse,
+            "teacher_temperature": torch.tensor(float(temperature), dtype=torch.float64)}
 
 
 def record_reference(trainer, batch):

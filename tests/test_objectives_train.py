@@ -101,3 +101,28 @@ def test_example(dev, monkeypatch, dist_env):
     first, last = out["preference_loss"]
     assert abs(first - 0.6931) < 1e-2 and last < 0.5 * first and min(out["margins"]) > 0
     sys.modules.pop("distill_and_prefer", None)
+
+
+def test_teacher_of_another_temperature():
+    """teacher_lse is of one temperature; a batch that says which is refused at another one, where the rest is used."""
+    from micro_engram.train.objectives import Distillation, record_teacher
+
+    shard, _ = _shard("cpu", V=40)
+    h = torch.randn(6, 64)
+
+    class Teacher:
+        vocab = shard
+
+        def hidden(self, batch):
+            return batch["h"]
+
+    batch = {"h": h, "labels": torch.arange(6)}
+    recorded = record_teacher(Teacher(), batch, 5, temperature=2.0)
+    assert float(Distillation(2.0, with_rest=True)(shard, h, recorded)) < 1e-3
+    with pytest.raises(ValueError, match="temperature"):
+        Distillation(1.0, with_rest=True)(shard, h, recorded)
+    with pytest.raises(ValueError, match="temperature"):
+        Distillation(2.0, with_rest=True)(shard, h, record_teacher(Teacher(), batch, 5))
+    Distillation(1.0)(shard, h, recorded)  # the entries alone are of no temperature
+    own = {k: v for k, v in recorded.items() if k != "teacher_temperature"}  # records that do not say
+    assert torch.equal(Distillation(2.0, with_rest=True)(shard, h, own), Distillation(2.0, with_rest=True)(shard, h, recorded))
