@@ -36,7 +36,7 @@ from . import model as M
 from .checkpoint import Checkpoints
 from .data import EpochPlan, collate, prepare
 from .faults import FaultHook
-from .objectives import NextToken
+from .objectives import NextToken, trained_tokens
 from .offload import ActivationOffload
 from .report import Reporter, to_host
 
@@ -295,6 +295,13 @@ class Trainer:
         batch = collate(self.samples, bins, self.cfg.sequence_len, self.pad_id, pin=self.device.type == "cuda")
         return {k: v.to(self.device, non_blocking=True) for k, v in batch.items()}
 
+    def _check_fed(self):
+        """The data set's batches hold input_ids, labels and position_ids: an objective that needs more is refused."""
+        missing = set(getattr(self.objective, "fields", ())) - {"input_ids", "labels", "position_ids"}
+        if missing:
+            raise ValueError(f"{type(self.objective).__name__} needs {', '.join(sorted(missing))}, which the data set's "
+                             "batches do not have: record them and call train_step(None, batches=[...])")
+
     def hidden(self, batch):
         """Final hidden states [tokens, d] of one micro-batch."""
         ids, pos = (batch[k].reshape(1, -1) for k in ("input_ids", "position_ids"))  # one row
@@ -331,11 +338,13 @@ class Trainer:
         numbers with sync (the public API), device tensors without (the training loop, which
         reads them at logging steps only)."""
         if batches is None:
+            self._check_fed()
             batches = [self._micro_batch(b) for b in micro]
-        tokens = torch.stack([self.objective.terms(b) for b in batches]).sum()
+        counts = torch.stack([torch.stack([trained_tokens(b), self.objective.terms(b)]) for b in batches]).sum(0)
         if self.world > 1:
-            dist.all_reduce(tokens)
-        count = tokens.clamp_min(1).float()
+            dist.all_reduce(counts)
+        tokens, terms = counts
+        count = terms.clamp_min(1).float()
         scale = self.world / count   # mean over every micro-batch's and rank's terms (trained tokens; loss * world / N)
         loss = torch.zeros((), device=self.device)
         for b in batches:
@@ -401,6 +410,7 @@ class Trainer:
         write_config(build_config(self.base_conf, self.slots, lambda _slot: rows_dir), self.cfg.output_dir)
 
     def train(self):
+        self._check_fed()
         cfg = self.cfg
         self._maybe_resume()
         self._publish_config(None)

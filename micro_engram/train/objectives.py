@@ -2,7 +2,8 @@
 recorded top logits, or a preference loss over packed chosen / rejected sequences.
 
 An objective is given to the trainer before its steps (``trainer.objective = Distillation()``); it gets the
-final hidden states of a micro-batch and the batch's tensors, and returns the sum of its terms:
+final hidden states of a micro-batch and the batch's tensors, and returns the sum of its terms. ``fields`` names what it
+needs of a batch beside input_ids and position_ids:
 
   NextToken     labels
   Distillation  teacher_ids, teacher_logits [tokens, k] (and teacher_lse [tokens] with the temperature that it is of,
@@ -10,10 +11,12 @@ final hidden states of a micro-batch and the batch's tensors, and returns the su
   Preference    ref_logps [tokens] (record_reference()) and cu_seqlens [2 pairs + 1]; one micro-batch
                 holds whole pairs
 
+The data set's batches have labels alone, so the last two run through ``trainer.train_step(None, batches=[...])`` on
+batches that the caller records; ``trainer.train()``, which draws its batches from the data set, refuses them.
+
 Teacher and reference are models of the same vocabulary. A natural reference policy is the frozen base
 without its engram; natural teachers are the bf16 base of an NF4 run and a larger model. The last two
-need the whole head on each GPU (VocabShard with world 1): a trainer on one GPU, or one whose head is
-replicated.
+need the whole head on the GPU, as a trainer on one GPU has it (VocabShard with world 1).
 """
 import torch
 
@@ -26,11 +29,17 @@ def _flat(batch, key):
     return batch[key].reshape(-1)
 
 
+def trained_tokens(batch):
+    return (batch["labels"] != IGNORE).sum()
+
+
 class NextToken:
     """Summed cross entropy of the trained tokens."""
+    fields = ("labels",)
 
     def terms(self, batch):
-        return (batch["labels"] != IGNORE).sum()
+        """How many terms the sum has (the step minimises their mean): here the trained tokens."""
+        return trained_tokens(batch)
 
     def __call__(self, vocab, hidden, batch):
         return vocab.loss_sum(hidden, _flat(batch, "labels"))[0]
@@ -43,6 +52,7 @@ class Distillation(NextToken):
 
     def __init__(self, temperature=1.0, with_rest=False):
         self.temperature, self.with_rest = float(temperature), with_rest
+        self.fields = ("labels", "teacher_ids", "teacher_logits") + (("teacher_lse",) if with_rest else ())
 
     def __call__(self, vocab, hidden, batch):
         lse = None
@@ -60,13 +70,15 @@ class Distillation(NextToken):
 
 class Preference:
     """Summed loss of the micro-batch's pairs; `rewards` [pairs, 2] of the last call."""
+    fields = ("labels", "ref_logps", "cu_seqlens")
 
     def __init__(self, beta=0.1, label_smoothing=0.0, kind="sigmoid"):
         self.args = (beta, label_smoothing, kind)
         self.rewards = None
 
     def terms(self, batch):
-        return torch.tensor(batch["cu_seqlens"].numel() // 2, device=batch["cu_seqlens"].device)
+        cu = batch["cu_seqlens"]
+        return torch.full((), cu.numel() // 2, dtype=torch.int64, device=cu.device)
 
     def __call__(self, vocab, hidden, batch):
         logps = vocab.token_logprobs(hidden, _flat(batch, "labels"))

@@ -126,3 +126,38 @@ def test_teacher_of_another_temperature():
     Distillation(1.0)(shard, h, recorded)  # the entries alone are of no temperature
     own = {k: v for k, v in recorded.items() if k != "teacher_temperature"}  # records that do not say
     assert torch.equal(Distillation(2.0, with_rest=True)(shard, h, own), Distillation(2.0, with_rest=True)(shard, h, recorded))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_trainer_feeds_the_objective(dev, monkeypatch, dist_env, tmp_path):
+    """train() and train_step(bins) have the data set's batches only: an objective that needs more is refused before
+    anything runs; the step's token count stays that of the trained tokens whatever the objective counts."""
+    if dev == "cpu":
+        monkeypatch.setenv("MICRO_ENGRAM_CPU", "1")
+    monkeypatch.syspath_prepend(os.path.join(ROOT, "examples"))
+    import distill_and_prefer as example
+    from micro_engram.train.objectives import Distillation, NextToken, Preference, record_reference, record_teacher
+
+    seq, vocab = 96, 4096
+    trainer = example.make_trainer(str(tmp_path), seq, vocab)
+    micro = trainer.plan.micro_batches(0, 0, 0)
+    for objective, field in ((Distillation(), "teacher_ids"), (Distillation(with_rest=True), "teacher_lse"),
+                             (Preference(), "cu_seqlens")):
+        trainer.objective = objective
+        for call in (trainer.train, lambda: trainer.train_step(micro)):
+            with pytest.raises(ValueError, match=field):
+                call()
+    assert trainer.global_step == 0 and not os.path.exists(trainer.cfg.output_dir)
+    lengths = [32, 24, 19, 16]
+    batch = example.packed(lengths, vocab, seq, torch.Generator().manual_seed(1), trainer.device)
+    batch["cu_seqlens"] = torch.tensor([0] + lengths, device=trainer.device).cumsum(0)
+    trained = int((batch["labels"] != -100).sum())
+    batch = record_reference(trainer, record_teacher(trainer, batch, 8))
+    for objective in (NextToken(), Distillation(), Preference()):
+        trainer.objective = objective
+        logs = trainer.train_step(None, batches=[batch, batch])
+        assert logs["tokens"] == 2 * trained
+    assert abs(logs["loss"] - 0.6931) < 0.05  # a mean over the pairs
+    trainer.objective = NextToken()
+    assert trainer.train_step(micro)["tokens"] > 0
+    sys.modules.pop("distill_and_prefer", None)
