@@ -198,12 +198,16 @@ class _HeadObjective(torch.autograd.Function):
                 else:
                     dh[a:b] = (z @ shard.weight).float()
             del z, padded
-        ctx.dh, ctx.hdtype = dh, hidden.dtype
+        if need_grad:
+            ctx.save_for_backward(dh)  # kept for as long as the graph is
+        ctx.hdtype = hidden.dtype
         return values
 
     @staticmethod
     def backward(ctx, g):
-        dh, ctx.dh = ctx.dh, None
+        if torch.is_grad_enabled():
+            raise RuntimeError("the gradient of this objective cannot be differentiated (create_graph)")
+        dh, = ctx.saved_tensors
         return (dh * g.float().unsqueeze(1)).to(ctx.hdtype), None, None, None
 
 

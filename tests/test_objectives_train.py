@@ -161,3 +161,20 @@ def test_trainer_feeds_the_objective(dev, monkeypatch, dist_env, tmp_path):
     trainer.objective = NextToken()
     assert trainer.train_step(micro)["tokens"] > 0
     sys.modules.pop("distill_and_prefer", None)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_head_backward_again(dev):
+    """The gradient is kept for a graph that is retained, released with one that is not, and not differentiable itself."""
+    shard, W = _shard(dev, V=200)
+    h = torch.randn(9, 64, device=dev).to(torch.bfloat16).requires_grad_()
+    labels = torch.arange(9, device=dev)
+    values = shard.token_logprobs(h, labels)
+    first, = torch.autograd.grad(values.sum(), h, retain_graph=True)
+    again, = torch.autograd.grad((2 * values).sum(), h)
+    assert torch.equal(again, 2 * first)
+    with pytest.raises(RuntimeError, match="second time|retain_graph"):
+        torch.autograd.grad(values.sum(), h)
+    values = shard.distill(h, labels[:, None], torch.zeros(9, 1, device=dev))
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(values.sum(), h, create_graph=True)
