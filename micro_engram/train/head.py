@@ -134,6 +134,11 @@ class VocabShard:
             raise ValueError(f"hidden states [tokens, {self.d}] are needed, got {tuple(hidden.shape)}")
         return _chunks(hidden.shape[0], self.chunk_bf16 if use_native(hidden) else self.chunk)
 
+    def _per_token(self, hidden, **given):
+        for name, t in given.items():
+            if t is not None and tuple(t.shape[:1]) != tuple(hidden.shape[:1]):
+                raise ValueError(f"{name}: one value (or row) a token is needed ({hidden.shape[0]}), got shape {tuple(t.shape)}")
+
     def _logits(self, hidden):
         """(raw logits [n, V], the same with the padding columns that the GEMMs want)."""
         h = hidden.detach().to(self.weight.dtype).contiguous()
@@ -157,6 +162,8 @@ class VocabShard:
 
     def token_logprobs(self, hidden, labels):
         """log p(label) of each token, fp32 [N] (0 where the label is -100), differentiable in hidden."""
+        self._per_token(hidden, labels=labels)
+
         def chunk(z, a, b, out):
             if out is None:
                 return objectives.token_logprobs(z, labels[a:b], self.softcap)
@@ -167,6 +174,9 @@ class VocabShard:
     def distill(self, hidden, teacher_ids, teacher_logits, teacher_lse=None, weights=None, temperature=1.0):
         """The weighted divergence from a teacher's top logits of each token, fp32 [N], differentiable in
         hidden; see ops.objectives.distill_loss."""
+        self._per_token(hidden, teacher_ids=teacher_ids, teacher_logits=teacher_logits, teacher_lse=teacher_lse,
+                        weights=weights)
+
         def chunk(z, a, b, out):
             args = (z, teacher_ids[a:b], teacher_logits[a:b], None if teacher_lse is None else teacher_lse[a:b],
                     None if weights is None else weights[a:b], self.softcap, temperature)

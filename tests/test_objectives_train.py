@@ -178,3 +178,21 @@ def test_head_backward_again(dev):
     values = shard.distill(h, labels[:, None], torch.zeros(9, 1, device=dev))
     with pytest.raises(RuntimeError, match="create_graph"):
         torch.autograd.grad(values.sum(), h, create_graph=True)
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+def test_head_refuses_other_lengths(dev):
+    """One value a token: longer or shorter arguments are refused, not cut to the hidden states."""
+    shard, _ = _shard(dev, V=200)  # chunks of 16
+    h = torch.randn(20, 64, device=dev).to(torch.bfloat16)
+    for n in (0, 16, 19, 21, 32, 40):
+        labels = torch.zeros(n, dtype=torch.int64, device=dev)
+        ids, top, one = labels[:, None], torch.zeros(n, 1, device=dev), torch.ones(n, device=dev)
+        good = torch.zeros(20, 1, dtype=torch.int64, device=dev), torch.zeros(20, 1, device=dev)
+        for call in (lambda: shard.token_logprobs(h, labels), lambda: shard.distill(h, ids, top),
+                     lambda: shard.distill(h, good[0], top), lambda: shard.distill(h, *good, one),
+                     lambda: shard.distill(h, *good, None, one), lambda: shard.token_logprobs(h[:0], labels) if n else shard.distill(h, ids, top)):
+            with pytest.raises(ValueError):
+                call()
+    with pytest.raises(ValueError):
+        shard.token_logprobs(h, torch.zeros(20, 1, dtype=torch.int64, device=dev))
