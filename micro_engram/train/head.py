@@ -120,7 +120,7 @@ class VocabShard:
         grad; labels [N] with -100 untrained. Collective: every rank calls it with the same N."""
         count = (labels != IGNORE).sum()
         labels = labels.to(hidden.device)
-        if use_native(hidden) and self.weight.dtype == torch.bfloat16:
+        if self._on_gemm(hidden):
             total = _FusedVocabCE.apply(hidden, labels, self, torch.is_grad_enabled() and hidden.requires_grad)
         else:
             total = _VocabParallelCE.apply(hidden, labels, self)
@@ -132,7 +132,11 @@ class VocabShard:
             raise ValueError("this objective needs the whole head on one GPU: VocabShard(weight, rank=0, world=1)")
         if hidden.dim() != 2 or hidden.shape[1] != self.d:
             raise ValueError(f"hidden states [tokens, {self.d}] are needed, got {tuple(hidden.shape)}")
-        return _chunks(hidden.shape[0], self.chunk_bf16 if use_native(hidden) else self.chunk)
+        return _chunks(hidden.shape[0], self.chunk_bf16 if self._on_gemm(hidden) else self.chunk)
+
+    def _on_gemm(self, t):
+        """Whether the head's products run on the tcgen05 GEMM (bf16 in)."""
+        return use_native(t) and self.weight.dtype == torch.bfloat16
 
     def _per_token(self, hidden, **given):
         for name, t in given.items():
@@ -142,7 +146,7 @@ class VocabShard:
     def _logits(self, hidden):
         """(raw logits [n, V], the same with the padding columns that the GEMMs want)."""
         h = hidden.detach().to(self.weight.dtype).contiguous()
-        if use_native(h):
+        if self._on_gemm(h):
             from micro_engram_fork_b200 import native
 
             z = native().gemm(h, self.gemm_weight, True, None)
@@ -201,7 +205,7 @@ class _HeadObjective(torch.autograd.Function):
             z, padded = shard._logits(hidden[a:b])
             values[a:b] = chunk(z, a, b, z if need_grad else None)
             if need_grad:
-                if use_native(padded):
+                if shard._on_gemm(padded):
                     from micro_engram_fork_b200 import native
 
                     dh[a:b] = native().gemm_f32(padded, w)

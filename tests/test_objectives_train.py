@@ -196,3 +196,29 @@ def test_head_refuses_other_lengths(dev):
                 call()
     with pytest.raises(ValueError):
         shard.token_logprobs(h, torch.zeros(20, 1, dtype=torch.int64, device=dev))
+
+
+@pytest.mark.parametrize("dev", DEVICES)
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16])
+def test_head_of_another_type(dev, dtype):
+    """A head that is not bf16 has the other objectives too, as it has the cross entropy."""
+    from micro_engram.train.head import VocabShard
+
+    torch.manual_seed(0)
+    W = torch.randn(203, 64).to(dtype)
+    shard = VocabShard(W * 0.3, 0, 1, softcap=30.0, chunk_tokens=16, device=dev)
+    h = torch.randn(21, 64, device=dev).to(dtype).requires_grad_()
+    labels = torch.randint(0, 203, (21,), device=dev)
+    labels[::4] = -100
+    ce, _ = shard.loss_sum(h, labels)
+    lp = shard.token_logprobs(h, labels)
+    # the logits are one product of `dtype` in both; fp32 sums of up to 21 values of 10
+    tol = 1e-3 if dtype == torch.float32 else 3e-2
+    assert abs(float(ce.detach()) + float(lp.detach().sum())) < tol
+    a, = torch.autograd.grad(ce, h)
+    b, = torch.autograd.grad(-lp.sum(), h)
+    assert torch.allclose(a, b, rtol=1e-2, atol=tol)
+    values, ids, lse = shard.top_logits(h, 5)
+    assert bool((values.diff(dim=1) <= 0).all())
+    loss = shard.distill(h, ids, values, lse)
+    assert float(loss.abs().max()) < tol  # the model is its own teacher
