@@ -564,6 +564,14 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
     // (m is rounded: what separates it from the shift that was taken goes into s)
     out.m = kCap ? ref * sc.inv_temp : ref;
     out.s = kCap ? s * exp2_fast((float)(shift - 1.4426950408889634 * out.m)) : s;
+    // A reference far below the largest: a gradient's coefficient over s has to stay a normal number, so m takes the
+    // whole part of log s (the exponential is of an exact argument; m's own rounding goes into s).
+    if (out.s > 1e12f) {
+      const float up = rintf(logf(out.s));
+      const double m = (double)out.m + up;
+      out.m = (float)m;
+      out.s *= expf(-up) * (1.f + (float)(m - out.m));
+    }
   } else {
     for (int i = 0; i < count; ++i) {
       const uint32_t out_mask = drop(sl.vec(i));

@@ -568,3 +568,25 @@ def test_overwritten_logits_of_inference():
         logp, dx = O.token_logprobs_grad(x.clone(), t)
         logp2, dx2 = O.token_logprobs_grad(x, t, out=x)
     assert dx2 is x and torch.equal(dx, x) and torch.equal(logp, logp2)
+
+
+@pytest.mark.parametrize("cap", [None, 40.0])
+def test_small_coefficients_far_from_the_reference(cap):
+    """Most logits 76 below the largest one, which no thread sees first: the sums are of e^76 then, and a small
+    coefficient divided by one has to keep its digits."""
+    N, V = 5, 262144
+    x = torch.randn(N, V, device=DEV, generator=_gen(1)) * 0.3 - 75.0
+    t = torch.arange(N, device=DEV)
+    x[:, V - 100] = 75.0 if cap else 1.0
+    coef = torch.tensor([1.0, 1e-6, 1e-9, 1e-11, -1e-12], device=DEV)
+    logp, dx = O.token_logprobs_grad(x, t, coef, softcap=cap)
+    want, grad, mass = oracle.logprobs(x, t, cap, coef)
+    oracle.close_logp(logp, want, x, cap)
+    oracle.close_grad(dx, grad, coef, mass, FP)
+    w = coef.abs()
+    ids, top = torch.stack([t, t + 9], 1), torch.zeros(N, 2, device=DEV)
+    for lse in (None, torch.full((N,), 2.0, device=DEV)):
+        loss, dx = O.distill_loss_grad(x, ids, top, lse, w, softcap=cap)
+        want, grad, mass = oracle.distill(x, ids, top, lse, w, cap, 1.0)
+        oracle.close_logp(loss, want, x, cap, factor=8)
+        oracle.close_grad(dx, grad, w, mass + oracle.rest_mass(x, ids, top, lse, cap, 1.0), FP)
