@@ -82,7 +82,8 @@ __global__ void __launch_bounds__(kPairThreads) preference_kernel(
   const float h = sums.x - sums.y, u = beta * h;
   float l, d;
   if (kind == 0) {
-    l = (1.f - smooth) * softplus(-u) + smooth * softplus(u);
+    l = (1.f - smooth) * softplus(-u);
+    if (smooth > 0.f) l += smooth * softplus(u);  // (0 times infinity where the rejected answer is impossible)
     d = beta * (smooth - 1.f / (1.f + expf(u)));
   } else if (kind == 1) {
     l = u < 1.f ? 1.f - u : (u == u ? 0.f : u);

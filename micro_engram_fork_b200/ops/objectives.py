@@ -237,11 +237,13 @@ def preference_ref(logps, ref_logps, cu_seqlens, kind=0, beta=0.1, smooth=0.0, s
     h = sums[:, 0] - sums[:, 1]
     u = beta * h
     if kind == 0:
-        loss = (1 - smooth) * torch.nn.functional.softplus(-u) + smooth * torch.nn.functional.softplus(u)
+        loss = (1 - smooth) * torch.nn.functional.softplus(-u)
+        if smooth:  # (0 times infinity where the rejected answer is impossible)
+            loss = loss + smooth * torch.nn.functional.softplus(u)
         d = beta * (smooth - torch.sigmoid(-u))
     elif kind == 1:
         loss = (1 - u).clamp_min(0)
-        d = torch.where(u < 1, -beta, 0.0) + 0.0 * u
+        d = torch.where(u.isnan(), u, torch.where(u < 1, -beta, 0.0))
     else:
         loss = (h - 0.5 / beta).square()
         d = 2 * (h - 0.5 / beta)

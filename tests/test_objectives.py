@@ -257,3 +257,27 @@ def test_overwritten_logits():
     for y in overwritten("cpu"):
         with pytest.raises(RuntimeError, match="inplace"):
             y.sum().backward()
+
+
+def impossible_answers(dev):
+    """Pairs whose rejected / chosen answer has a token of probability 0, per kind: (loss, rewards, gradient) as the
+    limits of the formulas have them (a NaN only where a difference of infinities has no limit)."""
+    inf = float("inf")
+    lp = torch.tensor([-1.0, -inf, -inf, -1.0, -1.0, -1.0], device=dev)
+    ref = torch.zeros(6, device=dev)
+    cu = torch.tensor([0, 1, 2, 3, 4, 5, 6], device=dev)  # rejected impossible, chosen impossible, neither
+    want = {("sigmoid", 0.0): ([0.0, inf, 0.6931472], [0, 0, -0.1, 0.1, -0.05, 0.05]),
+            ("sigmoid", 0.25): ([inf, inf, 0.6931472], [0.025, -0.025, -0.075, 0.075, -0.025, 0.025]),
+            ("hinge", 0.0): ([0.0, inf, 1.0], [0, 0, -0.1, 0.1, -0.1, 0.1])}
+    for (kind, smooth), (loss, grad) in want.items():
+        got = O.preference_loss_grad(lp, ref, cu, 0.1, smooth, kind, scale=1.0)
+        leaf = lp.clone().requires_grad_()
+        auto, _ = O.preference_loss(leaf, ref, cu, 0.1, smooth, kind)
+        for value, d in ((got[0], got[2]), (auto.detach(), torch.autograd.grad(auto.sum(), leaf)[0])):
+            assert torch.allclose(value.cpu(), torch.tensor(loss)), (kind, smooth, value)
+            assert torch.allclose(d.cpu(), torch.tensor(grad, dtype=torch.float32), atol=1e-7), (kind, smooth, d)
+        assert torch.allclose(got[1].cpu(), torch.tensor([[-0.1, -inf], [-inf, -0.1], [-0.1, -0.1]]))
+
+
+def test_impossible_answers():
+    impossible_answers("cpu")

@@ -7,7 +7,7 @@ import torch
 
 import objective_oracle as oracle
 from micro_engram_fork_b200.ops import objectives as O
-from test_objectives import overwritten, refusals
+from test_objectives import impossible_answers, overwritten, refusals
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -590,3 +590,7 @@ def test_small_coefficients_far_from_the_reference(cap):
         want, grad, mass = oracle.distill(x, ids, top, lse, w, cap, 1.0)
         oracle.close_logp(loss, want, x, cap, factor=8)
         oracle.close_grad(dx, grad, w, mass + oracle.rest_mass(x, ids, top, lse, cap, 1.0), FP)
+
+
+def test_impossible_answers():
+    impossible_answers(DEV)
