@@ -484,7 +484,7 @@ ME_DEVICE void stream(const uint4* src, int count, Ring& ring, First&& first, F&
 // is carried. A share that this does not suit (a sum out of range, a NaN or +inf anywhere) is added again element by element with a running maximum.
 //
 // With a softcap the exponential is ex2 of the difference times log2 e / tau (an argument's rounding
-// moves a term by 1e-6 at most, and the softcap's own rounding is as large); without one exp_pair(),
+// moves a term by 1e-6 at c / tau = 30 and 3e-6 at most, and the softcap's own rounding is as large); without one exp_pair(),
 // since nothing else is rounded then.
 // watch(x, i): sees the thread's vectors from the i-th on, one or two at a time, in order.
 struct WatchNothing {
@@ -559,8 +559,10 @@ ME_DEVICE MaxSum slice_sum(const Slice<T>& sl, const Scale& sc, const Drop& drop
         }
       });
   const float s = sum0 + sum1;
-  const float far = kCap ? (sc.cap - ref) * sc.inv_temp : big.value() * sc.inv_temp - ref;  // the largest exponent
-  if (count > 0 && s > 1e-20f && s < 1e37f && far < 80.f) {  // (masked columns add 2e-38 each)
+  // exp_pair's range; ex2 leaves its own with an infinity, which the sum shows. (Not the largest exponent that the cap
+  // allows: that sent every row with 2 cap / tau near 160 to the slow form, 122 -> 801 us for top logits of 1024 x 262144.)
+  const bool in_range = kCap || big.value() * sc.inv_temp - ref < 80.f;
+  if (count > 0 && s > 1e-20f && s < 1e37f && in_range) {  // (masked columns add 2e-38 each)
     // (m is rounded: what separates it from the shift that was taken goes into s)
     out.m = kCap ? ref * sc.inv_temp : ref;
     out.s = kCap ? s * exp2_fast((float)(shift - 1.4426950408889634 * out.m)) : s;

@@ -594,3 +594,58 @@ def test_small_coefficients_far_from_the_reference(cap):
 
 def test_impossible_answers():
     impossible_answers(DEV)
+
+
+WIDE = [(BF, 50.0, 0.25, None), (BF, 100.0, 1.0, None), (FP, 100.0, 1.0, None), (HF, 200.0, 0.7, None), (BF, None, 1.0, -1e9),
+        (FP, None, 1.0, -1e9), (HF, None, 1.0, -3e4), (BF, None, 2.0, -1e4)]
+
+
+def _wide_row(N, V, dtype, masked, seed=1):
+    """An ordinary body with a few peaks; `masked` is the value of all columns but the last 9000."""
+    x = torch.randn(N, V, device=DEV, generator=_gen(seed)) * 2.5 - 5.0
+    x[:, 5::V // 12] = 12.0
+    if masked is not None:
+        x[:, : V - 9000] = masked
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype,cap,temp,masked", WIDE)
+def test_wide_caps_and_finite_masks(dtype, cap, temp, masked):
+    N, V = 6, 100003
+    x = _wide_row(N, V, dtype, masked)
+    x[0] = (x[0].float() * 8).to(dtype)  # beyond what one reference can hold
+    t = torch.randint(V - 9000, V, (N,), device=DEV, generator=_gen(2))
+    coef = torch.randn(N, device=DEV, generator=_gen(3))
+    logp, dx = O.token_logprobs_grad(x, t, coef, softcap=cap)
+    want, grad, mass = oracle.logprobs(x, t, cap, coef)
+    big = torch.where(x < -9000, 0.0, x.float())  # what the sums are formed of
+    oracle.close_logp(logp, want, big, cap)
+    oracle.close_grad(dx, grad, coef, mass, dtype)
+    lse = O.top_logits(x, 4, softcap=cap, temperature=temp)[2]
+    oracle.close_logp(lse, torch.logsumexp(oracle.z64(x, cap) / temp, 1), big, cap, temp)
+    ids, top, w = t[:, None], torch.zeros(N, 1, device=DEV), torch.ones(N, device=DEV)
+    for rest in (None, torch.ones(N, device=DEV)):
+        loss, dx = O.distill_loss_grad(x, ids, top, rest, w, softcap=cap, temperature=temp)
+        want, grad, mass = oracle.distill(x, ids, top, rest, w, cap, temp)
+        oracle.close_logp(loss, want, big, cap, temp, factor=8)
+        oracle.close_grad(dx, grad, w * temp, mass + oracle.rest_mass(x, ids, top, rest, cap, temp), dtype)
+
+
+@pytest.mark.parametrize("dtype,cap,temp", [w[:3] for w in WIDE if w[0] != HF and w[1]])
+def test_wide_caps_take_the_fast_sum(dtype, cap, temp):
+    """The time of one call against that with cap 30 at temperature 1: the element by element form takes more than four
+    times as long."""
+    def best(x, cap, temp):
+        O.top_logits(x, 20, cap, temp)
+        times = []
+        for _ in range(7):
+            a, b = (torch.cuda.Event(enable_timing=True) for _ in range(2))
+            a.record()
+            O.top_logits(x, 20, cap, temp)
+            b.record()
+            b.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    x = _wide_row(1024, 262144, dtype, None)
+    assert best(x, cap, temp) < 2.5 * best(x, 30.0, 1.0)
