@@ -46,10 +46,21 @@ ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float 
 #pragma unroll
           for (int p = 0; p < kP; ++p) {
             const f32x2 zp = z[u][p];
-            // (a 16-bit result is rounded at 2^-9 or 2^-12: the exponent's rounding, 2e-6, may stay)
-            const float2 a = unpack2(sizeof(T) == 4 ? mul2(fma2(zp, both2(sc.inv_temp), both2(-m)), both2(kLog2e))
-                                                    : fma2(zp, both2(k), both2(-shift)));
-            const f32x2 e = pack2(exp2_fast(a.x), exp2_fast(a.y));
+            // (a 16-bit result is rounded at 2^-9 or 2^-12, a 32-bit z under a softcap at up to 1e-6: the exponent's
+            // rounding, 2e-6, may stay)
+            float2 a;
+            if constexpr (sizeof(T) == 4) a = unpack2(fma2(zp, both2(sc.inv_temp), both2(-m)));
+            else a = unpack2(fma2(zp, both2(k), both2(-shift)));
+            f32x2 e;
+            if constexpr (sizeof(T) == 4 && !kCap) {
+              const float2 r = unpack2(exp_pair(pack2(a.x, a.y)));  // down to e^-87; 0 below, for masked columns too
+              e = pack2(a.x < -87.f ? 0.f : r.x, a.y < -87.f ? 0.f : r.y);
+            } else if constexpr (sizeof(T) == 4) {
+              a = unpack2(mul2(pack2(a.x, a.y), both2(kLog2e)));
+              e = pack2(exp2_fast(a.x), exp2_fast(a.y));
+            } else {
+              e = pack2(exp2_fast(a.x), exp2_fast(a.y));
+            }
             z[u][p] = mul2(e, kCap ? fma2(mul2(zp, both2(coef_slope)), zp, both2(coef)) : both2(coef));
           }
           Vec16<T> r;
@@ -66,12 +77,14 @@ ME_DEVICE void write_vectors(const Slice<T>& sl, T* out, const Scale& sc, float 
 }
 template <typename T, bool kCap>
 ME_DEVICE void write_slice(const Slice<T>& sl, T* out, const Scale& sc, float m, float coef, Ring& ring) {
+  if (m == -INFINITY) coef = NAN;  // nothing but masked columns (every other NaN of a row is in coef already)
   if ((reinterpret_cast<uintptr_t>(out + sl.head) & 15) == 0) write_vectors<T, kCap, true>(sl, out, sc, m, coef, ring);
   else write_vectors<T, kCap, false>(sl, out, sc, m, coef, ring);
   const int j = sl.single();
   if (j >= 0) {
-    const float z = softcap(to_f<T>(sl.row[j]), sc.cap);
-    out[j] = from_f<T>(coef * exp2_fast((z * sc.inv_temp - m) * kLog2e) * softcap_slope(z, sc.cap));
+    const float z = softcap(to_f<T>(sl.row[j]), sc.cap), y = z * sc.inv_temp - m;
+    const float e = sizeof(T) == 4 ? expf(y) : exp2_fast(y * kLog2e);
+    out[j] = from_f<T>(coef * e * softcap_slope(z, sc.cap));
   }
 }
 
