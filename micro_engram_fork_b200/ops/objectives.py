@@ -24,7 +24,8 @@ and are the tests' second opinion. Rules that hold for both:
   logits        V is at most 2^31 - 4097 for the kernels, k (teacher's entries, top logits) at most 256
   teacher_ids   an id outside [0, V) is an unused entry; ids of one row are distinct (a repeated id
                 counts as the sum of its probabilities)
-  weights       0 is an untrained token: loss 0, gradient 0, whatever its logits hold
+  weights       0 is an untrained token: loss 0, gradient 0, whatever its logits hold (as where there is nothing to
+                match: no entry, and no teacher_lse)
   non-finite    -inf logits have probability 0; a NaN or +inf logit makes its row's results NaN
                 (with a softcap +-inf are +-c)
 """
@@ -219,8 +220,9 @@ def distill_ref(x, ids, top, lse=None, weights=None, cap=0.0, temperature=1.0):
         d = torch.where(some, p, 0.0)
     d = d.scatter_add(1, col, -torch.where(used, q, 0.0)) * slope * temperature
     w = torch.ones(N, dtype=z.dtype, device=x.device) if weights is None else weights.to(z.dtype)
-    loss = torch.where(w != 0, w * temperature ** 2 * kl, 0.0)
-    return loss, torch.where((w != 0).unsqueeze(1), w.unsqueeze(1) * d, 0.0).to(x.dtype)
+    on = w != 0 if lse is not None else (w != 0) & some.squeeze(1)  # (no entry and no rest: nothing to match)
+    return (torch.where(on, w * temperature ** 2 * kl, 0.0),
+            torch.where(on.unsqueeze(1), w.unsqueeze(1) * d, 0.0).to(x.dtype))
 
 
 def preference_ref(logps, ref_logps, cu_seqlens, kind=0, beta=0.1, smooth=0.0, scale=1.0, targets=None):

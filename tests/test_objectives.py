@@ -281,3 +281,24 @@ def impossible_answers(dev):
 
 def test_impossible_answers():
     impossible_answers("cpu")
+
+
+def nothing_to_match(dev):
+    """Rows without an entry and without a rest: value 0 and gradient 0, whatever their logits hold."""
+    nan, inf = float("nan"), float("inf")
+    x = torch.randn(5, 40, device=dev)
+    x[1, 3], x[2, 4], x[3] = nan, inf, -inf
+    ids = torch.tensor([[-1, 40], [-1, -7], [41, -1], [-1, -1], [2, 3]], device=dev)
+    top = torch.zeros(5, 2, device=dev)
+    top[4] = -inf  # entries of probability 0 are none
+    for cap in (None, 30.0):
+        loss, dx = O.distill_loss_grad(x, ids, top, softcap=cap)
+        leaf = x.clone().requires_grad_()
+        auto = O.distill_loss(leaf, ids, top, softcap=cap)
+        auto.sum().backward()
+        for t in (loss, dx, auto.detach(), leaf.grad):
+            assert bool((t == 0).all()), (cap, t)
+
+
+def test_nothing_to_match():
+    nothing_to_match("cpu")

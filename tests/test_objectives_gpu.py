@@ -7,7 +7,7 @@ import torch
 
 import objective_oracle as oracle
 from micro_engram_fork_b200.ops import objectives as O
-from test_objectives import impossible_answers, overwritten, refusals
+from test_objectives import impossible_answers, nothing_to_match, overwritten, refusals
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -665,3 +665,7 @@ def test_small_probabilities_of_fp32_gradients():
     _, dx = O.distill_loss_grad(x, ids, top)
     want, grad, _ = oracle.distill(x, ids, top, None, torch.ones(N, device=DEV), None, 1.0)
     assert float((dx.double() / grad - 1)[:, 1:].abs().max()) < 2.0 ** -21
+
+
+def test_nothing_to_match():
+    nothing_to_match(DEV)
