@@ -104,7 +104,7 @@ ME_DEVICE void zero_slice(const Slice<T>& sl, T* out) {
 
 // ------------------------------------------------------------------------------------ log-probabilities
 // One cluster a row, one walk. Bound by issue slots under a softcap (97 for 8 logits a thread): 2048 x 262144 bf16,
-// softcap 30, 198 us, 0.82 of the copy rate with every row counted; fp32 without one runs at the copy rate.
+// softcap 30, 204 us, 0.80 of the copy rate with every row counted; fp32 without one runs at the copy rate.
 template <typename T, bool kCap>
 __global__ void __launch_bounds__(kThreads, 4) logprob_fwd_kernel(Rows<const T> x, int V, int lg_ranks,
                                                                   const int64_t* __restrict__ target, Scale sc,

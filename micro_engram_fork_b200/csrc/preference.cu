@@ -8,7 +8,9 @@
 // and dL / d logp_t = +-dL/dh for the tokens of the chosen / rejected sequence.
 //
 // One block a pair: it adds its two sequences (fp32, fixed order) and writes their tokens' gradient, so that value and
-// gradient are one launch. Bound by the launch: 4 pairs over 6000 tokens, 9 us a call, of which the host takes 8.
+// gradient are one launch. Bound by the launch: 4 pairs over 6000 tokens, 9 us a call, of which the host takes 8. (A
+// block reads all offsets ahead of its pair's, so that malformed ones cost no launch of their own: nothing for hundreds of
+// pairs, 29 us for 4096, 164 us for 16384.)
 #include "objectives.cuh"
 
 using namespace me;

@@ -9,8 +9,9 @@
 // (k groups hold one each that is as large), so only the groups that reach it are read again, about k of
 // them, and their logits above the bound, a little more than k, are ranked by counting. Where that
 // does not end in few candidates (many equal logits, few columns, a NaN), the row's first block finds the
-// exact k-th logit by radix selection, some passes over the row. 2048 x 262144 bf16, softcap 30, k 64: 258 us (one
-// read takes 164 us at the copy rate); bound by issue slots, the sum's 97 for 8 logits a thread and 12 for the maxima.
+// exact k-th logit by radix selection, some passes over the row. 2048 x 262144 bf16, softcap 30, k 64: 268 us (one
+// read takes 164 us at the copy rate). Three quarters of the issue slots are taken (the sum's 97 for 8 logits a thread, 12
+// for the maxima); the selection, which follows a row's walk, and three blocks an SM instead of four leave the rest.
 #include "objectives.cuh"
 
 #include <algorithm>
