@@ -93,6 +93,13 @@ std::vector<torch::Tensor> preference_logits(torch::Tensor x, torch::Tensor targ
                                              torch::Tensor cu, int64_t kind, double beta, double smooth,
                                              c10::optional<double> scale, c10::optional<double> cap,
                                              c10::optional<torch::Tensor> out);
+// paged_torch.cpp (paged_append.cu, paged_attention.cu)
+torch::Tensor paged_append(torch::Tensor qkv, torch::Tensor q_w, torch::Tensor k_w, torch::Tensor inv_freq, torch::Tensor k_pages,
+                           torch::Tensor v_pages, torch::Tensor table, torch::Tensor cu, torch::Tensor lens, int64_t q_heads,
+                           bool kv_shared, double eps);
+std::vector<torch::Tensor> paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor table,
+                                           torch::Tensor cu, torch::Tensor lens, int64_t window, double scale, int64_t max_q,
+                                           c10::optional<torch::Tensor> out);
 // attention.cu
 std::vector<torch::Tensor> attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor doc_start,
                                     int64_t window, double scale);
@@ -183,6 +190,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preference_loss", &preference_loss);
   m.def("preference_pairs", &preference_pairs);
   m.def("preference_logits", &preference_logits);
+  m.def("paged_append", &paged_append);
+  m.def("paged_attention", &paged_attention);
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
   m.def("attn_fwd_tc", &attn_fwd_tc);

@@ -1,0 +1,487 @@
+// Attention of new tokens over a paged cache.
+//
+// Rows (token, query head) of a sequence whose query heads share a key head read the same keys, so a unit of
+// work is (sequence, key head, 8 of those rows) over blocks of 64 keys. One new token a sequence, 2 to 8 query heads a key head: two
+// products of 2 to 8 rows with each 2-byte element, far below what the tensor cores need to be busy; the keys' and values' way
+// from memory is the bound, and everything here is for keeping loads in flight:
+//
+//   * All units' blocks are one line, cut into as many equal pieces as blocks fit on the GPU (two on an SM): whatever the
+//     lengths, every SM reads the same number of bytes. A piece that begins or ends inside a unit leaves (max, sum, output) of its part
+//     in the workspace, and a second kernel joins them; it is launched beside the first one's end (programmatic
+//     dependent launch).
+//   * A warp works alone: its own 16 keys of each block, its own ring of shared memory (24 KB, cp.async, rows outside the
+//     range and pages that are none filled with zeros), its own running maximum and sum. The 4 warps meet at a unit's end.
+//   * Keys are the M side of mma.m16n8k16 and the 8 rows its N side: S^T = K Q^T, O^T += V^T P^T. The rows of S^T become the
+//     B operand of the second product through movmatrix, without shared memory. P goes as two bf16 terms (its value rounded and
+//     what the rounding left, relative error 2^-17), which the idle tensor cores give for nothing: the output is as exact as its own
+//     rounding.
+#include <algorithm>
+
+#include "paged.cuh"
+
+namespace me {
+namespace {
+using namespace paged;
+
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// The running maximum (in log2 units) moves only when a score is this far above it: p stays below 2^8.
+constexpr float kSlack = 8.f;
+
+ME_DEVICE uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+ME_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// 16 bytes global -> shared; `bytes` 0: zeros, nothing is read.
+ME_DEVICE void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+ME_DEVICE void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+ME_DEVICE void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+ME_DEVICE void ldsm4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+ME_DEVICE void ldsm4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+ME_DEVICE uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+ME_DEVICE void mma16n8k16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// A part's sum (of terms below its own maximum) next to the whole's maximum.
+ME_DEVICE float share(float2 max_sum, float top) {
+  return max_sum.y == 0.f || max_sum.x == -INFINITY ? max_sum.y : max_sum.y * ex2(max_sum.x - top);
+}
+ME_DEVICE uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// ------------------------------------------------------------------------------- few rows a key head
+constexpr int kRows = 8, kWarps = 4, kTile = 16, kBlock = kWarps * kTile, kThreads = kWarps * 32;
+
+template <int D>
+struct Cfg {
+  static constexpr int UC = D < 256 ? D : 256;  // columns of a unit of the ring
+  static constexpr int UNIT = kTile * UC * 2;
+  static constexpr int PARTS = D / UC;          // units a tile of K
+  static constexpr int RING = 24 * 1024 / UNIT;
+  static constexpr int PITCH = D + 4;           // floats of a row where the warps meet: no bank conflicts
+  static constexpr int SMEM = kWarps * RING * UNIT;
+  static_assert(kWarps * kRows * PITCH * 4 <= SMEM, "the warps meet in the ring");
+  static_assert(2 * (SMEM + 2048) <= 227 * 1024, "two blocks an SM");
+};
+
+struct RowsArgs {
+  PagedAttentionArgs a;
+  float* part_o;   // [slots][kRows][D]
+  float2* part_ml; // [slots][kRows] (maximum, sum)
+  int pieces;      // blocks of the grid
+  int plog;
+};
+
+struct UnitsOf {
+  int tiles;   // row tiles of the sequence
+  int blocks;  // blocks of 64 keys of each
+};
+ME_DEVICE UnitsOf units_of(const PagedAttentionArgs& a, int b, const Sequence& s) {
+  if (s.count == 0) return {0, 0};
+  const int group = a.q_heads / a.cache.heads;
+  const Keys k = keys_of(a.batch, a.cache.page, s, 0, s.count - 1, a.window);
+  return {(s.count * group + kRows - 1) / kRows, max((k.hi + kBlock - 1) / kBlock - k.lo / kBlock, 1)};
+}
+
+template <int D>
+__global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs args) {
+  using C = Cfg<D>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ WorkLine<kThreads>::Shared line_shared;
+  __shared__ float2 warp_ml[kWarps][kRows];
+  const PagedAttentionArgs& a = args.a;
+  const PagedBatch& p = a.batch;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int hk = a.cache.heads, group = a.q_heads / hk, plog = args.plog;
+  const int g = lane >> 2, t4 = lane & 3;  // a fragment's row and column pair
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // rows of no sequence
+  if (a.clear_rest) {
+    const int head = p.seqs ? min(max(p.cu[0], 0), p.tokens) : p.tokens;
+    const int tail = p.seqs ? min(max(p.cu[p.seqs], head), p.tokens) : p.tokens;
+    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)(head + p.tokens - tail) * a.q_heads;
+         i += (int64_t)gridDim.x * kThreads) {
+      const int h = (int)(i % a.q_heads), n = (int)(i / a.q_heads), t = n < head ? n : n - head + tail;
+      bf16* o = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head;
+      for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+      a.lse[(int64_t)h * p.tokens + t] = -INFINITY;
+    }
+  }
+
+  auto count = [&](int b) -> int64_t {
+    const UnitsOf u = units_of(a, b, sequence_of(p, b));
+    return (int64_t)u.tiles * hk * u.blocks;
+  };
+  WorkLine<kThreads> line(line_shared);
+  const int64_t total = line.total(p.seqs, count);
+  const int64_t pieces = min((int64_t)args.pieces, total);
+  if (blockIdx.x >= pieces) return;
+  const int64_t x0 = blockIdx.x * total / pieces, x1 = (blockIdx.x + 1) * total / pieces;
+  int64_t x = x0, before;
+  int b = line.find(p.seqs, count, x, before);
+
+  const uint32_t my_ring = smem_u32(ring) + warp * (C::RING * C::UNIT);
+  constexpr int CPR = C::UC / 8, RPP = 32 / CPR;  // 16-byte chunks a row, rows a pass of the warp
+  const int c_row = lane / CPR, c_col = lane % CPR;
+  const int l_row = (lane & 7) + ((lane >> 3) & 1) * 8;
+
+  while (x < x1) {
+    const Sequence s = sequence_of(p, b);
+    const UnitsOf u = units_of(a, b, s);
+    const int64_t in_seq = x - before;
+    if (in_seq >= (int64_t)u.tiles * hk * u.blocks) {  // on to the next sequence that has any
+      before += (int64_t)u.tiles * hk * u.blocks;
+      ++b;
+      continue;
+    }
+    const int unit = (int)(in_seq / u.blocks), first_block = (int)(in_seq % u.blocks);
+    const int blocks = (int)min((int64_t)(u.blocks - first_block), x1 - x);
+    const int tile = unit % u.tiles, kv = unit / u.tiles;  // a head's row tiles lie together: their keys meet in L2
+    const int r0 = tile * kRows, rows = min(kRows, s.count * group - r0);
+    const Keys keys = keys_of(p, a.cache.page, s, r0 / group, (r0 + rows - 1) / group, a.window);
+    const int seq_lo = keys_of(p, a.cache.page, s, 0, s.count - 1, a.window).lo;
+    const int start = (seq_lo / kBlock + first_block) * kBlock + warp * kTile;  // this warp's first key; a tile a block
+
+    // this lane's two rows of S^T: their last and first keys
+    int last[2], from[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = r0 + 2 * t4 + e, pos = s.context + r / group;
+      last[e] = r < r0 + rows ? pos : -1;
+      from[e] = a.window > 0 ? pos - a.window + 1 : 0;
+    }
+    const int all_last = s.context + r0 / group;
+    const int all_from = a.window > 0 ? s.context + (r0 + rows - 1) / group - a.window + 1 : 0;
+
+    uint32_t qf[D / 16][2];
+    {
+      const int r = r0 + g;
+      const bf16* q = reinterpret_cast<const bf16*>(a.q) + (int64_t)(s.first + r / group) * a.q_token + (kv * group + r % group) * a.q_head + 2 * t4;
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        qf[k][0] = g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
+        qf[k][1] = g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+      }
+    }
+    const bf16* kbase = reinterpret_cast<const bf16*>(a.cache.k) + ((int64_t)kv * D << plog);
+    const bf16* vbase = reinterpret_cast<const bf16*>(a.cache.v) + ((int64_t)kv * D << plog);
+
+    int ids = -1;        // pages of the 32 tiles around the one that is loaded next, one a lane
+    uint32_t there = 0;  // bit j % 32: tile j has a page
+    int slot_in = 0, slot_out = 0;
+    auto issue = [&](int j, int part) {  // part of tile j: columns of K, then of V
+      if (j < blocks) {
+        if (part == 0) {
+          if ((j & 31) == 0) {
+            const int key = start + (j + lane) * kBlock;
+            ids = j + lane < blocks && key < keys.hi && key + kTile > keys.lo ? page_at(p, a.cache.pages, b, key >> plog) : -1;
+          }
+          const int id = __shfl_sync(0xffffffffu, ids, j & 31);
+          there = (there & ~(1u << (j & 31))) | ((id >= 0 ? 1u : 0u) << (j & 31));
+        }
+        const int id = __shfl_sync(0xffffffffu, ids, j & 31);
+        const int key = start + j * kBlock;
+        const bool is_v = part >= C::PARTS;
+        const bf16* src = (is_v ? vbase : kbase) + (id < 0 ? 0 : id * (is_v ? a.cache.v_stride : a.cache.k_stride)) +
+                          (int64_t)((key & (a.cache.page - 1)) + c_row) * D + (part % C::PARTS) * C::UC + c_col * 8;
+        const uint32_t dst = my_ring + slot_in * C::UNIT;
+#pragma unroll
+        for (int i = 0; i < kTile / RPP; ++i) {
+          const int row = i * RPP + c_row;
+          const bool in = id >= 0 && key + row >= keys.lo && key + row < keys.hi;
+          cp_async16(dst + row * (C::UC * 2) + ((c_col ^ (row & 7)) << 4), in ? src + i * RPP * D : kbase, in ? 16 : 0);
+        }
+        slot_in = slot_in + 1 == C::RING ? 0 : slot_in + 1;
+      }
+      cp_commit();
+    };
+
+    float acc[D / 16][4];
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
+    float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    const float to_log2 = a.scale * kLog2e;
+
+    constexpr int UPT = 2 * C::PARTS;
+#pragma unroll
+    for (int i = 0; i < C::RING; ++i) issue(i / UPT, i % UPT);
+    for (int j = 0; j < blocks; ++j) {
+      float sc[2][4] = {};
+      uint32_t ph[2], pl[2];
+#pragma unroll
+      for (int part = 0; part < UPT; ++part) {
+        cp_wait<C::RING - 1>();
+        __syncwarp();
+        const uint32_t at = my_ring + slot_out * C::UNIT + l_row * (C::UC * 2);
+        if (part < C::PARTS) {
+#pragma unroll
+          for (int k = 0; k < C::UC / 16; ++k) {
+            uint32_t f[4];
+            ldsm4(f, at + (((2 * k + (lane >> 4)) ^ (l_row & 7)) << 4));
+            mma16n8k16(sc[k & 1], f, qf[part * (C::UC / 16) + k][0], qf[part * (C::UC / 16) + k][1]);
+          }
+        } else {
+          if (part == C::PARTS) {  // the scores are whole: softmax
+            const int key = start + j * kBlock + g;
+            float v[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = (sc[0][e] + sc[1][e]) * to_log2;
+            const bool page = (there >> (j & 31)) & 1;
+            const int key0 = start + j * kBlock;
+            if (!(page && key0 >= all_from && key0 + kTile - 1 <= all_last && key0 + kTile <= keys.hi)) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int at_key = key + (e >> 1) * 8;
+                if (!page || at_key > last[e & 1] || at_key < from[e & 1] || at_key >= keys.hi) v[e] = -INFINITY;
+              }
+            }
+            float mx[2] = {fmaxf(v[0], v[2]), fmaxf(v[1], v[3])};
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+              mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+              mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+            }
+            const bool up0 = mx[0] > m[0] + kSlack, up1 = mx[1] > m[1] + kSlack;  // -inf + slack = -inf: any score is above it
+            if (__any_sync(0xffffffffu, up0 || up1)) {
+              const float f0 = up0 ? ex2(m[0] - mx[0]) : 1.f, f1 = up1 ? ex2(m[1] - mx[1]) : 1.f;
+              if (up0) m[0] = mx[0];
+              if (up1) m[1] = mx[1];
+              sum[0] *= f0, sum[1] *= f1;
+#pragma unroll
+              for (int i = 0; i < D / 16; ++i) acc[i][0] *= f0, acc[i][1] *= f1, acc[i][2] *= f0, acc[i][3] *= f1;
+            }
+            const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1];
+            v[0] = ex2(v[0] - z0), v[1] = ex2(v[1] - z1), v[2] = ex2(v[2] - z0), v[3] = ex2(v[3] - z1);
+            sum[0] += v[0] + v[2], sum[1] += v[1] + v[3];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t h = pack2(v[2 * e], v[2 * e + 1]);
+              const float h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xffff0000u);
+              ph[e] = transpose8x8(h);
+              pl[e] = transpose8x8(pack2(v[2 * e] - h0, v[2 * e + 1] - h1));
+            }
+          }
+          // V^T: the transposed reads give dimensions as rows
+          const uint32_t vat = my_ring + slot_out * C::UNIT + ((lane & 7) + (lane >> 4) * 8) * (C::UC * 2);
+#pragma unroll
+          for (int k = 0; k < C::UC / 16; ++k) {
+            uint32_t f[4];
+            ldsm4_t(f, vat + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
+            mma16n8k16(acc[(part - C::PARTS) * (C::UC / 16) + k], f, ph[0], ph[1]);
+            mma16n8k16(acc[(part - C::PARTS) * (C::UC / 16) + k], f, pl[0], pl[1]);
+          }
+        }
+        __syncwarp();
+        slot_out = slot_out + 1 == C::RING ? 0 : slot_out + 1;
+        issue(j + (part + C::RING) / UPT, (part + C::RING) % UPT);
+      }
+    }
+
+    // ---- the four warps meet
+#pragma unroll
+    for (int o = 4; o < 32; o <<= 1) {
+      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
+      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
+    }
+    if (g == 0) {
+      warp_ml[warp][2 * t4] = make_float2(m[0], sum[0]);
+      warp_ml[warp][2 * t4 + 1] = make_float2(m[1], sum[1]);
+    }
+    cp_wait<0>();
+    __syncthreads();
+    float* meet = reinterpret_cast<float*>(ring);
+    {
+      float f[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][2 * t4 + e].x);
+        f[e] = m[e] == -INFINITY ? 0.f : ex2(m[e] - top);
+      }
+      float* out = meet + (warp * kRows + 2 * t4) * C::PITCH + g;
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        out[i * 16] = acc[i][0] * f[0], out[C::PITCH + i * 16] = acc[i][1] * f[1];
+        out[i * 16 + 8] = acc[i][2] * f[0], out[C::PITCH + i * 16 + 8] = acc[i][3] * f[1];
+      }
+    }
+    __syncthreads();
+    const bool whole = blocks == u.blocks;
+    const int64_t slot = 2 * (int64_t)blockIdx.x + (x == x0 ? 0 : 1);
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kThreads) {
+      const int r = i / (D / 4), c = i % (D / 4) * 4;
+      float top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][r].x);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) l += share(warp_ml[w][r], top);
+      float4 o = *reinterpret_cast<const float4*>(meet + r * C::PITCH + c);
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 y = *reinterpret_cast<const float4*>(meet + (w * kRows + r) * C::PITCH + c);
+        o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+      }
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int t = s.first + (r0 + r) / group, h = kv * group + (r0 + r) % group;
+        uint2 b4;
+        b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
+        *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + c) = b4;
+        if (c == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+      } else {
+        *reinterpret_cast<float4*>(args.part_o + (slot * kRows + r) * D + c) = o;
+        if (c == 0) args.part_ml[slot * kRows + r] = make_float2(top, l);
+      }
+    }
+    __syncthreads();  // the ring is free again
+    x += blocks;
+  }
+}
+
+// Joins the parts of units that were cut. One block a unit and row at a time; groups of D / 4 threads take a part each.
+constexpr int kJoinThreads = 256;
+
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs args) {
+  constexpr int PER = D / 4, GROUPS = kJoinThreads / PER;
+  __shared__ WorkLine<kJoinThreads>::Shared line_shared;
+  __shared__ float4 meet[kJoinThreads];
+  __shared__ float2 meet_ml[GROUPS];
+  const PagedAttentionArgs& a = args.a;
+  const PagedBatch& p = a.batch;
+  const int hk = a.cache.heads, group = a.q_heads / hk;
+  auto blocks_of = [&](int b) -> int64_t {
+    const UnitsOf u = units_of(a, b, sequence_of(p, b));
+    return (int64_t)u.tiles * hk * u.blocks;
+  };
+  WorkLine<kJoinThreads> line(line_shared);
+  const int64_t total = line.total(p.seqs, blocks_of);
+  const int64_t pieces = min((int64_t)args.pieces, total);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  // Only units that a border between two pieces lies in were cut: border i is before block x of the line.
+  for (int64_t i = 1 + blockIdx.x; i < pieces; i += gridDim.x) {
+    const int64_t x = i * total / pieces;
+    int64_t before;
+    const int b = line.find(p.seqs, blocks_of, x, before);
+    const Sequence s = sequence_of(p, b);
+    const UnitsOf u = units_of(a, b, s);
+    const int unit = (int)((x - before) / u.blocks);
+    const int64_t begin = before + (int64_t)unit * u.blocks, end = begin + u.blocks;
+    if (x == begin) continue;                                // it separates two units
+    if ((i - 1) * total / pieces > begin) continue;          // an earlier border joins this unit
+    const int tile = unit % u.tiles, kv = unit / u.tiles, r0 = tile * kRows, rows = min(kRows, s.count * group - r0);
+    const int64_t from = i - 1, to = (end * pieces - 1) / total;  // pieces of the unit: the one with its last block
+    const int c = threadIdx.x % PER * 4, part = threadIdx.x / PER;
+    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
+      float top = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int64_t k = from + part; k <= to; k += GROUPS) {
+        const int64_t slot = 2 * k + (k * total / pieces >= begin ? 0 : 1);
+        const float2 ml = args.part_ml[slot * kRows + r];
+        const float4 y = *reinterpret_cast<const float4*>(args.part_o + (slot * kRows + r) * D + c);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float up = fmaxf(top, ml.x);
+        const float f0 = top == -INFINITY ? 0.f : ex2(top - up), f1 = ex2(ml.x - up);
+        o.x = o.x * f0 + y.x * f1, o.y = o.y * f0 + y.y * f1, o.z = o.z * f0 + y.z * f1, o.w = o.w * f0 + y.w * f1;
+        l = l * f0 + ml.y * f1;
+        top = up;
+      }
+      __syncthreads();
+      meet[threadIdx.x] = o;
+      if (c == 0) meet_ml[part] = make_float2(top, l);
+      __syncthreads();
+      if (part == 0) {
+        float best = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < GROUPS; ++w) best = fmaxf(best, meet_ml[w].x);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+        l = 0.f;
+#pragma unroll
+        for (int w = 0; w < GROUPS; ++w) {
+          const float2 ml = meet_ml[w];
+          if (ml.x == -INFINITY && ml.y == 0.f) continue;
+          const float f = ex2(ml.x - best);
+          const float4 y = meet[w * PER + threadIdx.x];
+          sum.x += y.x * f, sum.y += y.y * f, sum.z += y.z * f, sum.w += y.w * f;
+          l += share(ml, best);
+        }
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        const int t = s.first + (r0 + r) / group, h = kv * group + (r0 + r) % group;
+        uint2 b4;
+        b4.x = pack2(sum.x * inv, sum.y * inv), b4.y = pack2(sum.z * inv, sum.w * inv);
+        *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + c) = b4;
+        if (c == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (best + log2f(l)) * kLn2;
+      }
+      __syncthreads();
+    }
+  }
+}
+
+template <int D>
+void launch_rows(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  using C = Cfg<D>;
+  RowsArgs args;
+  args.a = a;
+  args.pieces = 2 * sms;
+  args.part_o = static_cast<float*>(workspace);
+  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * args.pieces * kRows * D);
+  args.plog = 0;
+  while ((1 << args.plog) < a.cache.page) ++args.plog;
+  cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  paged_rows_kernel<D><<<args.pieces, kThreads, C::SMEM, stream>>>(args);
+  // one block a border between two pieces and a row
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(args.pieces - 1, std::min<int64_t>(kRows, (int64_t)a.q_heads / a.cache.heads * a.max_q));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, (const RowsArgs)args);
+}
+
+}  // namespace
+
+int64_t paged_attention_workspace(const PagedAttentionArgs& a, int sms) {
+  return (int64_t)2 * 2 * sms * kRows * (a.cache.dim + 2) * 4;
+}
+
+void launch_paged_attention(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  switch (a.cache.dim) {
+    case 64: return launch_rows<64>(a, workspace, sms, stream);
+    case 128: return launch_rows<128>(a, workspace, sms, stream);
+    case 256: return launch_rows<256>(a, workspace, sms, stream);
+    default: return launch_rows<512>(a, workspace, sms, stream);
+  }
+}
+
+}  // namespace me

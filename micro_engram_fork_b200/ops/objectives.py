@@ -41,7 +41,7 @@ KINDS = ("sigmoid", "hinge", "ipo")
 
 # ------------------------------------------------------------------------- argument checks
 # (of the plain forms; the kernels' entry points check the same in C++, where it costs a call next to nothing)
-def _kernel(name, *args):
+def kernel_call(name, *args):
     """A kernel's entry point; its complaints about an argument's value are ValueErrors."""
     try:
         return getattr(native(), name)(*args)
@@ -264,7 +264,7 @@ def top_logits(logits, k, softcap=None, temperature=1.0):
         values, ids, lse = top_logits(_rows(logits), k, softcap, temperature)
         return values.view(*lead, k), ids.view(*lead, k), lse.view(lead)
     if use_native(logits):
-        return tuple(_kernel("top_logits", logits, k, softcap, temperature))
+        return tuple(kernel_call("top_logits", logits, k, softcap, temperature))
     x, cap, temperature = _rows(logits), _cap(softcap), _temperature(temperature)
     if not 1 <= k <= min(x.shape[1], MAX_TOP):
         raise ValueError(f"k: 1 to {min(x.shape[1], MAX_TOP)}, got {k}")
@@ -293,7 +293,7 @@ def token_logprobs(logits, targets, softcap=None):
         lead = logits.shape[:-1]
         return token_logprobs(_rows(logits), _per_row(targets, lead, "targets"), softcap).view(lead)
     if use_native(logits):
-        return _kernel("token_logprobs", logits, targets, softcap)
+        return kernel_call("token_logprobs", logits, targets, softcap)
     return _TokenLogprobsRef.apply(_rows(logits), _targets(targets, logits.shape[:1]), _cap(softcap))
 
 
@@ -306,7 +306,7 @@ def token_logprobs_grad(logits, targets, coefficients=None, softcap=None, out=No
                                        _per_row(coefficients, lead, "coefficients"), softcap, _out_rows(out, logits))
         return logp.view(lead), dx.view(logits.shape) if out is None else out
     if use_native(logits):
-        logp, dx = _kernel("token_logprobs_grad", logits, targets, coefficients, softcap, out)
+        logp, dx = kernel_call("token_logprobs_grad", logits, targets, coefficients, softcap, out)
         return logp, dx if out is None else out
     x, lead = _rows(logits), logits.shape[:1]
     t, g = _targets(targets, lead), _per_row(coefficients, lead, "coefficients")
@@ -355,7 +355,7 @@ def distill_loss(logits, teacher_ids, teacher_logits, teacher_lse=None, weights=
         flat = _flat_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights)
         return distill_loss(*flat, softcap, temperature).view(logits.shape[:-1])
     if use_native(logits):
-        return _kernel("distill_loss", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
+        return kernel_call("distill_loss", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
     return _DistillRef.apply(*_checked_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap,
                                                temperature))
 
@@ -370,7 +370,7 @@ def distill_loss_grad(logits, teacher_ids, teacher_logits, teacher_lse=None, wei
         loss, dx = distill_loss_grad(*flat, softcap, temperature, _out_rows(out, logits))
         return loss.view(logits.shape[:-1]), dx.view(logits.shape) if out is None else out
     if use_native(logits):
-        loss, dx = _kernel("distill_grad", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature,
+        loss, dx = kernel_call("distill_grad", logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature,
                                          out)
         return loss, dx if out is None else out
     args = _checked_teacher(logits, teacher_ids, teacher_logits, teacher_lse, weights, softcap, temperature)
@@ -416,7 +416,7 @@ def preference_loss(logps, ref_logps, cu_seqlens, beta=0.1, label_smoothing=0.0,
     kind: "sigmoid" (with label_smoothing, the share of wrong labels), "hinge" or "ipo"."""
     kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
     if use_native(logps):
-        return tuple(_kernel("preference_loss", logps, ref_logps, cu_seqlens, kind, beta, smooth))
+        return tuple(kernel_call("preference_loss", logps, ref_logps, cu_seqlens, kind, beta, smooth))
     _check_tokens(logps, ref_logps)
     _check_offsets(cu_seqlens)
     return _PreferenceRef.apply(logps, ref_logps, cu_seqlens, kind, beta, smooth)
@@ -431,7 +431,7 @@ def preference_loss_grad(logps, ref_logps, cu_seqlens, beta=0.1, label_smoothing
     mean over the pairs."""
     kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
     if use_native(logps):
-        return tuple(_kernel("preference_pairs", logps, ref_logps, cu_seqlens, kind, beta, smooth, scale, None))
+        return tuple(kernel_call("preference_pairs", logps, ref_logps, cu_seqlens, kind, beta, smooth, scale, None))
     _check_tokens(logps, ref_logps)
     _check_offsets(cu_seqlens)
     with torch.no_grad():
@@ -445,7 +445,7 @@ def preference_logits_grad(logits, targets, ref_logps, cu_seqlens, beta=0.1, lab
     scale * gradient of sum(loss) in the logits [T, V]). `out` as in distill_loss_grad."""
     kind, beta, smooth = _pair_args(beta, label_smoothing, kind)
     if use_native(logits):
-        loss, rewards, logps, dx = _kernel("preference_logits", logits, targets, ref_logps, cu_seqlens, kind, beta, smooth,
+        loss, rewards, logps, dx = kernel_call("preference_logits", logits, targets, ref_logps, cu_seqlens, kind, beta, smooth,
                                                               scale, softcap, out)
         return loss, rewards, logps, dx if out is None else out
     if logits.dim() != 2:

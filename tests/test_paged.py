@@ -1,0 +1,201 @@
+"""The paged cache's operators on CPU: the plain forms against the 64-bit definitions, edge rules, refusals."""
+import math
+
+import pytest
+import torch
+
+import paged_oracle as oracle
+from micro_engram_fork_b200.ops import paged
+
+F32, F64 = torch.float32, torch.float64
+
+
+def append_inputs(batch, kv_shared, dtype, seed=1):
+    g = torch.Generator().manual_seed(seed)
+    heads = batch.hq + (1 if kv_shared else 2) * batch.hk
+    dev = batch.q.device
+    qkv = (torch.randn(batch.tokens, heads * batch.d, generator=g) * 1.5).to(dtype).to(dev)
+    w = (1 + 0.2 * torch.randn(2, batch.d, generator=g)).to(dev)
+    inv_freq = (10000.0 ** (-torch.arange(0, batch.d, 2).float() / batch.d)).to(dev)
+    return qkv, w[0], w[1], inv_freq
+
+
+def check_append(batch, kv_shared, dtype, call, eps=1e-6):
+    """Appends to the batch's cache and looks at every row of it."""
+    qkv, q_w, k_w, inv_freq = append_inputs(batch, kv_shared, dtype)
+    before_k, before_v = batch.k.clone(), batch.v.clone()
+    q = call(qkv, q_w, k_w, inv_freq, batch.k, batch.v, batch.table, batch.cu, batch.seq_lens, batch.hq, kv_shared, eps)
+    want_q, want_k, want_v, q_size, k_size, where = oracle.appended(batch, qkv, q_w, k_w, inv_freq, kv_shared, eps)
+    mine = torch.zeros(batch.tokens, dtype=torch.bool)
+    mine[list(where.values())] = True
+    oracle.close_append(q[mine], want_q[mine], q_size[mine], dtype)
+    assert bool((q[~mine] == 0).all())
+    for (b, pos), t in where.items():
+        page, row = int(batch.table[b, pos // batch.page]), pos % batch.page
+        oracle.close_append(batch.k[page, :, row], want_k[t], k_size[t], dtype)
+        oracle.close_append(batch.v[page, :, row], want_v[t], want_v[t].abs(), dtype)
+        before_k[page, :, row], before_v[page, :, row] = batch.k[page, :, row], batch.v[page, :, row]
+    # nothing else was touched (NaN rows included)
+    as_int = torch.int64 if dtype == F64 else torch.int32 if dtype == F32 else torch.int16
+    for now, was in ((batch.k, before_k), (batch.v, before_v)):
+        assert torch.equal(now.contiguous().view(as_int), was.contiguous().view(as_int))
+
+
+@pytest.mark.parametrize("dtype", [F32, F64])
+@pytest.mark.parametrize("lens,window", [([(0, 1)], None), ([(5, 3), (0, 17), (40, 0), (31, 1)], None), ([(70, 9), (3, 30)], 20)])
+def test_attention(lens, window, dtype):
+    batch = oracle.Batch(lens, 6, 2, 64, 16, window, dtype, before=1, after=2)
+    got = paged.paged_attention(batch.q, *batch.args(), window=window, scale=0.7)
+    oracle.close_attention(got, oracle.attention(batch, 0.7), 64, False, dtype)
+    assert bool((got[0][0] == 0).all()) and bool((got[0][-2:] == 0).all()) and bool((got[1][:, -2:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("kv_shared", [False, True])
+@pytest.mark.parametrize("dtype", [F32, F64])
+def test_append(dtype, kv_shared):
+    batch = oracle.Batch([(5, 3), (0, 17), (40, 0), (100000, 2)], 3, 1, 64, 16, None, dtype, before=2, after=1)
+    check_append(batch, kv_shared, dtype, paged.qkv_norm_rope_append)
+
+
+def bad_pages(device, dtype):
+    """A batch one of whose sequences has numbers that are no pages, another a length past its table's row: (batch,
+    the same with those keys left out as a list of visible keys for each sequence)."""
+    batch = oracle.Batch([(60, 2), (33, 1), (10, 1)], 4, 2, 64, 16, None, dtype, device)
+    batch.table[0, 1] = batch.k.shape[0]
+    batch.table[0, 2] = -7
+    batch.seq_lens[2] = 16 * batch.table.shape[1] + 5  # its row ends: the new token has no place, and sees what there is
+    batch.table[2] = batch.table[1]                    # (pages that hold numbers: all but the last are whole)
+    batch.table[2, 2:] = -1
+    return batch
+
+
+def check_bad_pages(device, dtype, single):
+    batch = bad_pages(device, dtype)
+    o, lse = paged.paged_attention(batch.q, *batch.args())
+    assert bool(o.isfinite().all()) and bool(lse.isfinite().all())
+    seen = {0: [0, 3], 1: [0, 1, 2], 2: [0, 1]}
+    for b, (first, count, length) in enumerate([(0, 2, 62), (2, 1, 34), (3, 1, 32)]):
+        ids = [int(batch.table[b, col]) for col in seen[b]]
+        key = torch.cat([torch.arange(16 * c, 16 * c + 16) for c in seen[b]]).to(device)
+        for i in range(count):
+            pos = length - count + i
+            ok = key <= pos if b < 2 else key < 32
+            k = torch.cat([batch.k[p] for p in ids], 1)[:, ok].double()
+            v = torch.cat([batch.v[p] for p in ids], 1)[:, ok].double()
+            x = torch.einsum("hgd,hkd->hgk", batch.q[first + i].double().view(2, 2, 64), k)
+            want = torch.einsum("hgk,hkd->hgd", torch.softmax(x, -1), v).reshape(4, 64)
+            assert float((o[first + i].double() - want).abs().max()) < 2.0 ** -7 * float(v.abs().max())
+            assert float((lse[:, first + i].double() - torch.logsumexp(x, -1).reshape(4)).abs().max()) < 1e-4
+    # appending there stores nothing but in pages
+    batch = bad_pages(device, dtype)
+    batch.seq_lens[1] = 0  # one new token, none in all: its position is negative
+    k, v = batch.k.clone(), batch.v.clone()
+    q = paged.qkv_norm_rope_append(*append_inputs(batch, False, dtype), *batch.args(), 4)
+    assert bool((q[2] == 0).all()) and bool((q[[0, 1, 3]] != 0).any(-1).all())
+    page = int(batch.table[0, 3])
+    k[page, :, 12:14], v[page, :, 12:14] = batch.k[page, :, 12:14], batch.v[page, :, 12:14]
+    assert torch.equal(k.nan_to_num(7.0), batch.k.nan_to_num(7.0)) and torch.equal(v.nan_to_num(7.0), batch.v.nan_to_num(7.0))
+    assert bool(batch.k[page, :, 12:14].isfinite().all())
+    o, lse = paged.paged_attention(batch.q, *batch.args())
+    assert bool((o[2] == 0).all()) and bool((lse[:, 2] == -math.inf).all())
+
+
+def test_bad_pages():
+    check_bad_pages("cpu", F32, False)
+
+
+def check_bad_offsets(device, dtype):
+    """cu_seqlens that leave the batch are taken within it."""
+    batch = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    want = paged.paged_attention(batch.q, *batch.args())
+    batch.cu[0], batch.cu[2] = -5, 1000
+    got = paged.paged_attention(batch.q[:, :], *batch.args())
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    batch.cu[1] = 900  # the first sequence takes all five tokens, the second none
+    o, lse = paged.paged_attention(batch.q, *batch.args())
+    assert o.shape == batch.q.shape and bool(o.isfinite().all())
+    batch.cu[:] = torch.tensor([4, 3, 2])
+    o, lse = paged.paged_attention(batch.q, *batch.args())
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+
+
+def test_bad_offsets():
+    check_bad_offsets("cpu", F32)
+
+
+def refusals(device, dtype):
+    """(error, call) for every argument that is refused alike on CPU and GPU."""
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    k, v, table, cu, lens = b.args()
+    qkv, q_w, k_w, f = append_inputs(b, False, dtype)
+    att = lambda *a, **kw: lambda: paged.paged_attention(*a, **kw)  # noqa: E731
+    app = lambda *a, **kw: lambda: paged.qkv_norm_rope_append(*a, **kw)  # noqa: E731
+    odd = k[:, :, :12].contiguous()
+    calls = [
+        att(b.q, k, v[:1], table, cu, lens), att(b.q, k[0], v[0], table, cu, lens), att(b.q, odd, odd, table, cu, lens),
+        att(b.q, k[..., :32].contiguous(), v[..., :32].contiguous(), table, cu, lens), att(b.q, k, v, table[:1], cu, lens),
+        att(b.q, k, v, table[0], cu, lens), att(b.q, k, v, table, cu[:2], lens), att(b.q, k, v, table, cu, lens.float()),
+        att(b.q, k, v, table.float(), cu, lens), att(b.q[:, :3], k, v, table, cu, lens), att(b.q[..., :32], k, v, table, cu, lens),
+        att(b.q[0], k, v, table, cu, lens), att(b.q, k, v, table, cu, lens, window=0), att(b.q, k, v, table, cu, lens, window=-3),
+        att(b.q, k, v, table, cu, lens, max_q=0), att(b.q, k, v, table, cu, lens, scale=math.nan),
+        att(b.q, k, v, table, cu, lens, scale=math.inf), att(b.q, k, v, table, cu, lens, out=b.q[:2].clone()),
+        att(b.q.clone().requires_grad_(), k, v, table, cu, lens), att(b.q, k[:0], v[:0], table, cu, lens),
+        app(qkv, q_w, k_w, f, k, v, table, cu, lens, 5), app(qkv, q_w, k_w, f, k, v, table, cu, lens, 4, True),
+        app(qkv, q_w, k_w, f, k, v, table, cu, lens, 0), app(qkv[0], q_w, k_w, f, k, v, table, cu, lens, 4),
+        app(qkv, q_w[:32], k_w, f, k, v, table, cu, lens, 4), app(qkv, q_w, k_w[None], f, k, v, table, cu, lens, 4),
+        app(qkv, q_w, k_w, q_w, k, v, table, cu, lens, 4), app(qkv, q_w, k_w, f, k, v[1:], table, cu, lens, 4),
+        app(qkv, q_w.clone().requires_grad_(), k_w, f, k, v, table, cu, lens, 4), app(qkv, q_w, k_w, f, k, v, table, cu[1:], lens, 4),
+    ]
+    return [(ValueError, c) for c in calls]
+
+
+def test_refusals():
+    for i, (error, call) in enumerate(refusals("cpu", F32)):
+        with pytest.raises(error):
+            call()
+            pytest.fail(f"call {i} was taken")
+
+
+def test_empty():
+    b = oracle.Batch([(20, 0), (9, 0)], 4, 2, 64, 16, None, F32)
+    o, lse = paged.paged_attention(b.q, *b.args())
+    assert o.shape == (0, 4, 64) and lse.shape == (4, 0)
+    none = torch.zeros(0, dtype=torch.int32)
+    o, lse = paged.paged_attention(torch.ones(3, 4, 64), b.k, b.v, b.table[:0], torch.zeros(1, dtype=torch.int32), none)
+    assert bool((o == 0).all()) and bool((lse == -math.inf).all())
+    qkv, q_w, k_w, f = append_inputs(b, False, F32)
+    assert paged.qkv_norm_rope_append(qkv, q_w, k_w, f, *b.args(), 4).shape == (0, 4, 64)
+
+
+def test_out():
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, F32, before=1, after=2)
+    want, _ = paged.paged_attention(b.q, *b.args())
+    out = torch.full_like(b.q, 9.0)
+    got, lse = paged.paged_attention(b.q, *b.args(), out=out)
+    assert got is out and torch.equal(out[1:-2], want[1:-2]) and bool((out[0] == 9).all()) and bool((out[-2:] == 9).all())
+
+
+def test_together():
+    """Appending a prompt in pieces and attending gives what the whole prompt gives at once."""
+    from micro_engram_fork_b200.ops.attention import attention_ref
+    from micro_engram_fork_b200.ops import norm as N
+
+    g = torch.Generator().manual_seed(0)
+    hq, hk, d, T = 4, 2, 64, 50
+    qkv = torch.randn(T, (hq + 2 * hk) * d, generator=g)
+    q_w, k_w = 1 + 0.1 * torch.randn(2, d, generator=g)
+    f = 10000.0 ** (-torch.arange(0, d, 2).float() / d)
+    cos, sin = N.rope_cos_sin(torch.arange(T), f, F32)
+    x = qkv.view(T, -1, d)
+    q = N.rope_ref(N.rmsnorm_ref(x[:, :hq], q_w), cos[:, None], sin[:, None])
+    k = N.rope_ref(N.rmsnorm_ref(x[:, hq:hq + hk], k_w), cos[:, None], sin[:, None])
+    want, _ = attention_ref(q, k, N.rmsnorm_ref(x[:, hq + hk:]), torch.zeros(T), 20, 0.3)
+    kp, vp = torch.full((2, 5, hk, 16, d), math.nan)
+    table = torch.tensor([[3, 0, 4, 1]], dtype=torch.int32)
+    parts, at = [], 0
+    for n in (7, 1, 30, 1, 11):
+        cu, lens = torch.tensor([0, n]), torch.tensor([at + n])
+        rows = paged.qkv_norm_rope_append(qkv[at:at + n], q_w, k_w, f, kp, vp, table, cu, lens, hq)
+        parts.append(paged.paged_attention(rows, kp, vp, table, cu, lens, window=20, scale=0.3)[0])
+        at += n
+    assert float((torch.cat(parts) - want).abs().max()) < 1e-5
