@@ -100,6 +100,7 @@ torch::Tensor paged_append(torch::Tensor qkv, torch::Tensor q_w, torch::Tensor k
 std::vector<torch::Tensor> paged_attention(torch::Tensor q, torch::Tensor k_pages, torch::Tensor v_pages, torch::Tensor table,
                                            torch::Tensor cu, torch::Tensor lens, int64_t window, double scale, int64_t max_q,
                                            c10::optional<torch::Tensor> out);
+std::vector<int64_t> paged_status(int64_t device);
 // attention.cu
 std::vector<torch::Tensor> attn_fwd(torch::Tensor q, torch::Tensor k, torch::Tensor v, torch::Tensor doc_start,
                                     int64_t window, double scale);
@@ -192,6 +193,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("preference_logits", &preference_logits);
   m.def("paged_append", &paged_append);
   m.def("paged_attention", &paged_attention);
+  m.def("paged_status", &paged_status);
   m.def("attn_fwd", &attn_fwd);
   m.def("attn_bwd", &attn_bwd);
   m.def("attn_fwd_tc", &attn_fwd_tc);

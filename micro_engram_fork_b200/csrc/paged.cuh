@@ -105,5 +105,40 @@ struct WorkLine {
   }
 };
 
+// ------------------------------------------------------------------------------- attention
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// A running maximum (in log2 units) moves only when a score is this far above it: p stays below 2^8.
+constexpr float kSlack = 8.f;
+
+ME_DEVICE float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// A part's sum (of terms below its own maximum) next to the whole's maximum.
+ME_DEVICE float share(float2 max_sum, float top) {
+  return max_sum.y == 0.f || max_sum.x == -INFINITY ? max_sum.y : max_sum.y * ex2(max_sum.x - top);
+}
+ME_DEVICE uint32_t pack2(float a, float b) {
+  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&x);
+}
+
+// Zeros for the rows of no sequence.
+template <int D>
+ME_DEVICE void clear_rest(const PagedAttentionArgs& a, int threads) {
+  if (!a.clear_rest) return;
+  const PagedBatch& p = a.batch;
+  const int head = p.seqs ? min(max(p.cu[0], 0), p.tokens) : p.tokens;
+  const int tail = p.seqs ? min(max(p.cu[p.seqs], head), p.tokens) : p.tokens;
+  for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < (int64_t)(head + p.tokens - tail) * a.q_heads;
+       i += (int64_t)gridDim.x * threads) {
+    const int h = (int)(i % a.q_heads), n = (int)(i / a.q_heads), t = n < head ? n : n - head + tail;
+    bf16* o = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head;
+    for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
+    a.lse[(int64_t)h * p.tokens + t] = -INFINITY;
+  }
+}
+
 }  // namespace paged
 }  // namespace me

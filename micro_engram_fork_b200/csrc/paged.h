@@ -50,8 +50,14 @@ struct PagedAttentionArgs {
   bool clear_rest;       // rows of no sequence: zeros (else left as they are)
   int max_q;             // the longest run of new tokens, as far as the caller knows
 };
-// Bytes of workspace that the call needs (16-byte aligned).
+// Bytes of workspace that the call needs (16-byte aligned), and the call; what is wrong, if anything is.
 int64_t paged_attention_workspace(const PagedAttentionArgs& a, int sms);
-void launch_paged_attention(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream);
+const char* launch_paged_attention(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream);
+
+// Its part for sequences with more than `least_rows` rows (new tokens times query heads of a key head): paged_tiles.cu.
+int64_t paged_tiles_workspace(const PagedAttentionArgs& a);
+const char* launch_paged_tiles(const PagedAttentionArgs& a, int least_rows, void* workspace, cudaStream_t stream);
+// The current device's first wait that ran out (a StatusCode, 0: none; waits for the device).
+int paged_status(int* detail);
 
 }  // namespace me

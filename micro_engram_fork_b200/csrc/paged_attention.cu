@@ -23,16 +23,7 @@ namespace me {
 namespace {
 using namespace paged;
 
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// The running maximum (in log2 units) moves only when a score is this far above it: p stays below 2^8.
-constexpr float kSlack = 8.f;
-
 ME_DEVICE uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-ME_DEVICE float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 // 16 bytes global -> shared; `bytes` 0: zeros, nothing is read.
 ME_DEVICE void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
@@ -65,15 +56,6 @@ ME_DEVICE void mma16n8k16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, ui
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// A part's sum (of terms below its own maximum) next to the whole's maximum.
-ME_DEVICE float share(float2 max_sum, float top) {
-  return max_sum.y == 0.f || max_sum.x == -INFINITY ? max_sum.y : max_sum.y * ex2(max_sum.x - top);
-}
-ME_DEVICE uint32_t pack2(float a, float b) {
-  const __nv_bfloat162 x = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&x);
-}
-
 // ------------------------------------------------------------------------------- few rows a key head
 constexpr int kRows = 8, kWarps = 4, kTile = 16, kBlock = kWarps * kTile, kThreads = kWarps * 32;
 
@@ -95,15 +77,17 @@ struct RowsArgs {
   float2* part_ml; // [slots][kRows] (maximum, sum)
   int pieces;      // blocks of the grid
   int plog;
+  int most_rows;   // sequences with more rows are the tensor cores' (paged_tiles.cu)
 };
 
 struct UnitsOf {
   int tiles;   // row tiles of the sequence
   int blocks;  // blocks of 64 keys of each
 };
-ME_DEVICE UnitsOf units_of(const PagedAttentionArgs& a, int b, const Sequence& s) {
-  if (s.count == 0) return {0, 0};
+ME_DEVICE UnitsOf units_of(const RowsArgs& args, int b, const Sequence& s) {
+  const PagedAttentionArgs& a = args.a;
   const int group = a.q_heads / a.cache.heads;
+  if (s.count == 0 || (int64_t)s.count * group > args.most_rows) return {0, 0};
   const Keys k = keys_of(a.batch, a.cache.page, s, 0, s.count - 1, a.window);
   return {(s.count * group + kRows - 1) / kRows, max((k.hi + kBlock - 1) / kBlock - k.lo / kBlock, 1)};
 }
@@ -121,21 +105,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
   const int g = lane >> 2, t4 = lane & 3;  // a fragment's row and column pair
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-  // rows of no sequence
-  if (a.clear_rest) {
-    const int head = p.seqs ? min(max(p.cu[0], 0), p.tokens) : p.tokens;
-    const int tail = p.seqs ? min(max(p.cu[p.seqs], head), p.tokens) : p.tokens;
-    for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < (int64_t)(head + p.tokens - tail) * a.q_heads;
-         i += (int64_t)gridDim.x * kThreads) {
-      const int h = (int)(i % a.q_heads), n = (int)(i / a.q_heads), t = n < head ? n : n - head + tail;
-      bf16* o = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head;
-      for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
-      a.lse[(int64_t)h * p.tokens + t] = -INFINITY;
-    }
-  }
+  clear_rest<D>(a, kThreads);
 
   auto count = [&](int b) -> int64_t {
-    const UnitsOf u = units_of(a, b, sequence_of(p, b));
+    const UnitsOf u = units_of(args, b, sequence_of(p, b));
     return (int64_t)u.tiles * hk * u.blocks;
   };
   WorkLine<kThreads> line(line_shared);
@@ -153,7 +126,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
 
   while (x < x1) {
     const Sequence s = sequence_of(p, b);
-    const UnitsOf u = units_of(a, b, s);
+    const UnitsOf u = units_of(args, b, s);
     const int64_t in_seq = x - before;
     if (in_seq >= (int64_t)u.tiles * hk * u.blocks) {  // on to the next sequence that has any
       before += (int64_t)u.tiles * hk * u.blocks;
@@ -378,7 +351,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs
   const PagedBatch& p = a.batch;
   const int hk = a.cache.heads, group = a.q_heads / hk;
   auto blocks_of = [&](int b) -> int64_t {
-    const UnitsOf u = units_of(a, b, sequence_of(p, b));
+    const UnitsOf u = units_of(args, b, sequence_of(p, b));
     return (int64_t)u.tiles * hk * u.blocks;
   };
   WorkLine<kJoinThreads> line(line_shared);
@@ -391,7 +364,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs
     int64_t before;
     const int b = line.find(p.seqs, blocks_of, x, before);
     const Sequence s = sequence_of(p, b);
-    const UnitsOf u = units_of(a, b, s);
+    const UnitsOf u = units_of(args, b, s);
     const int unit = (int)((x - before) / u.blocks);
     const int64_t begin = before + (int64_t)unit * u.blocks, end = begin + u.blocks;
     if (x == begin) continue;                                // it separates two units
@@ -445,7 +418,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs
 }
 
 template <int D>
-void launch_rows(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream) {
+void launch_rows(const PagedAttentionArgs& a, int most_rows, void* workspace, int sms, cudaStream_t stream) {
   using C = Cfg<D>;
   RowsArgs args;
   args.a = a;
@@ -454,6 +427,7 @@ void launch_rows(const PagedAttentionArgs& a, void* workspace, int sms, cudaStre
   args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * args.pieces * kRows * D);
   args.plog = 0;
   while ((1 << args.plog) < a.cache.page) ++args.plog;
+  args.most_rows = most_rows;
   cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   paged_rows_kernel<D><<<args.pieces, kThreads, C::SMEM, stream>>>(args);
   // one block a border between two pieces and a row
@@ -469,19 +443,38 @@ void launch_rows(const PagedAttentionArgs& a, void* workspace, int sms, cudaStre
   cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, (const RowsArgs)args);
 }
 
+// Which kernel takes which sequence: up to kFewRows rows this file's, which reads a sequence's keys once for every 8 of them; more
+// the tensor cores'.
+constexpr int kFewRows = 16;
+// A batch of this many sequences may hold single tokens beside chunks; below, the tensor cores' kernel takes them all.
+constexpr int kMixed = 4;
+
+enum Which { kRowsOnly, kTilesOnly, kBoth };
+Which which(const PagedAttentionArgs& a) {
+  if ((int64_t)a.max_q * (a.q_heads / a.cache.heads) <= kFewRows) return kRowsOnly;
+  return a.batch.seqs < kMixed ? kTilesOnly : kBoth;
+}
+
 }  // namespace
 
 int64_t paged_attention_workspace(const PagedAttentionArgs& a, int sms) {
-  return (int64_t)2 * 2 * sms * kRows * (a.cache.dim + 2) * 4;
+  const int64_t rows = (int64_t)2 * 2 * sms * kRows * (a.cache.dim + 2) * 4;
+  const Which w = which(a);
+  return w == kRowsOnly ? rows : w == kTilesOnly ? paged_tiles_workspace(a) : std::max(rows, paged_tiles_workspace(a));
 }
 
-void launch_paged_attention(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream) {
-  switch (a.cache.dim) {
-    case 64: return launch_rows<64>(a, workspace, sms, stream);
-    case 128: return launch_rows<128>(a, workspace, sms, stream);
-    case 256: return launch_rows<256>(a, workspace, sms, stream);
-    default: return launch_rows<512>(a, workspace, sms, stream);
+const char* launch_paged_attention(const PagedAttentionArgs& a, void* workspace, int sms, cudaStream_t stream) {
+  const Which w = which(a);
+  if (w != kTilesOnly) {
+    const int most = w == kRowsOnly ? INT32_MAX : kFewRows;
+    switch (a.cache.dim) {
+      case 64: launch_rows<64>(a, most, workspace, sms, stream); break;
+      case 128: launch_rows<128>(a, most, workspace, sms, stream); break;
+      case 256: launch_rows<256>(a, most, workspace, sms, stream); break;
+      default: launch_rows<512>(a, most, workspace, sms, stream);
+    }
   }
+  return w == kRowsOnly ? nullptr : launch_paged_tiles(a, w == kBoth ? kFewRows : 0, workspace, stream);
 }
 
 }  // namespace me

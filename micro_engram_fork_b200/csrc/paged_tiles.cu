@@ -1,0 +1,791 @@
+// Attention of chunks of new tokens over a paged cache, on the tensor cores.
+//
+// Many rows a key head: S = Q K^T and O += P V are bound by the tensor cores, and next by the L2 cache, out of which every tile of
+// rows reads its sequence's keys and values again. So two SMs work as one (cta_group::2): 256 rows (new token, query head of the
+// key head's group) a pair, 128 of them in each SM's tensor memory, and each SM loads half of every block of 128 keys, which halves what
+// both read. Per SM and block at dim 256: 64 KB in 2048 clocks of the tensor core.
+//
+//   warp 0     loads: rows of Q once a unit, then K and V through a ring of 16 KB stages (TMA; a page is a run of rows of the tensor
+//              map's second dimension, a page that is none is an index past its third, which reads zeros)
+//   warp 1     issues the products (one lane of the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
+//              softmax has the time of two products
+//   warps 2-5  softmax, a thread a row: 128 scores from tensor memory, running maximum (O is rescaled only when it grows by
+//              more than 2^8), P rounded to bf16 and put back over its scores, from where it is the A operand of P V. O is divided by the sum of
+//              the rounded terms, so that a row's one large term does not keep its rounding; the log-sum-exp is of the others.
+//              At a unit's end: O / sum to global memory
+//
+// Tensor memory: O in columns 0-255, two S (P) buffers of 128. dim 512 has no room for both halves of O: a unit takes one half of the
+// columns, and S is computed twice (4/3 of the operations).
+// Rows of V that no row of the sequence may see (past its end, before its first window) can hold anything, and 0 * NaN is not 0: in blocks that have
+// such rows the softmax threads wait for V themselves and put zeros there.
+//
+// Units (sequence, tile of rows, key head, half of the columns) are dealt to the pairs in turn, the longest of a sequence first. With few of them a
+// sequence's keys are cut into chunks, whose (max, sum, O) a second kernel joins.
+// Every wait is bounded (2 s); a timeout records ME_ERR_TIMEOUT in the status word and the kernel frees tensor memory and returns.
+#include <cudaTypedefs.h>
+
+#include <algorithm>
+#include <mutex>
+#include <unordered_map>
+
+#include "paged.cuh"
+#include "tc_common.cuh"
+
+namespace me {
+namespace {
+using namespace paged;
+using namespace tc;
+
+constexpr int kThreads = 192, kSoftWarps = 4;
+constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
+constexpr int kStage = 16 * 1024;
+constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
+constexpr int kDeals = 4;             // units a pair that cutting aims at
+
+template <int D>
+struct Cfg {
+  static constexpr int DV = D < 256 ? D : 256;       // columns of O a unit
+  static constexpr int HALVES = D / DV;
+  static constexpr int NV = D == 64 ? 128 : DV;      // columns of the P V product (dim 64: the odd SM's half is past the row, zeros)
+  static constexpr int VC = NV / 2;                  // of them in this SM
+  static constexpr int Q_BYTES = BM * D * 2;
+  static constexpr int K_STAGES = D <= 128 ? 1 : D / 128;  // stages of a block's K: 64 keys x 128 columns
+  static constexpr int V_KEYS = kStage / (VC * 2);         // keys of a stage of V
+  static constexpr int V_STAGES = BN / V_KEYS;
+  static constexpr int K_COLS = D < 128 ? D : 128;
+  static constexpr int K_BYTES = 64 * K_COLS * 2;
+  static constexpr int RING = (224 * 1024 - Q_BYTES) / kStage > 12 ? 12 : (224 * 1024 - Q_BYTES) / kStage;
+  static constexpr int BAR_OFF = Q_BYTES + RING * kStage;
+  static constexpr int SMEM = BAR_OFF + 1024 + 1024;
+  static_assert(SMEM + 256 <= 232448, "shared memory");
+  static_assert(8 * (K_STAGES + V_STAGES) > RING, "v_here");
+};
+// Blocks that loads can be ahead of the products: V of block i + 8 needs a stage that V of block i has given back.
+constexpr int kVHere = 8;
+constexpr int kO = 0, kS = 256;  // columns of tensor memory
+
+struct TilesArgs {
+  PagedAttentionArgs a;
+  float* part_o;    // [slots][slot_rows][DV]
+  float2* part_ml;  // [slots][slot_rows]
+  int slot_rows;    // a sequence with more rows is not cut, unless 256
+  int pairs;
+  int plog;
+  int least_rows;   // sequences with up to this many rows are others' work
+};
+// The first wait that ran out (ME_ERR_TIMEOUT, where): a device's own word, not an allocation that a captured graph could own.
+__device__ int g_status[2];
+
+// ------------------------------------------------------------------------------- units of work
+struct UnitsOf {
+  int tiles, chunks, per;  // tiles of rows, chunks of keys, blocks of a chunk
+  int first, blocks;       // the sequence's blocks of keys
+};
+template <int D>
+ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut) {
+  const PagedAttentionArgs& a = t.a;
+  const int group = a.q_heads / a.cache.heads, tokens = 2 * (BM / group);
+  if (s.count == 0 || (int64_t)s.count * group <= t.least_rows) return {0, 1, 0, 0, 0};
+  const Keys k = keys_of(a.batch, a.cache.page, s, 0, s.count - 1, a.window);
+  UnitsOf u;
+  u.tiles = (s.count + tokens - 1) / tokens;
+  u.first = k.lo / BN;
+  u.blocks = max((k.hi + BN - 1) / BN - u.first, 1);
+  const bool whole = cut <= 0 || (t.slot_rows < 2 * BM && (int64_t)s.count * group > t.slot_rows);
+  u.chunks = whole ? 1 : (u.blocks + cut - 1) / cut;
+  u.per = (u.blocks + u.chunks - 1) / u.chunks;
+  return u;
+}
+
+// Blocks a chunk that make about kDeals units a pair, 0: no cutting. At most 2 kDeals units a pair come of it: as many
+// as there were (fewer than kDeals) and one for every `cut` blocks.
+template <int D, int NT>
+ME_DEVICE int cut_of(const TilesArgs& t, typename WorkLine<NT>::Shared& sh, int64_t& units) {
+  WorkLine<NT> line(sh);
+  const PagedBatch& p = t.a.batch;
+  const int each = t.a.cache.heads * Cfg<D>::HALVES;
+  units = line.total(p.seqs, [&](int b) -> int64_t { return (int64_t)units_of<D>(t, b, sequence_of(p, b), 0).tiles * each; });
+  if (units == 0 || units >= (int64_t)kDeals * t.pairs) return 0;
+  const int64_t blocks = line.total(p.seqs, [&](int b) -> int64_t {
+    const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), 0);
+    return (int64_t)u.tiles * each * u.blocks;
+  });
+  const int64_t aim = (int64_t)kDeals * t.pairs;
+  return (int)max((blocks + aim - 1) / aim, (int64_t)kLeastBlocks);
+}
+
+struct Unit {
+  Sequence s;
+  int b, tile, kv, half;
+  int kb0, kb1;  // its blocks of keys, kb1 <= kb0: none
+  int chunk, chunks;
+};
+
+// A warp's way along the units: 32 sequences at a time, a lane each.
+template <int D>
+struct Walk {
+  const TilesArgs& t;
+  int cut, c = 0;
+  int64_t base = 0, mine = 0, upto = 0, all = 0;
+
+  ME_DEVICE Walk(const TilesArgs& args, int cut_blocks) : t(args), cut(cut_blocks) { scan(); }
+  ME_DEVICE void scan() {
+    const PagedBatch& p = t.a.batch;
+    const int lane = threadIdx.x & 31, b = c + lane;
+    mine = 0;
+    if (b < p.seqs) {
+      const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), cut);
+      mine = (int64_t)u.tiles * u.chunks * t.a.cache.heads * Cfg<D>::HALVES;
+    }
+    upto = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int64_t x = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += x;
+    }
+    all = __shfl_sync(0xffffffffu, upto, 31);
+  }
+  // Unit x (not below an earlier one's); false: there is none.
+  ME_DEVICE bool at(int64_t x, Unit& out) {
+    while (x >= base + all) {
+      base += all;
+      c += 32;
+      if (c >= t.a.batch.seqs) return false;
+      scan();
+    }
+    const uint32_t here = __ballot_sync(0xffffffffu, x - base < upto);
+    const int src = __ffs(here) - 1;
+    const int64_t before = base + __shfl_sync(0xffffffffu, upto - mine, src);
+    const PagedAttentionArgs& a = t.a;
+    out.b = c + src;
+    out.s = sequence_of(a.batch, out.b);
+    const UnitsOf u = units_of<D>(t, out.b, out.s, cut);
+    int64_t i = x - before;
+    out.half = (int)(i % Cfg<D>::HALVES), i /= Cfg<D>::HALVES;
+    out.kv = (int)(i % a.cache.heads), i /= a.cache.heads;
+    out.chunk = (int)(i % u.chunks), out.chunks = u.chunks;
+    out.tile = u.tiles - 1 - (int)(i / u.chunks);  // the last rows see the most keys
+    const int tokens = 2 * (BM / (a.q_heads / a.cache.heads));
+    const int i0 = out.tile * tokens, i1 = min(i0 + tokens, out.s.count) - 1;
+    const Keys k = keys_of(a.batch, a.cache.page, out.s, i0, i1, a.window);
+    out.kb0 = max(k.lo / BN, u.first + out.chunk * u.per);
+    out.kb1 = min(k.hi <= k.lo ? 0 : (k.hi + BN - 1) / BN, u.first + (out.chunk + 1) * u.per);
+    return true;
+  }
+};
+
+// ------------------------------------------------------------------------------- instructions
+ME_DEVICE void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
+      "[%2];" ::"r"(smem_addr(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      : "memory");
+}
+// A (P) from tensor memory.
+ME_DEVICE void umma_bf16_pair_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+}
+// 32 columns of this warp's lanes, not yet there until tmem_wait_ld().
+ME_DEVICE void tmem_issue_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+// The loads' results pass through here, so that no use of them moves ahead of the wait.
+ME_DEVICE void tmem_wait_ld(uint32_t (&r)[32]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]),
+                 "+r"(r[17]), "+r"(r[18]), "+r"(r[19]), "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]),
+                 "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+               :
+               : "memory");
+}
+ME_DEVICE void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
+      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+      "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]), "r"(v[19]), "r"(v[20]),
+      "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]),
+      "r"(v[31])
+      : "memory");
+}
+
+// ------------------------------------------------------------------------------- the kernel
+template <int D>
+__global__ void __launch_bounds__(kThreads, 1)
+    paged_tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
+                       const __grid_constant__ TilesArgs args) {
+  using C = Cfg<D>;
+  constexpr int RING = C::RING;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* sQ = smem;
+  uint8_t* sR = smem + C::Q_BYTES;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [RING], the even SM's counts for both
+  uint64_t* empty = full + RING;     // [RING]
+  uint64_t* q_full = empty + RING;   // the even SM's
+  uint64_t* q_empty = q_full + 1;
+  uint64_t* s_full = q_empty + 1;    // [2]
+  uint64_t* p_full = s_full + 2;     // [2], the even SM's: 4 warps of both
+  uint64_t* v_here = p_full + 2;     // [kVHere] V of a block whose rows are put right here
+  uint64_t* pv_done = v_here + kVHere;
+  uint64_t* o_free = pv_done + 1;    // the even SM's
+  uint64_t* all_done = o_free + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  __shared__ typename WorkLine<kThreads>::Shared line_shared;
+
+  const PagedAttentionArgs& a = args.a;
+  const PagedBatch& p = a.batch;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const bool leader = rank == 0;
+  const int pair = blockIdx.x >> 1;
+  const int group = a.q_heads / a.cache.heads, tokens = BM / group;  // new tokens an SM
+  int* status = g_status;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < RING; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 2 * kSoftWarps);
+    for (int i = 0; i < kVHere; ++i) mbar_init(&v_here[i], 1);
+    mbar_init(pv_done, 1);
+    mbar_init(o_free, 2 * kSoftWarps);
+    mbar_init(all_done, 1);
+    *abort = 0;
+    fence_barrier_init();
+    prefetch_tmap(&tq);
+    prefetch_tmap(&tk);
+    prefetch_tmap(&tv);
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  if (args.least_rows == 0) clear_rest<D>(a, kThreads);  // (else the kernel of few rows does)
+  int64_t units0;
+  const int cut = cut_of<D, kThreads>(args, line_shared, units0);
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  // In a block with rows of V that may hold anything, V arrives at v_here and the softmax threads put zeros there.
+  auto has_stale = [&](const Keys& seq, int kb) { return kb * BN < seq.lo || (kb + 1) * BN > seq.hi; };
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- loads
+    const uint32_t full_leader = mapa_shared(smem_addr(full), 0), q_leader = mapa_shared(smem_addr(q_full), 0);
+    const int box = min(a.cache.page, 64);          // rows of a load
+    const int per_sub = 64 / box;                   // loads of 64 keys x 64 columns
+    int g = 0;                                      // stages so far
+    int blocks_before = 0, live = 0;
+    bool ok = true;
+    Walk<D> walk(args, cut);
+    Unit u;
+    auto take = [&]() -> int {  // a stage that is free, on the whole warp
+      const int st = g % RING, r = g / RING;
+      if (r > 0 && !mbar_wait(&empty[st], (r - 1) & 1, status, 50, abort)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      ++g;
+      return st;
+    };
+    for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
+      const int n = u.kb1 - u.kb0;
+      if (n <= 0) continue;
+      const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
+      const int y0 = u.kv << args.plog;
+      // pages of a block, a lane for each 16 keys; an index past the cache where there is none
+      auto pages_of = [&](int kb) {
+        int id = -1;
+        if (lane < 8) id = page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog);
+        return id < 0 ? a.cache.pages : id;
+      };
+      auto load_k = [&](int kb, int ids) {  // this SM's 64 keys
+#pragma unroll 1
+        for (int c = 0; c < C::K_STAGES; ++c) {
+          const int st = take();
+          if (!ok) return;
+          if (leader && lane == 0) mbar_expect_tx(&full[st], 2 * C::K_BYTES);
+          const int i = lane / per_sub, r = lane % per_sub * box;  // lane: columns i, keys from r
+          const int key = kb * BN + (int)rank * 64 + r;
+          const int id = __shfl_sync(0xffffffffu, ids, (((int)rank * 64 + r) / 16) & 7);
+          if (i < C::K_COLS / 64)
+            tma_load_3d_pair(sR + st * kStage + i * (64 * 128) + r * 128, &tk, full_leader + st * 8, c * 128 + i * 64, y0 + (key & (a.cache.page - 1)), id);
+        }
+      };
+      auto load_v = [&](int kb, int ids, int count) {
+        const bool stale = has_stale(seq, kb);
+        if (stale && lane == 0) mbar_expect_tx(&v_here[count % kVHere], C::V_STAGES * kStage);
+        __syncwarp();
+#pragma unroll 1
+        for (int c = 0; c < C::V_STAGES; ++c) {
+          const int st = take();
+          if (!ok) return;
+          if (leader && lane == 0) {
+            if (stale) mbar_arrive(&full[st]);
+            else mbar_expect_tx(&full[st], 2 * kStage);
+          }
+          // 64 keys x 64 columns after another: columns first (2 x 64 keys of a stage where VC is 128, else 128 keys)
+          constexpr int SUBS = kStage / (64 * 128);
+          const int i = lane / per_sub, r = lane % per_sub * box;
+          const int col = C::VC == 128 ? i * 64 : 0, row = C::VC == 128 ? c * 64 + r : i * 64 + r;
+          const int key = kb * BN + row;
+          const int id = __shfl_sync(0xffffffffu, ids, (row / 16) & 7);
+          const uint32_t bar = stale ? mapa_shared(smem_addr(&v_here[count % kVHere]), rank) : full_leader + st * 8;
+          if (i < SUBS)
+            tma_load_3d_pair(sR + st * kStage + i * (64 * 128) + r * 128, &tv, bar, u.half * C::DV + (int)rank * C::VC + col, y0 + (key & (a.cache.page - 1)), id);
+        }
+      };
+      int ids = pages_of(u.kb0), next = n > 1 ? pages_of(u.kb0 + 1) : 0;
+      load_k(u.kb0, ids);
+      if (live > 0 && ok && !mbar_wait(q_empty, (live - 1) & 1, status, 51, abort)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      if (ok && lane == 0) {
+        if (leader) mbar_expect_tx(q_full, 2 * (D / 64) * tokens * group * 128);
+        for (int c = 0; c < D / 64; ++c)
+          tma_load_3d_pair(sQ + c * (BM * 128), &tq, q_leader, c * 64, u.kv * group, u.s.first + u.tile * 2 * tokens + (int)rank * tokens);
+      }
+      __syncwarp();
+      for (int j = 0; j < n && ok; ++j) {
+        const int after = j + 2 < n ? pages_of(u.kb0 + j + 2) : 0;
+        if (j + 1 < n) load_k(u.kb0 + j + 1, next);
+        if (ok) load_v(u.kb0 + j, ids, blocks_before + j);
+        ids = next, next = after;
+      }
+      blocks_before += n;
+      ++live;
+    }
+    // Every stage this SM filled is given back by the products that read it: then no copy is in flight.
+    for (int i = max(0, g - RING); i < g; ++i) {
+      if (*abort && !leader) break;
+      mbar_wait(&empty[i % RING], (i / RING) & 1, status, 52, abort, 500000000ull);
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    if (leader) {
+      const uint32_t id_s = idesc_bf16(2 * BM, BN), id_o = idesc_bf16(2 * BM, C::NV, true);
+      const uint32_t aQ = smem_addr(sQ), aR = smem_addr(sR);
+      int g = 0, gb = 0, live = 0;  // stages, blocks, units so far
+      bool ok = true;
+      Walk<D> walk(args, cut);
+      Unit u;
+      for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
+        const int n = u.kb1 - u.kb0;
+        if (n <= 0) continue;
+        if (lane == 0) {
+          ok = mbar_wait(q_full, live & 1, status, 60, abort);
+          auto product_pv = [&](int i) {  // block i of all
+            if (!ok) return;
+            if (!mbar_wait_cluster(&p_full[i & 1], (i >> 1) & 1, status, 61, abort)) {
+              ok = false;
+              return;
+            }
+#pragma unroll 1
+            for (int c = 0; c < C::V_STAGES; ++c, ++g) {
+              const int st = g % RING;
+              if (!mbar_wait(&full[st], (g / RING) & 1, status, 62, abort)) {
+                ok = false;
+                return;
+              }
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < C::V_KEYS / 16; ++kk)
+                umma_bf16_pair_ts(tmem + kO, tmem + kS + (i & 1) * BN + (c * (C::V_KEYS / 16) + kk) * 8,
+                                  desc_mn_sw128(aR + st * kStage + kk * 2048, 64 * 128, 1024), id_o, (i > gb || c > 0 || kk > 0) ? 1u : 0u);
+              umma_commit_pair(&empty[st], 0x3);
+            }
+            umma_commit_pair(pv_done, 0x3);
+          };
+          for (int j = 0; j < n && ok; ++j) {
+            const int i = gb + j;
+#pragma unroll 1
+            for (int c = 0; c < C::K_STAGES; ++c, ++g) {
+              const int st = g % RING;
+              if (!mbar_wait(&full[st], (g / RING) & 1, status, 63, abort)) {
+                ok = false;
+                break;
+              }
+              tc_fence_after();
+#pragma unroll
+              for (int kk = 0; kk < C::K_COLS / 16; ++kk)
+                umma_bf16_pair(tmem + kS + (i & 1) * BN, desc_sw128(aQ + (c * 2 + kk / 4) * (BM * 128) + (kk & 3) * 32),
+                               desc_sw128(aR + st * kStage + (kk / 4) * (64 * 128) + (kk & 3) * 32), id_s, (c | kk) != 0);
+              umma_commit_pair(&empty[st], 0x3);
+            }
+            if (!ok) break;
+            umma_commit_pair(&s_full[i & 1], 0x3);
+            if (j == n - 1) umma_commit_pair(q_empty, 0x3);
+            if (j == 1 && live > 0 && !mbar_wait_cluster(o_free, (live - 1) & 1, status, 64, abort)) ok = false;
+            if (j >= 1) product_pv(i - 1);
+          }
+          if (ok && n == 1 && live > 0 && !mbar_wait_cluster(o_free, (live - 1) & 1, status, 64, abort)) ok = false;
+          if (ok) product_pv(gb + n - 1);
+          gb += n;
+        }
+        ok = __all_sync(0xffffffffu, ok);
+        ++live;
+      }
+      if (lane == 0) {  // every product has ended before tensor memory is freed
+        umma_commit_pair(all_done, 0x1);
+        mbar_wait(all_done, 0, status, 65, nullptr, 500000000ull);
+      }
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax
+    const int quarter = warp & 3, r = quarter * 32 + lane;  // row of the SM
+    const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
+    const uint32_t p_leader = mapa_shared(smem_addr(p_full), 0), o_leader = mapa_shared(smem_addr(o_free), 0);
+    const float to_log2 = a.scale * kLog2e;
+    const int ti = r / group, head = r % group;
+    int g = 0, gb = 0;       // stages, blocks so far
+    uint32_t v_phases = 0;   // bit i: parity of v_here[i]
+    bool ok = true;
+    Walk<D> walk(args, cut);
+    Unit u;
+    for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
+      const int n = max(u.kb1 - u.kb0, 0);
+      const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
+      const int token = u.tile * 2 * tokens + (int)rank * tokens + ti;  // of the sequence's new ones
+      const bool mine = ti < tokens && token < u.s.count;
+      const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
+      const int from = a.window > 0 ? u.s.context + token - a.window + 1 : 0;
+      float m = -INFINITY, l = 0.f, l_rounded = 0.f;  // sums of p, and of p as the product takes it
+      auto pages_of = [&](int kb) {  // bit i: keys 16 i of the block have a page
+        const bool is = lane < 8 && page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog) >= 0;
+        return __ballot_sync(0xffffffffu, is);
+      };
+      uint32_t there = n > 0 ? pages_of(u.kb0) : 0;
+      for (int j = 0; j < n && ok; ++j) {
+        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN;
+        const uint32_t there_next = j + 1 < n ? pages_of(kb + 1) : 0;
+        if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, status, 70, abort)) ok = false;
+        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        tc_fence_after();
+        uint32_t s[4][32];
+        const uint32_t at = tmem + lanes + kS + (i & 1) * BN;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_issue_ld32(at + c * 32, s[c]);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
+        const bool open = there == 0xffu && ((key0 >= from && key0 + BN - 1 <= last) || !mine);
+        if (!__all_sync(0xffffffffu, open)) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int key = key0 + c * 32 + e;
+              if (key > last || key < from || !((there >> (c * 2 + e / 16)) & 1)) s[c][e] = 0xff800000u;  // -inf
+            }
+        }
+        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
+        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+        bool resc = false;
+        float alpha = 1.f;
+        if (top > m + kSlack) {
+          if (m != -INFINITY) alpha = ex2(m - top), resc = true;
+          m = top;
+        }
+        const float z = m == -INFINITY ? 0.f : m;
+        float sum[2] = {0.f, 0.f}, rounded[2] = {0.f, 0.f};
+        uint32_t pk[2][32];
+#pragma unroll
+        for (int c = 0; c < 4; ++c)
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), to_log2, -z));
+            const uint32_t h = pack2(p0, p1);
+            sum[0] += p0, sum[1] += p1;
+            rounded[0] += __uint_as_float(h << 16), rounded[1] += __uint_as_float(h & 0xffff0000u);
+            pk[c >> 1][(c & 1) * 16 + e / 2] = h;
+          }
+        l = l * alpha + (sum[0] + sum[1]);
+        l_rounded = l_rounded * alpha + (rounded[0] + rounded[1]);
+        tmem_st32u(at, pk[0]);
+        tmem_st32u(at + 32, pk[1]);
+        if (__any_sync(0xffffffffu, resc) && j > 0) {  // O stands still once the product before has ended
+          if (!mbar_wait(pv_done, (i - 1) & 1, status, 71, abort)) ok = false;
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          tc_fence_after();
+#pragma unroll 1
+          for (int c = 0; c < C::DV / 32; ++c) {
+            uint32_t o[32];
+            tmem_issue_ld32(tmem + lanes + kO + c * 32, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st32u(tmem + lanes + kO + c * 32, o);
+          }
+        }
+        if (has_stale(seq, kb)) {  // thread r: key r of the block, this SM's columns
+          if (!mbar_wait(&v_here[i % kVHere], (v_phases >> (i % kVHere)) & 1, status, 72, abort)) ok = false;
+          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          v_phases ^= 1u << (i % kVHere);
+          const int key = key0 + r;
+          if (key < seq.lo || key >= seq.hi) {
+            // V's stages of block j come after those of K of the blocks up to j + 1
+            const int st = (g + min(j + 2, n) * C::K_STAGES + j * C::V_STAGES + (C::VC == 128 ? r / 64 : 0)) % RING;
+#pragma unroll
+            for (int c = 0; c < C::VC / 8; ++c) {
+              const int sub = C::VC == 128 ? c / 8 : r / 64;
+              *reinterpret_cast<uint4*>(sR + st * kStage + sub * (64 * 128) + (r & 63) * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
+            }
+          }
+          fence_async_smem();
+        }
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(p_leader + (i & 1) * 8);
+        there = there_next;
+      }
+      // ---- the unit's end
+      if (n > 0 && ok) {
+        // a phase at a time: the last but one may still be open
+        if (n > 1 && !mbar_wait(pv_done, (gb + n - 2) & 1, status, 73, abort)) ok = false;
+        if (ok && !mbar_wait(pv_done, (gb + n - 1) & 1, status, 74, abort)) ok = false;
+        ok = __all_sync(0xffffffffu, ok);
+      }
+      if (!ok) break;
+      tc_fence_after();
+      // a part's O goes with the sum l
+      const float inv = l_rounded == 0.f ? 0.f : (u.chunks > 1 ? l : 1.f) / l_rounded;
+      const int t = u.s.first + token, h = u.kv * group + head;
+      const int64_t slot = (x * args.slot_rows + (int)rank * tokens * group + r);
+#pragma unroll 1
+      for (int c = 0; c < C::DV / 32; ++c) {
+        uint32_t o[32];
+        if (n > 0) {
+          tmem_issue_ld32(tmem + lanes + kO + c * 32, o);
+          tmem_wait_ld(o);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 32; ++e) o[e] = 0;
+        }
+        if (!mine) continue;
+        if (u.chunks > 1) {
+          float* dst = args.part_o + slot * C::DV + c * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                                              __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+        } else {
+          bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + c * 32;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
+            uint4 v;
+            v.x = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            v.y = pack2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            v.z = pack2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
+            v.w = pack2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
+            *reinterpret_cast<uint4*>(dst + e) = v;
+          }
+        }
+      }
+      if (n > 0) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cluster(o_leader);
+      }
+      if (mine) {
+        if (u.chunks > 1) args.part_ml[slot] = make_float2(m, l);
+        else if (u.half == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+      }
+      gb += n;
+      g += n * (C::K_STAGES + C::V_STAGES);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();  // both SMs are done with every product, copy and remote arrival
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+// Joins the chunks of sequences that were cut: a block takes a unit's first chunk and every gridDim.y-th group of its rows.
+constexpr int kJoinThreads = 256;
+template <int D>
+__global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
+  using C = Cfg<D>;
+  constexpr int PER = C::DV / 4, ROWS = kJoinThreads / PER;
+  __shared__ typename WorkLine<kJoinThreads>::Shared line_shared;
+  const PagedAttentionArgs& a = args.a;
+  int64_t units;
+  const int cut = cut_of<D, kJoinThreads>(args, line_shared, units);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (cut == 0) return;
+  const int group = a.q_heads / a.cache.heads, tokens = 2 * (BM / group);
+  Walk<D> walk(args, cut);
+  Unit u;
+  for (int64_t x = blockIdx.x; walk.at(x, u); x += gridDim.x) {
+    if (u.chunks == 1 || u.chunk != 0) continue;
+    const int64_t stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
+    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group;
+    const int c = threadIdx.x % PER * 4;
+    for (int r = blockIdx.y * ROWS + threadIdx.x / PER; r < rows; r += gridDim.y * ROWS) {
+      float top = -INFINITY, l = 0.f;
+      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int k = 0; k < u.chunks; ++k) {
+        const int64_t slot = (x + k * stride) * args.slot_rows + r;
+        const float2 ml = args.part_ml[slot];
+        const float4 y = *reinterpret_cast<const float4*>(args.part_o + slot * C::DV + c);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float up = fmaxf(top, ml.x);
+        const float f0 = top == -INFINITY ? 0.f : ex2(top - up), f1 = ex2(ml.x - up);
+        o.x = o.x * f0 + y.x * f1, o.y = o.y * f0 + y.y * f1, o.z = o.z * f0 + y.z * f1, o.w = o.w * f0 + y.w * f1;
+        l = l * f0 + ml.y * f1;
+        top = up;
+      }
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t = u.s.first + i0 + r / group, h = u.kv * group + r % group;
+      uint2 b4;
+      b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + c) = b4;
+      if (c == 0 && u.half == 0) a.lse[(int64_t)h * a.batch.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------- host
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* f = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) != cudaSuccess) f = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(f);
+  }();
+  return fn;
+}
+
+// [z][y][x] bf16 with boxes of 64 columns, 128-byte swizzle.
+bool make_map(CUtensorMap* map, const void* ptr, int64_t x, int64_t y, int64_t z, int64_t y_stride, int64_t z_stride, int box_y, int box_z) {
+  cuuint64_t dims[3] = {(cuuint64_t)x, (cuuint64_t)y, (cuuint64_t)z};
+  cuuint64_t strides[2] = {(cuuint64_t)y_stride * 2, (cuuint64_t)z_stride * 2};
+  cuuint32_t box[3] = {64, (cuuint32_t)box_y, (cuuint32_t)box_z}, one[3] = {1, 1, 1};
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int D>
+int resident_pairs() {
+  static std::mutex mu;
+  static std::unordered_map<int, int> known;
+  int dev = 0;
+  cudaGetDevice(&dev);
+  std::lock_guard<std::mutex> lk(mu);
+  auto it = known.find(dev);
+  if (it != known.end()) return it->second;
+  cudaFuncSetAttribute(paged_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  int sms = 0, n = 0;
+  cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(sms & ~1);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = Cfg<D>::SMEM;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  if (cudaOccupancyMaxActiveClusters(&n, paged_tiles_kernel<D>, &cfg) != cudaSuccess || n <= 0) {
+    (void)cudaGetLastError();
+    n = sms / 2;
+  }
+  return known[dev] = n;
+}
+
+template <int D>
+int slot_rows_of(const PagedAttentionArgs& a) {
+  return (int)std::min<int64_t>(2 * BM, ((int64_t)a.max_q * (a.q_heads / a.cache.heads) + 7) / 8 * 8);
+}
+template <int D>
+int64_t workspace(const PagedAttentionArgs& a) {
+  return (int64_t)2 * kDeals * resident_pairs<D>() * slot_rows_of<D>(a) * (Cfg<D>::DV + 2) * 4;
+}
+
+template <int D>
+const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cudaStream_t stream) {
+  using C = Cfg<D>;
+  if (encode_fn() == nullptr) return "cuTensorMapEncodeTiled is unavailable";
+  TilesArgs args;
+  args.a = a;
+  args.pairs = resident_pairs<D>();
+  args.slot_rows = slot_rows_of<D>(a);
+  args.part_o = static_cast<float*>(space);
+  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * kDeals * args.pairs * args.slot_rows * C::DV);
+  args.plog = 0;
+  while ((1 << args.plog) < a.cache.page) ++args.plog;
+  args.least_rows = least_rows;
+  bind_primary_context();
+  const int group = a.q_heads / a.cache.heads, box = std::min(a.cache.page, 64);
+  CUtensorMap tq, tk, tv;
+  if (!make_map(&tq, a.q, D, a.q_heads, a.batch.tokens, a.q_head, a.q_token, group, BM / group) ||
+      !make_map(&tk, a.cache.k, D, (int64_t)a.cache.heads * a.cache.page, a.cache.pages, D, a.cache.k_stride, box, 1) ||
+      !make_map(&tv, a.cache.v, D, (int64_t)a.cache.heads * a.cache.page, a.cache.pages, D, a.cache.v_stride, box, 1))
+    return "cuTensorMapEncodeTiled failed";
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = 2, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.gridDim = dim3(2 * args.pairs);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = C::SMEM;
+  cfg.stream = stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D>, tq, tk, tv, args);
+  if (e != cudaSuccess) return cudaGetErrorString(e);
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(2 * kDeals * args.pairs, std::max(1, std::min(8, args.slot_rows / 8)));
+  cfg.blockDim = dim3(kJoinThreads);
+  cfg.dynamicSmemBytes = 0;
+  e = cudaLaunchKernelEx(&cfg, paged_join_tiles_kernel<D>, args);
+  return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
+}
+
+}  // namespace
+
+int paged_status(int* detail) {
+  int word[2] = {0, 0};
+  cudaMemcpyFromSymbol(word, g_status, sizeof word);
+  *detail = word[1];
+  return word[0];
+}
+
+int64_t paged_tiles_workspace(const PagedAttentionArgs& a) {
+  switch (a.cache.dim) {
+    case 64: return workspace<64>(a);
+    case 128: return workspace<128>(a);
+    case 256: return workspace<256>(a);
+    default: return workspace<512>(a);
+  }
+}
+
+const char* launch_paged_tiles(const PagedAttentionArgs& a, int least_rows, void* space, cudaStream_t stream) {
+  switch (a.cache.dim) {
+    case 64: return launch<64>(a, least_rows, space, stream);
+    case 128: return launch<128>(a, least_rows, space, stream);
+    case 256: return launch<256>(a, least_rows, space, stream);
+    default: return launch<512>(a, least_rows, space, stream);
+  }
+}
+
+}  // namespace me

@@ -80,9 +80,13 @@ const float* check_weight(const Tensor& w, const Tensor& pages, int64_t n, const
 
 int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; }
 
-bool rows_fit(const Tensor& t) {  // 16-byte vectors of heads [T, H, D]
-  return t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) % 8 == 0) && (t.size(0) <= 1 || t.stride(0) % 8 == 0) && aligned(t);
+// Heads [T, H, D] as the kernels and their tensor maps take them: contiguous, a multiple of 8 elements apart.
+bool rows_fit(const Tensor& t) {
+  auto fits = [&](int i) { return t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0); };
+  return t.stride(2) == 1 && fits(0) && fits(1) && aligned(t);
 }
+int64_t head_stride(const Tensor& t) { return t.size(1) <= 1 ? t.size(2) : t.stride(1); }
+int64_t token_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0); }
 
 }  // namespace
 
@@ -131,7 +135,7 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   ME_CHECK_VALUE(q_heads >= heads && q_heads % heads == 0 && q_heads / heads <= 128, "q: heads a multiple of the pages' ", text(heads),
                  " (up to 128 times) are needed, got ", text(q_heads));
   ME_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window: a positive number or None, got ", text(window));
-  ME_CHECK_VALUE(scale == scale && scale < INFINITY && scale > -INFINITY, "scale: a finite number is needed");
+  ME_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale: a positive number is needed");
   ME_CHECK_VALUE(max_q >= 0, "max_q: a positive number or None, got ", text(max_q));
   const Batch batch = check_batch(k_pages, table, cu, lens, tokens);
   a.batch = batch.args;
@@ -149,9 +153,9 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   Tensor lse = torch::empty({q_heads, tokens}, q.options().dtype(torch::kFloat32).requires_grad(false));
   if (tokens == 0) return {o, lse};
   a.q = q.data_ptr();
-  a.q_token = q.stride(0), a.q_head = q.stride(1);
+  a.q_token = token_stride(q), a.q_head = head_stride(q);
   a.o = o.data_ptr();
-  a.o_token = o.stride(0), a.o_head = o.stride(1);
+  a.o_token = token_stride(o), a.o_head = head_stride(o);
   a.lse = lse.data_ptr<float>();
   a.q_heads = (int)q_heads;
   a.window = (int)window;
@@ -159,7 +163,16 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   a.clear_rest = !out.has_value();
   a.max_q = (int)std::min(max_q ? max_q : tokens, tokens);
   Tensor workspace = torch::empty({me::paged_attention_workspace(a, sms())}, q.options().dtype(torch::kByte).requires_grad(false));
-  me::launch_paged_attention(a, workspace.data_ptr(), sms(), at::cuda::getCurrentCUDAStream());
+  const char* wrong = me::launch_paged_attention(a, workspace.data_ptr(), sms(), at::cuda::getCurrentCUDAStream());
+  TORCH_CHECK(wrong == nullptr, "paged_attention: ", wrong);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {o, lse};
+}
+
+// (code, where) of the first device wait that ran out in the attention on this device; (0, 0): none.
+std::vector<int64_t> paged_status(int64_t device) {
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
+  int detail = 0;
+  const int code = me::paged_status(&detail);
+  return {code, detail};
 }

@@ -11,7 +11,7 @@ tokens in all, so its new tokens have the positions seq_lens[b] - (their number)
   paged_attention       the new tokens' attention over all that their sequence has in the cache, themselves
                         included (what ops.attention.attention_fwd does, with a cache)
 
-CUDA tensors run the sm_100a kernels (csrc/paged_append.cu, paged_attention.cu) on the current stream; nothing is read
+CUDA tensors run the sm_100a kernels (csrc/paged_append.cu, paged_attention.cu, paged_tiles.cu) on the current stream; nothing is read
 back to the host, so a call can be captured into a graph and replayed with other lengths and pages of the same shapes.
 CPU tensors run the plain PyTorch forms below, which compute in fp32 (fp64 for fp64 inputs). Rules that hold for both:
 
@@ -182,8 +182,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         raise ValueError(f"q: [tokens, heads, {d}] is needed, got {tuple(q.shape)}")
     if q.shape[1] < hk or q.shape[1] % hk or q.shape[1] // hk > 128:
         raise ValueError(f"q: heads a multiple of the pages' {hk} (up to 128 times) are needed, got {q.shape[1]}")
-    if not abs(float(scale)) < float("inf"):
-        raise ValueError(f"scale: a finite number is needed, got {scale}")
+    if not 0 < float(scale) < float("inf"):
+        raise ValueError(f"scale: a positive number is needed, got {scale}")
     if out is not None and out.shape != q.shape:
         raise ValueError(f"out: q's shape {tuple(q.shape)} is needed, got {tuple(out.shape)}")
     with torch.no_grad():

@@ -24,7 +24,7 @@ CXX = ["-O3", "-std=c++17"]
 SOURCES = [os.path.join(CSRC, f) for f in (
     "bindings.cpp", "symm.cpp", "engram.cu", "norm.cu", "ce.cu", "attention.cu", "attention_tc.cu", "gemm.cu", "gemm_fused.cu", "gemm_nf4.cu",
     "p2p.cu", "nf4.cu", "objectives_torch.cpp", "objectives.cu", "top_logits.cu", "preference.cu",
-    "paged_torch.cpp", "paged_append.cu", "paged_attention.cu",
+    "paged_torch.cpp", "paged_append.cu", "paged_attention.cu", "paged_tiles.cu",
 )]
 
 setup(

@@ -138,7 +138,7 @@ def refusals(device, dtype):
         att(b.q, k, v, table.float(), cu, lens), att(b.q[:, :3], k, v, table, cu, lens), att(b.q[..., :32], k, v, table, cu, lens),
         att(b.q[0], k, v, table, cu, lens), att(b.q, k, v, table, cu, lens, window=0), att(b.q, k, v, table, cu, lens, window=-3),
         att(b.q, k, v, table, cu, lens, max_q=0), att(b.q, k, v, table, cu, lens, scale=math.nan),
-        att(b.q, k, v, table, cu, lens, scale=math.inf), att(b.q, k, v, table, cu, lens, out=b.q[:2].clone()),
+        att(b.q, k, v, table, cu, lens, scale=math.inf), att(b.q, k, v, table, cu, lens, scale=0.0), att(b.q, k, v, table, cu, lens, scale=-1.0), att(b.q, k, v, table, cu, lens, out=b.q[:2].clone()),
         att(b.q.clone().requires_grad_(), k, v, table, cu, lens), att(b.q, k[:0], v[:0], table, cu, lens),
         app(qkv, q_w, k_w, f, k, v, table, cu, lens, 5), app(qkv, q_w, k_w, f, k, v, table, cu, lens, 4, True),
         app(qkv, q_w, k_w, f, k, v, table, cu, lens, 0), app(qkv[0], q_w, k_w, f, k, v, table, cu, lens, 4),

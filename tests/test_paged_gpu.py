@@ -17,6 +17,14 @@ BF = torch.bfloat16
 HEADS = [(32, 16, 256), (32, 4, 512), (4, 2, 64), (4, 1, 128), (3, 3, 128), (15, 3, 128), (16, 1, 64), (6, 2, 256), (2, 2, 512), (9, 1, 512)]
 
 
+@pytest.fixture(autouse=True)
+def no_wait_ran_out():
+    yield
+    from micro_engram_fork_b200 import native
+
+    assert native().paged_status(0) == [0, 0]
+
+
 def _attend(batch, single, scale=1.0, max_q=None):
     got = paged.paged_attention(batch.q, *batch.args(), window=batch.window, scale=scale, max_q=max_q)
     oracle.close_attention(got, oracle.attention(batch, scale), batch.d, single)
