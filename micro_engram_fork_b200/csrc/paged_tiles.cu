@@ -9,8 +9,8 @@
 //              map's second dimension, a page that is none is an index past its third, which reads zeros)
 //   warp 1     issues the products (one lane of the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
 //              softmax has the time of two products
-//   warps 2-5  softmax, a thread a row: 128 scores from tensor memory, running maximum (O is rescaled only when it grows by
-//              more than 2^8), P rounded to bf16 and put back over its scores, from where it is the A operand of P V. O is divided by the sum of
+//   warps 2-9  softmax, two threads a row (the halves of a block's keys; they agree on the maximum in shared memory): 64 scores from
+//              tensor memory, running maximum (O is rescaled only when it grows by more than 2^8), P rounded to bf16 and put back over its scores, from where it is the A operand of P V. O is divided by the sum of
 //              the rounded terms, so that a row's one large term does not keep its rounding; the log-sum-exp is of the others.
 //              At a unit's end: O / sum to global memory
 //
@@ -36,7 +36,7 @@ namespace {
 using namespace paged;
 using namespace tc;
 
-constexpr int kThreads = 192, kSoftWarps = 4;
+constexpr int kThreads = 320, kSoftWarps = 8;
 constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
 constexpr int kStage = 16 * 1024;
 constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
@@ -56,8 +56,9 @@ struct Cfg {
   static constexpr int K_BYTES = 64 * K_COLS * 2;
   static constexpr int RING = (224 * 1024 - Q_BYTES) / kStage > 12 ? 12 : (224 * 1024 - Q_BYTES) / kStage;
   static constexpr int BAR_OFF = Q_BYTES + RING * kStage;
-  static constexpr int SMEM = BAR_OFF + 1024 + 1024;
-  static_assert(SMEM + 256 <= 232448, "shared memory");
+  static constexpr int MEET_OFF = BAR_OFF + 512;   // [parity][half][BM] floats: maxima, then sums
+  static constexpr int SMEM = MEET_OFF + 2 * 2 * BM * 4;
+  static_assert(SMEM <= 232448, "shared memory");
   static_assert(8 * (K_STAGES + V_STAGES) > RING, "v_here");
 };
 // Blocks that loads can be ahead of the products: V of block i + 8 needs a stage that V of block i has given back.
@@ -222,6 +223,17 @@ ME_DEVICE void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
       : "memory");
 }
 
+// Arrive on a barrier of either SM of the pair. The release is this SM's alone: enough for what tensor memory holds, and without the
+// wait for all earlier memory operations that one at cluster scope costs (1000 clocks a block).
+ME_DEVICE void mbar_arrive_cta(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cta.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+ME_DEVICE void st_global32(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]),
+               "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
 // ------------------------------------------------------------------------------- the kernel
 template <int D>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -229,8 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                        const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
   constexpr int RING = C::RING;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  extern __shared__ __align__(1024) uint8_t smem[];  // (no room to align it here: there is no other shared memory)
   uint8_t* sQ = smem;
   uint8_t* sR = smem + C::Q_BYTES;
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [RING], the even SM's counts for both
@@ -238,14 +249,16 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = empty + RING;   // the even SM's
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;    // [2]
-  uint64_t* p_full = s_full + 2;     // [2], the even SM's: 4 warps of both
+  uint64_t* p_full = s_full + 2;     // [2], the even SM's: 8 warps of both
   uint64_t* v_here = p_full + 2;     // [kVHere] V of a block whose rows are put right here
   uint64_t* pv_done = v_here + kVHere;
   uint64_t* o_free = pv_done + 1;    // the even SM's
   uint64_t* all_done = o_free + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  uint64_t* meet_bar = all_done + 1;  // [4] the two warps of the same rows
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet_bar + 4);
+  float* meet = reinterpret_cast<float*>(smem + C::MEET_OFF);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  __shared__ typename WorkLine<kThreads>::Shared line_shared;
+  auto& line_shared = *reinterpret_cast<typename WorkLine<kThreads>::Shared*>(sQ);  // before Q comes
 
   const PagedAttentionArgs& a = args.a;
   const PagedBatch& p = a.batch;
@@ -255,6 +268,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int pair = blockIdx.x >> 1;
   const int group = a.q_heads / a.cache.heads, tokens = BM / group;  // new tokens an SM
   int* status = g_status;
+  if (smem_addr(smem) & 1023) {
+    report(status, ME_ERR_ALIGN, 76);
+    return;
+  }
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < RING; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
@@ -265,6 +282,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(pv_done, 1);
     mbar_init(o_free, 2 * kSoftWarps);
     mbar_init(all_done, 1);
+    for (int i = 0; i < 4; ++i) mbar_init(&meet_bar[i], 2);
     *abort = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -444,14 +462,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else {
     // ---------------------------------------------------------------- softmax
-    const int quarter = warp & 3, r = quarter * 32 + lane;  // row of the SM
+    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;  // half of a block's keys; row of the SM
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t p_leader = mapa_shared(smem_addr(p_full), 0), o_leader = mapa_shared(smem_addr(o_free), 0);
     const float to_log2 = a.scale * kLog2e;
     const int ti = r / group, head = r % group;
-    int g = 0, gb = 0;       // stages, blocks so far
-    uint32_t v_phases = 0;   // bit i: parity of v_here[i]
+    // 32-byte stores of O where its rows allow them
+    const bool wide = reinterpret_cast<uintptr_t>(a.o) % 32 == 0 && a.o_token % 16 == 0 && a.o_head % 16 == 0;
+    int g = 0, gb = 0, met = 0;  // stages, blocks, meetings so far
+    uint32_t v_phases = 0;       // bit i: parity of v_here[i]
     bool ok = true;
+    // The other half's x of this row.
+    auto other = [&](float x) {
+      meet[((met & 1) * 2 + half) * BM + r] = x;
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&meet_bar[quarter]);
+      if (!mbar_wait(&meet_bar[quarter], met & 1, status, 75, abort)) ok = false;
+      ok = __all_sync(0xffffffffu, ok);
+      const float y = meet[((met & 1) * 2 + (half ^ 1)) * BM + r];
+      ++met;
+      return y;
+    };
     Walk<D> walk(args, cut);
     Unit u;
     for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
@@ -461,40 +492,48 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = ti < tokens && token < u.s.count;
       const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
       const int from = a.window > 0 ? u.s.context + token - a.window + 1 : 0;
-      float m = -INFINITY, l = 0.f, l_rounded = 0.f;  // sums of p, and of p as the product takes it
-      auto pages_of = [&](int kb) {  // bit i: keys 16 i of the block have a page
-        const bool is = lane < 8 && page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog) >= 0;
-        return __ballot_sync(0xffffffffu, is);
+      float m = -INFINITY, l = 0.f, l_rounded = 0.f;  // of this half: sums of p, and of p as the product takes it
+      auto pages_of = [&](int kb) {  // bit i: keys 16 i of the four blocks from kb on have a page
+        return __ballot_sync(0xffffffffu, page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog) >= 0);
       };
-      uint32_t there = n > 0 ? pages_of(u.kb0) : 0;
+      uint32_t there = n > 0 ? pages_of(u.kb0) : 0, there_next = 0;
       for (int j = 0; j < n && ok; ++j) {
-        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN;
-        const uint32_t there_next = j + 1 < n ? pages_of(kb + 1) : 0;
+        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN + half * 64;
+        if ((j & 3) == 0) {
+          if (j > 0) there = there_next;
+          if (j + 4 < n) there_next = pages_of(kb + 4);
+        }
+        const uint32_t pages = (there >> ((j & 3) * 8 + half * 4)) & 0xf;
         if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, status, 70, abort)) ok = false;
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
-        uint32_t s[4][32];
+        uint32_t s[2][32];
         const uint32_t at = tmem + lanes + kS + (i & 1) * BN;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_issue_ld32(at + c * 32, s[c]);
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_wait_ld(s[c]);
-        const bool open = there == 0xffu && ((key0 >= from && key0 + BN - 1 <= last) || !mine);
+        tmem_issue_ld32(at + half * 64, s[0]);
+        tmem_issue_ld32(at + half * 64 + 32, s[1]);
+        tmem_wait_ld(s[0]);
+        tmem_wait_ld(s[1]);
+        const bool open = pages == 0xfu && ((key0 >= from && key0 + 63 <= last) || !mine);
         if (!__all_sync(0xffffffffu, open)) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
+          for (int c = 0; c < 2; ++c) {
+            // bits from .. last of these 32 keys that have a page
+            const int k0 = key0 + c * 32, lo = min(max(from - k0, 0), 32), hi = min(max(last + 1 - k0, 0), 32);
+            uint32_t seen = (uint32_t)(((1ull << hi) - 1) & ~((1ull << lo) - 1));
+            seen &= ((pages >> (2 * c)) & 1 ? 0xffffu : 0u) | ((pages >> (2 * c + 1)) & 1 ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int key = key0 + c * 32 + e;
-              if (key > last || key < from || !((there >> (c * 2 + e / 16)) & 1)) s[c][e] = 0xff800000u;  // -inf
-            }
+            for (int e = 0; e < 32; ++e)
+              if (!(seen & (1u << e))) s[c][e] = 0xff800000u;  // -inf
+          }
         }
         float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
-        const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
+        top = fmaxf(top, other(top));  // (both halves have read their scores now: P may go over them)
+        if (!ok) break;
         bool resc = false;
         float alpha = 1.f;
         if (top > m + kSlack) {
@@ -503,47 +542,49 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         const float z = m == -INFINITY ? 0.f : m;
         float sum[2] = {0.f, 0.f}, rounded[2] = {0.f, 0.f};
-        uint32_t pk[2][32];
+        uint32_t pk[32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+        for (int c = 0; c < 2; ++c)
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
             const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), to_log2, -z));
             const uint32_t h = pack2(p0, p1);
             sum[0] += p0, sum[1] += p1;
             rounded[0] += __uint_as_float(h << 16), rounded[1] += __uint_as_float(h & 0xffff0000u);
-            pk[c >> 1][(c & 1) * 16 + e / 2] = h;
+            pk[c * 16 + e / 2] = h;
           }
         l = l * alpha + (sum[0] + sum[1]);
         l_rounded = l_rounded * alpha + (rounded[0] + rounded[1]);
-        tmem_st32u(at, pk[0]);
-        tmem_st32u(at + 32, pk[1]);
+        tmem_st32u(at + half * 32, pk);
         if (__any_sync(0xffffffffu, resc) && j > 0) {  // O stands still once the product before has ended
           if (!mbar_wait(pv_done, (i - 1) & 1, status, 71, abort)) ok = false;
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < C::DV / 32; ++c) {
+          for (int c = 0; c < C::DV / 64; ++c) {
             uint32_t o[32];
-            tmem_issue_ld32(tmem + lanes + kO + c * 32, o);
+            const uint32_t col = tmem + lanes + kO + half * (C::DV / 2) + c * 32;
+            tmem_issue_ld32(col, o);
             tmem_wait_ld(o);
 #pragma unroll
             for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32u(tmem + lanes + kO + c * 32, o);
+            tmem_st32u(col, o);
           }
         }
-        if (has_stale(seq, kb)) {  // thread r: key r of the block, this SM's columns
+        const bool stale = has_stale(seq, kb);
+        if (stale) {  // row r: key r of the block, a half of this SM's columns
           if (!mbar_wait(&v_here[i % kVHere], (v_phases >> (i % kVHere)) & 1, status, 72, abort)) ok = false;
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           v_phases ^= 1u << (i % kVHere);
-          const int key = key0 + r;
+          const int key = kb * BN + r;
           if (key < seq.lo || key >= seq.hi) {
             // V's stages of block j come after those of K of the blocks up to j + 1
             const int st = (g + min(j + 2, n) * C::K_STAGES + j * C::V_STAGES + (C::VC == 128 ? r / 64 : 0)) % RING;
 #pragma unroll
-            for (int c = 0; c < C::VC / 8; ++c) {
+            for (int c = half * (C::VC / 16); c < (half + 1) * (C::VC / 16); ++c) {
               const int sub = C::VC == 128 ? c / 8 : r / 64;
-              *reinterpret_cast<uint4*>(sR + st * kStage + sub * (64 * 128) + (r & 63) * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
+              const int chunk = C::VC == 128 ? (c + r) & 7 : c;  // any order, together all of them
+              *reinterpret_cast<uint4*>(sR + st * kStage + sub * (64 * 128) + (r & 63) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
             }
           }
           fence_async_smem();
@@ -551,8 +592,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(p_leader + (i & 1) * 8);
-        there = there_next;
+        if (lane == 0) {
+          // P is in tensor memory, which the fences above order; what was written to shared memory has to be there for the other SM's eyes
+          if (stale) mbar_arrive_cluster(p_leader + (i & 1) * 8);
+          else mbar_arrive_cta(p_leader + (i & 1) * 8);
+        }
       }
       // ---- the unit's end
       if (n > 0 && ok) {
@@ -563,48 +607,65 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       tc_fence_after();
-      // a part's O goes with the sum l
-      const float inv = l_rounded == 0.f ? 0.f : (u.chunks > 1 ? l : 1.f) / l_rounded;
+      l += other(l);
+      l_rounded += other(l_rounded);
+      if (!ok) break;
+      const float inv = l_rounded == 0.f ? 0.f : (u.chunks > 1 ? l : 1.f) / l_rounded;  // (a part's O goes with the sum l)
       const int t = u.s.first + token, h = u.kv * group + head;
-      const int64_t slot = (x * args.slot_rows + (int)rank * tokens * group + r);
+      const int64_t slot = x * args.slot_rows + (int)rank * tokens * group + r;
+      const int col0 = half * (C::DV / 2);
+      if (u.chunks > 1) {
 #pragma unroll 1
-      for (int c = 0; c < C::DV / 32; ++c) {
-        uint32_t o[32];
-        if (n > 0) {
-          tmem_issue_ld32(tmem + lanes + kO + c * 32, o);
-          tmem_wait_ld(o);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 32; ++e) o[e] = 0;
-        }
-        if (!mine) continue;
-        if (u.chunks > 1) {
-          float* dst = args.part_o + slot * C::DV + c * 32;
-#pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(dst + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                                              __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-        } else {
-          bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + c * 32;
-#pragma unroll
-          for (int e = 0; e < 32; e += 8) {
-            uint4 v;
-            v.x = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
-            v.y = pack2(__uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
-            v.z = pack2(__uint_as_float(o[e + 4]) * inv, __uint_as_float(o[e + 5]) * inv);
-            v.w = pack2(__uint_as_float(o[e + 6]) * inv, __uint_as_float(o[e + 7]) * inv);
-            *reinterpret_cast<uint4*>(dst + e) = v;
+        for (int c = 0; c < C::DV / 64; ++c) {
+          uint32_t o[32];
+          if (n > 0) {
+            tmem_issue_ld32(tmem + lanes + kO + col0 + c * 32, o);
+            tmem_wait_ld(o);
           }
+          float* dst = args.part_o + slot * C::DV + col0 + c * 32;
+          if (mine)
+#pragma unroll
+            for (int e = 0; e < 32; e += 4)
+              *reinterpret_cast<float4*>(dst + e) =
+                  n > 0 ? make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv,
+                                      __uint_as_float(o[e + 3]) * inv)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
         }
-      }
-      if (n > 0) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive_cluster(o_leader);
-      }
-      if (mine) {
-        if (u.chunks > 1) args.part_ml[slot] = make_float2(m, l);
-        else if (u.half == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        if (n > 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cta(o_leader);
+        }
+        if (mine && half == 0) args.part_ml[slot] = make_float2(m, l);
+      } else {
+        // all of O into registers first: the next unit's products may begin
+        uint32_t out[C::DV / 4] = {};
+        if (n > 0) {
+#pragma unroll
+          for (int c = 0; c < C::DV / 64; ++c) {
+            uint32_t o[32];
+            tmem_issue_ld32(tmem + lanes + kO + col0 + c * 32, o);
+            tmem_wait_ld(o);
+#pragma unroll
+            for (int e = 0; e < 32; e += 2) out[c * 16 + e / 2] = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive_cta(o_leader);
+        }
+        if (mine) {
+          bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + col0;
+#pragma unroll
+          for (int e = 0; e < C::DV / 4; e += 8) {
+            if (wide) {
+              st_global32(dst + e * 2, &out[e]);
+            } else {
+              *reinterpret_cast<uint4*>(dst + e * 2) = make_uint4(out[e], out[e + 1], out[e + 2], out[e + 3]);
+              *reinterpret_cast<uint4*>(dst + e * 2 + 8) = make_uint4(out[e + 4], out[e + 5], out[e + 6], out[e + 7]);
+            }
+          }
+          if (u.half == 0 && half == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
       }
       gb += n;
       g += n * (C::K_STAGES + C::V_STAGES);
