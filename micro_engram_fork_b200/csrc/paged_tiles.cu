@@ -5,14 +5,15 @@
 // key head's group) a pair, 128 of them in each SM's tensor memory, and each SM loads half of every block of 128 keys, which halves what
 // both read. Per SM and block at dim 256: 64 KB in 2048 clocks of the tensor core.
 //
-//   warp 0     loads: rows of Q once a unit, then K and V through a ring of 16 KB stages (TMA; a page is a run of rows of the tensor
-//              map's second dimension, a page that is none is an index past its third, which reads zeros)
-//   warp 1     issues the products (one lane of the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
+//   warps 0, 2 loads: rows of Q once a unit, and K; V (TMA, each through a ring of its own; a page is a run of rows of the tensor
+//              map, a page that is none is an index past its last dimension, which reads zeros)
+//   warp 1     issues the products (from the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
 //              softmax has the time of two products
-//   warps 2-9  softmax, two threads a row (the halves of a block's keys; they agree on the maximum in shared memory): 64 scores from
-//              tensor memory, running maximum (O is rescaled only when it grows by more than 2^8), P rounded to bf16 and put back over its scores, from where it is the A operand of P V. O is divided by the sum of
-//              the rounded terms, so that a row's one large term does not keep its rounding; the log-sum-exp is of the others.
-//              At a unit's end: O / sum to global memory
+//   warps 4-11 softmax, two threads a row (a half of a block's keys each): 64 scores from tensor memory; p = 2^(s - m) by the
+//              maximum m that the row's threads had agreed on a block before, for the maximum of this block comes round through shared
+//              memory while they compute (a row that has none yet, or jumps by more than 2^60, waits for it). O is rescaled
+//              only when m grows by more than 2^8. P is rounded to bf16 (as what it is multiplied with is) and put back over its scores, from where
+//              it is the A operand of P V; the sum is of the terms before that. At a unit's end: O / sum to global memory
 //
 // Tensor memory: O in columns 0-255, two S (P) buffers of 128. dim 512 has no room for both halves of O: a unit takes one half of the
 // columns, and S is computed twice (4/3 of the operations).
@@ -26,6 +27,7 @@
 
 #include <algorithm>
 #include <mutex>
+#include <type_traits>
 #include <unordered_map>
 
 #include "paged.cuh"
@@ -36,9 +38,8 @@ namespace {
 using namespace paged;
 using namespace tc;
 
-constexpr int kThreads = 320, kSoftWarps = 8;
+constexpr int kParts = 2, kSoftWarps = 4 * kParts, kFirstSoft = 4, kThreads = (kFirstSoft + kSoftWarps) * 32;  // kParts softmax threads a row
 constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
-constexpr int kStage = 16 * 1024;
 constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
 constexpr int kDeals = 4;             // units a pair that cutting aims at
 
@@ -49,21 +50,17 @@ struct Cfg {
   static constexpr int NV = D == 64 ? 128 : DV;      // columns of the P V product (dim 64: the odd SM's half is past the row, zeros)
   static constexpr int VC = NV / 2;                  // of them in this SM
   static constexpr int Q_BYTES = BM * D * 2;
-  static constexpr int K_STAGES = D <= 128 ? 1 : D / 128;  // stages of a block's K: 64 keys x 128 columns
-  static constexpr int V_KEYS = kStage / (VC * 2);         // keys of a stage of V
-  static constexpr int V_STAGES = BN / V_KEYS;
-  static constexpr int K_COLS = D < 128 ? D : 128;
-  static constexpr int K_BYTES = 64 * K_COLS * 2;
-  static constexpr int RING = (224 * 1024 - Q_BYTES) / kStage > 12 ? 12 : (224 * 1024 - Q_BYTES) / kStage;
-  static constexpr int BAR_OFF = Q_BYTES + RING * kStage;
-  static constexpr int MEET_OFF = BAR_OFF + 512;   // [parity][half][BM] floats: maxima, then sums
-  static constexpr int SMEM = MEET_OFF + 2 * 2 * BM * 4;
+  // a stage of K: this SM's 64 keys of a block x KC columns; of V: 128 keys x VC, one set of 64 keys after the other
+  static constexpr int KC = D < 256 ? D : 256, K_STAGES = D / KC;
+  static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = BN * VC * 2;
+  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 1 : D == 256 ? 2 : 6;  // stages
+  static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KR * K_BYTES, BAR_OFF = V_OFF + VR * V_BYTES;
+  static constexpr int MEET_OFF = BAR_OFF + 512;   // [4 blocks][BM]: maxima; [kParts][BM]: sums
+  static constexpr int SMEM = MEET_OFF + 4 * BM * 4;
   static_assert(SMEM <= 232448, "shared memory");
-  static_assert(8 * (K_STAGES + V_STAGES) > RING, "v_here");
 };
-// Blocks that loads can be ahead of the products: V of block i + 8 needs a stage that V of block i has given back.
-constexpr int kVHere = 8;
 constexpr int kO = 0, kS = 256;  // columns of tensor memory
+constexpr float kJump = 60.f;   // a score this far above m (log2) does not wait for the next block
 
 struct TilesArgs {
   PagedAttentionArgs a;
@@ -176,20 +173,56 @@ struct Walk {
 };
 
 // ------------------------------------------------------------------------------- instructions
-ME_DEVICE void tma_load_3d_pair(void* dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z) {
+// A load by the lanes of `issue`, into this SM's shared memory; `bar_cluster` may be the other's.
+ME_DEVICE void tma_load_3d_pair_if(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z, uint32_t issue) {
   asm volatile(
-      "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], "
-      "[%2];" ::"r"(smem_addr(dst)),
-      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z)
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];\n\t}" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "r"(issue)
       : "memory");
 }
-// A (P) from tensor memory.
-ME_DEVICE void umma_bf16_pair_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
+ME_DEVICE void tma_load_4d_pair_if(uint32_t dst, const CUtensorMap* map, uint32_t bar_cluster, int x, int y, int z, int w, uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];\n\t}" ::"r"(
+          dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "r"(w), "r"(issue)
+      : "memory");
+}
+// The order of floats as that of integers, and back.
+ME_DEVICE int ordered(float x) {
+  const int i = __float_as_int(x);
+  return i ^ ((i >> 31) & 0x7fffffff);
+}
+ME_DEVICE float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
+
+// The pair's product and its commits, by the lanes of `issue` (one lane of the warp that goes along).
+ME_DEVICE void umma_bf16_pair_if(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate));
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue));
+}
+// A (P) from tensor memory.
+ME_DEVICE void umma_bf16_pair_ts_if(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue));
+}
+ME_DEVICE void umma_commit_pair_if(uint64_t* bar, uint32_t issue, uint16_t mask = 0x3) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(smem_addr(bar)),
+      "h"(mask), "r"(issue)
+      : "memory");
 }
 // 32 columns of this warp's lanes, not yet there until tmem_wait_ld().
 ME_DEVICE void tmem_issue_ld32(uint32_t taddr, uint32_t (&r)[32]) {
@@ -212,6 +245,27 @@ ME_DEVICE void tmem_wait_ld(uint32_t (&r)[32]) {
                :
                : "memory");
 }
+ME_DEVICE void tmem_issue_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+ME_DEVICE void tmem_wait_ld(uint32_t (&r)[16]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]),
+                 "+r"(r[9]), "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+               :
+               : "memory");
+}
+ME_DEVICE void tmem_st16u(uint32_t taddr, const uint32_t (&v)[16]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+               "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), "r"(v[10]),
+               "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+               : "memory");
+}
+
 ME_DEVICE void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
@@ -222,7 +276,6 @@ ME_DEVICE void tmem_st32u(uint32_t taddr, const uint32_t (&v)[32]) {
       "r"(v[31])
       : "memory");
 }
-
 // Arrive on a barrier of either SM of the pair. The release is this SM's alone: enough for what tensor memory holds, and without the
 // wait for all earlier memory operations that one at cluster scope costs (1000 clocks a block).
 ME_DEVICE void mbar_arrive_cta(uint32_t cluster_addr) {
@@ -240,24 +293,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     paged_tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
-  constexpr int RING = C::RING;
+  constexpr int KR = C::KR, VR = C::VR;
   extern __shared__ __align__(1024) uint8_t smem[];  // (no room to align it here: there is no other shared memory)
-  uint8_t* sQ = smem;
-  uint8_t* sR = smem + C::Q_BYTES;
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [RING], the even SM's counts for both
-  uint64_t* empty = full + RING;     // [RING]
-  uint64_t* q_full = empty + RING;   // the even SM's
+  uint8_t *sQ = smem, *sK = smem + C::K_OFF, *sV = smem + C::V_OFF;
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + C::BAR_OFF);  // [KR], the even SM's counts for both
+  uint64_t* k_empty = k_full + KR;
+  uint64_t* v_full = k_empty + KR;   // [VR], the even SM's
+  uint64_t* v_empty = v_full + VR;
+  uint64_t* v_here = v_empty + VR;   // [VR] V of a block whose rows are put right here
+  uint64_t* q_full = v_here + VR;    // the even SM's
   uint64_t* q_empty = q_full + 1;
   uint64_t* s_full = q_empty + 1;    // [2]
-  uint64_t* p_full = s_full + 2;     // [2], the even SM's: 8 warps of both
-  uint64_t* v_here = p_full + 2;     // [kVHere] V of a block whose rows are put right here
-  uint64_t* pv_done = v_here + kVHere;
-  uint64_t* o_free = pv_done + 1;    // the even SM's
+  uint64_t* p_full = s_full + 2;     // [2], the even SM's: the softmax warps of both
+  uint64_t* pv_done = p_full + 2;    // [2]
+  uint64_t* o_full = pv_done + 2;    // once a unit
+  uint64_t* o_free = o_full + 1;     // the even SM's
   uint64_t* all_done = o_free + 1;
-  uint64_t* meet_bar = all_done + 1;  // [4] the two warps of the same rows
+  uint64_t* meet_bar = all_done + 1;  // [4] the warps of the same rows
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet_bar + 4);
-  float* meet = reinterpret_cast<float*>(smem + C::MEET_OFF);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* tops = reinterpret_cast<int*>(smem + C::MEET_OFF);       // [4][BM] ordered()
+  float* sums = reinterpret_cast<float*>(smem + C::MEET_OFF);   // [kParts][BM]
   auto& line_shared = *reinterpret_cast<typename WorkLine<kThreads>::Shared*>(sQ);  // before Q comes
 
   const PagedAttentionArgs& a = args.a;
@@ -274,15 +330,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < RING; ++i) mbar_init(&full[i], 1), mbar_init(&empty[i], 1);
+    for (int i = 0; i < KR; ++i) mbar_init(&k_full[i], 1), mbar_init(&k_empty[i], 1);
+    for (int i = 0; i < VR; ++i) mbar_init(&v_full[i], 1), mbar_init(&v_empty[i], 1), mbar_init(&v_here[i], 1);
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 2 * kSoftWarps);
-    for (int i = 0; i < kVHere; ++i) mbar_init(&v_here[i], 1);
-    mbar_init(pv_done, 1);
+    for (int i = 0; i < 2; ++i) mbar_init(&s_full[i], 1), mbar_init(&p_full[i], 2 * kSoftWarps), mbar_init(&pv_done[i], 1);
+    mbar_init(o_full, 1);
     mbar_init(o_free, 2 * kSoftWarps);
     mbar_init(all_done, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&meet_bar[i], 2);
+    for (int i = 0; i < 4; ++i) mbar_init(&meet_bar[i], kParts);
     *abort = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -290,37 +346,48 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tv);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  for (int i = threadIdx.x; i < 4 * BM; i += kThreads) tops[i] = ordered(-INFINITY);
   if (args.least_rows == 0) clear_rest<D>(a, kThreads);  // (else the kernel of few rows does)
   int64_t units0;
   const int cut = cut_of<D, kThreads>(args, line_shared, units0);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
+  constexpr uint32_t tmem = 0;  // all columns are this kernel's, so they begin at 0 (and addresses need no register)
+  if (*tmem_slot != tmem) {
+    if (threadIdx.x == 0) report(status, ME_ERR_ALIGN, 77), *abort = 1;
+  }
+  __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
   // In a block with rows of V that may hold anything, V arrives at v_here and the softmax threads put zeros there.
   auto has_stale = [&](const Keys& seq, int kb) { return kb * BN < seq.lo || (kb + 1) * BN > seq.hi; };
 
-  if (warp == 0) {
+  if (warp == 0 || warp == 2) {
     // ---------------------------------------------------------------- loads
+    // (the whole warp goes along and its lane 0 issues, as for the products)
+    const bool of_k = warp == 0;
+    uint64_t *full = of_k ? k_full : v_full, *empty = of_k ? k_empty : v_empty;
+    const int ring = of_k ? KR : VR;
     const uint32_t full_leader = mapa_shared(smem_addr(full), 0), q_leader = mapa_shared(smem_addr(q_full), 0);
-    const int box = min(a.cache.page, 64);          // rows of a load
-    const int per_sub = 64 / box;                   // loads of 64 keys x 64 columns
-    int g = 0;                                      // stages so far
-    int blocks_before = 0, live = 0;
+    const uint32_t v_here_own = mapa_shared(smem_addr(v_here), rank), aQ = smem_addr(sQ), aK = smem_addr(sK), aV = smem_addr(sV);
+    // rows of a load; pages of 64 and more: all columns of a stage at once
+    const int box = min(a.cache.page, 64), page_mask = a.cache.page - 1;
+    const uint32_t one = lane == 0;
+    int st = 0, round = 0, g = 0;   // the ring's next stage; stages so far
+    int live = 0;
     bool ok = true;
     Walk<D> walk(args, cut);
     Unit u;
-    auto take = [&]() -> int {  // a stage that is free, on the whole warp
-      const int st = g % RING, r = g / RING;
-      if (r > 0 && !mbar_wait(&empty[st], (r - 1) & 1, status, 50, abort)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
+    auto free_stage = [&] {
+      if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1, status, of_k ? 50 : 53, abort));
+    };
+    auto next_stage = [&] {
       ++g;
-      return st;
+      if (++st == ring) st = 0, ++round;
     };
     for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
-      const int n = u.kb1 - u.kb0;
+      const int n = __shfl_sync(0xffffffffu, u.kb1 - u.kb0, 0);
       if (n <= 0) continue;
       const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
       const int y0 = u.kv << args.plog;
@@ -330,158 +397,162 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane < 8) id = page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog);
         return id < 0 ? a.cache.pages : id;
       };
-      auto load_k = [&](int kb, int ids) {  // this SM's 64 keys
-#pragma unroll 1
-        for (int c = 0; c < C::K_STAGES; ++c) {
-          const int st = take();
-          if (!ok) return;
-          if (leader && lane == 0) mbar_expect_tx(&full[st], 2 * C::K_BYTES);
-          const int i = lane / per_sub, r = lane % per_sub * box;  // lane: columns i, keys from r
-          const int key = kb * BN + (int)rank * 64 + r;
-          const int id = __shfl_sync(0xffffffffu, ids, (((int)rank * 64 + r) / 16) & 7);
-          if (i < C::K_COLS / 64)
-            tma_load_3d_pair(sR + st * kStage + i * (64 * 128) + r * 128, &tk, full_leader + st * 8, c * 128 + i * 64, y0 + (key & (a.cache.page - 1)), id);
-        }
-      };
-      auto load_v = [&](int kb, int ids, int count) {
-        const bool stale = has_stale(seq, kb);
-        if (stale && lane == 0) mbar_expect_tx(&v_here[count % kVHere], C::V_STAGES * kStage);
-        __syncwarp();
-#pragma unroll 1
-        for (int c = 0; c < C::V_STAGES; ++c) {
-          const int st = take();
-          if (!ok) return;
-          if (leader && lane == 0) {
-            if (stale) mbar_arrive(&full[st]);
-            else mbar_expect_tx(&full[st], 2 * kStage);
+      // 64 keys from `in` of block kb, NC x 64 columns from chunk x on
+      auto load64 = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int kb, int in, int ids, int x, auto NC) {
+        if (box == 64) {
+          const int id = __shfl_sync(0xffffffffu, ids, in / 16);
+          tma_load_4d_pair_if(dst, map, bar, 0, y0 + ((kb * BN + in) & page_mask), x, id, one);
+        } else {
+          for (int row = 0; row < 64; row += box) {
+            const int id = __shfl_sync(0xffffffffu, ids, (in + row) / 16);
+#pragma unroll
+            for (int i = 0; i < decltype(NC)::value; ++i)
+              tma_load_4d_pair_if(dst + i * (64 * 128) + row * 128, map, bar, 0, y0 + ((kb * BN + in + row) & page_mask), x + i, id, one);
           }
-          // 64 keys x 64 columns after another: columns first (2 x 64 keys of a stage where VC is 128, else 128 keys)
-          constexpr int SUBS = kStage / (64 * 128);
-          const int i = lane / per_sub, r = lane % per_sub * box;
-          const int col = C::VC == 128 ? i * 64 : 0, row = C::VC == 128 ? c * 64 + r : i * 64 + r;
-          const int key = kb * BN + row;
-          const int id = __shfl_sync(0xffffffffu, ids, (row / 16) & 7);
-          const uint32_t bar = stale ? mapa_shared(smem_addr(&v_here[count % kVHere]), rank) : full_leader + st * 8;
-          if (i < SUBS)
-            tma_load_3d_pair(sR + st * kStage + i * (64 * 128) + r * 128, &tv, bar, u.half * C::DV + (int)rank * C::VC + col, y0 + (key & (a.cache.page - 1)), id);
         }
       };
-      int ids = pages_of(u.kb0), next = n > 1 ? pages_of(u.kb0 + 1) : 0;
-      load_k(u.kb0, ids);
-      if (live > 0 && ok && !mbar_wait(q_empty, (live - 1) & 1, status, 51, abort)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      if (ok && lane == 0) {
-        if (leader) mbar_expect_tx(q_full, 2 * (D / 64) * tokens * group * 128);
-        for (int c = 0; c < D / 64; ++c)
-          tma_load_3d_pair(sQ + c * (BM * 128), &tq, q_leader, c * 64, u.kv * group, u.s.first + u.tile * 2 * tokens + (int)rank * tokens);
-      }
-      __syncwarp();
+      int ids = pages_of(u.kb0);
       for (int j = 0; j < n && ok; ++j) {
-        const int after = j + 2 < n ? pages_of(u.kb0 + j + 2) : 0;
-        if (j + 1 < n) load_k(u.kb0 + j + 1, next);
-        if (ok) load_v(u.kb0 + j, ids, blocks_before + j);
-        ids = next, next = after;
+        const int next = j + 1 < n ? pages_of(u.kb0 + j + 1) : 0, kb = u.kb0 + j;
+        if (of_k) {
+#pragma unroll
+          for (int c = 0; c < C::K_STAGES; ++c) {
+            free_stage();
+            if (!ok) break;
+            if (leader && one) mbar_expect_tx(&full[st], 2 * C::K_BYTES);
+            __syncwarp();
+            load64(aK + st * C::K_BYTES, &tk, full_leader + st * 8, kb, (int)rank * 64, ids, c * (C::KC / 64), std::integral_constant<int, C::KC / 64>());
+            next_stage();
+          }
+          if (j == 0 && ok) {  // Q, once the unit before is done with it
+            if (live > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (live - 1) & 1, status, 51, abort));
+            if (!ok) break;
+            if (leader && one) mbar_expect_tx(q_full, 2 * (D / 64) * tokens * group * 128);
+            __syncwarp();
+#pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+              tma_load_3d_pair_if(aQ + c * (BM * 128), &tq, q_leader, c * 64, u.kv * group, u.s.first + u.tile * 2 * tokens + (int)rank * tokens, one);
+          }
+        } else {
+          const bool stale = has_stale(seq, kb);
+          free_stage();
+          if (!ok) break;
+          if (one) {
+            if (stale) mbar_expect_tx(&v_here[st], C::V_BYTES);
+            if (leader && stale) mbar_arrive(&full[st]);
+            if (leader && !stale) mbar_expect_tx(&full[st], 2 * C::V_BYTES);
+          }
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            load64(aV + st * C::V_BYTES + c * (C::V_BYTES / 2), &tv, stale ? v_here_own + st * 8 : full_leader + st * 8, kb, c * 64, ids,
+                   (u.half * C::DV + (int)rank * C::VC) / 64, std::integral_constant<int, C::VC / 64>());
+          next_stage();
+        }
+        ids = next;
       }
-      blocks_before += n;
       ++live;
     }
     // Every stage this SM filled is given back by the products that read it: then no copy is in flight.
-    for (int i = max(0, g - RING); i < g; ++i) {
+    for (int i = max(0, g - ring); i < g; ++i) {
       if (*abort && !leader) break;
-      mbar_wait(&empty[i % RING], (i / RING) & 1, status, 52, abort, 500000000ull);
+      mbar_wait(&empty[i % ring], (i / ring) & 1, status, 52, abort, 500000000ull);
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products
+    // The whole warp goes along, so that descriptors stay in uniform registers; its lane 0 issues. (With lane 0 alone in here an
+    // issue took 110 to 180 clocks, more than the product.)
     if (leader) {
       const uint32_t id_s = idesc_bf16(2 * BM, BN), id_o = idesc_bf16(2 * BM, C::NV, true);
-      const uint32_t aQ = smem_addr(sQ), aR = smem_addr(sR);
-      int g = 0, gb = 0, live = 0;  // stages, blocks, units so far
+      const uint64_t dQ = desc_sw128(smem_addr(sQ)), dK = desc_sw128(smem_addr(sK)), dV = desc_mn_sw128(smem_addr(sV), 64 * 128, 1024);
+      const uint32_t one = lane == 0;
+      int kst = 0, kphase = 0, vst = 0, vphase = 0;  // the rings' next stages
+      int gb = 0, live = 0;    // blocks, units so far
       bool ok = true;
+      auto wait = [&](uint64_t* bar, int parity, int where) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, status, where, abort)); };
       Walk<D> walk(args, cut);
       Unit u;
       for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
-        const int n = u.kb1 - u.kb0;
+        const int n = __shfl_sync(0xffffffffu, u.kb1 - u.kb0, 0);
         if (n <= 0) continue;
-        if (lane == 0) {
-          ok = mbar_wait(q_full, live & 1, status, 60, abort);
-          auto product_pv = [&](int i) {  // block i of all
-            if (!ok) return;
-            if (!mbar_wait_cluster(&p_full[i & 1], (i >> 1) & 1, status, 61, abort)) {
-              ok = false;
-              return;
-            }
-#pragma unroll 1
-            for (int c = 0; c < C::V_STAGES; ++c, ++g) {
-              const int st = g % RING;
-              if (!mbar_wait(&full[st], (g / RING) & 1, status, 62, abort)) {
-                ok = false;
-                return;
-              }
-              tc_fence_after();
+        const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
+        wait(q_full, live & 1, 60);
+        for (int j = 0; j <= n && ok; ++j) {
+          if (j < n) {
+            const uint32_t to = kS + ((gb + j) & 1) * BN;
 #pragma unroll
-              for (int kk = 0; kk < C::V_KEYS / 16; ++kk)
-                umma_bf16_pair_ts(tmem + kO, tmem + kS + (i & 1) * BN + (c * (C::V_KEYS / 16) + kk) * 8,
-                                  desc_mn_sw128(aR + st * kStage + kk * 2048, 64 * 128, 1024), id_o, (i > gb || c > 0 || kk > 0) ? 1u : 0u);
-              umma_commit_pair(&empty[st], 0x3);
-            }
-            umma_commit_pair(pv_done, 0x3);
-          };
-          for (int j = 0; j < n && ok; ++j) {
-            const int i = gb + j;
-#pragma unroll 1
-            for (int c = 0; c < C::K_STAGES; ++c, ++g) {
-              const int st = g % RING;
-              if (!mbar_wait(&full[st], (g / RING) & 1, status, 63, abort)) {
-                ok = false;
-                break;
-              }
+            for (int c = 0; c < C::K_STAGES; ++c) {
+              wait(&k_full[kst], kphase, 63);
+              if (!ok) break;
               tc_fence_after();
+              const uint64_t dk = dK + (kst * C::K_BYTES >> 4);
 #pragma unroll
-              for (int kk = 0; kk < C::K_COLS / 16; ++kk)
-                umma_bf16_pair(tmem + kS + (i & 1) * BN, desc_sw128(aQ + (c * 2 + kk / 4) * (BM * 128) + (kk & 3) * 32),
-                               desc_sw128(aR + st * kStage + (kk / 4) * (64 * 128) + (kk & 3) * 32), id_s, (c | kk) != 0);
-              umma_commit_pair(&empty[st], 0x3);
+              for (int kk = 0; kk < C::KC / 16; ++kk)
+                umma_bf16_pair_if(to, dQ + (((c * (C::KC / 64) + kk / 4) * (BM * 128) + (kk & 3) * 32) >> 4),
+                                  dk + (((kk / 4) * (64 * 128) + (kk & 3) * 32) >> 4), id_s, (c | kk) != 0, one);
+              umma_commit_pair_if(&k_empty[kst], one);
+              if (++kst == KR) kst = 0, kphase ^= 1;
             }
             if (!ok) break;
-            umma_commit_pair(&s_full[i & 1], 0x3);
-            if (j == n - 1) umma_commit_pair(q_empty, 0x3);
-            if (j == 1 && live > 0 && !mbar_wait_cluster(o_free, (live - 1) & 1, status, 64, abort)) ok = false;
-            if (j >= 1) product_pv(i - 1);
+            umma_commit_pair_if(&s_full[(gb + j) & 1], one);
+            if (j == n - 1) umma_commit_pair_if(q_empty, one);
           }
-          if (ok && n == 1 && live > 0 && !mbar_wait_cluster(o_free, (live - 1) & 1, status, 64, abort)) ok = false;
-          if (ok) product_pv(gb + n - 1);
-          gb += n;
+          if (j > 0) {
+            const int i = gb + j - 1;  // block of all
+            if (j == 1 && live > 0) wait(o_free, (live - 1) & 1, 64);
+            if (!ok) break;
+            if (has_stale(seq, u.kb0 + j - 1))  // the other SM's shared memory was written
+              ok = __all_sync(0xffffffffu, mbar_wait_cluster(&p_full[i & 1], (i >> 1) & 1, status, 61, abort));
+            else if (ok)
+              wait(&p_full[i & 1], (i >> 1) & 1, 61);
+            if (!ok) break;
+            wait(&v_full[vst], vphase, 62);
+            if (!ok) break;
+            tc_fence_after();
+            const uint64_t dv = dV + (vst * C::V_BYTES >> 4);
+#pragma unroll
+            for (int kk = 0; kk < BN / 16; ++kk)
+              umma_bf16_pair_ts_if(kO, kS + (i & 1) * BN + kk * 8, dv + (((kk / 4) * (C::V_BYTES / 2) + (kk & 3) * 2048) >> 4), id_o, (j > 1 || kk > 0), one);
+            umma_commit_pair_if(&v_empty[vst], one);
+            if (++vst == VR) vst = 0, vphase ^= 1;
+            umma_commit_pair_if(&pv_done[i & 1], one);
+            if (j == n) umma_commit_pair_if(o_full, one);
+          }
         }
-        ok = __all_sync(0xffffffffu, ok);
+        gb += n;
         ++live;
       }
-      if (lane == 0) {  // every product has ended before tensor memory is freed
-        umma_commit_pair(all_done, 0x1);
-        mbar_wait(all_done, 0, status, 65, nullptr, 500000000ull);
-      }
+      // every product has ended before tensor memory is freed
+      umma_commit_pair_if(all_done, one, 0x1);
+      if (one) mbar_wait(all_done, 0, status, 65, nullptr, 500000000ull);
+      __syncwarp();
     }
-  } else {
+  } else if (warp >= kFirstSoft) {
     // ---------------------------------------------------------------- softmax
-    const int quarter = warp & 3, half = (warp - 2) >> 2, r = quarter * 32 + lane;  // half of a block's keys; row of the SM
+    const int quarter = warp & 3, part = (warp - kFirstSoft) >> 2, r = quarter * 32 + lane;  // part of a block's keys; row of the SM
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t p_leader = mapa_shared(smem_addr(p_full), 0), o_leader = mapa_shared(smem_addr(o_free), 0);
+    constexpr int HB = BN / kParts;  // keys a thread
     const float to_log2 = a.scale * kLog2e;
     const int ti = r / group, head = r % group;
     // 32-byte stores of O where its rows allow them
     const bool wide = reinterpret_cast<uintptr_t>(a.o) % 32 == 0 && a.o_token % 16 == 0 && a.o_head % 16 == 0;
-    int g = 0, gb = 0, met = 0;  // stages, blocks, meetings so far
-    uint32_t v_phases = 0;       // bit i: parity of v_here[i]
+    int gb = 0, live = 0, met = 0;  // blocks, units with any, meetings so far
+    uint32_t v_phases = 0;          // bit i: parity of v_here[i]
     bool ok = true;
-    // The other half's x of this row.
-    auto other = [&](float x) {
-      meet[((met & 1) * 2 + half) * BM + r] = x;
+    // The row's four warps meet: what each wrote before come_by() is there after meet().
+    auto come_by = [&] {
       __syncwarp();
       if (lane == 0) mbar_arrive(&meet_bar[quarter]);
-      if (!mbar_wait(&meet_bar[quarter], met & 1, status, 75, abort)) ok = false;
-      ok = __all_sync(0xffffffffu, ok);
-      const float y = meet[((met & 1) * 2 + (half ^ 1)) * BM + r];
-      ++met;
-      return y;
+    };
+    auto meet = [&] { ok = __all_sync(0xffffffffu, mbar_wait(&meet_bar[quarter], met++ & 1, status, 75, abort)); };
+    // The sum of all parts' x, in the parts' order. (sums lies over tops: both are idle at a unit's end.)
+    auto sum_up = [&](float x) {
+      sums[part * BM + r] = x;
+      come_by(), meet();
+      const float all = sums[r] + sums[BM + r];
+      come_by(), meet();
+      return all;
     };
     Walk<D> walk(args, cut);
     Unit u;
@@ -492,99 +563,120 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool mine = ti < tokens && token < u.s.count;
       const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
       const int from = a.window > 0 ? u.s.context + token - a.window + 1 : 0;
-      float m = -INFINITY, l = 0.f, l_rounded = 0.f;  // of this half: sums of p, and of p as the product takes it
+      float m = -INFINITY, l = 0.f;  // l: this part's sum of p
+      float alpha = 1.f;             // what O has to be rescaled by
       auto pages_of = [&](int kb) {  // bit i: keys 16 i of the four blocks from kb on have a page
         return __ballot_sync(0xffffffffu, page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog) >= 0);
       };
       uint32_t there = n > 0 ? pages_of(u.kb0) : 0, there_next = 0;
       for (int j = 0; j < n && ok; ++j) {
-        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN + half * 64;
+        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN + part * HB;
         if ((j & 3) == 0) {
           if (j > 0) there = there_next;
           if (j + 4 < n) there_next = pages_of(kb + 4);
         }
-        const uint32_t pages = (there >> ((j & 3) * 8 + half * 4)) & 0xf;
+        const uint32_t pages = (there >> ((j & 3) * 8 + part * (HB / 16))) & 0xfu;
         if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, status, 70, abort)) ok = false;
         if (!(ok = __all_sync(0xffffffffu, ok))) break;
         tc_fence_after();
-        uint32_t s[2][32];
         const uint32_t at = tmem + lanes + kS + (i & 1) * BN;
-        tmem_issue_ld32(at + half * 64, s[0]);
-        tmem_issue_ld32(at + half * 64 + 32, s[1]);
-        tmem_wait_ld(s[0]);
-        tmem_wait_ld(s[1]);
-        const bool open = pages == 0xfu && ((key0 >= from && key0 + 63 <= last) || !mine);
-        if (!__all_sync(0xffffffffu, open)) {
+        const bool open = pages == 0xfu && ((key0 >= from && key0 + HB - 1 <= last) || !mine), all_open = __all_sync(0xffffffffu, open);
+        float top = -INFINITY, sum[2];
+        uint32_t pk[HB / 2];
+        int passes = 0;  // a second one, from the scores again, for a row that jumps
+#pragma unroll 1
+        for (;;) {
+          uint32_t s[HB];
+          uint32_t(&low)[32] = reinterpret_cast<uint32_t(&)[32]>(s[0]), (&high)[32] = reinterpret_cast<uint32_t(&)[32]>(s[32]);
+          tmem_issue_ld32(at + part * HB, low);
+          tmem_issue_ld32(at + part * HB + 32, high);
+          tmem_wait_ld(low);
+          tmem_wait_ld(high);
+          if (!all_open) {
 #pragma unroll
-          for (int c = 0; c < 2; ++c) {
-            // bits from .. last of these 32 keys that have a page
-            const int k0 = key0 + c * 32, lo = min(max(from - k0, 0), 32), hi = min(max(last + 1 - k0, 0), 32);
-            uint32_t seen = (uint32_t)(((1ull << hi) - 1) & ~((1ull << lo) - 1));
-            seen &= ((pages >> (2 * c)) & 1 ? 0xffffu : 0u) | ((pages >> (2 * c + 1)) & 1 ? 0xffff0000u : 0u);
+            for (int c = 0; c < HB; c += 32) {
+              // bits from .. last of these 32 keys that have a page
+              const int lo = min(max(from - key0 - c, 0), 32), hi = min(max(last + 1 - key0 - c, 0), 32);
+              uint32_t seen = (uint32_t)(((1ull << hi) - 1) & ~((1ull << lo) - 1));
+              seen &= ((pages >> (c / 16)) & 1 ? 0xffffu : 0u) | ((pages >> (c / 16)) & 2 ? 0xffff0000u : 0u);
 #pragma unroll
-            for (int e = 0; e < 32; ++e)
-              if (!(seen & (1u << e))) s[c][e] = 0xff800000u;  // -inf
+              for (int e = 0; e < 32; ++e)
+                if (!(seen & (1u << e))) s[c + e] = 0xff800000u;  // -inf
+            }
           }
-        }
-        float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+          bool wait_here = passes > 0;  // the maximum of this block has come round before the exponentials
+          if (passes++ == 0) {
+            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int c = 0; c < 2; ++c)
+            for (int e = 0; e < HB; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
+            atomicMax(&tops[(i & 3) * BM + r], ordered(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
+            if (part == 0) tops[((i + 2) & 3) * BM + r] = ordered(-INFINITY);  // block i - 2's, which all have read: its P has been taken
+            come_by();
+            if (__any_sync(0xffffffffu, m == -INFINITY && mine)) {
+              meet();
+              if (!ok) break;
+              top = unordered(tops[(i & 3) * BM + r]) * to_log2;
+              if (m == -INFINITY) m = top;
+              wait_here = true;
+            }
+          }
+          const float z = m == -INFINITY ? 0.f : m;
+          sum[0] = sum[1] = 0.f;
 #pragma unroll
-          for (int e = 0; e < 32; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[c][e]));
-        float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * to_log2;
-        top = fmaxf(top, other(top));  // (both halves have read their scores now: P may go over them)
-        if (!ok) break;
-        bool resc = false;
-        float alpha = 1.f;
-        if (top > m + kSlack) {
-          if (m != -INFINITY) alpha = ex2(m - top), resc = true;
-          m = top;
-        }
-        const float z = m == -INFINITY ? 0.f : m;
-        float sum[2] = {0.f, 0.f}, rounded[2] = {0.f, 0.f};
-        uint32_t pk[32];
-#pragma unroll
-        for (int c = 0; c < 2; ++c)
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[c][e]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[c][e + 1]), to_log2, -z));
-            const uint32_t h = pack2(p0, p1);
+          for (int e = 0; e < HB; e += 2) {
+            const float p0 = ex2(fmaf(__uint_as_float(s[e]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[e + 1]), to_log2, -z));
             sum[0] += p0, sum[1] += p1;
-            rounded[0] += __uint_as_float(h << 16), rounded[1] += __uint_as_float(h & 0xffff0000u);
-            pk[c * 16 + e / 2] = h;
+            pk[e / 2] = pack2(p0, p1);
           }
-        l = l * alpha + (sum[0] + sum[1]);
-        l_rounded = l_rounded * alpha + (rounded[0] + rounded[1]);
-        tmem_st32u(at + half * 32, pk);
-        if (__any_sync(0xffffffffu, resc) && j > 0) {  // O stands still once the product before has ended
-          if (!mbar_wait(pv_done, (i - 1) & 1, status, 71, abort)) ok = false;
+          if (!wait_here) {
+            meet();  // (and all have read their scores: P may go over them)
+            if (!ok) break;
+            top = unordered(tops[(i & 3) * BM + r]) * to_log2;
+          }
+          if (!__any_sync(0xffffffffu, top > m + kJump)) break;  // (the row's threads see the same numbers)
+          if (top > m + kJump) {
+            const float f = ex2(m - top);
+            alpha *= f, l *= f;
+            m = top;
+          }
+        }
+        if (!ok) break;
+        l += sum[0] + sum[1];
+        tmem_st32u(at + part * (HB / 2), pk);
+        if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {  // O stands still once the product before has ended
+          if (!mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, status, 71, abort)) ok = false;
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < C::DV / 64; ++c) {
-            uint32_t o[32];
-            const uint32_t col = tmem + lanes + kO + half * (C::DV / 2) + c * 32;
-            tmem_issue_ld32(col, o);
+          for (int c = 0; c < C::DV / kParts; c += 16) {
+            uint32_t o[16];
+            const uint32_t col = tmem + lanes + kO + part * (C::DV / kParts) + c;
+            tmem_issue_ld16(col, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st32u(col, o);
+            for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+            tmem_st16u(col, o);
           }
         }
+        alpha = 1.f;
+        if (top > m + kSlack) {  // from the next block on
+          alpha = ex2(m - top);
+          l *= alpha;
+          m = top;
+        }
         const bool stale = has_stale(seq, kb);
-        if (stale) {  // row r: key r of the block, a half of this SM's columns
-          if (!mbar_wait(&v_here[i % kVHere], (v_phases >> (i % kVHere)) & 1, status, 72, abort)) ok = false;
+        if (stale) {  // row r: key r of the block, a part of this SM's columns
+          const int st = i % VR;
+          if (!mbar_wait(&v_here[st], (v_phases >> st) & 1, status, 72, abort)) ok = false;
           if (!(ok = __all_sync(0xffffffffu, ok))) break;
-          v_phases ^= 1u << (i % kVHere);
+          v_phases ^= 1u << st;
           const int key = kb * BN + r;
           if (key < seq.lo || key >= seq.hi) {
-            // V's stages of block j come after those of K of the blocks up to j + 1
-            const int st = (g + min(j + 2, n) * C::K_STAGES + j * C::V_STAGES + (C::VC == 128 ? r / 64 : 0)) % RING;
 #pragma unroll
-            for (int c = half * (C::VC / 16); c < (half + 1) * (C::VC / 16); ++c) {
-              const int sub = C::VC == 128 ? c / 8 : r / 64;
-              const int chunk = C::VC == 128 ? (c + r) & 7 : c;  // any order, together all of them
-              *reinterpret_cast<uint4*>(sR + st * kStage + sub * (64 * 128) + (r & 63) * 128 + chunk * 16) = make_uint4(0, 0, 0, 0);
+            for (int i8 = 0; i8 < C::VC / 8 / kParts; ++i8) {
+              const int c = part * (C::VC / 8 / kParts) + i8;  // of its 16-byte chunks
+              *reinterpret_cast<uint4*>(sV + st * C::V_BYTES + (r / 64) * (C::V_BYTES / 2) + (c / 8) * (64 * 128) + (r & 63) * 128 + (c & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
             }
           }
           fence_async_smem();
@@ -599,64 +691,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // ---- the unit's end
+      float o_scale = 1.f;
       if (n > 0 && ok) {
-        // a phase at a time: the last but one may still be open
-        if (n > 1 && !mbar_wait(pv_done, (gb + n - 2) & 1, status, 73, abort)) ok = false;
-        if (ok && !mbar_wait(pv_done, (gb + n - 1) & 1, status, 74, abort)) ok = false;
+        o_scale = alpha;  // a rescaling that no block was left for
+        come_by(), meet();  // all have read the last maxima
+        if (ok) l = sum_up(l);
+        tops[part * BM + r] = tops[(part + 2) * BM + r] = ordered(-INFINITY);
+        come_by();
+        if (ok) meet();
+        if (ok && !mbar_wait(o_full, live & 1, status, 73, abort)) ok = false;
         ok = __all_sync(0xffffffffu, ok);
+        ++live;
       }
       if (!ok) break;
       tc_fence_after();
-      l += other(l);
-      l_rounded += other(l_rounded);
-      if (!ok) break;
-      const float inv = l_rounded == 0.f ? 0.f : (u.chunks > 1 ? l : 1.f) / l_rounded;  // (a part's O goes with the sum l)
+      const float inv = u.chunks > 1 ? o_scale : l == 0.f ? 0.f : o_scale / l;  // (a part keeps its sum)
       const int t = u.s.first + token, h = u.kv * group + head;
       const int64_t slot = x * args.slot_rows + (int)rank * tokens * group + r;
-      const int col0 = half * (C::DV / 2);
+      constexpr int PC = C::DV / kParts, PS = PC < 32 ? PC : 32;  // this part's columns of O, and of a step
+      const int col0 = part * PC;
+      auto release = [&] {  // O has been read: the next unit's products may go over it
+        if (n == 0) return;
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive_cta(o_leader);
+      };
       if (u.chunks > 1) {
+        float* dst = args.part_o + slot * C::DV + col0;
 #pragma unroll 1
-        for (int c = 0; c < C::DV / 64; ++c) {
-          uint32_t o[32];
+        for (int c = 0; c < PC; c += PS) {
+          uint32_t o[32] = {};
           if (n > 0) {
-            tmem_issue_ld32(tmem + lanes + kO + col0 + c * 32, o);
+            tmem_issue_ld32(tmem + lanes + kO + col0 + c, o);
             tmem_wait_ld(o);
           }
-          float* dst = args.part_o + slot * C::DV + col0 + c * 32;
           if (mine)
 #pragma unroll
-            for (int e = 0; e < 32; e += 4)
-              *reinterpret_cast<float4*>(dst + e) =
-                  n > 0 ? make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv, __uint_as_float(o[e + 2]) * inv,
-                                      __uint_as_float(o[e + 3]) * inv)
-                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int e = 0; e < PS; e += 4)
+              *reinterpret_cast<float4*>(dst + c + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
+                                                                    __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
         }
-        if (n > 0) {
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cta(o_leader);
-        }
-        if (mine && half == 0) args.part_ml[slot] = make_float2(m, l);
+        if (mine && part == 0) args.part_ml[slot] = make_float2(m, l);
+        release();
       } else {
-        // all of O into registers first: the next unit's products may begin
-        uint32_t out[C::DV / 4] = {};
+        uint32_t out[PC / 2] = {};
         if (n > 0) {
 #pragma unroll
-          for (int c = 0; c < C::DV / 64; ++c) {
+          for (int c = 0; c < PC; c += PS) {
             uint32_t o[32];
-            tmem_issue_ld32(tmem + lanes + kO + col0 + c * 32, o);
+            tmem_issue_ld32(tmem + lanes + kO + col0 + c, o);
             tmem_wait_ld(o);
 #pragma unroll
-            for (int e = 0; e < 32; e += 2) out[c * 16 + e / 2] = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+            for (int e = 0; e < PS; e += 2) out[(c + e) / 2] = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
           }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive_cta(o_leader);
         }
+        release();
         if (mine) {
           bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + col0;
 #pragma unroll
-          for (int e = 0; e < C::DV / 4; e += 8) {
+          for (int e = 0; e < PC / 2; e += 8) {
             if (wide) {
               st_global32(dst + e * 2, &out[e]);
             } else {
@@ -664,11 +757,10 @@ __global__ void __launch_bounds__(kThreads, 1)
               *reinterpret_cast<uint4*>(dst + e * 2 + 8) = make_uint4(out[e + 4], out[e + 5], out[e + 6], out[e + 7]);
             }
           }
-          if (u.half == 0 && half == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+          if (u.half == 0 && part == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
       }
       gb += n;
-      g += n * (C::K_STAGES + C::V_STAGES);
     }
   }
   tc_fence_before();
@@ -735,12 +827,14 @@ PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   return fn;
 }
 
-// [z][y][x] bf16 with boxes of 64 columns, 128-byte swizzle.
-bool make_map(CUtensorMap* map, const void* ptr, int64_t x, int64_t y, int64_t z, int64_t y_stride, int64_t z_stride, int box_y, int box_z) {
-  cuuint64_t dims[3] = {(cuuint64_t)x, (cuuint64_t)y, (cuuint64_t)z};
-  cuuint64_t strides[2] = {(cuuint64_t)y_stride * 2, (cuuint64_t)z_stride * 2};
-  cuuint32_t box[3] = {64, (cuuint32_t)box_y, (cuuint32_t)box_z}, one[3] = {1, 1, 1};
-  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+// bf16, a box of 64 elements of the first dimension, 128-byte swizzle. Strides in elements, of the dimensions from the second on.
+template <int N>
+bool make_map(CUtensorMap* map, const void* ptr, const int64_t (&dim)[N], const int64_t (&stride)[N - 1], const int (&box)[N - 1]) {
+  cuuint64_t dims[N], strides[N - 1];
+  cuuint32_t boxes[N] = {64}, one[N];
+  for (int i = 0; i < N; ++i) dims[i] = dim[i], one[i] = 1;
+  for (int i = 0; i + 1 < N; ++i) strides[i] = stride[i] * 2, boxes[i + 1] = box[i];
+  return encode_fn()(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, N, const_cast<void*>(ptr), dims, strides, boxes, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -796,10 +890,13 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
   args.least_rows = least_rows;
   bind_primary_context();
   const int group = a.q_heads / a.cache.heads, box = std::min(a.cache.page, 64);
+  const int64_t rows = (int64_t)a.cache.heads * a.cache.page;
+  // pages as [page][64 columns of the head][head, position][column]
+  const int64_t dims[4] = {64, rows, D / 64, a.cache.pages};
   CUtensorMap tq, tk, tv;
-  if (!make_map(&tq, a.q, D, a.q_heads, a.batch.tokens, a.q_head, a.q_token, group, BM / group) ||
-      !make_map(&tk, a.cache.k, D, (int64_t)a.cache.heads * a.cache.page, a.cache.pages, D, a.cache.k_stride, box, 1) ||
-      !make_map(&tv, a.cache.v, D, (int64_t)a.cache.heads * a.cache.page, a.cache.pages, D, a.cache.v_stride, box, 1))
+  if (!make_map<3>(&tq, a.q, {D, a.q_heads, a.batch.tokens}, {a.q_head, a.q_token}, {group, BM / group}) ||
+      !make_map<4>(&tk, a.cache.k, dims, {D, 64, a.cache.k_stride}, {box, box == 64 ? C::KC / 64 : 1, 1}) ||
+      !make_map<4>(&tv, a.cache.v, dims, {D, 64, a.cache.v_stride}, {box, box == 64 ? C::VC / 64 : 1, 1}))
     return "cuTensorMapEncodeTiled failed";
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr;
