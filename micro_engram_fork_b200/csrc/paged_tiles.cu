@@ -9,6 +9,7 @@
 //              map, a page that is none is an index past its last dimension, which reads zeros)
 //   warp 1     issues the products (from the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
 //              softmax has the time of two products
+//   warp 3     finds the pair's next unit while the others are at work, two ahead
 //   warps 4-11 softmax, two threads a row (a half of a block's keys each): 64 scores from tensor memory; p = 2^(s - m) by the
 //              maximum m that the row's threads had agreed on a block before, for the maximum of this block comes round through shared
 //              memory while they compute (a row that has none yet, or jumps by more than 2^60, waits for it). O is rescaled
@@ -55,9 +56,10 @@ struct Cfg {
   static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = BN * VC * 2;
   static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 1 : D == 256 ? 2 : 6;  // stages
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KR * K_BYTES, BAR_OFF = V_OFF + VR * V_BYTES;
-  static constexpr int MEET_OFF = BAR_OFF + 512;   // [4 blocks][BM]: maxima; [kParts][BM]: sums
+  static constexpr int MEET_OFF = BAR_OFF + 640;   // [4 blocks][BM]: maxima; [kParts][BM]: sums
   static constexpr int SMEM = MEET_OFF + 4 * BM * 4;
   static_assert(SMEM <= 232448, "shared memory");
+  static_assert((2 * KR + 3 * VR + 19) * 8 <= 496, "barriers");
 };
 constexpr int kO = 0, kS = 256;  // columns of tensor memory
 constexpr float kJump = 60.f;   // a score this far above m (log2) does not wait for the next block
@@ -95,20 +97,22 @@ ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut
   return u;
 }
 
-// Blocks a chunk that make about kDeals units a pair, 0: no cutting. At most 2 kDeals units a pair come of it: as many
-// as there were (fewer than kDeals) and one for every `cut` blocks.
+// Blocks a chunk that make about kDeals units a pair, 0: no cutting, where the units as they are keep four pairs of five busy. At most 2 kDeals
+// units a pair come of it: as many as there were (fewer than kDeals) and one for every `cut` blocks.
 template <int D, int NT>
 ME_DEVICE int cut_of(const TilesArgs& t, typename WorkLine<NT>::Shared& sh, int64_t& units) {
   WorkLine<NT> line(sh);
   const PagedBatch& p = t.a.batch;
   const int each = t.a.cache.heads * Cfg<D>::HALVES;
   units = line.total(p.seqs, [&](int b) -> int64_t { return (int64_t)units_of<D>(t, b, sequence_of(p, b), 0).tiles * each; });
-  if (units == 0 || units >= (int64_t)kDeals * t.pairs) return 0;
+  const int64_t aim = (int64_t)kDeals * t.pairs;
+  if (units == 0 || units >= aim) return 0;
+  const int few = (int)units, deals = (few + t.pairs - 1) / t.pairs;
+  if (few * 5 >= deals * t.pairs * 4) return 0;
   const int64_t blocks = line.total(p.seqs, [&](int b) -> int64_t {
     const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), 0);
     return (int64_t)u.tiles * each * u.blocks;
   });
-  const int64_t aim = (int64_t)kDeals * t.pairs;
   return (int)max((blocks + aim - 1) / aim, (int64_t)kLeastBlocks);
 }
 
@@ -158,11 +162,11 @@ struct Walk {
     out.b = c + src;
     out.s = sequence_of(a.batch, out.b);
     const UnitsOf u = units_of<D>(t, out.b, out.s, cut);
-    int64_t i = x - before;
-    out.half = (int)(i % Cfg<D>::HALVES), i /= Cfg<D>::HALVES;
-    out.kv = (int)(i % a.cache.heads), i /= a.cache.heads;
-    out.chunk = (int)(i % u.chunks), out.chunks = u.chunks;
-    out.tile = u.tiles - 1 - (int)(i / u.chunks);  // the last rows see the most keys
+    unsigned i = (unsigned)(x - before);  // (a sequence's units: the host checks that they fit)
+    out.half = i % Cfg<D>::HALVES, i /= Cfg<D>::HALVES;
+    out.kv = i % a.cache.heads, i /= a.cache.heads;
+    out.chunk = i % u.chunks, out.chunks = u.chunks, i /= u.chunks;
+    out.tile = u.tiles - 1 - (int)i;  // the last rows see the most keys
     const int tokens = 2 * (BM / (a.q_heads / a.cache.heads));
     const int i0 = out.tile * tokens, i1 = min(i0 + tokens, out.s.count) - 1;
     const Keys k = keys_of(a.batch, a.cache.page, out.s, i0, i1, a.window);
@@ -310,7 +314,10 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_free = o_full + 1;     // the even SM's
   uint64_t* all_done = o_free + 1;
   uint64_t* meet_bar = all_done + 1;  // [4] the warps of the same rows
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(meet_bar + 4);
+  uint64_t* next_full = meet_bar + 4;   // [2]
+  uint64_t* next_empty = next_full + 2; // [2]
+  int* next_unit = reinterpret_cast<int*>(smem + C::BAR_OFF + 496);  // [2][16]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 624);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* tops = reinterpret_cast<int*>(smem + C::MEET_OFF);       // [4][BM] ordered()
   float* sums = reinterpret_cast<float*>(smem + C::MEET_OFF);   // [kParts][BM]
@@ -339,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(o_free, 2 * kSoftWarps);
     mbar_init(all_done, 1);
     for (int i = 0; i < 4; ++i) mbar_init(&meet_bar[i], kParts);
+    for (int i = 0; i < 2; ++i) mbar_init(&next_full[i], 1), mbar_init(&next_empty[i], 2 + kSoftWarps + (leader ? 1 : 0));
     *abort = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
@@ -360,6 +368,29 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+  // The `it`-th unit of the pair, by warp 3; false: there is none, or a wait ran out. Whole warps; the numbers are the same in all lanes, and
+  // pass a reduction so that they are known to be, and addresses and descriptors that come of them stay in uniform registers.
+  auto uniform = [](int x) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)x); };
+  auto wait_u = [&](uint64_t* bar, int parity, int where) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, status, where, abort));
+  };
+  Unit u;
+  Keys seq;
+  int unit_x = 0;
+  auto take_unit = [&](int it, int where) {
+    if (!wait_u(&next_full[it & 1], (it >> 1) & 1, where)) return false;
+    const int mine = next_unit[(it & 1) * 16 + (lane & 15)];
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&next_empty[it & 1]);
+    auto field = [&](int i) { return uniform(__shfl_sync(0xffffffffu, mine, i)); };
+    u.s = {field(1), field(2), field(3)};
+    u.b = field(4), u.tile = field(5), u.kv = field(6), u.half = field(7);
+    u.kb0 = field(8), u.kb1 = field(9), u.chunk = field(10), u.chunks = field(11);
+    seq = {field(12), field(13)};
+    unit_x = field(14);
+    return field(0) != 0;
+  };
+
   // In a block with rows of V that may hold anything, V arrives at v_here and the softmax threads put zeros there.
   auto has_stale = [&](const Keys& seq, int kb) { return kb * BN < seq.lo || (kb + 1) * BN > seq.hi; };
 
@@ -377,19 +408,16 @@ __global__ void __launch_bounds__(kThreads, 1)
     int st = 0, round = 0, g = 0;   // the ring's next stage; stages so far
     int live = 0;
     bool ok = true;
-    Walk<D> walk(args, cut);
-    Unit u;
     auto free_stage = [&] {
-      if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&empty[st], (round - 1) & 1, status, of_k ? 50 : 53, abort));
+      if (round > 0) ok = wait_u(&empty[st], (round - 1) & 1, of_k ? 50 : 53);
     };
     auto next_stage = [&] {
       ++g;
       if (++st == ring) st = 0, ++round;
     };
-    for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
-      const int n = __shfl_sync(0xffffffffu, u.kb1 - u.kb0, 0);
+    for (int it = 0; ok && take_unit(it, of_k ? 54 : 55); ++it) {
+      const int n = u.kb1 - u.kb0;
       if (n <= 0) continue;
-      const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
       const int y0 = u.kv << args.plog;
       // pages of a block, a lane for each 16 keys; an index past the cache where there is none
       auto pages_of = [&](int kb) {
@@ -425,7 +453,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             next_stage();
           }
           if (j == 0 && ok) {  // Q, once the unit before is done with it
-            if (live > 0) ok = __all_sync(0xffffffffu, mbar_wait(q_empty, (live - 1) & 1, status, 51, abort));
+            if (live > 0) ok = wait_u(q_empty, (live - 1) & 1, 51);
             if (!ok) break;
             if (leader && one) mbar_expect_tx(q_full, 2 * (D / 64) * tokens * group * 128);
             __syncwarp();
@@ -469,13 +497,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       int kst = 0, kphase = 0, vst = 0, vphase = 0;  // the rings' next stages
       int gb = 0, live = 0;    // blocks, units so far
       bool ok = true;
-      auto wait = [&](uint64_t* bar, int parity, int where) { ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, status, where, abort)); };
-      Walk<D> walk(args, cut);
-      Unit u;
-      for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
-        const int n = __shfl_sync(0xffffffffu, u.kb1 - u.kb0, 0);
+      auto wait = [&](uint64_t* bar, int parity, int where) { ok = wait_u(bar, parity, where); };
+      for (int it = 0; ok && take_unit(it, 66); ++it) {
+        const int n = u.kb1 - u.kb0;
         if (n <= 0) continue;
-        const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
         wait(q_full, live & 1, 60);
         for (int j = 0; j <= n && ok; ++j) {
           if (j < n) {
@@ -527,6 +552,24 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (one) mbar_wait(all_done, 0, status, 65, nullptr, 500000000ull);
       __syncwarp();
     }
+  } else if (warp == 3) {
+    // ---------------------------------------------------------------- units
+    Walk<D> walk(args, cut);
+    Unit w = {};
+    bool more = true;
+    for (int it = 0; more; ++it) {
+      const int64_t x = pair + (int64_t)it * args.pairs;
+      more = __all_sync(0xffffffffu, walk.at(x, w));
+      const Keys k = keys_of(p, a.cache.page, w.s, 0, w.s.count - 1, a.window);
+      if (it >= 2 && !wait_u(&next_empty[it & 1], ((it >> 1) - 1) & 1, 80)) break;
+      int* to = next_unit + (it & 1) * 16;
+      if (lane == 0) {
+        to[0] = more, to[1] = w.s.first, to[2] = w.s.count, to[3] = w.s.context, to[4] = w.b, to[5] = w.tile, to[6] = w.kv, to[7] = w.half;
+        to[8] = w.kb0, to[9] = w.kb1, to[10] = w.chunk, to[11] = w.chunks, to[12] = k.lo, to[13] = k.hi, to[14] = (int)x;
+        mbar_arrive(&next_full[it & 1]);
+      }
+      __syncwarp();
+    }
   } else if (warp >= kFirstSoft) {
     // ---------------------------------------------------------------- softmax
     const int quarter = warp & 3, part = (warp - kFirstSoft) >> 2, r = quarter * 32 + lane;  // part of a block's keys; row of the SM
@@ -545,7 +588,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       __syncwarp();
       if (lane == 0) mbar_arrive(&meet_bar[quarter]);
     };
-    auto meet = [&] { ok = __all_sync(0xffffffffu, mbar_wait(&meet_bar[quarter], met++ & 1, status, 75, abort)); };
+    auto meet = [&] { ok = wait_u(&meet_bar[quarter], met & 1, 75), ++met; };
     // The sum of all parts' x, in the parts' order. (sums lies over tops: both are idle at a unit's end.)
     auto sum_up = [&](float x) {
       sums[part * BM + r] = x;
@@ -554,11 +597,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       come_by(), meet();
       return all;
     };
-    Walk<D> walk(args, cut);
-    Unit u;
-    for (int64_t x = pair; ok && walk.at(x, u); x += args.pairs) {
+    for (int it = 0; ok && take_unit(it, 77); ++it) {
       const int n = max(u.kb1 - u.kb0, 0);
-      const Keys seq = keys_of(p, a.cache.page, u.s, 0, u.s.count - 1, a.window);
       const int token = u.tile * 2 * tokens + (int)rank * tokens + ti;  // of the sequence's new ones
       const bool mine = ti < tokens && token < u.s.count;
       const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
@@ -576,14 +616,13 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (j + 4 < n) there_next = pages_of(kb + 4);
         }
         const uint32_t pages = (there >> ((j & 3) * 8 + part * (HB / 16))) & 0xfu;
-        if (!mbar_wait(&s_full[i & 1], (i >> 1) & 1, status, 70, abort)) ok = false;
-        if (!(ok = __all_sync(0xffffffffu, ok))) break;
+        const bool open = pages == 0xfu && ((key0 >= from && key0 + HB - 1 <= last) || !mine), all_open = __all_sync(0xffffffffu, open);
+        if (!(ok = wait_u(&s_full[i & 1], (i >> 1) & 1, 70))) break;
         tc_fence_after();
         const uint32_t at = tmem + lanes + kS + (i & 1) * BN;
-        const bool open = pages == 0xfu && ((key0 >= from && key0 + HB - 1 <= last) || !mine), all_open = __all_sync(0xffffffffu, open);
         float top = -INFINITY, sum[2];
         uint32_t pk[HB / 2];
-        int passes = 0;  // a second one, from the scores again, for a row that jumps
+        bool first = true;  // a second pass, from the scores again, for a row that jumps
 #pragma unroll 1
         for (;;) {
           uint32_t s[HB];
@@ -604,8 +643,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!(seen & (1u << e))) s[c + e] = 0xff800000u;  // -inf
             }
           }
-          bool wait_here = passes > 0;  // the maximum of this block has come round before the exponentials
-          if (passes++ == 0) {
+          bool wait_here = !first;  // the maximum of this block has come round before the exponentials
+          if (first) {
+            first = false;
             float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
             for (int e = 0; e < HB; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
@@ -644,8 +684,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += sum[0] + sum[1];
         tmem_st32u(at + part * (HB / 2), pk);
         if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {  // O stands still once the product before has ended
-          if (!mbar_wait(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, status, 71, abort)) ok = false;
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          if (!(ok = wait_u(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 71))) break;
           tc_fence_after();
 #pragma unroll 1
           for (int c = 0; c < C::DV / kParts; c += 16) {
@@ -667,8 +706,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const bool stale = has_stale(seq, kb);
         if (stale) {  // row r: key r of the block, a part of this SM's columns
           const int st = i % VR;
-          if (!mbar_wait(&v_here[st], (v_phases >> st) & 1, status, 72, abort)) ok = false;
-          if (!(ok = __all_sync(0xffffffffu, ok))) break;
+          if (!(ok = wait_u(&v_here[st], (v_phases >> st) & 1, 72))) break;
           v_phases ^= 1u << st;
           const int key = kb * BN + r;
           if (key < seq.lo || key >= seq.hi) {
@@ -699,15 +737,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         tops[part * BM + r] = tops[(part + 2) * BM + r] = ordered(-INFINITY);
         come_by();
         if (ok) meet();
-        if (ok && !mbar_wait(o_full, live & 1, status, 73, abort)) ok = false;
-        ok = __all_sync(0xffffffffu, ok);
+        if (ok) ok = wait_u(o_full, live & 1, 73);
         ++live;
       }
       if (!ok) break;
       tc_fence_after();
       const float inv = u.chunks > 1 ? o_scale : l == 0.f ? 0.f : o_scale / l;  // (a part keeps its sum)
       const int t = u.s.first + token, h = u.kv * group + head;
-      const int64_t slot = x * args.slot_rows + (int)rank * tokens * group + r;
+      const int64_t slot = (int64_t)unit_x * args.slot_rows + (int)rank * tokens * group + r;
       constexpr int PC = C::DV / kParts, PS = PC < 32 ? PC : 32;  // this part's columns of O, and of a step
       const int col0 = part * PC;
       auto release = [&] {  // O has been read: the next unit's products may go over it
@@ -772,12 +809,12 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the chunks of sequences that were cut: a block takes a unit's first chunk and every gridDim.y-th group of its rows.
-constexpr int kJoinThreads = 256;
+// Joins the chunks of sequences that were cut: a block takes every gridDim.x-th 32 rows of units.
+constexpr int kJoinThreads = 256, kJoinRows = 32;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
-  constexpr int PER = C::DV / 4, ROWS = kJoinThreads / PER;
+  constexpr int PER = C::DV / 4, ROWS = kJoinThreads / PER, STEPS = 2 * BM / kJoinRows;
   __shared__ typename WorkLine<kJoinThreads>::Shared line_shared;
   const PagedAttentionArgs& a = args.a;
   int64_t units;
@@ -787,12 +824,12 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __
   const int group = a.q_heads / a.cache.heads, tokens = 2 * (BM / group);
   Walk<D> walk(args, cut);
   Unit u;
-  for (int64_t x = blockIdx.x; walk.at(x, u); x += gridDim.x) {
+  for (int64_t i = blockIdx.x; walk.at(i / STEPS, u); i += gridDim.x) {
     if (u.chunks == 1 || u.chunk != 0) continue;
-    const int64_t stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
-    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group;
+    const int64_t x = i / STEPS, stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
+    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r0 = (int)(i % STEPS) * kJoinRows;
     const int c = threadIdx.x % PER * 4;
-    for (int r = blockIdx.y * ROWS + threadIdx.x / PER; r < rows; r += gridDim.y * ROWS) {
+    for (int r = r0 + threadIdx.x / PER; r < min(rows, r0 + kJoinRows); r += ROWS) {
       float top = -INFINITY, l = 0.f;
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int k = 0; k < u.chunks; ++k) {
@@ -912,7 +949,7 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
   if (e != cudaSuccess) return cudaGetErrorString(e);
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3(2 * kDeals * args.pairs, std::max(1, std::min(8, args.slot_rows / 8)));
+  cfg.gridDim = dim3(8 * args.pairs);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
   e = cudaLaunchKernelEx(&cfg, paged_join_tiles_kernel<D>, args);

@@ -134,6 +134,7 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   const int64_t tokens = q.size(0), q_heads = q.size(1);
   ME_CHECK_VALUE(q_heads >= heads && q_heads % heads == 0 && q_heads / heads <= 128, "q: heads a multiple of the pages' ", text(heads),
                  " (up to 128 times) are needed, got ", text(q_heads));
+  ME_CHECK_VALUE(tokens * q_heads < (1ll << 31), "q: fewer than 2^31 rows (tokens times heads) are needed, got ", shape(q));
   ME_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window: a positive number or None, got ", text(window));
   ME_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale: a positive number is needed");
   ME_CHECK_VALUE(max_q >= 0, "max_q: a positive number or None, got ", text(max_q));
