@@ -10,11 +10,11 @@
 //   warp 1     issues the products (from the even SM): S of block j + 1 goes ahead of P V of block j, so that block j's
 //              softmax has the time of two products
 //   warp 3     finds the pair's next unit while the others are at work, two ahead
-//   warps 4-11 softmax, two threads a row (a half of a block's keys each): 64 scores from tensor memory; p = 2^(s - m) by the
-//              maximum m that the row's threads had agreed on a block before, for the maximum of this block comes round through shared
-//              memory while they compute (a row that has none yet, or jumps by more than 2^60, waits for it). O is rescaled
-//              only when m grows by more than 2^8. P is rounded to bf16 (as what it is multiplied with is) and put back over its scores, from where
-//              it is the A operand of P V; the sum is of the terms before that. At a unit's end: O / sum to global memory
+//   warps 4-7  softmax, a thread a row: 128 scores from tensor memory, running
+//              maximum (O is rescaled only when it grows by more than 2^8), P rounded to bf16 (as what it is multiplied with is) and put
+//              back over its scores, from where it is the A operand of P V; the sum is of the terms before that. At a unit's end:
+//              O / sum to global memory. One warp a scheduler: what a block costs beside its exponentials is paid once, and nothing is
+//              exchanged (two threads a row: 3100 clocks a block at dim 256, four: 3200, every second block to another four warps: 3450)
 //
 // Tensor memory: O in columns 0-255, two S (P) buffers of 128. dim 512 has no room for both halves of O: a unit takes one half of the
 // columns, and S is computed twice (4/3 of the operations).
@@ -39,7 +39,7 @@ namespace {
 using namespace paged;
 using namespace tc;
 
-constexpr int kParts = 2, kSoftWarps = 4 * kParts, kFirstSoft = 4, kThreads = (kFirstSoft + kSoftWarps) * 32;  // kParts softmax threads a row
+constexpr int kSoftWarps = 4, kFirstSoft = 4, kThreads = (kFirstSoft + kSoftWarps) * 32;
 constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
 constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
 constexpr int kDeals = 4;             // units a pair that cutting aims at
@@ -51,24 +51,24 @@ struct Cfg {
   static constexpr int NV = D == 64 ? 128 : DV;      // columns of the P V product (dim 64: the odd SM's half is past the row, zeros)
   static constexpr int VC = NV / 2;                  // of them in this SM
   static constexpr int Q_BYTES = BM * D * 2;
-  // a stage of K: this SM's 64 keys of a block x KC columns; of V: 128 keys x VC, one set of 64 keys after the other
+  // a stage of K: this SM's 64 keys of a block x KC columns; of V: V_KEYS keys x VC
   static constexpr int KC = D < 256 ? D : 256, K_STAGES = D / KC;
-  static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = BN * VC * 2;
-  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 1 : D == 256 ? 2 : 6;  // stages
+  static constexpr int V_KEYS = VC == 128 ? 64 : 128, V_STAGES = BN / V_KEYS;
+  static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = V_KEYS * VC * 2;
+  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 2 : D == 256 ? 4 : 6;  // stages
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KR * K_BYTES, BAR_OFF = V_OFF + VR * V_BYTES;
-  static constexpr int MEET_OFF = BAR_OFF + 640;   // [4 blocks][BM]: maxima; [kParts][BM]: sums
-  static constexpr int SMEM = MEET_OFF + 4 * BM * 4;
+  static constexpr int SMEM = BAR_OFF + 640;
   static_assert(SMEM <= 232448, "shared memory");
-  static_assert((2 * KR + 3 * VR + 19) * 8 <= 496, "barriers");
+  static_assert((2 * KR + 3 * VR + 15) * 8 <= 496, "barriers");
 };
 constexpr int kO = 0, kS = 256;  // columns of tensor memory
-constexpr float kJump = 60.f;   // a score this far above m (log2) does not wait for the next block
 
 struct TilesArgs {
   PagedAttentionArgs a;
-  float* part_o;    // [slots][slot_rows][DV]
+  float4* part_o;   // [slots][DV / 4][slot_rows]: a warp's rows lie together
   float2* part_ml;  // [slots][slot_rows]
   int slot_rows;    // a sequence with more rows is not cut, unless 256
+  int group, tokens;  // query heads a key head, new tokens an SM
   int pairs;
   int plog;
   int least_rows;   // sequences with up to this many rows are others' work
@@ -84,7 +84,7 @@ struct UnitsOf {
 template <int D>
 ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut) {
   const PagedAttentionArgs& a = t.a;
-  const int group = a.q_heads / a.cache.heads, tokens = 2 * (BM / group);
+  const int group = t.group, tokens = 2 * t.tokens;
   if (s.count == 0 || (int64_t)s.count * group <= t.least_rows) return {0, 1, 0, 0, 0};
   const Keys k = keys_of(a.batch, a.cache.page, s, 0, s.count - 1, a.window);
   UnitsOf u;
@@ -97,23 +97,33 @@ ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut
   return u;
 }
 
-// Blocks a chunk that make about kDeals units a pair, 0: no cutting, where the units as they are keep four pairs of five busy. At most 2 kDeals
-// units a pair come of it: as many as there were (fewer than kDeals) and one for every `cut` blocks.
-template <int D, int NT>
-ME_DEVICE int cut_of(const TilesArgs& t, typename WorkLine<NT>::Shared& sh, int64_t& units) {
-  WorkLine<NT> line(sh);
+// Blocks a chunk, 0: no cutting. By a whole warp. Uncut, the last pair is done about after the mean of the blocks and, where units
+// differ, most of the longest one; cut to about kDeals units a pair, after 1.15 times the mean and what four blocks take for the parts.
+// At most 2 kDeals units a pair come of it: as many as there were (fewer than kDeals) and one for every `cut` blocks.
+template <int D>
+ME_DEVICE int cut_of(const TilesArgs& t) {
   const PagedBatch& p = t.a.batch;
-  const int each = t.a.cache.heads * Cfg<D>::HALVES;
-  units = line.total(p.seqs, [&](int b) -> int64_t { return (int64_t)units_of<D>(t, b, sequence_of(p, b), 0).tiles * each; });
-  const int64_t aim = (int64_t)kDeals * t.pairs;
-  if (units == 0 || units >= aim) return 0;
-  const int few = (int)units, deals = (few + t.pairs - 1) / t.pairs;
-  if (few * 5 >= deals * t.pairs * 4) return 0;
-  const int64_t blocks = line.total(p.seqs, [&](int b) -> int64_t {
+  int64_t units = 0, blocks = 0;
+  int most = 0;
+#pragma unroll 4
+  for (int b = threadIdx.x & 31; b < p.seqs; b += 32) {
     const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), 0);
-    return (int64_t)u.tiles * each * u.blocks;
-  });
-  return (int)max((blocks + aim - 1) / aim, (int64_t)kLeastBlocks);
+    units += u.tiles, blocks += (int64_t)u.tiles * u.blocks;
+    most = max(most, u.blocks);
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    units += __shfl_xor_sync(0xffffffffu, units, o);
+    blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
+  }
+  most = __reduce_max_sync(0xffffffffu, most);
+  const int each = t.a.cache.heads * Cfg<D>::HALVES, aim = kDeals * t.pairs;
+  units *= each, blocks *= each;
+  if (units == 0 || units >= aim) return 0;
+  const float mean = (float)blocks / t.pairs;
+  const float uncut = blocks == units * most ? (float)((int)(units + t.pairs - 1) / t.pairs * most) : mean + 0.75f * most;
+  if (uncut <= 1.15f * mean + 4.f) return 0;
+  return max((int)((blocks + aim - 1) / aim), kLeastBlocks);
 }
 
 struct Unit {
@@ -167,7 +177,7 @@ struct Walk {
     out.kv = i % a.cache.heads, i /= a.cache.heads;
     out.chunk = i % u.chunks, out.chunks = u.chunks, i /= u.chunks;
     out.tile = u.tiles - 1 - (int)i;  // the last rows see the most keys
-    const int tokens = 2 * (BM / (a.q_heads / a.cache.heads));
+    const int tokens = 2 * t.tokens;
     const int i0 = out.tile * tokens, i1 = min(i0 + tokens, out.s.count) - 1;
     const Keys k = keys_of(a.batch, a.cache.page, out.s, i0, i1, a.window);
     out.kb0 = max(k.lo / BN, u.first + out.chunk * u.per);
@@ -195,13 +205,6 @@ ME_DEVICE void tma_load_4d_pair_if(uint32_t dst, const CUtensorMap* map, uint32_
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "r"(w), "r"(issue)
       : "memory");
 }
-// The order of floats as that of integers, and back.
-ME_DEVICE int ordered(float x) {
-  const int i = __float_as_int(x);
-  return i ^ ((i >> 31) & 0x7fffffff);
-}
-ME_DEVICE float unordered(int i) { return __int_as_float(i ^ ((i >> 31) & 0x7fffffff)); }
-
 // The pair's product and its commits, by the lanes of `issue` (one lane of the warp that goes along).
 ME_DEVICE void umma_bf16_pair_if(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
   asm volatile(
@@ -313,15 +316,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* o_full = pv_done + 2;    // once a unit
   uint64_t* o_free = o_full + 1;     // the even SM's
   uint64_t* all_done = o_free + 1;
-  uint64_t* meet_bar = all_done + 1;  // [4] the warps of the same rows
-  uint64_t* next_full = meet_bar + 4;   // [2]
+  uint64_t* next_full = all_done + 1;   // [2]
   uint64_t* next_empty = next_full + 2; // [2]
   int* next_unit = reinterpret_cast<int*>(smem + C::BAR_OFF + 496);  // [2][16]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + C::BAR_OFF + 624);
   volatile int* abort = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  int* tops = reinterpret_cast<int*>(smem + C::MEET_OFF);       // [4][BM] ordered()
-  float* sums = reinterpret_cast<float*>(smem + C::MEET_OFF);   // [kParts][BM]
-  auto& line_shared = *reinterpret_cast<typename WorkLine<kThreads>::Shared*>(sQ);  // before Q comes
 
   const PagedAttentionArgs& a = args.a;
   const PagedBatch& p = a.batch;
@@ -329,7 +328,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const uint32_t rank = cluster_ctarank();
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1;
-  const int group = a.q_heads / a.cache.heads, tokens = BM / group;  // new tokens an SM
+  const int group = args.group, tokens = args.tokens;
   int* status = g_status;
   if (smem_addr(smem) & 1023) {
     report(status, ME_ERR_ALIGN, 76);
@@ -345,7 +344,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(o_full, 1);
     mbar_init(o_free, 2 * kSoftWarps);
     mbar_init(all_done, 1);
-    for (int i = 0; i < 4; ++i) mbar_init(&meet_bar[i], kParts);
     for (int i = 0; i < 2; ++i) mbar_init(&next_full[i], 1), mbar_init(&next_empty[i], 2 + kSoftWarps + (leader ? 1 : 0));
     *abort = 0;
     fence_barrier_init();
@@ -354,10 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&tv);
   }
   if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
-  for (int i = threadIdx.x; i < 4 * BM; i += kThreads) tops[i] = ordered(-INFINITY);
   if (args.least_rows == 0) clear_rest<D>(a, kThreads);  // (else the kernel of few rows does)
-  int64_t units0;
-  const int cut = cut_of<D, kThreads>(args, line_shared, units0);
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
@@ -377,6 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   Unit u;
   Keys seq;
   int unit_x = 0;
+  bool whole = true;  // every page of the unit's keys is one
   auto take_unit = [&](int it, int where) {
     if (!wait_u(&next_full[it & 1], (it >> 1) & 1, where)) return false;
     const int mine = next_unit[(it & 1) * 16 + (lane & 15)];
@@ -387,7 +383,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     u.b = field(4), u.tile = field(5), u.kv = field(6), u.half = field(7);
     u.kb0 = field(8), u.kb1 = field(9), u.chunk = field(10), u.chunks = field(11);
     seq = {field(12), field(13)};
-    unit_x = field(14);
+    unit_x = field(14), whole = field(15);
     return field(0) != 0;
   };
 
@@ -419,29 +415,33 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int n = u.kb1 - u.kb0;
       if (n <= 0) continue;
       const int y0 = u.kv << args.plog;
-      // pages of a block, a lane for each 16 keys; an index past the cache where there is none
+      // The table's entries for four blocks, a lane for each 16 keys: read four blocks ahead and looked at when they are needed (a look at
+      // once would wait for memory in every block, which held most SMs at 5000 to 6000 clocks a block).
       auto pages_of = [&](int kb) {
-        int id = -1;
-        if (lane < 8) id = page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog);
-        return id < 0 ? a.cache.pages : id;
+        const int col = (kb * BN + lane * 16) >> args.plog;
+        return col < p.width ? p.table[u.b * p.table_stride + col] : -1;
       };
       // 64 keys from `in` of block kb, NC x 64 columns from chunk x on
       auto load64 = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int kb, int in, int ids, int x, auto NC) {
         if (box == 64) {
-          const int id = __shfl_sync(0xffffffffu, ids, in / 16);
+          const int id = __shfl_sync(0xffffffffu, ids, (kb - u.kb0) % 4 * 8 + in / 16);
           tma_load_4d_pair_if(dst, map, bar, 0, y0 + ((kb * BN + in) & page_mask), x, id, one);
         } else {
           for (int row = 0; row < 64; row += box) {
-            const int id = __shfl_sync(0xffffffffu, ids, (in + row) / 16);
+            const int id = __shfl_sync(0xffffffffu, ids, (kb - u.kb0) % 4 * 8 + (in + row) / 16);
 #pragma unroll
             for (int i = 0; i < decltype(NC)::value; ++i)
               tma_load_4d_pair_if(dst + i * (64 * 128) + row * 128, map, bar, 0, y0 + ((kb * BN + in + row) & page_mask), x + i, id, one);
           }
         }
       };
-      int ids = pages_of(u.kb0);
+      int raw = pages_of(u.kb0), ids = 0;
       for (int j = 0; j < n && ok; ++j) {
-        const int next = j + 1 < n ? pages_of(u.kb0 + j + 1) : 0, kb = u.kb0 + j;
+        const int kb = u.kb0 + j;
+        if ((j & 3) == 0) {
+          ids = raw >= 0 && raw < a.cache.pages ? raw : a.cache.pages;  // none: an index past the cache
+          if (j + 4 < n) raw = pages_of(kb + 4);
+        }
         if (of_k) {
 #pragma unroll
           for (int c = 0; c < C::K_STAGES; ++c) {
@@ -463,21 +463,23 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           const bool stale = has_stale(seq, kb);
-          free_stage();
-          if (!ok) break;
-          if (one) {
-            if (stale) mbar_expect_tx(&v_here[st], C::V_BYTES);
-            if (leader && stale) mbar_arrive(&full[st]);
-            if (leader && !stale) mbar_expect_tx(&full[st], 2 * C::V_BYTES);
-          }
-          __syncwarp();
 #pragma unroll
-          for (int c = 0; c < 2; ++c)
-            load64(aV + st * C::V_BYTES + c * (C::V_BYTES / 2), &tv, stale ? v_here_own + st * 8 : full_leader + st * 8, kb, c * 64, ids,
-                   (u.half * C::DV + (int)rank * C::VC) / 64, std::integral_constant<int, C::VC / 64>());
-          next_stage();
+          for (int c = 0; c < C::V_STAGES; ++c) {
+            free_stage();
+            if (!ok) break;
+            if (one) {
+              if (stale) mbar_expect_tx(&v_here[st], C::V_BYTES);
+              if (leader && stale) mbar_arrive(&full[st]);
+              if (leader && !stale) mbar_expect_tx(&full[st], 2 * C::V_BYTES);
+            }
+            __syncwarp();
+#pragma unroll
+            for (int in = 0; in < C::V_KEYS; in += 64)
+              load64(aV + st * C::V_BYTES + in * 128, &tv, stale ? v_here_own + st * 8 : full_leader + st * 8, kb, c * C::V_KEYS + in, ids,
+                     (u.half * C::DV + (int)rank * C::VC) / 64, std::integral_constant<int, C::VC / 64>());
+            next_stage();
+          }
         }
-        ids = next;
       }
       ++live;
     }
@@ -505,16 +507,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int j = 0; j <= n && ok; ++j) {
           if (j < n) {
             const uint32_t to = kS + ((gb + j) & 1) * BN;
-#pragma unroll
+#pragma unroll 1
             for (int c = 0; c < C::K_STAGES; ++c) {
               wait(&k_full[kst], kphase, 63);
               if (!ok) break;
               tc_fence_after();
-              const uint64_t dk = dK + (kst * C::K_BYTES >> 4);
+              const uint64_t dk = dK + (kst * C::K_BYTES >> 4), dq = dQ + (c * (C::KC / 64) * (BM * 128) >> 4);
+#pragma unroll 1
+              for (int k4 = 0; k4 < C::KC / 64; ++k4)
 #pragma unroll
-              for (int kk = 0; kk < C::KC / 16; ++kk)
-                umma_bf16_pair_if(to, dQ + (((c * (C::KC / 64) + kk / 4) * (BM * 128) + (kk & 3) * 32) >> 4),
-                                  dk + (((kk / 4) * (64 * 128) + (kk & 3) * 32) >> 4), id_s, (c | kk) != 0, one);
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_bf16_pair_if(to, dq + ((k4 * (BM * 128) + kk * 32) >> 4), dk + ((k4 * (64 * 128) + kk * 32) >> 4), id_s, (c | k4 | kk) != 0, one);
               umma_commit_pair_if(&k_empty[kst], one);
               if (++kst == KR) kst = 0, kphase ^= 1;
             }
@@ -531,15 +534,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             else if (ok)
               wait(&p_full[i & 1], (i >> 1) & 1, 61);
             if (!ok) break;
-            wait(&v_full[vst], vphase, 62);
-            if (!ok) break;
-            tc_fence_after();
-            const uint64_t dv = dV + (vst * C::V_BYTES >> 4);
+#pragma unroll 1
+            for (int c = 0; c < C::V_STAGES; ++c) {
+              wait(&v_full[vst], vphase, 62);
+              if (!ok) break;
+              tc_fence_after();
+              const uint64_t dv = dV + (vst * C::V_BYTES >> 4);
+              const uint32_t from_p = kS + (i & 1) * BN + c * (C::V_KEYS / 16) * 8;
+#pragma unroll 1
+              for (int k4 = 0; k4 < C::V_KEYS / 64; ++k4)
 #pragma unroll
-            for (int kk = 0; kk < BN / 16; ++kk)
-              umma_bf16_pair_ts_if(kO, kS + (i & 1) * BN + kk * 8, dv + (((kk / 4) * (C::V_BYTES / 2) + (kk & 3) * 2048) >> 4), id_o, (j > 1 || kk > 0), one);
-            umma_commit_pair_if(&v_empty[vst], one);
-            if (++vst == VR) vst = 0, vphase ^= 1;
+                for (int kk = 0; kk < 4; ++kk)
+                  umma_bf16_pair_ts_if(kO, from_p + (k4 * 4 + kk) * 8, dv + ((k4 * 4 + kk) * 2048 >> 4), id_o, (j > 1 || c > 0 || k4 > 0 || kk > 0), one);
+              umma_commit_pair_if(&v_empty[vst], one);
+              if (++vst == VR) vst = 0, vphase ^= 1;
+            }
+            if (!ok) break;
             umma_commit_pair_if(&pv_done[i & 1], one);
             if (j == n) umma_commit_pair_if(o_full, one);
           }
@@ -554,168 +564,135 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- units
-    Walk<D> walk(args, cut);
+    Walk<D> walk(args, cut_of<D>(args));
     Unit w = {};
     bool more = true;
     for (int it = 0; more; ++it) {
       const int64_t x = pair + (int64_t)it * args.pairs;
       more = __all_sync(0xffffffffu, walk.at(x, w));
       const Keys k = keys_of(p, a.cache.page, w.s, 0, w.s.count - 1, a.window);
+      bool all = true;
+      for (int kb = w.kb0 + lane / 8; more && kb < w.kb1; kb += 4) {  // a lane for 16 keys
+        const int key = kb * BN + lane % 8 * 16;
+        if (key + 15 >= k.lo && key < k.hi) all = all && page_at(p, a.cache.pages, w.b, key >> args.plog) >= 0;
+      }
+      all = __all_sync(0xffffffffu, all);
       if (it >= 2 && !wait_u(&next_empty[it & 1], ((it >> 1) - 1) & 1, 80)) break;
       int* to = next_unit + (it & 1) * 16;
       if (lane == 0) {
         to[0] = more, to[1] = w.s.first, to[2] = w.s.count, to[3] = w.s.context, to[4] = w.b, to[5] = w.tile, to[6] = w.kv, to[7] = w.half;
-        to[8] = w.kb0, to[9] = w.kb1, to[10] = w.chunk, to[11] = w.chunks, to[12] = k.lo, to[13] = k.hi, to[14] = (int)x;
+        to[8] = w.kb0, to[9] = w.kb1, to[10] = w.chunk, to[11] = w.chunks, to[12] = k.lo, to[13] = k.hi, to[14] = (int)x, to[15] = all;
         mbar_arrive(&next_full[it & 1]);
       }
       __syncwarp();
     }
   } else if (warp >= kFirstSoft) {
     // ---------------------------------------------------------------- softmax
-    const int quarter = warp & 3, part = (warp - kFirstSoft) >> 2, r = quarter * 32 + lane;  // part of a block's keys; row of the SM
+    const int quarter = warp & 3, r = quarter * 32 + lane;  // row of the SM
     const uint32_t lanes = (uint32_t)(quarter * 32) << 16;
     const uint32_t p_leader = mapa_shared(smem_addr(p_full), 0), o_leader = mapa_shared(smem_addr(o_free), 0);
-    constexpr int HB = BN / kParts;  // keys a thread
     const float to_log2 = a.scale * kLog2e;
     const int ti = r / group, head = r % group;
     // 32-byte stores of O where its rows allow them
     const bool wide = reinterpret_cast<uintptr_t>(a.o) % 32 == 0 && a.o_token % 16 == 0 && a.o_head % 16 == 0;
-    int gb = 0, live = 0, met = 0;  // blocks, units with any, meetings so far
-    uint32_t v_phases = 0;          // bit i: parity of v_here[i]
+    int gb = 0, live = 0;   // blocks, units with any so far
+    uint32_t v_phases = 0;  // bit i: parity of v_here[i]
     bool ok = true;
-    // The row's four warps meet: what each wrote before come_by() is there after meet().
-    auto come_by = [&] {
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&meet_bar[quarter]);
-    };
-    auto meet = [&] { ok = wait_u(&meet_bar[quarter], met & 1, 75), ++met; };
-    // The sum of all parts' x, in the parts' order. (sums lies over tops: both are idle at a unit's end.)
-    auto sum_up = [&](float x) {
-      sums[part * BM + r] = x;
-      come_by(), meet();
-      const float all = sums[r] + sums[BM + r];
-      come_by(), meet();
-      return all;
-    };
     for (int it = 0; ok && take_unit(it, 77); ++it) {
       const int n = max(u.kb1 - u.kb0, 0);
       const int token = u.tile * 2 * tokens + (int)rank * tokens + ti;  // of the sequence's new ones
-      const bool mine = ti < tokens && token < u.s.count;
+      const bool mine = ti < tokens && token < u.s.count, any_mine = __any_sync(0xffffffffu, mine);
       const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
       const int from = a.window > 0 ? u.s.context + token - a.window + 1 : 0;
-      float m = -INFINITY, l = 0.f;  // l: this part's sum of p
-      float alpha = 1.f;             // what O has to be rescaled by
-      auto pages_of = [&](int kb) {  // bit i: keys 16 i of the four blocks from kb on have a page
-        return __ballot_sync(0xffffffffu, page_at(p, a.cache.pages, u.b, (kb * BN + lane * 16) >> args.plog) >= 0);
-      };
-      uint32_t there = n > 0 ? pages_of(u.kb0) : 0, there_next = 0;
-      for (int j = 0; j < n && ok; ++j) {
-        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN + part * HB;
-        if ((j & 3) == 0) {
-          if (j > 0) there = there_next;
-          if (j + 4 < n) there_next = pages_of(kb + 4);
-        }
-        const uint32_t pages = (there >> ((j & 3) * 8 + part * (HB / 16))) & 0xfu;
-        const bool open = pages == 0xfu && ((key0 >= from && key0 + HB - 1 <= last) || !mine), all_open = __all_sync(0xffffffffu, open);
+      float m = -INFINITY, l = 0.f;
+      for (int j = 0; j < n; ++j) {
+        const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN;
+        const uint32_t at = lanes + kS + (i & 1) * BN;
+        const bool stale = has_stale(seq, kb);
+        float alpha = 1.f;
         if (!(ok = wait_u(&s_full[i & 1], (i >> 1) & 1, 70))) break;
         tc_fence_after();
-        const uint32_t at = tmem + lanes + kS + (i & 1) * BN;
-        float top = -INFINITY, sum[2];
-        uint32_t pk[HB / 2];
-        bool first = true;  // a second pass, from the scores again, for a row that jumps
+        if (any_mine) {  // (rows of nothing: P may be what it is)
+          uint32_t pages = 0xff;
+          if (!whole) pages = __ballot_sync(0xffffffffu, lane < 8 && page_at(p, a.cache.pages, u.b, (key0 + (lane & 7) * 16) >> args.plog) >= 0);
+          const bool open = __all_sync(0xffffffffu, pages == 0xffu && ((key0 >= from && key0 + BN - 1 <= last) || !mine));
+          // 64 scores from column c on, -inf where the row does not see the key
+          auto scores = [&](int c, uint32_t(&s)[2][32]) {
+            tmem_issue_ld32(at + c, s[0]);
+            tmem_issue_ld32(at + c + 32, s[1]);
+            tmem_wait_ld(s[0]);
+            tmem_wait_ld(s[1]);
+            if (!open) {
+              // bits from .. last of these keys that have a page
+              const int lo = min(max(from - key0 - c, 0), 64), hi = min(max(last + 1 - key0 - c, 0), 64);
+              const uint64_t seen = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                const uint32_t two = pages >> (c / 16 + 2 * h);
+                const uint32_t bits = (uint32_t)(seen >> (32 * h)) & ((two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u));
+#pragma unroll
+                for (int e = 0; e < 32; ++e)
+                  if (!(bits & (1u << e))) s[h][e] = 0xff800000u;  // -inf
+              }
+            }
+          };
+          // (Rolled loops: with 128 scores unrolled the roles' code together does not fit the instruction caches, and the SMs of a
+          // full GPC took 4000 to 5000 clocks for what takes 1400.)
+          float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll 1
-        for (;;) {
-          uint32_t s[HB];
-          uint32_t(&low)[32] = reinterpret_cast<uint32_t(&)[32]>(s[0]), (&high)[32] = reinterpret_cast<uint32_t(&)[32]>(s[32]);
-          tmem_issue_ld32(at + part * HB, low);
-          tmem_issue_ld32(at + part * HB + 32, high);
-          tmem_wait_ld(low);
-          tmem_wait_ld(high);
-          if (!all_open) {
+          for (int c = 0; c < BN; c += 64) {
+            uint32_t s[2][32];
+            scores(c, s);
 #pragma unroll
-            for (int c = 0; c < HB; c += 32) {
-              // bits from .. last of these 32 keys that have a page
-              const int lo = min(max(from - key0 - c, 0), 32), hi = min(max(last + 1 - key0 - c, 0), 32);
-              uint32_t seen = (uint32_t)(((1ull << hi) - 1) & ~((1ull << lo) - 1));
-              seen &= ((pages >> (c / 16)) & 1 ? 0xffffu : 0u) | ((pages >> (c / 16)) & 2 ? 0xffff0000u : 0u);
-#pragma unroll
-              for (int e = 0; e < 32; ++e)
-                if (!(seen & (1u << e))) s[c + e] = 0xff800000u;  // -inf
-            }
+            for (int e = 0; e < 64; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(s[e / 32][e % 32]));
           }
-          bool wait_here = !first;  // the maximum of this block has come round before the exponentials
-          if (first) {
-            first = false;
-            float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int e = 0; e < HB; ++e) mx[e & 3] = fmaxf(mx[e & 3], __uint_as_float(s[e]));
-            atomicMax(&tops[(i & 3) * BM + r], ordered(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))));
-            if (part == 0) tops[((i + 2) & 3) * BM + r] = ordered(-INFINITY);  // block i - 2's, which all have read: its P has been taken
-            come_by();
-            if (__any_sync(0xffffffffu, m == -INFINITY && mine)) {
-              meet();
-              if (!ok) break;
-              top = unordered(tops[(i & 3) * BM + r]) * to_log2;
-              if (m == -INFINITY) m = top;
-              wait_here = true;
-            }
-          }
-          const float z = m == -INFINITY ? 0.f : m;
-          sum[0] = sum[1] = 0.f;
-#pragma unroll
-          for (int e = 0; e < HB; e += 2) {
-            const float p0 = ex2(fmaf(__uint_as_float(s[e]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[e + 1]), to_log2, -z));
-            sum[0] += p0, sum[1] += p1;
-            pk[e / 2] = pack2(p0, p1);
-          }
-          if (!wait_here) {
-            meet();  // (and all have read their scores: P may go over them)
-            if (!ok) break;
-            top = unordered(tops[(i & 3) * BM + r]) * to_log2;
-          }
-          if (!__any_sync(0xffffffffu, top > m + kJump)) break;  // (the row's threads see the same numbers)
-          if (top > m + kJump) {
-            const float f = ex2(m - top);
-            alpha *= f, l *= f;
+          const float top = fmaxf(mx[0], mx[1]) * to_log2;
+          if (top > m + kSlack) {
+            if (m != -INFINITY) alpha = ex2(m - top), l *= alpha;  // (before its first score a row's O is zero)
             m = top;
           }
+          const float z = m == -INFINITY ? 0.f : m;
+          float sum[2] = {0.f, 0.f};
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 64) {
+            uint32_t s[2][32], pk[32];
+            scores(c, s);
+#pragma unroll
+            for (int e = 0; e < 64; e += 2) {
+              const float p0 = ex2(fmaf(__uint_as_float(s[e / 32][e % 32]), to_log2, -z)), p1 = ex2(fmaf(__uint_as_float(s[e / 32][e % 32 + 1]), to_log2, -z));
+              sum[0] += p0, sum[1] += p1;
+              pk[e / 2] = pack2(p0, p1);
+            }
+            tmem_st32u(at + c / 2, pk);  // over scores of keys up to c + 63, which have been read
+          }
+          l += sum[0] + sum[1];
         }
-        if (!ok) break;
-        l += sum[0] + sum[1];
-        tmem_st32u(at + part * (HB / 2), pk);
-        if (__any_sync(0xffffffffu, alpha != 1.f) && j > 0) {  // O stands still once the product before has ended
+        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {  // O stands still once the product before has ended
           if (!(ok = wait_u(&pv_done[(i - 1) & 1], ((i - 1) >> 1) & 1, 71))) break;
           tc_fence_after();
 #pragma unroll 1
-          for (int c = 0; c < C::DV / kParts; c += 16) {
+          for (int c = 0; c < C::DV; c += 16) {
             uint32_t o[16];
-            const uint32_t col = tmem + lanes + kO + part * (C::DV / kParts) + c;
-            tmem_issue_ld16(col, o);
+            tmem_issue_ld16(lanes + kO + c, o);
             tmem_wait_ld(o);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
-            tmem_st16u(col, o);
+            tmem_st16u(lanes + kO + c, o);
           }
         }
-        alpha = 1.f;
-        if (top > m + kSlack) {  // from the next block on
-          alpha = ex2(m - top);
-          l *= alpha;
-          m = top;
-        }
-        const bool stale = has_stale(seq, kb);
-        if (stale) {  // row r: key r of the block, a part of this SM's columns
-          const int st = i % VR;
-          if (!(ok = wait_u(&v_here[st], (v_phases >> st) & 1, 72))) break;
-          v_phases ^= 1u << st;
-          const int key = kb * BN + r;
+        if (stale) {  // thread r: key r of the block, this SM's columns
+          for (int c = 0; c < C::V_STAGES && ok; ++c) {
+            const int st = (i * C::V_STAGES + c) % VR;
+            ok = wait_u(&v_here[st], (v_phases >> st) & 1, 72);
+            v_phases ^= 1u << st;
+          }
+          if (!ok) break;
+          const int key = key0 + r;
           if (key < seq.lo || key >= seq.hi) {
+            const int st = (i * C::V_STAGES + r / C::V_KEYS) % VR, row = r % C::V_KEYS;
 #pragma unroll
-            for (int i8 = 0; i8 < C::VC / 8 / kParts; ++i8) {
-              const int c = part * (C::VC / 8 / kParts) + i8;  // of its 16-byte chunks
-              *reinterpret_cast<uint4*>(sV + st * C::V_BYTES + (r / 64) * (C::V_BYTES / 2) + (c / 8) * (64 * 128) + (r & 63) * 128 + (c & 7) * 16) =
-                  make_uint4(0, 0, 0, 0);
-            }
+            for (int c = 0; c < C::VC / 8; ++c)  // its 16-byte chunks; the warp's rows in different banks
+              *reinterpret_cast<uint4*>(sV + st * C::V_BYTES + (c / 8) * (C::V_KEYS * 128) + row * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
         }
@@ -729,72 +706,65 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
       }
       // ---- the unit's end
-      float o_scale = 1.f;
-      if (n > 0 && ok) {
-        o_scale = alpha;  // a rescaling that no block was left for
-        come_by(), meet();  // all have read the last maxima
-        if (ok) l = sum_up(l);
-        tops[part * BM + r] = tops[(part + 2) * BM + r] = ordered(-INFINITY);
-        come_by();
-        if (ok) meet();
-        if (ok) ok = wait_u(o_full, live & 1, 73);
-        ++live;
-      }
+      if (n > 0 && ok) ok = wait_u(o_full, live & 1, 73), ++live;
       if (!ok) break;
       tc_fence_after();
-      const float inv = u.chunks > 1 ? o_scale : l == 0.f ? 0.f : o_scale / l;  // (a part keeps its sum)
       const int t = u.s.first + token, h = u.kv * group + head;
-      const int64_t slot = (int64_t)unit_x * args.slot_rows + (int)rank * tokens * group + r;
-      constexpr int PC = C::DV / kParts, PS = PC < 32 ? PC : 32;  // this part's columns of O, and of a step
-      const int col0 = part * PC;
+      const int64_t slot = unit_x, row = (int64_t)(int)rank * tokens * group + r;
       auto release = [&] {  // O has been read: the next unit's products may go over it
         if (n == 0) return;
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive_cta(o_leader);
       };
-      if (u.chunks > 1) {
-        float* dst = args.part_o + slot * C::DV + col0;
+      if (!any_mine) {
+        release();
+      } else if (u.chunks > 1) {
+        float4* dst = args.part_o + slot * (C::DV / 4) * args.slot_rows + row;
 #pragma unroll 1
-        for (int c = 0; c < PC; c += PS) {
+        for (int c = 0; c < C::DV; c += 32) {
           uint32_t o[32] = {};
           if (n > 0) {
-            tmem_issue_ld32(tmem + lanes + kO + col0 + c, o);
+            tmem_issue_ld32(lanes + kO + c, o);
             tmem_wait_ld(o);
           }
+          if (c + 32 == C::DV) release();
           if (mine)
 #pragma unroll
-            for (int e = 0; e < PS; e += 4)
-              *reinterpret_cast<float4*>(dst + c + e) = make_float4(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv,
-                                                                    __uint_as_float(o[e + 2]) * inv, __uint_as_float(o[e + 3]) * inv);
+            for (int e = 0; e < 32; e += 4)
+              dst[(int64_t)((c + e) / 4) * args.slot_rows] = make_float4(__uint_as_float(o[e]), __uint_as_float(o[e + 1]), __uint_as_float(o[e + 2]),
+                                                                         __uint_as_float(o[e + 3]));
         }
-        if (mine && part == 0) args.part_ml[slot] = make_float2(m, l);
-        release();
+        if (mine) args.part_ml[slot * args.slot_rows + row] = make_float2(m, l);
       } else {
-        uint32_t out[PC / 2] = {};
-        if (n > 0) {
-#pragma unroll
-          for (int c = 0; c < PC; c += PS) {
-            uint32_t o[32];
-            tmem_issue_ld32(tmem + lanes + kO + col0 + c, o);
-            tmem_wait_ld(o);
-#pragma unroll
-            for (int e = 0; e < PS; e += 2) out[(c + e) / 2] = pack2(__uint_as_float(o[e]) * inv, __uint_as_float(o[e + 1]) * inv);
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV;
+#pragma unroll 1
+        for (int c = 0; c < C::DV; c += 64) {
+          uint32_t o[2][32] = {};
+          if (n > 0) {
+            tmem_issue_ld32(lanes + kO + c, o[0]);
+            tmem_issue_ld32(lanes + kO + c + 32, o[1]);
+            tmem_wait_ld(o[0]);
+            tmem_wait_ld(o[1]);
           }
-        }
-        release();
-        if (mine) {
-          bf16* dst = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + col0;
+          if (c + 64 == C::DV) release();
+          if (!mine) continue;
+          uint32_t out[32];
 #pragma unroll
-          for (int e = 0; e < PC / 2; e += 8) {
+          for (int e = 0; e < 64; e += 2) out[e / 2] = pack2(__uint_as_float(o[e / 32][e % 32]) * inv, __uint_as_float(o[e / 32][e % 32 + 1]) * inv);
+#pragma unroll
+          for (int e = 0; e < 32; e += 8) {
             if (wide) {
-              st_global32(dst + e * 2, &out[e]);
+              st_global32(dst + c + e * 2, &out[e]);
             } else {
-              *reinterpret_cast<uint4*>(dst + e * 2) = make_uint4(out[e], out[e + 1], out[e + 2], out[e + 3]);
-              *reinterpret_cast<uint4*>(dst + e * 2 + 8) = make_uint4(out[e + 4], out[e + 5], out[e + 6], out[e + 7]);
+              *reinterpret_cast<uint4*>(dst + c + e * 2) = make_uint4(out[e], out[e + 1], out[e + 2], out[e + 3]);
+              *reinterpret_cast<uint4*>(dst + c + e * 2 + 8) = make_uint4(out[e + 4], out[e + 5], out[e + 6], out[e + 7]);
             }
           }
-          if (u.half == 0 && part == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
+        }
+        if (mine) {
+          if (u.half == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
         }
       }
       gb += n;
@@ -809,47 +779,46 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the chunks of sequences that were cut: a block takes every gridDim.x-th 32 rows of units.
-constexpr int kJoinThreads = 256, kJoinRows = 32;
+// Joins the chunks of sequences that were cut: a block takes every gridDim.x-th (unit, 32 rows), its lanes a row each and its warps every
+// eighth 4 columns.
+constexpr int kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
-  constexpr int PER = C::DV / 4, ROWS = kJoinThreads / PER, STEPS = 2 * BM / kJoinRows;
-  __shared__ typename WorkLine<kJoinThreads>::Shared line_shared;
+  constexpr int STEPS = 2 * BM / 32;
   const PagedAttentionArgs& a = args.a;
-  int64_t units;
-  const int cut = cut_of<D, kJoinThreads>(args, line_shared, units);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int cut = cut_of<D>(args);
   if (cut == 0) return;
-  const int group = a.q_heads / a.cache.heads, tokens = 2 * (BM / group);
   Walk<D> walk(args, cut);
   Unit u;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = args.group, tokens = 2 * args.tokens;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int64_t i = blockIdx.x; walk.at(i / STEPS, u); i += gridDim.x) {
     if (u.chunks == 1 || u.chunk != 0) continue;
     const int64_t x = i / STEPS, stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
-    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r0 = (int)(i % STEPS) * kJoinRows;
-    const int c = threadIdx.x % PER * 4;
-    for (int r = r0 + threadIdx.x / PER; r < min(rows, r0 + kJoinRows); r += ROWS) {
-      float top = -INFINITY, l = 0.f;
+    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r = (int)(i % STEPS) * 32 + lane;
+    if (r >= rows) continue;
+    float top = -INFINITY, l = 0.f;
+    for (int k = 0; k < u.chunks; ++k) top = fmaxf(top, args.part_ml[(x + k * stride) * args.slot_rows + r].x);
+    for (int k = 0; k < u.chunks; ++k) l += share(args.part_ml[(x + k * stride) * args.slot_rows + r], top);
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int t = u.s.first + i0 + r / group, h = u.kv * group + r % group;
+    bf16* out = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV;
+    for (int c = warp; c < C::DV / 4; c += kJoinThreads / 32) {
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
       for (int k = 0; k < u.chunks; ++k) {
-        const int64_t slot = (x + k * stride) * args.slot_rows + r;
-        const float2 ml = args.part_ml[slot];
-        const float4 y = *reinterpret_cast<const float4*>(args.part_o + slot * C::DV + c);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float up = fmaxf(top, ml.x);
-        const float f0 = top == -INFINITY ? 0.f : ex2(top - up), f1 = ex2(ml.x - up);
-        o.x = o.x * f0 + y.x * f1, o.y = o.y * f0 + y.y * f1, o.z = o.z * f0 + y.z * f1, o.w = o.w * f0 + y.w * f1;
-        l = l * f0 + ml.y * f1;
-        top = up;
+        const int64_t slot = x + k * stride;
+        const float2 ml = args.part_ml[slot * args.slot_rows + r];
+        const float4 y = args.part_o[(slot * (C::DV / 4) + c) * args.slot_rows + r];
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2(ml.x - top);  // (a NaN stays one)
+        o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
       }
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      const int t = u.s.first + i0 + r / group, h = u.kv * group + r % group;
       uint2 b4;
       b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + c) = b4;
-      if (c == 0 && u.half == 0) a.lse[(int64_t)h * a.batch.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+      *reinterpret_cast<uint2*>(out + c * 4) = b4;
     }
+    if (warp == 0 && u.half == 0) a.lse[(int64_t)h * a.batch.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
   }
 }
 
@@ -920,18 +889,19 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
   args.a = a;
   args.pairs = resident_pairs<D>();
   args.slot_rows = slot_rows_of<D>(a);
-  args.part_o = static_cast<float*>(space);
-  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * kDeals * args.pairs * args.slot_rows * C::DV);
+  args.part_o = static_cast<float4*>(space);
+  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * kDeals * args.pairs * args.slot_rows * (C::DV / 4));
+  args.group = a.q_heads / a.cache.heads, args.tokens = BM / args.group;
   args.plog = 0;
   while ((1 << args.plog) < a.cache.page) ++args.plog;
   args.least_rows = least_rows;
   bind_primary_context();
-  const int group = a.q_heads / a.cache.heads, box = std::min(a.cache.page, 64);
+  const int box = std::min(a.cache.page, 64);
   const int64_t rows = (int64_t)a.cache.heads * a.cache.page;
   // pages as [page][64 columns of the head][head, position][column]
   const int64_t dims[4] = {64, rows, D / 64, a.cache.pages};
   CUtensorMap tq, tk, tv;
-  if (!make_map<3>(&tq, a.q, {D, a.q_heads, a.batch.tokens}, {a.q_head, a.q_token}, {group, BM / group}) ||
+  if (!make_map<3>(&tq, a.q, {D, a.q_heads, a.batch.tokens}, {a.q_head, a.q_token}, {args.group, args.tokens}) ||
       !make_map<4>(&tk, a.cache.k, dims, {D, 64, a.cache.k_stride}, {box, box == 64 ? C::KC / 64 : 1, 1}) ||
       !make_map<4>(&tv, a.cache.v, dims, {D, 64, a.cache.v_stride}, {box, box == 64 ? C::VC / 64 : 1, 1}))
     return "cuTensorMapEncodeTiled failed";
