@@ -51,11 +51,11 @@ struct Cfg {
   static constexpr int NV = D == 64 ? 128 : DV;      // columns of the P V product (dim 64: the odd SM's half is past the row, zeros)
   static constexpr int VC = NV / 2;                  // of them in this SM
   static constexpr int Q_BYTES = BM * D * 2;
-  // a stage of K: this SM's 64 keys of a block x KC columns; of V: V_KEYS keys x VC
+  // a stage of K: this SM's 64 keys of a block x KC columns; of V: 128 keys x VC, one set of 64 keys after the other. (Stages of 16 KB, twice
+  // as many: 10% slower, for a stage costs its loader and the products' warp some hundred clocks.)
   static constexpr int KC = D < 256 ? D : 256, K_STAGES = D / KC;
-  static constexpr int V_KEYS = VC == 128 ? 64 : 128, V_STAGES = BN / V_KEYS;
-  static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = V_KEYS * VC * 2;
-  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 2 : D == 256 ? 4 : 6;  // stages
+  static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = BN * VC * 2;
+  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 1 : D == 256 ? 2 : 6;  // stages
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KR * K_BYTES, BAR_OFF = V_OFF + VR * V_BYTES;
   static constexpr int SMEM = BAR_OFF + 640;
   static_assert(SMEM <= 232448, "shared memory");
@@ -205,23 +205,26 @@ ME_DEVICE void tma_load_4d_pair_if(uint32_t dst, const CUtensorMap* map, uint32_
       "l"(reinterpret_cast<uint64_t>(map)), "r"(bar_cluster), "r"(x), "r"(y), "r"(z), "r"(w), "r"(issue)
       : "memory");
 }
-// The pair's product and its commits, by the lanes of `issue` (one lane of the warp that goes along).
-ME_DEVICE void umma_bf16_pair_if(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+// The pair's product and its commits, by the lanes of `issue` (one lane of the warp that goes along). Descriptors in halves: steps change the
+// low one alone.
+ME_DEVICE void umma_bf16_pair_if(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t hi, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 a, b;\n\t"
+      "mov.b64 a, {%1, %3};\n\tmov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_lo), "r"(b_lo), "r"(hi), "r"(idesc), "r"(accumulate), "r"(issue));
 }
 // A (P) from tensor memory.
-ME_DEVICE void umma_bf16_pair_ts_if(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+ME_DEVICE void umma_bf16_pair_ts_if(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t b_hi, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
   asm volatile(
-      "{\n\t.reg .pred p, q;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "setp.ne.b32 q, %5, 0;\n\t"
-      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(issue));
+      "{\n\t.reg .pred p, q;\n\t.reg .b64 b;\n\t"
+      "mov.b64 b, {%2, %3};\n\t"
+      "setp.ne.b32 p, %5, 0;\n\t"
+      "setp.ne.b32 q, %6, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %4, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "r"(b_lo), "r"(b_hi), "r"(idesc), "r"(accumulate), "r"(issue));
 }
 ME_DEVICE void umma_commit_pair_if(uint64_t* bar, uint32_t issue, uint16_t mask = 0x3) {
   asm volatile(
@@ -463,22 +466,19 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         } else {
           const bool stale = has_stale(seq, kb);
-#pragma unroll
-          for (int c = 0; c < C::V_STAGES; ++c) {
-            free_stage();
-            if (!ok) break;
-            if (one) {
-              if (stale) mbar_expect_tx(&v_here[st], C::V_BYTES);
-              if (leader && stale) mbar_arrive(&full[st]);
-              if (leader && !stale) mbar_expect_tx(&full[st], 2 * C::V_BYTES);
-            }
-            __syncwarp();
-#pragma unroll
-            for (int in = 0; in < C::V_KEYS; in += 64)
-              load64(aV + st * C::V_BYTES + in * 128, &tv, stale ? v_here_own + st * 8 : full_leader + st * 8, kb, c * C::V_KEYS + in, ids,
-                     (u.half * C::DV + (int)rank * C::VC) / 64, std::integral_constant<int, C::VC / 64>());
-            next_stage();
+          free_stage();
+          if (!ok) break;
+          if (one) {
+            if (stale) mbar_expect_tx(&v_here[st], C::V_BYTES);
+            if (leader && stale) mbar_arrive(&full[st]);
+            if (leader && !stale) mbar_expect_tx(&full[st], 2 * C::V_BYTES);
           }
+          __syncwarp();
+#pragma unroll
+          for (int c = 0; c < 2; ++c)
+            load64(aV + st * C::V_BYTES + c * (C::V_BYTES / 2), &tv, stale ? v_here_own + st * 8 : full_leader + st * 8, kb, c * 64, ids,
+                   (u.half * C::DV + (int)rank * C::VC) / 64, std::integral_constant<int, C::VC / 64>());
+          next_stage();
         }
       }
       ++live;
@@ -494,7 +494,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     // issue took 110 to 180 clocks, more than the product.)
     if (leader) {
       const uint32_t id_s = idesc_bf16(2 * BM, BN), id_o = idesc_bf16(2 * BM, C::NV, true);
-      const uint64_t dQ = desc_sw128(smem_addr(sQ)), dK = desc_sw128(smem_addr(sK)), dV = desc_mn_sw128(smem_addr(sV), 64 * 128, 1024);
+      const uint32_t dQ = (uint32_t)desc_sw128(smem_addr(sQ)), dK = (uint32_t)desc_sw128(smem_addr(sK)), hi = (uint32_t)(desc_sw128(0) >> 32);
+      const uint32_t dV = (uint32_t)desc_mn_sw128(smem_addr(sV), 64 * 128, 1024), hV = (uint32_t)(desc_mn_sw128(0, 64 * 128, 1024) >> 32);
       const uint32_t one = lane == 0;
       int kst = 0, kphase = 0, vst = 0, vphase = 0;  // the rings' next stages
       int gb = 0, live = 0;    // blocks, units so far
@@ -512,12 +513,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               wait(&k_full[kst], kphase, 63);
               if (!ok) break;
               tc_fence_after();
-              const uint64_t dk = dK + (kst * C::K_BYTES >> 4), dq = dQ + (c * (C::KC / 64) * (BM * 128) >> 4);
-#pragma unroll 1
+              const uint32_t dk = dK + (kst * C::K_BYTES >> 4), dq = dQ + (c * (C::KC / 64) * (BM * 128) >> 4);
+#pragma unroll
               for (int k4 = 0; k4 < C::KC / 64; ++k4)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                  umma_bf16_pair_if(to, dq + ((k4 * (BM * 128) + kk * 32) >> 4), dk + ((k4 * (64 * 128) + kk * 32) >> 4), id_s, (c | k4 | kk) != 0, one);
+                  umma_bf16_pair_if(to, dq + ((k4 * (BM * 128) + kk * 32) >> 4), dk + ((k4 * (64 * 128) + kk * 32) >> 4), hi, id_s, (c | k4 | kk) != 0, one);
               umma_commit_pair_if(&k_empty[kst], one);
               if (++kst == KR) kst = 0, kphase ^= 1;
             }
@@ -534,21 +535,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             else if (ok)
               wait(&p_full[i & 1], (i >> 1) & 1, 61);
             if (!ok) break;
-#pragma unroll 1
-            for (int c = 0; c < C::V_STAGES; ++c) {
-              wait(&v_full[vst], vphase, 62);
-              if (!ok) break;
-              tc_fence_after();
-              const uint64_t dv = dV + (vst * C::V_BYTES >> 4);
-              const uint32_t from_p = kS + (i & 1) * BN + c * (C::V_KEYS / 16) * 8;
-#pragma unroll 1
-              for (int k4 = 0; k4 < C::V_KEYS / 64; ++k4)
+            wait(&v_full[vst], vphase, 62);
+            if (!ok) break;
+            tc_fence_after();
+            const uint32_t dv = dV + (vst * C::V_BYTES >> 4), from_p = kS + (i & 1) * BN;
 #pragma unroll
-                for (int kk = 0; kk < 4; ++kk)
-                  umma_bf16_pair_ts_if(kO, from_p + (k4 * 4 + kk) * 8, dv + ((k4 * 4 + kk) * 2048 >> 4), id_o, (j > 1 || c > 0 || k4 > 0 || kk > 0), one);
-              umma_commit_pair_if(&v_empty[vst], one);
-              if (++vst == VR) vst = 0, vphase ^= 1;
-            }
+            for (int kk = 0; kk < BN / 16; ++kk)
+              umma_bf16_pair_ts_if(kO, from_p + kk * 8, dv + (((kk / 4) * (C::V_BYTES / 2) + (kk & 3) * 2048) >> 4), hV, id_o, (j > 1 || kk > 0), one);
+            umma_commit_pair_if(&v_empty[vst], one);
+            if (++vst == VR) vst = 0, vphase ^= 1;
             if (!ok) break;
             umma_commit_pair_if(&pv_done[i & 1], one);
             if (j == n) umma_commit_pair_if(o_full, one);
@@ -681,18 +676,15 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         if (stale) {  // thread r: key r of the block, this SM's columns
-          for (int c = 0; c < C::V_STAGES && ok; ++c) {
-            const int st = (i * C::V_STAGES + c) % VR;
-            ok = wait_u(&v_here[st], (v_phases >> st) & 1, 72);
-            v_phases ^= 1u << st;
-          }
-          if (!ok) break;
+          const int st = i % VR;
+          if (!(ok = wait_u(&v_here[st], (v_phases >> st) & 1, 72))) break;
+          v_phases ^= 1u << st;
           const int key = key0 + r;
           if (key < seq.lo || key >= seq.hi) {
-            const int st = (i * C::V_STAGES + r / C::V_KEYS) % VR, row = r % C::V_KEYS;
 #pragma unroll
             for (int c = 0; c < C::VC / 8; ++c)  // its 16-byte chunks; the warp's rows in different banks
-              *reinterpret_cast<uint4*>(sV + st * C::V_BYTES + (c / 8) * (C::V_KEYS * 128) + row * 128 + ((c + r) & 7) * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(sV + st * C::V_BYTES + (r / 64) * (C::V_BYTES / 2) + (c / 8) * (64 * 128) + (r & 63) * 128 + ((c + r) & 7) * 16) =
+                  make_uint4(0, 0, 0, 0);
           }
           fence_async_smem();
         }
