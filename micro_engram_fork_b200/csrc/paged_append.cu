@@ -67,9 +67,10 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
   }
   __syncthreads();
 
-  const int groups = (heads + HPW - 1) / HPW;
-  for (int g = blockIdx.y * kWarps + warp; g < groups; g += gridDim.y * kWarps) {
-    const int h = g * HPW + lane / L;
+  // A warp takes a group of heads; with fewer groups than warps several warps share one and take its tokens in turn.
+  const int groups = (heads + HPW - 1) / HPW, sharing = max(kWarps / groups, 1);
+  for (int g = sharing > 1 ? warp % groups : blockIdx.y * kWarps + warp; g < groups; g += gridDim.y * kWarps) {
+    const int h = g * HPW + lane / L, t0 = sharing > 1 ? warp / groups : 0;
     const bool live = h < heads;
     const bool is_q = h < hq, is_v = h >= hq + hk;
     const int src_h = !live ? 0 : (a.kv_shared && is_v) ? h - hk : h;
@@ -82,10 +83,16 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
       for (int e = 0; e < 8; ++e) wl[e] = w[l * 8 + e], wh[e] = w[HALF + l * 8 + e];
     }
     const bf16* src = reinterpret_cast<const bf16*>(a.qkv) + (int64_t)n0 * a.qkv_stride + (int64_t)src_h * D + l * 8;
-    for (int t = 0; t < n; ++t, src += a.qkv_stride) {
-      BF16x8 lo, hi;
-      lo.u = *reinterpret_cast<const uint4*>(src);
-      hi.u = *reinterpret_cast<const uint4*>(src + HALF);
+    BF16x8 lo, hi, next_lo, next_hi;
+    auto read = [&](int t, BF16x8& x, BF16x8& y) {
+      x.u = *reinterpret_cast<const uint4*>(src + t * a.qkv_stride);
+      y.u = *reinterpret_cast<const uint4*>(src + t * a.qkv_stride + HALF);
+    };
+    if (sharing > 1 && t0 >= sharing) break;  // (a warp left over)
+    if (t0 < n) read(t0, next_lo, next_hi);
+    for (int t = t0; t < n; t += sharing) {
+      lo.u = next_lo.u, hi.u = next_hi.u;
+      if (t + sharing < n) read(t + sharing, next_lo, next_hi);  // on its way while this one is worked on
       float xl[8], xh[8], ss = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
@@ -123,6 +130,7 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
         *reinterpret_cast<uint4*>(dst + HALF + l * 8) = hi.u;
       }
     }
+    if (sharing > 1) break;
   }
 }
 

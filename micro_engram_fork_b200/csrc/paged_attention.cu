@@ -92,6 +92,25 @@ ME_DEVICE UnitsOf units_of(const RowsArgs& args, int b, const Sequence& s) {
   return {(s.count * group + kRows - 1) / kRows, max((k.hi + kBlock - 1) / kBlock - k.lo / kBlock, 1)};
 }
 
+// The line of blocks in pieces of the same length, the first `rest` of them one longer.
+struct Cut {
+  int64_t total;
+  int pieces;
+  int64_t each;
+  int rest;
+  ME_DEVICE Cut(int64_t blocks, int most) : total(blocks), pieces((int)min((int64_t)most, blocks)) {
+    if (pieces == 0) each = 0, rest = 0;
+    else if (total <= UINT32_MAX) each = (uint32_t)total / (uint32_t)pieces, rest = (uint32_t)total % (uint32_t)pieces;
+    else each = total / pieces, rest = (int)(total % pieces);
+  }
+  ME_DEVICE int64_t start(int i) const { return i * each + min(i, rest); }
+  ME_DEVICE int owner(int64_t x) const {  // the piece that block x lies in
+    const int64_t longer = rest * (each + 1), in = x < longer ? x : x - longer, by = x < longer ? each + 1 : each;
+    const int n = in <= UINT32_MAX && by <= UINT32_MAX ? (int)((uint32_t)in / (uint32_t)by) : (int)(in / by);
+    return x < longer ? n : rest + n;
+  }
+};
+
 template <int D>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs args) {
   using C = Cfg<D>;
@@ -112,10 +131,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
     return (int64_t)u.tiles * hk * u.blocks;
   };
   WorkLine<kThreads> line(line_shared);
-  const int64_t total = line.total(p.seqs, count);
-  const int64_t pieces = min((int64_t)args.pieces, total);
-  if (blockIdx.x >= pieces) return;
-  const int64_t x0 = blockIdx.x * total / pieces, x1 = (blockIdx.x + 1) * total / pieces;
+  const Cut cut(line.total(p.seqs, count), args.pieces);
+  if (blockIdx.x >= cut.pieces) return;
+  const int64_t x0 = cut.start(blockIdx.x), x1 = cut.start(blockIdx.x + 1);
   int64_t x = x0, before;
   int b = line.find(p.seqs, count, x, before);
 
@@ -338,82 +356,80 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
   }
 }
 
-// Joins the parts of units that were cut. One block a unit and row at a time; groups of D / 4 threads take a part each.
-constexpr int kJoinThreads = 256;
+// Joins the parts of units that were cut. A block finds the unit that its border between two pieces lies in; the blocks of a unit's borders share its
+// rows, 128 columns at a time. Units of many parts: the block's warps take every eighth part of a task; of few: a task a warp.
+constexpr int kJoinThreads = 256, kJoinWarps = 8;
 
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs args) {
-  constexpr int PER = D / 4, GROUPS = kJoinThreads / PER;
+  constexpr int COLS = D < 128 ? D : 128, SETS = D / COLS;  // columns of a task
   __shared__ WorkLine<kJoinThreads>::Shared line_shared;
-  __shared__ float4 meet[kJoinThreads];
-  __shared__ float2 meet_ml[GROUPS];
+  __shared__ float4 meet[kJoinWarps][32];
+  __shared__ float meet_l[kJoinWarps];
   const PagedAttentionArgs& a = args.a;
   const PagedBatch& p = a.batch;
-  const int hk = a.cache.heads, group = a.q_heads / hk;
+  const int hk = a.cache.heads, group = a.q_heads / hk, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   auto blocks_of = [&](int b) -> int64_t {
     const UnitsOf u = units_of(args, b, sequence_of(p, b));
     return (int64_t)u.tiles * hk * u.blocks;
   };
   WorkLine<kJoinThreads> line(line_shared);
-  const int64_t total = line.total(p.seqs, blocks_of);
-  const int64_t pieces = min((int64_t)args.pieces, total);
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  // Only units that a border between two pieces lies in were cut: border i is before block x of the line.
-  for (int64_t i = 1 + blockIdx.x; i < pieces; i += gridDim.x) {
-    const int64_t x = i * total / pieces;
+  const Cut cut(line.total(p.seqs, blocks_of), args.pieces);
+  const int border = blockIdx.x + 1;
+  if (border < cut.pieces) {
+    const int64_t x = cut.start(border);  // the border is before block x of the line
     int64_t before;
     const int b = line.find(p.seqs, blocks_of, x, before);
     const Sequence s = sequence_of(p, b);
     const UnitsOf u = units_of(args, b, s);
-    const int unit = (int)((x - before) / u.blocks);
-    const int64_t begin = before + (int64_t)unit * u.blocks, end = begin + u.blocks;
-    if (x == begin) continue;                                // it separates two units
-    if ((i - 1) * total / pieces > begin) continue;          // an earlier border joins this unit
+    const int64_t in_seq = x - before;
+    const int unit = in_seq <= UINT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)u.blocks) : (int)(in_seq / u.blocks);
+    const int64_t begin = before + (int64_t)unit * u.blocks;
+    const int first = cut.owner(begin), count = cut.owner(begin + u.blocks - 1) - first + 1;  // the unit's pieces
     const int tile = unit % u.tiles, kv = unit / u.tiles, r0 = tile * kRows, rows = min(kRows, s.count * group - r0);
-    const int64_t from = i - 1, to = (end * pieces - 1) / total;  // pieces of the unit: the one with its last block
-    const int c = threadIdx.x % PER * 4, part = threadIdx.x / PER;
-    for (int r = blockIdx.y; r < rows; r += gridDim.y) {
-      float top = -INFINITY, l = 0.f;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (x == begin) return;  // it separates two units
+    const int borders = count - 1, mine = border - first - 1, tasks = rows * SETS;
+    const bool split = 2 * borders >= tasks;  // all warps on one task
+    for (int task = split ? mine : mine * kJoinWarps + warp; task < tasks; task += split ? borders : borders * kJoinWarps) {
+      const int r = task % rows, c = task / rows * COLS + lane * 4;
+      auto row_of = [&](int k) { return (2 * (int64_t)(first + k) + (cut.start(first + k) >= begin ? 0 : 1)) * kRows + r; };
+      float top = -INFINITY;
+      for (int k = lane; k < count; k += 32) top = fmaxf(top, args.part_ml[row_of(k)].x);
+      top = warp_max(top);
       float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      for (int64_t k = from + part; k <= to; k += GROUPS) {
-        const int64_t slot = 2 * k + (k * total / pieces >= begin ? 0 : 1);
-        const float2 ml = args.part_ml[slot * kRows + r];
-        const float4 y = *reinterpret_cast<const float4*>(args.part_o + (slot * kRows + r) * D + c);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float up = fmaxf(top, ml.x);
-        const float f0 = top == -INFINITY ? 0.f : ex2(top - up), f1 = ex2(ml.x - up);
-        o.x = o.x * f0 + y.x * f1, o.y = o.y * f0 + y.y * f1, o.z = o.z * f0 + y.z * f1, o.w = o.w * f0 + y.w * f1;
-        l = l * f0 + ml.y * f1;
-        top = up;
+      float l = 0.f;
+#pragma unroll 8
+      for (int k = split ? warp : 0; k < count; k += split ? kJoinWarps : 1) {
+        const float2 x = args.part_ml[row_of(k)];
+        const float4 y = lane * 4 < COLS ? *reinterpret_cast<const float4*>(args.part_o + row_of(k) * D + c) : o;
+        const float f = x.x == -INFINITY ? (x.y == 0.f ? 0.f : x.y) : ex2(x.x - top);  // (a NaN stays one)
+        l += share(x, top);
+        o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
       }
-      __syncthreads();
-      meet[threadIdx.x] = o;
-      if (c == 0) meet_ml[part] = make_float2(top, l);
-      __syncthreads();
-      if (part == 0) {
-        float best = -INFINITY;
+      if (split) {
+        __syncthreads();
+        meet[warp][lane] = o;
+        if (lane == 0) meet_l[warp] = l;
+        __syncthreads();
+        if (warp != 0) continue;
 #pragma unroll
-        for (int w = 0; w < GROUPS; ++w) best = fmaxf(best, meet_ml[w].x);
-        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-        l = 0.f;
-#pragma unroll
-        for (int w = 0; w < GROUPS; ++w) {
-          const float2 ml = meet_ml[w];
-          if (ml.x == -INFINITY && ml.y == 0.f) continue;
-          const float f = ex2(ml.x - best);
-          const float4 y = meet[w * PER + threadIdx.x];
-          sum.x += y.x * f, sum.y += y.y * f, sum.z += y.z * f, sum.w += y.w * f;
-          l += share(ml, best);
+        for (int w = 1; w < kJoinWarps; ++w) {
+          const float4 y = meet[w][lane];
+          o.x += y.x, o.y += y.y, o.z += y.z, o.w += y.w;
+          l += meet_l[w];
         }
-        const float inv = l == 0.f ? 0.f : 1.f / l;
-        const int t = s.first + (r0 + r) / group, h = kv * group + (r0 + r) % group;
-        uint2 b4;
-        b4.x = pack2(sum.x * inv, sum.y * inv), b4.y = pack2(sum.z * inv, sum.w * inv);
-        *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + c) = b4;
-        if (c == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (best + log2f(l)) * kLn2;
       }
-      __syncthreads();
+      if (lane * 4 >= COLS) continue;
+      const float inv = l == 0.f ? 0.f : 1.f / l;
+      const int t = s.first + (r0 + r) / group, h = kv * group + (r0 + r) % group;
+      uint2 b4;
+      b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
+      *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + c) = b4;
+      if (c == 0) a.lse[(int64_t)h * p.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
     }
+  } else {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
   }
 }
 
@@ -430,9 +446,9 @@ void launch_rows(const PagedAttentionArgs& a, int most_rows, void* workspace, in
   args.most_rows = most_rows;
   cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
   paged_rows_kernel<D><<<args.pieces, kThreads, C::SMEM, stream>>>(args);
-  // one block a border between two pieces and a row
+  // one block a border between two pieces
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(args.pieces - 1, std::min<int64_t>(kRows, (int64_t)a.q_heads / a.cache.heads * a.max_q));
+  cfg.gridDim = dim3(args.pieces - 1);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.stream = stream;
   cudaLaunchAttribute attr;

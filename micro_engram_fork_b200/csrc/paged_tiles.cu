@@ -430,11 +430,21 @@ __global__ void __launch_bounds__(kThreads, 1)
           const int id = __shfl_sync(0xffffffffu, ids, (kb - u.kb0) % 4 * 8 + in / 16);
           tma_load_4d_pair_if(dst, map, bar, 0, y0 + ((kb * BN + in) & page_mask), x, id, one);
         } else {
-          for (int row = 0; row < 64; row += box) {
-            const int id = __shfl_sync(0xffffffffu, ids, (kb - u.kb0) % 4 * 8 + (in + row) / 16);
+          // small pages: their numbers first, so that the loads go out one after the other
+          const int at = (kb - u.kb0) % 4 * 8 + in / 16, y = y0 + ((kb * BN + in) & page_mask);
+          int id[4];
 #pragma unroll
-            for (int i = 0; i < decltype(NC)::value; ++i)
-              tma_load_4d_pair_if(dst + i * (64 * 128) + row * 128, map, bar, 0, y0 + ((kb * BN + in + row) & page_mask), x + i, id, one);
+          for (int i = 0; i < 4; ++i) id[i] = __shfl_sync(0xffffffffu, ids, at + i);
+          if (box == 32) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+              for (int c = 0; c < decltype(NC)::value; ++c) tma_load_4d_pair_if(dst + c * (64 * 128) + i * (32 * 128), map, bar, 0, y, x + c, id[2 * i], one);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+              for (int c = 0; c < decltype(NC)::value; ++c) tma_load_4d_pair_if(dst + c * (64 * 128) + i * (16 * 128), map, bar, 0, y, x + c, id[i], one);
           }
         }
       };
@@ -777,18 +787,18 @@ constexpr int kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
-  constexpr int STEPS = 2 * BM / 32;
   const PagedAttentionArgs& a = args.a;
+  const int steps = (args.slot_rows + 31) / 32;
   const int cut = cut_of<D>(args);
   if (cut == 0) return;
   Walk<D> walk(args, cut);
   Unit u;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = args.group, tokens = 2 * args.tokens;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t i = blockIdx.x; walk.at(i / STEPS, u); i += gridDim.x) {
+  for (int64_t i = blockIdx.x; walk.at(i / steps, u); i += gridDim.x) {
     if (u.chunks == 1 || u.chunk != 0) continue;
-    const int64_t x = i / STEPS, stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
-    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r = (int)(i % STEPS) * 32 + lane;
+    const int64_t x = i / steps, stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
+    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r = (int)(i % steps) * 32 + lane;
     if (r >= rows) continue;
     float top = -INFINITY, l = 0.f;
     for (int k = 0; k < u.chunks; ++k) top = fmaxf(top, args.part_ml[(x + k * stride) * args.slot_rows + r].x);
