@@ -781,46 +781,50 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// Joins the chunks of sequences that were cut: a block takes every gridDim.x-th (unit, 32 rows), its lanes a row each and its warps every
-// eighth 4 columns.
+// Joins the chunks of sequences that were cut: a block takes every gridDim.x-th (unit, 32 rows, 32 columns), its lanes a row and its warps 4
+// columns each.
 constexpr int kJoinThreads = 256;
 template <int D>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
   using C = Cfg<D>;
+  constexpr int SETS = C::DV / 32;
   const PagedAttentionArgs& a = args.a;
-  const int steps = (args.slot_rows + 31) / 32;
-  const int cut = cut_of<D>(args);
-  if (cut == 0) return;
+  const int steps = (args.slot_rows + 31) / 32, cut = cut_of<D>(args);
+  if (cut == 0) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    return;
+  }
   Walk<D> walk(args, cut);
   Unit u;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = args.group, tokens = 2 * args.tokens;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  for (int64_t i = blockIdx.x; walk.at(i / steps, u); i += gridDim.x) {
+  for (int i = blockIdx.x; walk.at(i / (steps * SETS), u); i += gridDim.x) {  // (units are few where any is cut)
     if (u.chunks == 1 || u.chunk != 0) continue;
-    const int64_t x = i / steps, stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
-    const int i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r = (int)(i % steps) * 32 + lane;
+    const int64_t x = i / (steps * SETS), stride = (int64_t)a.cache.heads * C::HALVES;  // between a tile's chunks
+    const int set = i % SETS, i0 = u.tile * tokens, rows = min(tokens, u.s.count - i0) * group, r = i / SETS % steps * 32 + lane;
     if (r >= rows) continue;
+    const float2* mls = args.part_ml + x * args.slot_rows + r;
+    const int64_t ml_step = stride * args.slot_rows;
     float top = -INFINITY, l = 0.f;
-    for (int k = 0; k < u.chunks; ++k) top = fmaxf(top, args.part_ml[(x + k * stride) * args.slot_rows + r].x);
-    for (int k = 0; k < u.chunks; ++k) l += share(args.part_ml[(x + k * stride) * args.slot_rows + r], top);
+#pragma unroll 8
+    for (int k = 0; k < u.chunks; ++k) top = fmaxf(top, mls[k * ml_step].x);
+    const int c = set * 8 + warp;  // of the columns, 4 at a time
+    const float4* parts = args.part_o + (x * (C::DV / 4) + c) * args.slot_rows + r;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+    for (int k = 0; k < u.chunks; ++k) {
+      const float2 ml = mls[k * ml_step];
+      const float4 y = parts[k * ml_step * (C::DV / 4)];
+      const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2(ml.x - top);  // (a NaN stays one)
+      l += share(ml, top);
+      o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
+    }
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const int t = u.s.first + i0 + r / group, h = u.kv * group + r % group;
-    bf16* out = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV;
-    for (int c = warp; c < C::DV / 4; c += kJoinThreads / 32) {
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-      for (int k = 0; k < u.chunks; ++k) {
-        const int64_t slot = x + k * stride;
-        const float2 ml = args.part_ml[slot * args.slot_rows + r];
-        const float4 y = args.part_o[(slot * (C::DV / 4) + c) * args.slot_rows + r];
-        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : ml.y) : ex2(ml.x - top);  // (a NaN stays one)
-        o.x += y.x * f, o.y += y.y * f, o.z += y.z * f, o.w += y.w * f;
-      }
-      uint2 b4;
-      b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
-      *reinterpret_cast<uint2*>(out + c * 4) = b4;
-    }
-    if (warp == 0 && u.half == 0) a.lse[(int64_t)h * a.batch.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
+    uint2 b4;
+    b4.x = pack2(o.x * inv, o.y * inv), b4.y = pack2(o.z * inv, o.w * inv);
+    *reinterpret_cast<uint2*>(reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head + u.half * C::DV + c * 4) = b4;
+    if (c == 0 && u.half == 0) a.lse[(int64_t)h * a.batch.tokens + t] = l == 0.f ? -INFINITY : (top + log2f(l)) * kLn2;
   }
 }
 
