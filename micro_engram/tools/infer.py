@@ -1,13 +1,14 @@
 """Generation with HF transformers plus trained engram(s) (reference: infer_engram.py:90-334).
 
     python -m micro_engram.tools.infer --model MERGED_DIR --prompt "Hello"
-    python -m micro_engram.tools.infer --model BASE_DIR --engram-pt micro_engram.pt --prompt "Hello" [--no-engram]
+    python -m micro_engram.tools.infer --model BASE_DIR --engram-pt micro_engram.pt --prompt "Hello" [--no-engram] [--native]
 
 Settings are resolved per key as: explicit flag > engram config > what the saved tensors
 show (table count / shape, gate parameters) > defaults. A config listing several engrams
 loads each from its own "weights" by layer. On a GPU the engram runs on the sm_100a kernels
 (native hash and fused gate); the history of the current generation is kept, and only the
-tail that new positions' n-grams can reach is hashed each step.
+tail that new positions' n-grams can reach is hashed each step. --native generates with the framework's own
+decoder on its paged cache (micro_engram_fork_b200/models/generate.py) instead of HF's.
 """
 import argparse
 import glob
@@ -190,8 +191,8 @@ class EngramSession:
         return engram.inject(hidden, [i[:, -T:] for i in engram.hash_ids(reach)])
 
 
-def attach_planned(plans, model):
-    """Build every planned engram for `model`, check it against its tensors, attach them."""
+def planned_engrams(plans, model):
+    """[(engram, layer)]: every planned engram built for `model` and checked against its tensors."""
     text_cfg = getattr(model.config, "text_config", model.config)
     pad = getattr(text_cfg, "pad_token_id", None)
     attached = []
@@ -212,7 +213,12 @@ def attach_planned(plans, model):
         print(f"[engram] layer {s['layer']}: {len(sd)} tensors, output-weight magnitude "
               f"{out_w.float().abs().mean().item():.6f} ({engram.gate} gate; 0 = untrained or not loaded)")
         attached.append((engram, s["layer"]))
-    return EngramSession(model, attached)
+    return attached
+
+
+def attach_planned(plans, model):
+    """The planned engrams attached to an HF model."""
+    return EngramSession(model, planned_engrams(plans, model))
 
 
 def add_engram_args(ap):
@@ -224,6 +230,28 @@ def add_engram_args(ap):
     ap.add_argument("--dim", type=int, default=None)
     ap.add_argument("--heads", type=int, default=None)
     ap.add_argument("--gate", choices=MicroEngram.GATES, default=None)
+
+
+def load_native(args, sequences, max_len, chunk=1024):
+    """(Generator, tokenizer): the framework's own decoder on a paged cache, with the engram(s) `args` name."""
+    from transformers import AutoTokenizer
+
+    from micro_engram_fork_b200.models import gemma as G
+    from micro_engram_fork_b200.models.generate import Generator
+
+    plans = plan_engrams(args)
+    device = "cuda" if torch.cuda.is_available() else "cpu"
+    dtype = torch.bfloat16 if device == "cuda" else torch.float32
+    with torch.device("meta"):
+        model = G.GemmaForCausalLM(G.GemmaConfig.from_pretrained(args.model))
+    model = model.to_empty(device=device)
+    G.cast_projections_(model, dtype)
+    missing = G.load_hf_weights(model, args.model)
+    if missing:
+        raise SystemExit(f"{args.model} is missing weights: {missing[:8]}")
+    for engram, layer in planned_engrams(plans, model):
+        model.model.layers[layer].add_module("micro_engram", engram.to(device=device, dtype=dtype).eval())
+    return Generator(model.eval(), sequences, max_len, chunk), AutoTokenizer.from_pretrained(args.model)
 
 
 def load_model(args):
@@ -253,7 +281,21 @@ def main(argv=None):
     ap.add_argument("--max-new-tokens", type=int, default=2000)
     ap.add_argument("--temperature", type=float, default=0.8)
     ap.add_argument("--top-p", type=float, default=0.95)
+    ap.add_argument("--native", action="store_true", help="the framework's own decoder and paged cache instead of HF's")
+    ap.add_argument("--max-len", type=int, default=32768, help="--native: tokens of the prompt and the answer that the cache holds")
     args = ap.parse_args(argv)
+    if args.native:
+        gen, tok = load_native(args, 1, args.max_len)
+        gen.engrams_on = not args.no_engram
+        print(f"[engram] enabled: {gen.engrams_on}")
+        ids = _prompt_ids(tok, args.prompt, args.raw)[0].tolist()
+        room = gen.cache.max_len + 1 - len(ids)
+        if room < 1:
+            raise SystemExit(f"the prompt has {len(ids)} tokens: --max-len {len(ids) + args.max_new_tokens}")
+        answer = gen.generate([ids], min(args.max_new_tokens, room), args.temperature, args.top_p)[0]
+        print("\n--- output ---")
+        print(tok.decode(answer, skip_special_tokens=True))
+        return
     model, tok, session = load_model(args)
     session.enabled = not args.no_engram
     print(f"[engram] enabled: {session.enabled}")

@@ -17,6 +17,7 @@ Execution:
          the layer input (which the trainer's offload hooks can move to pinned host memory)
          and recomputes the layer in the backward.
   CPU    the same math in plain PyTorch autograd (oracle, gloo tests).
+  `forward_cached` runs a layer for new tokens of sequences in a paged cache (models/generate.py).
 The q/k/v and gate/up projections are stored fused; the HF-named Linear weights are views
 into the fused buffers, so loading an HF state dict fills them in place.
 """
@@ -30,6 +31,7 @@ import torch.nn.functional as F
 
 from ..ops import use_native
 from ..ops import norm as N
+from ..ops import paged
 from ..ops.attention import attention_torch, doc_starts
 from ..ops.linear import dgeglu_linear, geglu_linear, linear, linear_t
 
@@ -273,6 +275,27 @@ class GemmaLayer(nn.Module):
             return checkpoint(self._forward_torch, x, pos, doc_start, use_reentrant=False)
         return self._forward_torch(x, pos, doc_start)
 
+    @torch.no_grad()
+    def forward_cached(self, x, k_pages, v_pages, block_table, cu_seqlens, seq_lens, max_q=None):
+        """The layer for new tokens x [T, d] of sequences in a paged cache (ops/paged.py), which are appended to it."""
+        args = (k_pages, v_pages, block_table, cu_seqlens, seq_lens)
+        cfg, att = self.cfg, self.self_attn
+        eps = cfg.rms_norm_eps
+        _materialize(self, force=not use_native(x))
+        norms = (att.q_norm.weight, att.k_norm.weight, self.inv_freq)
+        if not use_native(x):
+            qkv = F.linear(self._norm(x, self.input_layernorm), self.qkv_weight)
+            q = paged.qkv_norm_rope_append(qkv, *norms, *args, self.n_q, self.kv_eq, eps)
+            a, _ = paged.paged_attention(q, *args, window=self.window)
+            return self._mlp_torch(x + self._norm(F.linear(a.flatten(1), att.o_proj.weight), self.post_attention_layernorm))
+        h, _ = N.rmsnorm(x, self.input_layernorm.weight, eps)
+        q = paged.qkv_norm_rope_append(_proj(self, "qkv", h), *norms, *args, self.n_q, self.kv_eq, eps)
+        a, _ = paged.paged_attention(q, *args, window=self.window, max_q=max_q)
+        o = _proj(self, "o", a.flatten(1))
+        x, h, _, _ = N.post_norm_add(x, o, self.post_attention_layernorm.weight, None, self.pre_feedforward_layernorm.weight, eps)
+        m, _ = _geglu_proj(self, h, False)
+        return N.post_norm_add(x, _proj(self, "down", m), self.post_feedforward_layernorm.weight, _ls(self), None, eps)[0]
+
     def _norm(self, x, norm, w_none=False):
         return N.rmsnorm_ref(x, None if w_none else norm.weight, self.cfg.rms_norm_eps)
 
@@ -291,7 +314,9 @@ class GemmaLayer(nn.Module):
         v = N.rmsnorm_ref(v, None, cfg.rms_norm_eps)
         a = attention_torch(q, k_n, v, doc_start, self.window, 1.0).reshape(T, -1)
         o = F.linear(a, att.o_proj.weight)
-        x = x + self._norm(o, self.post_attention_layernorm)
+        return self._mlp_torch(x + self._norm(o, self.post_attention_layernorm))
+
+    def _mlp_torch(self, x):
         h = self._norm(x, self.pre_feedforward_layernorm)
         gu = F.linear(h, self.gate_up_weight)
         m = N.geglu_ref(gu)
@@ -558,6 +583,9 @@ class GemmaTextModel(nn.Module):
         for layer in self.layers:
             out = layer(x, pos, ds)
             x = (out[0] if isinstance(out, tuple) else out).reshape(-1, d)  # an engram hook may add a batch dim
+        return self.final_norm(x)
+
+    def final_norm(self, x):
         if use_native(x):
             return _FinalNorm.apply(x, self.norm.weight, self.config.rms_norm_eps)
         return N.rmsnorm_ref(x, self.norm.weight, self.config.rms_norm_eps)

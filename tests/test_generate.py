@@ -1,0 +1,187 @@
+"""Generation with the native decoder on its paged cache, on CPU: the same hidden states and answers as whole forward passes."""
+import json
+import math
+
+import pytest
+import torch
+
+from micro_engram.module import MicroEngram, attach_engram
+from micro_engram_fork_b200.models import gemma as G
+from micro_engram_fork_b200.models.generate import Generator
+
+
+def small_model(device="cpu", dtype=torch.float32, engram=True, seed=0, **kw):
+    cfg = G.tiny_config(vocab_size=256, hidden_size=128, intermediate_size=256, sliding_window=20, **kw)
+    model = G.GemmaForCausalLM(cfg).to(device)
+    G.cast_projections_(model, dtype)
+    G.init_random_(model, seed=seed, std=0.08)
+    g = torch.Generator().manual_seed(seed)
+    for layer in model.model.layers:  # scores as trained norm weights leave them
+        layer.self_attn.q_norm.weight.copy_(0.3 + 0.1 * torch.rand(layer.head_dim, generator=g))
+        layer.self_attn.k_norm.weight.copy_(0.3 + 0.1 * torch.rand(layer.head_dim, generator=g))
+        layer.layer_scalar.fill_(0.8)
+    eng = None
+    if engram:
+        eng = MicroEngram(model_dim=128, vocab_size=256, table_size=97, engram_dim=16, num_heads=2, gate="scalar_sqrt", seed=3)
+        with torch.no_grad():
+            for p in eng.parameters():
+                p.copy_(torch.randn(p.shape, generator=g) * 0.2)
+        eng.eval()
+    return model, eng
+
+
+def whole_forward(model, eng, ids, layer=1):
+    """Final hidden states of one sequence by the decoder's forward pass over all of it, the engram by its hook."""
+    ids = torch.tensor([ids], device=model.model.embed_tokens.weight.device)
+    handles = []
+    if eng is not None:
+        _, handles = attach_engram(model, eng, layer, get_ids=lambda: (ids, None))
+    w = model.model.embed_tokens.weight
+    x = (w[ids[0]] * torch.tensor(model.model.embed_scale, dtype=w.dtype)).to(w.dtype)
+    with torch.no_grad():
+        h = model.model(x, torch.arange(ids.shape[1], device=x.device))
+    for handle in handles:
+        handle.remove()
+    return h
+
+
+PROMPTS = [[(7 * i * i + 3) % 256 for i in range(n)] for n in (70, 1, 33)]
+
+
+@pytest.mark.parametrize("engram", [False, True])
+@pytest.mark.parametrize("chunk", [16, 100])
+def test_extend_matches_whole_forward(chunk, engram):
+    model, eng = small_model(engram=engram)
+    want = [whole_forward(model, eng, p) for p in PROMPTS]
+    gen = Generator(model, 3, 90, chunk=chunk, page=16)
+    rest, got = [list(p) for p in PROMPTS], [[], [], []]
+    while any(rest):
+        now = [r[:chunk - 3 * b] for b, r in enumerate(rest)]
+        h, at = gen.extend(now), 0
+        for b, n in enumerate(now):
+            got[b].append(h[at:at + len(n)])
+            at += len(n)
+        rest = [r[len(n):] for r, n in zip(rest, now)]
+    for a, b in zip(got, want):
+        a = torch.cat(a)
+        assert float((a - b).abs().max()) <= 1e-4 * float(b.abs().max())
+    assert gen.lens == [70, 1, 33]
+
+
+def test_generate_matches_whole_forward():
+    """Greedy answers, token by token, past the window and round the sliding layers' rings."""
+    model, eng = small_model()
+    model.config.eos_token_id = None
+    model.model.layers[1].add_module("micro_engram", eng)
+    gen = Generator(model, 4, 120, chunk=16, page=16)
+    answers = gen.generate(PROMPTS, 40)
+    del model.model.layers[1].micro_engram
+    cap = model.config.final_logit_softcapping
+    for prompt, answer in zip(PROMPTS, answers):
+        assert len(answer) == 40
+        h = whole_forward(model, eng, prompt + answer)
+        if hasattr(model.model.layers[1], "micro_engram"):
+            del model.model.layers[1].micro_engram
+        z = (h @ model.model.embed_tokens.weight.t()).double()
+        z = cap * torch.tanh(z / cap)
+        for i, t in enumerate(answer):  # the likeliest, up to what the two ways differ by
+            row = z[len(prompt) - 1 + i]
+            assert float(row.max() - row[t]) <= 1e-3
+
+
+def test_generate_stops_and_samples():
+    model, _ = small_model(engram=False)
+    gen = Generator(model, 2, 100, chunk=32, page=16)
+    first = gen.generate(PROMPTS[:2], 20, eos=-1)
+    stop = first[0][3]
+    cut = gen.generate(PROMPTS[:2], 20, eos=stop)
+    assert cut[0] == first[0][:first[0].index(stop) + 1]
+    g = lambda: torch.Generator().manual_seed(5)  # noqa: E731
+    a = gen.generate(PROMPTS[:2], 20, temperature=1.5, top_p=0.9, eos=-1, generator=g())
+    assert a == gen.generate(PROMPTS[:2], 20, temperature=1.5, top_p=0.9, eos=-1, generator=g())
+    assert gen.generate(PROMPTS[:2], 20, temperature=1.5, top_p=1e-9, eos=-1, generator=g()) == first
+    assert gen.generate(PROMPTS[:2], 20, temperature=1.5, top_k=1, eos=-1, generator=g()) == first
+
+
+def test_sampling_follows_the_probabilities():
+    model, _ = small_model(engram=False)
+    gen = Generator(model, 1, 20, chunk=16, page=16)
+    h = gen.extend([[5, 9, 11]])[-1:]
+    z = (h @ model.model.embed_tokens.weight.t()).double()[0]
+    cap = model.config.final_logit_softcapping
+    p = torch.softmax(cap * torch.tanh(z / cap) / 0.7, 0)
+    order = p.sort(descending=True)
+    keep = order.values.cumsum(0) - order.values < 0.8
+    want = torch.zeros(256, dtype=torch.float64)
+    want[order.indices[keep]] = order.values[keep] / order.values[keep].sum()
+    n = 20000
+    drawn = gen.next_tokens(h.expand(n, -1), 0.7, 0.8, generator=torch.Generator().manual_seed(1))
+    got = torch.bincount(drawn, minlength=256).double() / n
+    assert float((got - want).abs().max()) <= 5 * math.sqrt(0.25 / n) and bool((got[want == 0] == 0).all())
+
+
+def test_refusals():
+    model, _ = small_model(engram=False)
+    with pytest.raises(ValueError):
+        Generator(model, 0, 10)
+    with pytest.raises(ValueError):
+        Generator(model, 1, 10, page=24)
+    gen = Generator(model, 2, 40, chunk=16, page=16)
+    for call in (lambda: gen.extend([[1]]), lambda: gen.extend([[1] * 17, []]), lambda: gen.generate([], 3), lambda: gen.generate([[1], []], 3),
+                 lambda: gen.generate([[1]] * 3, 3), lambda: gen.generate([[1] * 30], 12)):
+        with pytest.raises(ValueError):
+            call()
+    gen.extend([[1] * 16, []])
+    gen.extend([[1] * 16, []])
+    with pytest.raises(ValueError):
+        gen.extend([[1] * 9, []])
+    assert gen.extend([[], []]).shape == (0, 128)
+
+
+def test_sliding_layers_keep_a_ring():
+    model, _ = small_model(engram=False)
+    gen = Generator(model, 2, 2000, chunk=16, page=16)
+    full, ring = gen.cache.layers[3][0].shape[0], gen.cache.layers[0][0].shape[0]
+    assert full == 2 * 125 and ring == 2 * 4  # 20 + 16 - 1 positions lie in 4 pages at most
+
+
+def test_infer_native(tmp_path, monkeypatch, capsys):
+    """The inference tool's --native path: folder -> decoder, engram, cache -> text."""
+    from safetensors.torch import save_file
+
+    from micro_engram.tools import infer
+
+    model, eng = small_model()
+    conf = model.config.to_dict()
+    conf.update({"model_type": "gemma4_text", "eos_token_id": None})
+    (tmp_path / "config.json").write_text(json.dumps(conf))
+    save_file({k: v.clone().contiguous() for k, v in model.state_dict().items()}, str(tmp_path / "model.safetensors"))
+    torch.save(eng.state_dict(), tmp_path / "engram.pt")
+
+    class Tok:
+        def __call__(self, text, return_tensors=None):
+            return type("E", (), {"input_ids": torch.tensor([[ord(c) for c in text]])})
+
+        def decode(self, ids, skip_special_tokens=False):
+            return " ".join(map(str, ids))
+
+    import transformers
+
+    monkeypatch.setattr(transformers.AutoTokenizer, "from_pretrained", lambda *a, **k: Tok())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    args = ["--model", str(tmp_path), "--engram-pt", str(tmp_path / "engram.pt"), "--layer", "1", "--heads", "2", "--prompt", "hello",
+            "--max-new-tokens", "6", "--temperature", "0", "--native", "--max-len", "64"]
+    from unittest import mock
+
+    with mock.patch.dict(infer.DEFAULTS, {"seed": 3}):
+        infer.main(args)
+        with_engram = capsys.readouterr().out.rsplit("--- output ---\n", 1)[1].split()
+        infer.main([*args, "--no-engram"])
+        without = capsys.readouterr().out.rsplit("--- output ---\n", 1)[1].split()
+        with pytest.raises(SystemExit):
+            infer.main([*args[:-1], "3"])
+    model.config.eos_token_id = None
+    gen = Generator(model, 1, 64)
+    assert list(map(str, gen.generate([[ord(c) for c in "hello"]], 6)[0])) == without
+    model.model.layers[1].add_module("micro_engram", eng)
+    assert list(map(str, gen.generate([[ord(c) for c in "hello"]], 6)[0])) == with_engram
