@@ -462,13 +462,15 @@ void launch_rows(const PagedAttentionArgs& a, int most_rows, void* workspace, in
 // Which kernel takes which sequence: up to kFewRows rows this file's, which reads a sequence's keys once for every 8 of them; more
 // the tensor cores'.
 constexpr int kFewRows = 16;
-// A batch of this many sequences may hold single tokens beside chunks; below, the tensor cores' kernel takes them all.
-constexpr int kMixed = 4;
+// With this many rows a sequence on average (or very few sequences) the tensor cores' kernel takes all of them: single tokens among them cost it a
+// little more than they cost this one, and the two launches are saved.
+constexpr int kMeanRows = 32, kFewSequences = 4;
 
 enum Which { kRowsOnly, kTilesOnly, kBoth };
 Which which(const PagedAttentionArgs& a) {
-  if ((int64_t)a.max_q * (a.q_heads / a.cache.heads) <= kFewRows) return kRowsOnly;
-  return a.batch.seqs < kMixed ? kTilesOnly : kBoth;
+  const int64_t group = a.q_heads / a.cache.heads;
+  if (a.max_q * group <= kFewRows) return kRowsOnly;
+  return a.batch.seqs < kFewSequences || a.batch.tokens * group >= (int64_t)kMeanRows * a.batch.seqs ? kTilesOnly : kBoth;
 }
 
 }  // namespace

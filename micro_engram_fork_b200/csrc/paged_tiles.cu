@@ -44,18 +44,22 @@ constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
 constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
 constexpr int kDeals = 4;             // units a pair that cutting aims at
 
-template <int D>
+// QR: rows of Q an SM. 64 of them serve calls whose chunks are short (drafts): the product's other 64 rows are then what lies behind,
+// and nobody looks at them; what Q leaves goes to the rings, which such calls need most, for they wait for memory.
+template <int D, int QR>
 struct Cfg {
+  static constexpr int ROWS = QR;
   static constexpr int DV = D < 256 ? D : 256;       // columns of O a unit
   static constexpr int HALVES = D / DV;
   static constexpr int NV = D == 64 ? 128 : DV;      // columns of the P V product (dim 64: the odd SM's half is past the row, zeros)
   static constexpr int VC = NV / 2;                  // of them in this SM
-  static constexpr int Q_BYTES = BM * D * 2;
+  static constexpr int Q_BYTES = QR * D * 2;
   // a stage of K: this SM's 64 keys of a block x KC columns; of V: 128 keys x VC, one set of 64 keys after the other. (Stages of 16 KB, twice
   // as many: 10% slower, for a stage costs its loader and the products' warp some hundred clocks.)
   static constexpr int KC = D < 256 ? D : 256, K_STAGES = D / KC;
   static constexpr int K_BYTES = 64 * KC * 2, V_BYTES = BN * VC * 2;
-  static constexpr int KR = D == 512 ? 2 : D == 256 ? 3 : 6, VR = D == 512 ? 1 : D == 256 ? 2 : 6;  // stages
+  static constexpr int KR = D == 512 ? (QR == 64 ? 3 : 2) : D == 256 ? (QR == 64 ? 4 : 3) : 6;
+  static constexpr int VR = D == 512 ? (QR == 64 ? 2 : 1) : D == 256 ? 2 : 6;  // stages
   static constexpr int K_OFF = Q_BYTES, V_OFF = K_OFF + KR * K_BYTES, BAR_OFF = V_OFF + VR * V_BYTES;
   static constexpr int SMEM = BAR_OFF + 640;
   static_assert(SMEM <= 232448, "shared memory");
@@ -81,7 +85,7 @@ struct UnitsOf {
   int tiles, chunks, per;  // tiles of rows, chunks of keys, blocks of a chunk
   int first, blocks;       // the sequence's blocks of keys
 };
-template <int D>
+template <int D, int QR>
 ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut) {
   const PagedAttentionArgs& a = t.a;
   const int group = t.group, tokens = 2 * t.tokens;
@@ -91,7 +95,7 @@ ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut
   u.tiles = (s.count + tokens - 1) / tokens;
   u.first = k.lo / BN;
   u.blocks = max((k.hi + BN - 1) / BN - u.first, 1);
-  const bool whole = cut <= 0 || (t.slot_rows < 2 * BM && (int64_t)s.count * group > t.slot_rows);
+  const bool whole = cut <= 0 || (t.slot_rows < 2 * QR && (int64_t)s.count * group > t.slot_rows);
   u.chunks = whole ? 1 : (u.blocks + cut - 1) / cut;
   u.per = (u.blocks + u.chunks - 1) / u.chunks;
   return u;
@@ -100,14 +104,14 @@ ME_DEVICE UnitsOf units_of(const TilesArgs& t, int b, const Sequence& s, int cut
 // Blocks a chunk, 0: no cutting. By a whole warp. Uncut, the last pair is done about after the mean of the blocks and, where units
 // differ, most of the longest one; cut to about kDeals units a pair, after 1.15 times the mean and what four blocks take for the parts.
 // At most 2 kDeals units a pair come of it: as many as there were (fewer than kDeals) and one for every `cut` blocks.
-template <int D>
+template <int D, int QR>
 ME_DEVICE int cut_of(const TilesArgs& t) {
   const PagedBatch& p = t.a.batch;
   int64_t units = 0, blocks = 0;
   int most = 0;
 #pragma unroll 4
   for (int b = threadIdx.x & 31; b < p.seqs; b += 32) {
-    const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), 0);
+    const UnitsOf u = units_of<D, QR>(t, b, sequence_of(p, b), 0);
     units += u.tiles, blocks += (int64_t)u.tiles * u.blocks;
     most = max(most, u.blocks);
   }
@@ -117,7 +121,7 @@ ME_DEVICE int cut_of(const TilesArgs& t) {
     blocks += __shfl_xor_sync(0xffffffffu, blocks, o);
   }
   most = __reduce_max_sync(0xffffffffu, most);
-  const int each = t.a.cache.heads * Cfg<D>::HALVES, aim = kDeals * t.pairs;
+  const int each = t.a.cache.heads * Cfg<D, QR>::HALVES, aim = kDeals * t.pairs;
   units *= each, blocks *= each;
   if (units == 0 || units >= aim) return 0;
   const float mean = (float)blocks / t.pairs;
@@ -134,7 +138,7 @@ struct Unit {
 };
 
 // A warp's way along the units: 32 sequences at a time, a lane each.
-template <int D>
+template <int D, int QR>
 struct Walk {
   const TilesArgs& t;
   int cut, c = 0;
@@ -146,8 +150,8 @@ struct Walk {
     const int lane = threadIdx.x & 31, b = c + lane;
     mine = 0;
     if (b < p.seqs) {
-      const UnitsOf u = units_of<D>(t, b, sequence_of(p, b), cut);
-      mine = (int64_t)u.tiles * u.chunks * t.a.cache.heads * Cfg<D>::HALVES;
+      const UnitsOf u = units_of<D, QR>(t, b, sequence_of(p, b), cut);
+      mine = (int64_t)u.tiles * u.chunks * t.a.cache.heads * Cfg<D, QR>::HALVES;
     }
     upto = mine;
 #pragma unroll
@@ -171,9 +175,9 @@ struct Walk {
     const PagedAttentionArgs& a = t.a;
     out.b = c + src;
     out.s = sequence_of(a.batch, out.b);
-    const UnitsOf u = units_of<D>(t, out.b, out.s, cut);
+    const UnitsOf u = units_of<D, QR>(t, out.b, out.s, cut);
     unsigned i = (unsigned)(x - before);  // (a sequence's units: the host checks that they fit)
-    out.half = i % Cfg<D>::HALVES, i /= Cfg<D>::HALVES;
+    out.half = i % Cfg<D, QR>::HALVES, i /= Cfg<D, QR>::HALVES;
     out.kv = i % a.cache.heads, i /= a.cache.heads;
     out.chunk = i % u.chunks, out.chunks = u.chunks, i /= u.chunks;
     out.tile = u.tiles - 1 - (int)i;  // the last rows see the most keys
@@ -298,11 +302,11 @@ ME_DEVICE void st_global32(void* p, const uint32_t* v) {
 }
 
 // ------------------------------------------------------------------------------- the kernel
-template <int D>
+template <int D, int QR>
 __global__ void __launch_bounds__(kThreads, 1)
     paged_tiles_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv,
                        const __grid_constant__ TilesArgs args) {
-  using C = Cfg<D>;
+  using C = Cfg<D, QR>;
   constexpr int KR = C::KR, VR = C::VR;
   extern __shared__ __align__(1024) uint8_t smem[];  // (no room to align it here: there is no other shared memory)
   uint8_t *sQ = smem, *sK = smem + C::K_OFF, *sV = smem + C::V_OFF;
@@ -472,7 +476,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             __syncwarp();
 #pragma unroll
             for (int c = 0; c < D / 64; ++c)
-              tma_load_3d_pair_if(aQ + c * (BM * 128), &tq, q_leader, c * 64, u.kv * group, u.s.first + u.tile * 2 * tokens + (int)rank * tokens, one);
+              tma_load_3d_pair_if(aQ + c * (C::ROWS * 128), &tq, q_leader, c * 64, u.kv * group, u.s.first + u.tile * 2 * tokens + (int)rank * tokens, one);
           }
         } else {
           const bool stale = has_stale(seq, kb);
@@ -523,12 +527,12 @@ __global__ void __launch_bounds__(kThreads, 1)
               wait(&k_full[kst], kphase, 63);
               if (!ok) break;
               tc_fence_after();
-              const uint32_t dk = dK + (kst * C::K_BYTES >> 4), dq = dQ + (c * (C::KC / 64) * (BM * 128) >> 4);
+              const uint32_t dk = dK + (kst * C::K_BYTES >> 4), dq = dQ + (c * (C::KC / 64) * (C::ROWS * 128) >> 4);
 #pragma unroll
               for (int k4 = 0; k4 < C::KC / 64; ++k4)
 #pragma unroll
                 for (int kk = 0; kk < 4; ++kk)
-                  umma_bf16_pair_if(to, dq + ((k4 * (BM * 128) + kk * 32) >> 4), dk + ((k4 * (64 * 128) + kk * 32) >> 4), hi, id_s, (c | k4 | kk) != 0, one);
+                  umma_bf16_pair_if(to, dq + ((k4 * (C::ROWS * 128) + kk * 32) >> 4), dk + ((k4 * (64 * 128) + kk * 32) >> 4), hi, id_s, (c | k4 | kk) != 0, one);
               umma_commit_pair_if(&k_empty[kst], one);
               if (++kst == KR) kst = 0, kphase ^= 1;
             }
@@ -569,7 +573,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == 3) {
     // ---------------------------------------------------------------- units
-    Walk<D> walk(args, cut_of<D>(args));
+    Walk<D, QR> walk(args, cut_of<D, QR>(args));
     Unit w = {};
     bool more = true;
     for (int it = 0; more; ++it) {
@@ -784,17 +788,17 @@ __global__ void __launch_bounds__(kThreads, 1)
 // Joins the chunks of sequences that were cut: a block takes every gridDim.x-th (unit, 32 rows, 32 columns), its lanes a row and its warps 4
 // columns each.
 constexpr int kJoinThreads = 256;
-template <int D>
+template <int D, int QR>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_tiles_kernel(const __grid_constant__ TilesArgs args) {
-  using C = Cfg<D>;
+  using C = Cfg<D, QR>;
   constexpr int SETS = C::DV / 32;
   const PagedAttentionArgs& a = args.a;
-  const int steps = (args.slot_rows + 31) / 32, cut = cut_of<D>(args);
+  const int steps = (args.slot_rows + 31) / 32, cut = cut_of<D, QR>(args);
   if (cut == 0) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     return;
   }
-  Walk<D> walk(args, cut);
+  Walk<D, QR> walk(args, cut);
   Unit u;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = args.group, tokens = 2 * args.tokens;
   asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -850,7 +854,7 @@ bool make_map(CUtensorMap* map, const void* ptr, const int64_t (&dim)[N], const 
                      CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D>
+template <int D, int QR>
 int resident_pairs() {
   static std::mutex mu;
   static std::unordered_map<int, int> known;
@@ -859,7 +863,7 @@ int resident_pairs() {
   std::lock_guard<std::mutex> lk(mu);
   auto it = known.find(dev);
   if (it != known.end()) return it->second;
-  cudaFuncSetAttribute(paged_tiles_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D>::SMEM);
+  cudaFuncSetAttribute(paged_tiles_kernel<D, QR>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<D, QR>::SMEM);
   int sms = 0, n = 0;
   cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
   cudaLaunchConfig_t cfg = {};
@@ -868,36 +872,36 @@ int resident_pairs() {
   attr.val.clusterDim.x = 2, attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cfg.gridDim = dim3(sms & ~1);
   cfg.blockDim = dim3(kThreads);
-  cfg.dynamicSmemBytes = Cfg<D>::SMEM;
+  cfg.dynamicSmemBytes = Cfg<D, QR>::SMEM;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  if (cudaOccupancyMaxActiveClusters(&n, paged_tiles_kernel<D>, &cfg) != cudaSuccess || n <= 0) {
+  if (cudaOccupancyMaxActiveClusters(&n, paged_tiles_kernel<D, QR>, &cfg) != cudaSuccess || n <= 0) {
     (void)cudaGetLastError();
     n = sms / 2;
   }
   return known[dev] = n;
 }
 
-template <int D>
+template <int D, int QR>
 int slot_rows_of(const PagedAttentionArgs& a) {
-  return (int)std::min<int64_t>(2 * BM, ((int64_t)a.max_q * (a.q_heads / a.cache.heads) + 7) / 8 * 8);
+  return (int)std::min<int64_t>(2 * QR, ((int64_t)a.max_q * (a.q_heads / a.cache.heads) + 7) / 8 * 8);
 }
-template <int D>
+template <int D, int QR>
 int64_t workspace(const PagedAttentionArgs& a) {
-  return (int64_t)2 * kDeals * resident_pairs<D>() * slot_rows_of<D>(a) * (Cfg<D>::DV + 2) * 4;
+  return (int64_t)2 * kDeals * resident_pairs<D, QR>() * slot_rows_of<D, QR>(a) * (Cfg<D, QR>::DV + 2) * 4;
 }
 
-template <int D>
+template <int D, int QR>
 const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, QR>;
   if (encode_fn() == nullptr) return "cuTensorMapEncodeTiled is unavailable";
   TilesArgs args;
   args.a = a;
-  args.pairs = resident_pairs<D>();
-  args.slot_rows = slot_rows_of<D>(a);
+  args.pairs = resident_pairs<D, QR>();
+  args.slot_rows = slot_rows_of<D, QR>(a);
   args.part_o = static_cast<float4*>(space);
   args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * kDeals * args.pairs * args.slot_rows * (C::DV / 4));
-  args.group = a.q_heads / a.cache.heads, args.tokens = BM / args.group;
+  args.group = a.q_heads / a.cache.heads, args.tokens = QR / args.group;
   args.plog = 0;
   while ((1 << args.plog) < a.cache.page) ++args.plog;
   args.least_rows = least_rows;
@@ -921,14 +925,14 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D>, tq, tk, tv, args);
+  cudaError_t e = cudaLaunchKernelEx(&cfg, paged_tiles_kernel<D, QR>, tq, tk, tv, args);
   if (e != cudaSuccess) return cudaGetErrorString(e);
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
   cfg.gridDim = dim3(8 * args.pairs);
   cfg.blockDim = dim3(kJoinThreads);
   cfg.dynamicSmemBytes = 0;
-  e = cudaLaunchKernelEx(&cfg, paged_join_tiles_kernel<D>, args);
+  e = cudaLaunchKernelEx(&cfg, paged_join_tiles_kernel<D, QR>, args);
   return e == cudaSuccess ? nullptr : cudaGetErrorString(e);
 }
 
@@ -941,22 +945,31 @@ int paged_status(int* detail) {
   return word[0];
 }
 
-int64_t paged_tiles_workspace(const PagedAttentionArgs& a) {
+namespace {
+// Short chunks: a tile of 64 rows an SM holds them all. (Sharper: with more than 64 query heads a key head a token has no room there.)
+bool few(const PagedAttentionArgs& a) {
+  const int group = a.q_heads / a.cache.heads;
+  return group <= 64 && (int64_t)a.max_q * group <= 64;
+}
+template <class F>
+auto by_shape(const PagedAttentionArgs& a, F f) {
+  using std::integral_constant;
+  auto rows = [&](auto dim) { return few(a) ? f(dim, integral_constant<int, 64>()) : f(dim, integral_constant<int, 128>()); };
   switch (a.cache.dim) {
-    case 64: return workspace<64>(a);
-    case 128: return workspace<128>(a);
-    case 256: return workspace<256>(a);
-    default: return workspace<512>(a);
+    case 64: return rows(integral_constant<int, 64>());
+    case 128: return rows(integral_constant<int, 128>());
+    case 256: return rows(integral_constant<int, 256>());
+    default: return rows(integral_constant<int, 512>());
   }
+}
+}  // namespace
+
+int64_t paged_tiles_workspace(const PagedAttentionArgs& a) {
+  return by_shape(a, [&](auto d, auto rows) { return workspace<decltype(d)::value, decltype(rows)::value>(a); });
 }
 
 const char* launch_paged_tiles(const PagedAttentionArgs& a, int least_rows, void* space, cudaStream_t stream) {
-  switch (a.cache.dim) {
-    case 64: return launch<64>(a, least_rows, space, stream);
-    case 128: return launch<128>(a, least_rows, space, stream);
-    case 256: return launch<256>(a, least_rows, space, stream);
-    default: return launch<512>(a, least_rows, space, stream);
-  }
+  return by_shape(a, [&](auto d, auto rows) { return launch<decltype(d)::value, decltype(rows)::value>(a, least_rows, space, stream); });
 }
 
 }  // namespace me
