@@ -1,7 +1,7 @@
 // Attention of new tokens over a paged cache.
 //
 // Rows (token, query head) of a sequence whose query heads share a key head read the same keys, so a unit of
-// work is (sequence, key head, 8 of those rows) over blocks of 64 keys. One new token a sequence, 2 to 8 query heads a key head: two
+// work is (sequence, key head, 8 or 16 of those rows) over blocks of 64 keys. One new token a sequence, 2 to 8 query heads a key head: two
 // products of 2 to 8 rows with each 2-byte element, far below what the tensor cores need to be busy; the keys' and values' way
 // from memory is the bound, and everything here is for keeping loads in flight:
 //
@@ -11,7 +11,7 @@
 //     dependent launch).
 //   * A warp works alone: its own 16 keys of each block, its own ring of shared memory (24 KB, cp.async, rows outside the
 //     range and pages that are none filled with zeros), its own running maximum and sum. The 4 warps meet at a unit's end.
-//   * Keys are the M side of mma.m16n8k16 and the 8 rows its N side: S^T = K Q^T, O^T += V^T P^T. The rows of S^T become the
+//   * Keys are the M side of mma.m16n8k16 and 8 rows its N side: S^T = K Q^T, O^T += V^T P^T. The rows of S^T become the
 //     B operand of the second product through movmatrix, without shared memory. P goes as two bf16 terms (its value rounded and
 //     what the rounding left, relative error 2^-17), which the idle tensor cores give for nothing: the output is as exact as its own
 //     rounding.
@@ -57,24 +57,29 @@ ME_DEVICE void mma16n8k16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // ------------------------------------------------------------------------------- few rows a key head
-constexpr int kRows = 8, kWarps = 4, kTile = 16, kBlock = kWarps * kTile, kThreads = kWarps * 32;
+constexpr int kWarps = 4, kTile = 16, kBlock = kWarps * kTile, kThreads = kWarps * 32;
 
-template <int D>
+// NT: sets of 8 rows that go through the keys together. Two of them where a sequence has more than 8 rows and its O fits the registers (up
+// to dim 256): the keys are read once and not twice (64 sequences of 5 new tokens in a sliding layer: 345 -> 222 us, 8 tokens: 239; at
+// the copy rate 165). Where no sequence has more than 8 rows one set is enough: two would cost registers and empty products.
+template <int D, int NT>
 struct Cfg {
+  static constexpr int ROWS = 8 * NT;
   static constexpr int UC = D < 256 ? D : 256;  // columns of a unit of the ring
   static constexpr int UNIT = kTile * UC * 2;
   static constexpr int PARTS = D / UC;          // units a tile of K
   static constexpr int RING = 24 * 1024 / UNIT;
   static constexpr int PITCH = D + 4;           // floats of a row where the warps meet: no bank conflicts
   static constexpr int SMEM = kWarps * RING * UNIT;
-  static_assert(kWarps * kRows * PITCH * 4 <= SMEM, "the warps meet in the ring");
+  static_assert(kWarps * ROWS * PITCH * 4 <= SMEM, "the warps meet in the ring");
   static_assert(2 * (SMEM + 2048) <= 227 * 1024, "two blocks an SM");
 };
 
 struct RowsArgs {
   PagedAttentionArgs a;
-  float* part_o;   // [slots][kRows][D]
-  float2* part_ml; // [slots][kRows] (maximum, sum)
+  float* part_o;   // [slots][rows][D]
+  float2* part_ml; // [slots][rows] (maximum, sum)
+  int rows;        // of a unit
   int pieces;      // blocks of the grid
   int plog;
   int most_rows;   // sequences with more rows are the tensor cores' (paged_tiles.cu)
@@ -89,7 +94,7 @@ ME_DEVICE UnitsOf units_of(const RowsArgs& args, int b, const Sequence& s) {
   const int group = a.q_heads / a.cache.heads;
   if (s.count == 0 || (int64_t)s.count * group > args.most_rows) return {0, 0};
   const Keys k = keys_of(a.batch, a.cache.page, s, 0, s.count - 1, a.window);
-  return {(s.count * group + kRows - 1) / kRows, max((k.hi + kBlock - 1) / kBlock - k.lo / kBlock, 1)};
+  return {(s.count * group + args.rows - 1) / args.rows, max((k.hi + kBlock - 1) / kBlock - k.lo / kBlock, 1)};
 }
 
 // The line of blocks in pieces of the same length, the first `rest` of them one longer.
@@ -111,9 +116,10 @@ struct Cut {
   }
 };
 
-template <int D>
+template <int D, int NT>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs args) {
-  using C = Cfg<D>;
+  using C = Cfg<D, NT>;
+  constexpr int kRows = C::ROWS;
   extern __shared__ __align__(128) uint8_t ring[];
   __shared__ WorkLine<kThreads>::Shared line_shared;
   __shared__ float2 warp_ml[kWarps][kRows];
@@ -159,25 +165,26 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
     const int seq_lo = keys_of(p, a.cache.page, s, 0, s.count - 1, a.window).lo;
     const int start = (seq_lo / kBlock + first_block) * kBlock + warp * kTile;  // this warp's first key; a tile a block
 
-    // this lane's two rows of S^T: their last and first keys
-    int last[2], from[2];
+    // this lane's two rows of each S^T: their last and first keys
+    int last[2 * NT], from[2 * NT];
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int r = r0 + 2 * t4 + e, pos = s.context + r / group;
+    for (int e = 0; e < 2 * NT; ++e) {
+      const int r = r0 + e / 2 * 8 + 2 * t4 + e % 2, pos = s.context + r / group;
       last[e] = r < r0 + rows ? pos : -1;
       from[e] = a.window > 0 ? pos - a.window + 1 : 0;
     }
     const int all_last = s.context + r0 / group;
     const int all_from = a.window > 0 ? s.context + (r0 + rows - 1) / group - a.window + 1 : 0;
 
-    uint32_t qf[D / 16][2];
-    {
-      const int r = r0 + g;
+    uint32_t qf[NT][D / 16][2];
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
+      const int r = r0 + n * 8 + g;
       const bf16* q = reinterpret_cast<const bf16*>(a.q) + (int64_t)(s.first + r / group) * a.q_token + (kv * group + r % group) * a.q_head + 2 * t4;
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        qf[k][0] = g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
-        qf[k][1] = g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
+        qf[n][k][0] = n * 8 + g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16) : 0u;
+        qf[n][k][1] = n * 8 + g < rows ? *reinterpret_cast<const uint32_t*>(q + k * 16 + 8) : 0u;
       }
     }
     const bf16* kbase = reinterpret_cast<const bf16*>(a.cache.k) + ((int64_t)kv * D << plog);
@@ -213,18 +220,22 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
       cp_commit();
     };
 
-    float acc[D / 16][4];
+    float acc[NT][D / 16][4];
+    float m[2 * NT], sum[2 * NT];
 #pragma unroll
-    for (int i = 0; i < D / 16; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    float m[2] = {-INFINITY, -INFINITY}, sum[2] = {0.f, 0.f};
+    for (int n = 0; n < NT; ++n) {
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+      m[2 * n] = m[2 * n + 1] = -INFINITY, sum[2 * n] = sum[2 * n + 1] = 0.f;
+    }
     const float to_log2 = a.scale * kLog2e;
 
     constexpr int UPT = 2 * C::PARTS;
 #pragma unroll
     for (int i = 0; i < C::RING; ++i) issue(i / UPT, i % UPT);
     for (int j = 0; j < blocks; ++j) {
-      float sc[2][4] = {};
-      uint32_t ph[2], pl[2];
+      float sc[NT][2][4] = {};
+      uint32_t ph[NT][2], pl[NT][2];
 #pragma unroll
       for (int part = 0; part < UPT; ++part) {
         cp_wait<C::RING - 1>();
@@ -235,47 +246,53 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
           for (int k = 0; k < C::UC / 16; ++k) {
             uint32_t f[4];
             ldsm4(f, at + (((2 * k + (lane >> 4)) ^ (l_row & 7)) << 4));
-            mma16n8k16(sc[k & 1], f, qf[part * (C::UC / 16) + k][0], qf[part * (C::UC / 16) + k][1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) mma16n8k16(sc[n][k & 1], f, qf[n][part * (C::UC / 16) + k][0], qf[n][part * (C::UC / 16) + k][1]);
           }
         } else {
           if (part == C::PARTS) {  // the scores are whole: softmax
-            const int key = start + j * kBlock + g;
-            float v[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = (sc[0][e] + sc[1][e]) * to_log2;
+            const int key0 = start + j * kBlock, key = key0 + g;
             const bool page = (there >> (j & 31)) & 1;
-            const int key0 = start + j * kBlock;
-            if (!(page && key0 >= all_from && key0 + kTile - 1 <= all_last && key0 + kTile <= keys.hi)) {
+            const bool open = page && key0 >= all_from && key0 + kTile - 1 <= all_last && key0 + kTile <= keys.hi;
 #pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int at_key = key + (e >> 1) * 8;
-                if (!page || at_key > last[e & 1] || at_key < from[e & 1] || at_key >= keys.hi) v[e] = -INFINITY;
+            for (int n = 0; n < NT; ++n) {
+              float v[4];
+#pragma unroll
+              for (int e = 0; e < 4; ++e) v[e] = (sc[n][0][e] + sc[n][1][e]) * to_log2;
+              if (!open) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const int at_key = key + (e >> 1) * 8;
+                  if (!page || at_key > last[2 * n + (e & 1)] || at_key < from[2 * n + (e & 1)] || at_key >= keys.hi) v[e] = -INFINITY;
+                }
               }
-            }
-            float mx[2] = {fmaxf(v[0], v[2]), fmaxf(v[1], v[3])};
+              float& m0 = m[2 * n];
+              float& m1 = m[2 * n + 1];
+              float mx[2] = {fmaxf(v[0], v[2]), fmaxf(v[1], v[3])};
 #pragma unroll
-            for (int o = 4; o < 32; o <<= 1) {
-              mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
-              mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
-            }
-            const bool up0 = mx[0] > m[0] + kSlack, up1 = mx[1] > m[1] + kSlack;  // -inf + slack = -inf: any score is above it
-            if (__any_sync(0xffffffffu, up0 || up1)) {
-              const float f0 = up0 ? ex2(m[0] - mx[0]) : 1.f, f1 = up1 ? ex2(m[1] - mx[1]) : 1.f;
-              if (up0) m[0] = mx[0];
-              if (up1) m[1] = mx[1];
-              sum[0] *= f0, sum[1] *= f1;
+              for (int o = 4; o < 32; o <<= 1) {
+                mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], o));
+                mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], o));
+              }
+              const bool up0 = mx[0] > m0 + kSlack, up1 = mx[1] > m1 + kSlack;  // -inf + slack = -inf: any score is above it
+              if (__any_sync(0xffffffffu, up0 || up1)) {
+                const float f0 = up0 ? ex2(m0 - mx[0]) : 1.f, f1 = up1 ? ex2(m1 - mx[1]) : 1.f;
+                if (up0) m0 = mx[0];
+                if (up1) m1 = mx[1];
+                sum[2 * n] *= f0, sum[2 * n + 1] *= f1;
 #pragma unroll
-              for (int i = 0; i < D / 16; ++i) acc[i][0] *= f0, acc[i][1] *= f1, acc[i][2] *= f0, acc[i][3] *= f1;
-            }
-            const float z0 = m[0] == -INFINITY ? 0.f : m[0], z1 = m[1] == -INFINITY ? 0.f : m[1];
-            v[0] = ex2(v[0] - z0), v[1] = ex2(v[1] - z1), v[2] = ex2(v[2] - z0), v[3] = ex2(v[3] - z1);
-            sum[0] += v[0] + v[2], sum[1] += v[1] + v[3];
+                for (int i = 0; i < D / 16; ++i) acc[n][i][0] *= f0, acc[n][i][1] *= f1, acc[n][i][2] *= f0, acc[n][i][3] *= f1;
+              }
+              const float z0 = m0 == -INFINITY ? 0.f : m0, z1 = m1 == -INFINITY ? 0.f : m1;
+              v[0] = ex2(v[0] - z0), v[1] = ex2(v[1] - z1), v[2] = ex2(v[2] - z0), v[3] = ex2(v[3] - z1);
+              sum[2 * n] += v[0] + v[2], sum[2 * n + 1] += v[1] + v[3];
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t h = pack2(v[2 * e], v[2 * e + 1]);
-              const float h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xffff0000u);
-              ph[e] = transpose8x8(h);
-              pl[e] = transpose8x8(pack2(v[2 * e] - h0, v[2 * e + 1] - h1));
+              for (int e = 0; e < 2; ++e) {
+                const uint32_t h = pack2(v[2 * e], v[2 * e + 1]);
+                const float h0 = __uint_as_float(h << 16), h1 = __uint_as_float(h & 0xffff0000u);
+                ph[n][e] = transpose8x8(h);
+                pl[n][e] = transpose8x8(pack2(v[2 * e] - h0, v[2 * e + 1] - h1));
+              }
             }
           }
           // V^T: the transposed reads give dimensions as rows
@@ -284,8 +301,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
           for (int k = 0; k < C::UC / 16; ++k) {
             uint32_t f[4];
             ldsm4_t(f, vat + (((2 * k + ((lane >> 3) & 1)) ^ (lane & 7)) << 4));
-            mma16n8k16(acc[(part - C::PARTS) * (C::UC / 16) + k], f, ph[0], ph[1]);
-            mma16n8k16(acc[(part - C::PARTS) * (C::UC / 16) + k], f, pl[0], pl[1]);
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+              mma16n8k16(acc[n][(part - C::PARTS) * (C::UC / 16) + k], f, ph[n][0], ph[n][1]);
+              mma16n8k16(acc[n][(part - C::PARTS) * (C::UC / 16) + k], f, pl[n][0], pl[n][1]);
+            }
           }
         }
         __syncwarp();
@@ -296,31 +316,29 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
 
     // ---- the four warps meet
 #pragma unroll
-    for (int o = 4; o < 32; o <<= 1) {
-      sum[0] += __shfl_xor_sync(0xffffffffu, sum[0], o);
-      sum[1] += __shfl_xor_sync(0xffffffffu, sum[1], o);
-    }
-    if (g == 0) {
-      warp_ml[warp][2 * t4] = make_float2(m[0], sum[0]);
-      warp_ml[warp][2 * t4 + 1] = make_float2(m[1], sum[1]);
+    for (int e = 0; e < 2 * NT; ++e) {
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+      if (g == 0) warp_ml[warp][e / 2 * 8 + 2 * t4 + e % 2] = make_float2(m[e], sum[e]);
     }
     cp_wait<0>();
     __syncthreads();
     float* meet = reinterpret_cast<float*>(ring);
-    {
+#pragma unroll
+    for (int n = 0; n < NT; ++n) {
       float f[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float top = -INFINITY;
 #pragma unroll
-        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][2 * t4 + e].x);
-        f[e] = m[e] == -INFINITY ? 0.f : ex2(m[e] - top);
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, warp_ml[w][n * 8 + 2 * t4 + e].x);
+        f[e] = m[2 * n + e] == -INFINITY ? 0.f : ex2(m[2 * n + e] - top);
       }
-      float* out = meet + (warp * kRows + 2 * t4) * C::PITCH + g;
+      float* out = meet + (warp * kRows + n * 8 + 2 * t4) * C::PITCH + g;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        out[i * 16] = acc[i][0] * f[0], out[C::PITCH + i * 16] = acc[i][1] * f[1];
-        out[i * 16 + 8] = acc[i][2] * f[0], out[C::PITCH + i * 16 + 8] = acc[i][3] * f[1];
+        out[i * 16] = acc[n][i][0] * f[0], out[C::PITCH + i * 16] = acc[n][i][1] * f[1];
+        out[i * 16 + 8] = acc[n][i][2] * f[0], out[C::PITCH + i * 16 + 8] = acc[n][i][3] * f[1];
       }
     }
     __syncthreads();
@@ -386,14 +404,14 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs
     const int unit = in_seq <= UINT32_MAX ? (int)((uint32_t)in_seq / (uint32_t)u.blocks) : (int)(in_seq / u.blocks);
     const int64_t begin = before + (int64_t)unit * u.blocks;
     const int first = cut.owner(begin), count = cut.owner(begin + u.blocks - 1) - first + 1;  // the unit's pieces
-    const int tile = unit % u.tiles, kv = unit / u.tiles, r0 = tile * kRows, rows = min(kRows, s.count * group - r0);
+    const int tile = unit % u.tiles, kv = unit / u.tiles, r0 = tile * args.rows, rows = min(args.rows, s.count * group - r0);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (x == begin) return;  // it separates two units
     const int borders = count - 1, mine = border - first - 1, tasks = rows * SETS;
     const bool split = 2 * borders >= tasks;  // all warps on one task
     for (int task = split ? mine : mine * kJoinWarps + warp; task < tasks; task += split ? borders : borders * kJoinWarps) {
       const int r = task % rows, c = task / rows * COLS + lane * 4;
-      auto row_of = [&](int k) { return (2 * (int64_t)(first + k) + (cut.start(first + k) >= begin ? 0 : 1)) * kRows + r; };
+      auto row_of = [&](int k) { return (2 * (int64_t)(first + k) + (cut.start(first + k) >= begin ? 0 : 1)) * args.rows + r; };
       float top = -INFINITY;
       for (int k = lane; k < count; k += 32) top = fmaxf(top, args.part_ml[row_of(k)].x);
       top = warp_max(top);
@@ -433,19 +451,20 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const RowsArgs
   }
 }
 
-template <int D>
+template <int D, int NT>
 void launch_rows(const PagedAttentionArgs& a, int most_rows, void* workspace, int sms, cudaStream_t stream) {
-  using C = Cfg<D>;
+  using C = Cfg<D, NT>;
   RowsArgs args;
   args.a = a;
   args.pieces = 2 * sms;
   args.part_o = static_cast<float*>(workspace);
-  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * args.pieces * kRows * D);
+  args.part_ml = reinterpret_cast<float2*>(args.part_o + (int64_t)2 * args.pieces * C::ROWS * D);
+  args.rows = C::ROWS;
   args.plog = 0;
   while ((1 << args.plog) < a.cache.page) ++args.plog;
   args.most_rows = most_rows;
-  cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
-  paged_rows_kernel<D><<<args.pieces, kThreads, C::SMEM, stream>>>(args);
+  cudaFuncSetAttribute(paged_rows_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+  paged_rows_kernel<D, NT><<<args.pieces, kThreads, C::SMEM, stream>>>(args);
   // one block a border between two pieces
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(args.pieces - 1);
@@ -473,10 +492,13 @@ Which which(const PagedAttentionArgs& a) {
   return a.batch.seqs < kFewSequences || a.batch.tokens * group >= (int64_t)kMeanRows * a.batch.seqs ? kTilesOnly : kBoth;
 }
 
+// Sets of 8 rows a unit (see Cfg).
+int sets_of(const PagedAttentionArgs& a) { return a.cache.dim <= 256 && (int64_t)a.max_q * (a.q_heads / a.cache.heads) > 8 ? 2 : 1; }
+
 }  // namespace
 
 int64_t paged_attention_workspace(const PagedAttentionArgs& a, int sms) {
-  const int64_t rows = (int64_t)2 * 2 * sms * kRows * (a.cache.dim + 2) * 4;
+  const int64_t rows = (int64_t)2 * 2 * sms * 8 * sets_of(a) * (a.cache.dim + 2) * 4;
   const Which w = which(a);
   return w == kRowsOnly ? rows : w == kTilesOnly ? paged_tiles_workspace(a) : std::max(rows, paged_tiles_workspace(a));
 }
@@ -485,11 +507,12 @@ const char* launch_paged_attention(const PagedAttentionArgs& a, void* workspace,
   const Which w = which(a);
   if (w != kTilesOnly) {
     const int most = w == kRowsOnly ? INT32_MAX : kFewRows;
+    const bool two = sets_of(a) == 2;
     switch (a.cache.dim) {
-      case 64: launch_rows<64>(a, most, workspace, sms, stream); break;
-      case 128: launch_rows<128>(a, most, workspace, sms, stream); break;
-      case 256: launch_rows<256>(a, most, workspace, sms, stream); break;
-      default: launch_rows<512>(a, most, workspace, sms, stream);
+      case 64: two ? launch_rows<64, 2>(a, most, workspace, sms, stream) : launch_rows<64, 1>(a, most, workspace, sms, stream); break;
+      case 128: two ? launch_rows<128, 2>(a, most, workspace, sms, stream) : launch_rows<128, 1>(a, most, workspace, sms, stream); break;
+      case 256: two ? launch_rows<256, 2>(a, most, workspace, sms, stream) : launch_rows<256, 1>(a, most, workspace, sms, stream); break;
+      default: launch_rows<512, 1>(a, most, workspace, sms, stream);
     }
   }
   return w == kRowsOnly ? nullptr : launch_paged_tiles(a, w == kBoth ? kFewRows : 0, workspace, stream);
