@@ -140,10 +140,13 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   ME_CHECK_VALUE(max_q >= 0, "max_q: a positive number or None, got ", text(max_q));
   const Batch batch = check_batch(k_pages, table, cu, lens, tokens);
   a.batch = batch.args;
+  const Tensor given = q;
   if (!rows_fit(q)) q = q.clone(at::MemoryFormat::Contiguous);
   Tensor o;
   if (out.has_value()) {
     o = *out;
+    // (units read rows of q that others' rows of o may lie over by then; q itself, not its copy above)
+    ME_CHECK_VALUE(!o.numel() || !o.is_alias_of(given), "out: a tensor of its own is needed, not q's memory");
     ME_CHECK_VALUE(o.sizes() == q.sizes(), "out: q's shape ", shape(q), " is needed, got ", shape(o));
     TORCH_CHECK(o.device() == q.device() && o.scalar_type() == torch::kBFloat16 && rows_fit(o) && !o.is_alias_of(k_pages) && !o.is_alias_of(v_pages),
                 "out: bfloat16 on the pages' device is needed, heads contiguous and a multiple of 8 elements apart, 16-byte aligned, not the pages");

@@ -168,7 +168,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
     """(o [T, Hq, D], lse [Hq, T] fp32) of q [T, Hq, D]: softmax(scale q . k) v over the keys at positions
     [max(0, p - window + 1), p] of the row's sequence (p: the row's position; window None: all of them). Hq is a multiple of Hk; the
     pages hold the new tokens too (append first). max_q: the longest run of new tokens if the host knows it; with it a batch of
-    single tokens skips what only longer runs need (a longer run than max_q says is still right, and slower). out: where o goes."""
+    single tokens skips what only longer runs need (a longer run than max_q says is still right, and slower). out: where o goes,
+    a tensor of its own."""
     _no_gradient("paged_attention", q, k_pages, v_pages)
     if window is not None and window < 1 or max_q is not None and max_q < 1:
         raise ValueError(f"window, max_q: a positive number or None, got {window} and {max_q}")
@@ -186,5 +187,7 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         raise ValueError(f"scale: a positive number is needed, got {scale}")
     if out is not None and out.shape != q.shape:
         raise ValueError(f"out: q's shape {tuple(q.shape)} is needed, got {tuple(out.shape)}")
+    if out is not None and out.numel() and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
+        raise ValueError("out: a tensor of its own is needed, not q's memory")
     with torch.no_grad():
         return paged_attention_ref(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(window or 0), float(scale), out)

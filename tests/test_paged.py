@@ -199,3 +199,18 @@ def test_together():
         parts.append(paged.paged_attention(rows, kp, vp, table, cu, lens, window=20, scale=0.3)[0])
         at += n
     assert float((torch.cat(parts) - want).abs().max()) < 1e-5
+
+
+def alias_refusals(device, dtype):
+    """`out` in q's memory: units of work read q after others have written."""
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    two = torch.zeros(b.tokens, 8, 64, dtype=dtype, device=device)
+    odd = torch.zeros(b.tokens, 4, 66, dtype=dtype, device=device)[..., :64]  # (q is copied first)
+    return [lambda: paged.paged_attention(b.q, *b.args(), out=b.q), lambda: paged.paged_attention(two[:, :4], *b.args(), out=two[:, 2:6]),
+            lambda: paged.paged_attention(odd, *b.args(), out=odd)]
+
+
+def test_out_is_not_q():
+    for call in alias_refusals("cpu", F32):
+        with pytest.raises(ValueError):
+            call()

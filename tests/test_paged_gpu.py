@@ -7,7 +7,7 @@ import torch
 
 import paged_oracle as oracle
 from micro_engram_fork_b200.ops import paged
-from test_paged import append_inputs, check_append, check_bad_offsets, check_bad_pages, refusals
+from test_paged import alias_refusals, append_inputs, check_append, check_bad_offsets, check_bad_pages, refusals
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -275,3 +275,9 @@ def test_refusals():
         with pytest.raises(RuntimeError):
             call()
             pytest.fail(f"call {i} was taken")
+
+
+def test_out_is_not_q():
+    for call in alias_refusals(DEV, BF):
+        with pytest.raises(ValueError):
+            call()
