@@ -612,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int token = u.tile * 2 * tokens + (int)rank * tokens + ti;  // of the sequence's new ones
       const bool mine = ti < tokens && token < u.s.count, any_mine = __any_sync(0xffffffffu, mine);
       const int last = mine ? min(u.s.context + token, seq.hi - 1) : -1;
-      const int from = a.window > 0 ? u.s.context + token - a.window + 1 : 0;
+      const int from = a.window > 0 ? max(u.s.context + token, 0) - a.window + 1 : 0;
       float m = -INFINITY, l = 0.f;
       for (int j = 0; j < n; ++j) {
         const int i = gb + j, kb = u.kb0 + j, key0 = kb * BN;
@@ -940,7 +940,10 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
 
 int paged_status(int* detail) {
   int word[2] = {0, 0};
+  cudaDeviceSynchronize();  // (streams that do not wait for the default one)
   cudaMemcpyFromSymbol(word, g_status, sizeof word);
+  const int none[2] = {0, 0};
+  if (word[0] != 0) cudaMemcpyToSymbol(g_status, none, sizeof none);
   *detail = word[1];
   return word[0];
 }

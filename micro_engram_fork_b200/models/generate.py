@@ -70,6 +70,9 @@ class Generator:
         for b, n in enumerate(counts):
             if n > self.cache.chunk or self.lens[b] + n > self.cache.max_len:
                 raise ValueError(f"extend: sequence {b} has {self.lens[b]} tokens and gets {n}; a call takes {self.cache.chunk}, the cache {self.cache.max_len}")
+        vocab = self.text.embed_tokens.weight.shape[0]
+        if any(not 0 <= t < vocab for n in new for t in n):
+            raise ValueError(f"extend: token ids of 0 to {vocab - 1} are needed")
         ends = [a + n for a, n in zip(self.lens, counts)]
         starts = [0]
         for n in counts:
@@ -104,6 +107,8 @@ class Generator:
         cap = self.model.config.final_logit_softcapping
         if temperature <= 0:
             return top_logits(z, 1, softcap=cap)[1][:, 0]
+        if not top_p > 0 or top_k < 0:
+            raise ValueError(f"top_p: a positive number, top_k: 0 or more; got {top_p} and {top_k}")
         k = min(top_k or MAX_TOP, MAX_TOP, z.shape[1])
         values, ids, lse = top_logits(z, k, softcap=cap, temperature=temperature)
         p = torch.exp(values / temperature - lse[:, None])
@@ -150,4 +155,5 @@ class Generator:
             if not live or step + 1 == max_new_tokens:
                 break
             hidden = self.extend(new)
+        paged.check_waits(self.device)
         return answers

@@ -26,10 +26,14 @@ CPU tensors run the plain PyTorch forms below, which compute in fp32 (fp64 for f
              taken within [0, tokens]; a token whose position is negative is stored nowhere and sees nothing.
   empty rows a row that sees no key: 0, lse -inf.
 
+Every wait inside the attention kernels is bounded; one that ran out (which no input causes) leaves its results wrong
+and a code on the device: check_waits raises where there is one (it waits for the device, so callers do it where they do anyway).
+
 There is no gradient: a call on tensors that require one is refused while gradients are recorded.
 """
 import torch
 
+from .. import native
 from . import use_native
 from .objectives import kernel_call
 
@@ -121,7 +125,7 @@ def qkv_norm_rope_append(qkv, q_w, k_w, inv_freq, k_pages, v_pages, block_table,
     the raw k); k and v are written into their pages. Each head is normalised (y = x / sqrt(mean x^2 + eps)), q and k take their
     weights [D] and are rotated by position * inv_freq [D / 2] (fp32), v takes neither. All in 32 bits (the angle in 64), rounded
     once. Two new tokens must not share a place in the cache."""
-    _no_gradient("qkv_norm_rope_append", qkv, q_w, k_w, k_pages, v_pages)
+    _no_gradient("qkv_norm_rope_append", qkv, q_w, k_w, inv_freq, k_pages, v_pages)
     args = (qkv, q_w, k_w, inv_freq, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(q_heads), bool(kv_shared), float(eps))
     if use_native(qkv, k_pages):
         return kernel_call("paged_append", *args)
@@ -170,7 +174,7 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
     pages hold the new tokens too (append first). max_q: the longest run of new tokens if the host knows it; with it a batch of
     single tokens skips what only longer runs need (a longer run than max_q says is still right, and slower). out: where o goes,
     a tensor of its own."""
-    _no_gradient("paged_attention", q, k_pages, v_pages)
+    _no_gradient("paged_attention", q, k_pages, v_pages, *(() if out is None else (out,)))
     if window is not None and window < 1 or max_q is not None and max_q < 1:
         raise ValueError(f"window, max_q: a positive number or None, got {window} and {max_q}")
     if use_native(q, k_pages):
@@ -183,11 +187,21 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         raise ValueError(f"q: [tokens, heads, {d}] is needed, got {tuple(q.shape)}")
     if q.shape[1] < hk or q.shape[1] % hk or q.shape[1] // hk > 128:
         raise ValueError(f"q: heads a multiple of the pages' {hk} (up to 128 times) are needed, got {q.shape[1]}")
-    if not 0 < float(scale) < float("inf"):
-        raise ValueError(f"scale: a positive number is needed, got {scale}")
+    if not 0 < float(torch.tensor(scale, dtype=torch.float32)) < float("inf"):
+        raise ValueError(f"scale: a positive number (in 32 bits) is needed, got {scale}")
     if out is not None and out.shape != q.shape:
         raise ValueError(f"out: q's shape {tuple(q.shape)} is needed, got {tuple(out.shape)}")
     if out is not None and out.numel() and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
         raise ValueError("out: a tensor of its own is needed, not q's memory")
     with torch.no_grad():
         return paged_attention_ref(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(window or 0), float(scale), out)
+
+
+def check_waits(device):
+    """Raises if a bounded wait of the attention kernels ran out on this device since the last look."""
+    device = torch.device(device)
+    if device.type != "cuda":
+        return
+    code, where = native().paged_status(torch.cuda.current_device() if device.index is None else device.index)
+    if code:
+        raise RuntimeError(f"paged_attention: a wait on the device ran out (code {code}, at {where}); results since the last check are not valid")

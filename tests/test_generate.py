@@ -185,3 +185,21 @@ def test_infer_native(tmp_path, monkeypatch, capsys):
     assert list(map(str, gen.generate([[ord(c) for c in "hello"]], 6)[0])) == without
     model.model.layers[1].add_module("micro_engram", eng)
     assert list(map(str, gen.generate([[ord(c) for c in "hello"]], 6)[0])) == with_engram
+
+
+def test_wrong_tokens_and_sampling():
+    model, _ = small_model(engram=False)
+    gen = Generator(model, 2, 40, chunk=16, page=16)
+    for ids in ([256], [-1], [3, 10 ** 12]):
+        with pytest.raises(ValueError):
+            gen.extend([[1], ids])
+        with pytest.raises(ValueError):
+            gen.generate([ids], 3)
+    assert gen.lens == [0, 0]
+    h = gen.extend([[1], [2, 3]])
+    for kw in ({"top_p": 0.0}, {"top_p": -1.0}, {"top_p": math.nan}, {"top_k": -1}):
+        with pytest.raises(ValueError):
+            gen.next_tokens(h, temperature=1.0, **kw)
+    likeliest = gen.next_tokens(h)
+    assert torch.equal(gen.next_tokens(h, temperature=1.0, top_p=1e-6), likeliest)
+    assert torch.equal(gen.next_tokens(h, temperature=1.0, top_k=1), likeliest)
