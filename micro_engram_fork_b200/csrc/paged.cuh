@@ -32,7 +32,7 @@ struct Keys {
 ME_DEVICE Keys keys_of(const PagedBatch& p, int page, const Sequence& s, int i0, int i1, int window) {
   const int room = p.width * page;
   const int hi = min(max(s.context + i1 + 1, 0), room);
-  const int lo = window > 0 ? max(s.context + i0 - window + 1, 0) : 0;
+  const int lo = window > 0 ? max(max(s.context + i0, 0) - window + 1, 0) : 0;  // (in this order nothing passes 32 bits)
   return {min(lo, hi), hi};
 }
 

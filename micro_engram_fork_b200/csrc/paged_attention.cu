@@ -171,10 +171,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const RowsArgs 
     for (int e = 0; e < 2 * NT; ++e) {
       const int r = r0 + e / 2 * 8 + 2 * t4 + e % 2, pos = s.context + r / group;
       last[e] = r < r0 + rows ? pos : -1;
-      from[e] = a.window > 0 ? pos - a.window + 1 : 0;
+      from[e] = a.window > 0 ? max(pos, 0) - a.window + 1 : 0;
     }
     const int all_last = s.context + r0 / group;
-    const int all_from = a.window > 0 ? s.context + (r0 + rows - 1) / group - a.window + 1 : 0;
+    const int all_from = a.window > 0 ? max(s.context + (r0 + rows - 1) / group, 0) - a.window + 1 : 0;
 
     uint32_t qf[NT][D / 16][2];
 #pragma unroll

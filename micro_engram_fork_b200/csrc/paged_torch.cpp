@@ -43,10 +43,13 @@ me::PagedCache check_cache(const Tensor& k, const Tensor& v) {
   return {k.data_ptr(), v.data_ptr(), pages == 1 ? whole : k.stride(0), pages == 1 ? whole : v.stride(0), (int)pages, (int)heads, (int)page, (int)dim};
 }
 
+// int32: a number outside its range is no page and no position, and must not come back as another one.
+Tensor narrow(const Tensor& t) { return t.scalar_type() == torch::kInt ? t : t.clamp(-1, INT32_MAX).to(torch::kInt); }
+
 Tensor check_int(const Tensor& t, const Tensor& like, const char* what) {
   TORCH_CHECK(t.device() == like.device(), what, ": on another device than the pages");
   ME_CHECK_VALUE(t.scalar_type() == torch::kInt || t.scalar_type() == torch::kLong, what, ": int32 or int64 is needed, got ", t.scalar_type());
-  return t.scalar_type() == torch::kInt && t.is_contiguous() ? t : t.to(torch::kInt).contiguous();
+  return narrow(t).contiguous();
 }
 
 struct Batch {
@@ -66,7 +69,7 @@ Batch check_batch(const Tensor& pages, const Tensor& table, const Tensor& cu, co
   b.lens = check_int(lens, pages, "seq_lens");
   TORCH_CHECK(table.device() == pages.device(), "block_table: on another device than the pages");
   ME_CHECK_VALUE(table.scalar_type() == torch::kInt || table.scalar_type() == torch::kLong, "block_table: int32 or int64 is needed, got ", table.scalar_type());
-  b.table = table.scalar_type() == torch::kInt && (table.size(1) <= 1 || table.stride(1) == 1) ? table : table.to(torch::kInt).contiguous();
+  b.table = table.scalar_type() == torch::kInt && (table.size(1) <= 1 || table.stride(1) == 1) ? table : narrow(table).contiguous();
   b.args = {b.cu.data_ptr<int>(), b.lens.data_ptr<int>(), b.table.data_ptr<int>(), b.table.stride(0), (int)table.size(1), (int)lens.size(0), (int)tokens};
   return b;
 }
@@ -84,6 +87,13 @@ int sms() { return at::cuda::getCurrentDeviceProperties()->multiProcessorCount; 
 bool rows_fit(const Tensor& t) {
   auto fits = [&](int i) { return t.size(i) <= 1 || (t.stride(i) > 0 && t.stride(i) % 8 == 0); };
   return t.stride(2) == 1 && fits(0) && fits(1) && aligned(t);
+}
+// ... and as they are written: no two of them share memory.
+bool apart(const Tensor& t) {
+  const int64_t n = t.size(0), h = t.size(1), d = t.size(2);
+  if (n <= 1 || h <= 1) return (n <= 1 || t.stride(0) >= d) && (h <= 1 || t.stride(1) >= d);
+  return t.stride(1) <= t.stride(0) ? t.stride(1) >= d && t.stride(0) >= (h - 1) * t.stride(1) + d
+                                    : t.stride(0) >= d && t.stride(1) >= (n - 1) * t.stride(0) + d;
 }
 int64_t head_stride(const Tensor& t) { return t.size(1) <= 1 ? t.size(2) : t.stride(1); }
 int64_t token_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0); }
@@ -136,7 +146,7 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
                  " (up to 128 times) are needed, got ", text(q_heads));
   ME_CHECK_VALUE(tokens * q_heads < (1ll << 31), "q: fewer than 2^31 rows (tokens times heads) are needed, got ", shape(q));
   ME_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window: a positive number or None, got ", text(window));
-  ME_CHECK_VALUE(scale > 0 && scale < INFINITY, "scale: a positive number is needed");
+  ME_CHECK_VALUE((float)scale > 0 && (float)scale < INFINITY, "scale: a positive number (in 32 bits) is needed");
   ME_CHECK_VALUE(max_q >= 0, "max_q: a positive number or None, got ", text(max_q));
   const Batch batch = check_batch(k_pages, table, cu, lens, tokens);
   a.batch = batch.args;
@@ -148,8 +158,9 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
     // (units read rows of q that others' rows of o may lie over by then; q itself, not its copy above)
     ME_CHECK_VALUE(!o.numel() || !o.is_alias_of(given), "out: a tensor of its own is needed, not q's memory");
     ME_CHECK_VALUE(o.sizes() == q.sizes(), "out: q's shape ", shape(q), " is needed, got ", shape(o));
-    TORCH_CHECK(o.device() == q.device() && o.scalar_type() == torch::kBFloat16 && rows_fit(o) && !o.is_alias_of(k_pages) && !o.is_alias_of(v_pages),
-                "out: bfloat16 on the pages' device is needed, heads contiguous and a multiple of 8 elements apart, 16-byte aligned, not the pages");
+    TORCH_CHECK(o.device() == q.device() && o.scalar_type() == torch::kBFloat16 && rows_fit(o) && apart(o) && !o.is_alias_of(k_pages) && !o.is_alias_of(v_pages),
+                "out: bfloat16 on the pages' device is needed, heads contiguous, a multiple of 8 elements and at least dim apart, 16-byte aligned, "
+                "not the pages");
     o.unsafeGetTensorImpl()->bump_version();
   } else {
     o = torch::empty({tokens, q_heads, dim}, q.options().requires_grad(false));
@@ -173,7 +184,7 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   return {o, lse};
 }
 
-// (code, where) of the first device wait that ran out in the attention on this device; (0, 0): none.
+// (code, where) of the first device wait that ran out in the attention on this device since the last call; (0, 0): none.
 std::vector<int64_t> paged_status(int64_t device) {
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
   int detail = 0;

@@ -214,3 +214,65 @@ def test_out_is_not_q():
     for call in alias_refusals("cpu", F32):
         with pytest.raises(ValueError):
             call()
+
+
+def check_wide_numbers(device, dtype):
+    """64-bit page numbers that would be pages if they were cut to 32 bits are none."""
+    batch = oracle.Batch([(60, 2), (33, 1)], 4, 2, 64, 16, None, dtype, device)
+    table = batch.table.long()
+    table[0, 1] = -1
+    want = paged.paged_attention(batch.q, batch.k, batch.v, table, batch.cu, batch.seq_lens)
+    for wrong in (2 ** 32, -2 ** 32, 2 ** 63 - 1, -2 ** 63):
+        table[0, 1] = wrong + int(batch.table[0, 1]) if abs(wrong) == 2 ** 32 else wrong
+        got = paged.paged_attention(batch.q, batch.k, batch.v, table, batch.cu.long(), batch.seq_lens.long())
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_wide_numbers():
+    check_wide_numbers("cpu", F32)
+
+
+def check_negative_positions(device, dtype):
+    """Tokens at negative positions before others, under windows of any size: those see nothing, the others what they would alone."""
+    for count, max_q in ((6, None), (6, 1), (40, None)):
+        batch = oracle.Batch([(0, count), (20, 3)], 4, 2, 64, 16, None, dtype, device)
+        batch.seq_lens[0] = 2  # its last two tokens have positions 0 and 1
+        want = paged.paged_attention(batch.q, *batch.args(), max_q=max_q)
+        assert bool((want[0][:count - 2] == 0).all()) and bool((want[1][:, count - 2:] > -math.inf).all())
+        for window in (2 ** 31 - 1, 2 ** 31 - 3, 1000):  # no key lies that far back
+            got = paged.paged_attention(batch.q, *batch.args(), window=window, max_q=max_q)
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_negative_positions():
+    check_negative_positions("cpu", F32)
+
+
+def more_refusals(device, dtype):
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    qkv, q_w, k_w, f = append_inputs(b, False, dtype)
+    return [lambda: paged.paged_attention(b.q, *b.args(), scale=1e-60), lambda: paged.paged_attention(b.q, *b.args(), scale=1e60),
+            lambda: paged.paged_attention(b.q, *b.args(), out=torch.zeros_like(b.q).requires_grad_()),
+            lambda: paged.qkv_norm_rope_append(qkv, q_w, k_w, f.clone().requires_grad_(), *b.args(), 4)]
+
+
+def test_more_refusals():
+    for call in more_refusals("cpu", F32):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_a_wait_that_ran_out(monkeypatch):
+    class Native:
+        words = [(7, 71), (0, 0)]
+
+        def paged_status(self, device):
+            assert device == 3
+            return self.words.pop(0)
+
+    fake = Native()
+    monkeypatch.setattr(paged, "native", lambda: fake)
+    paged.check_waits("cpu")
+    with pytest.raises(RuntimeError, match="ran out"):
+        paged.check_waits("cuda:3")
+    paged.check_waits("cuda:3")

@@ -7,7 +7,7 @@ import torch
 
 import paged_oracle as oracle
 from micro_engram_fork_b200.ops import paged
-from test_paged import alias_refusals, append_inputs, check_append, check_bad_offsets, check_bad_pages, refusals
+from test_paged import alias_refusals, append_inputs, check_append, check_bad_offsets, check_bad_pages, check_negative_positions, check_wide_numbers, more_refusals, refusals
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -281,3 +281,24 @@ def test_out_is_not_q():
     for call in alias_refusals(DEV, BF):
         with pytest.raises(ValueError):
             call()
+
+
+def test_wide_numbers():
+    check_wide_numbers(DEV, BF)
+
+
+def test_negative_positions():
+    check_negative_positions(DEV, BF)
+
+
+def test_more_refusals():
+    for call in more_refusals(DEV, BF):
+        with pytest.raises(ValueError):
+            call()
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, BF, DEV)
+    room = torch.zeros(5 * 4 * 64, dtype=BF, device=DEV)
+    for strides in ((8, 64, 1), (256, 32, 1), (128, 64, 1), (64, 256, 1)):  # heads that lie over one another
+        with pytest.raises(RuntimeError):
+            paged.paged_attention(b.q, *b.args(), out=room.as_strided((5, 4, 64), strides))
+    got = paged.paged_attention(b.q, *b.args(), out=room.as_strided((5, 4, 64), (64, 320, 1)))[0]
+    assert torch.equal(got, paged.paged_attention(b.q, *b.args())[0])
