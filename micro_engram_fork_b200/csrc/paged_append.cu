@@ -9,6 +9,9 @@
 // Bound: memory. Each element is read once and written once. A lane holds 8 elements of each half of a head in two 16-byte
 // loads, so dim / 16 lanes share a head and a warp works on 512 / dim heads of one token; it keeps them for all tokens of its
 // block, with its heads' weights in registers, and reads the block's table of sines from shared memory.
+//
+// Measured: 8192 new tokens of a sliding layer (32 q, 16 + 16 kv heads of 256; 537 MB) 109 us, 0.75 of the copy rate (half of the issue slots:
+// 40 operations an element pair with its unpacking and packing). Small calls are the host's: one token 8.2 us, its kernel 3.3.
 #include <algorithm>
 
 #include "paged.cuh"

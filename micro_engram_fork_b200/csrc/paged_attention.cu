@@ -15,6 +15,10 @@
 //     B operand of the second product through movmatrix, without shared memory. P goes as two bf16 terms (its value rounded and
 //     what the rounding left, relative error 2^-17), which the idle tensor cores give for nothing: the output is as exact as its own
 //     rounding.
+//
+// Measured, single tokens: 128 sequences of 30 to 9000 tokens in a sliding layer (window 1024, 16 heads of 256; 2.0 GB) 311 us, 0.98 of the copy
+// rate; 64 of 100 to 16000 in a global one (4 heads of 512; 4.5 GB) 755 us, 0.92; one over 131072 (1.07 GB) 196 us, 0.84 (ramp, two partial
+// blocks each piece, the join: 25 us); one sliding sequence (16 MB) 14 us, two launches one after another.
 #include <algorithm>
 
 #include "paged.cuh"

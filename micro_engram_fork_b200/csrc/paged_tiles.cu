@@ -3,7 +3,7 @@
 // Many rows a key head: S = Q K^T and O += P V are bound by the tensor cores, and next by the L2 cache, out of which every tile of
 // rows reads its sequence's keys and values again. So two SMs work as one (cta_group::2): 256 rows (new token, query head of the
 // key head's group) a pair, 128 of them in each SM's tensor memory, and each SM loads half of every block of 128 keys, which halves what
-// both read. Per SM and block at dim 256: 64 KB in 2048 clocks of the tensor core.
+// both read. Per SM and block at dim 256: 64 KB of keys and values for 2048 clocks of the tensor core.
 //
 //   warps 0, 2 loads: rows of Q once a unit, and K; V (TMA, each through a ring of its own; a page is a run of rows of the tensor
 //              map, a page that is none is an index past its last dimension, which reads zeros)
@@ -14,16 +14,22 @@
 //              maximum (O is rescaled only when it grows by more than 2^8), P rounded to bf16 (as what it is multiplied with is) and put
 //              back over its scores, from where it is the A operand of P V; the sum is of the terms before that. At a unit's end:
 //              O / sum to global memory. One warp a scheduler: what a block costs beside its exponentials is paid once, and nothing is
-//              exchanged (two threads a row: 3100 clocks a block at dim 256, four: 3200, every second block to another four warps: 3450)
+//              exchanged (two and four threads a row were slower)
 //
 // Tensor memory: O in columns 0-255, two S (P) buffers of 128. dim 512 has no room for both halves of O: a unit takes one half of the
-// columns, and S is computed twice (4/3 of the operations).
+// columns, and S is computed twice (3/2 of the operations).
 // Rows of V that no row of the sequence may see (past its end, before its first window) can hold anything, and 0 * NaN is not 0: in blocks that have
 // such rows the softmax threads wait for V themselves and put zeros there.
 //
 // Units (sequence, tile of rows, key head, half of the columns) are dealt to the pairs in turn, the longest of a sequence first. With few of them a
 // sequence's keys are cut into chunks, whose (max, sum, O) a second kernel joins.
 // Every wait is bounded (2 s); a timeout records ME_ERR_TIMEOUT in the status word and the kernel frees tensor memory and returns.
+//
+// Measured: 2048 new tokens over 16048, 32 query heads on 4 of dim 512: 2.29 ms, 880 TFLOP/s of what has to be computed (0.53 of the measured
+// bf16 rate; the tensor cores are 78% busy, a third of it with S a second time). 4096 new tokens under a window of 1024, 32 heads on 16 of dim 256: 195 us,
+// 705 TFLOP/s (0.42): a block takes 2950 clocks, of them the softmax 2450 (128 exponentials a thread at 8 clocks a warp's, two
+// readings of the scores, the arrival), the rest the way of P to the products and of the next S back (two S buffers cover one of both); a unit of
+// 10 blocks has 7000 clocks between its last softmax and the next unit's first (its last product 1800, O out 4700).
 #include <cudaTypedefs.h>
 
 #include <algorithm>
@@ -625,13 +631,20 @@ __global__ void __launch_bounds__(kThreads, 1)
           uint32_t pages = 0xff;
           if (!whole) pages = __ballot_sync(0xffffffffu, lane < 8 && page_at(p, a.cache.pages, u.b, (key0 + (lane & 7) * 16) >> args.plog) >= 0);
           const bool open = __all_sync(0xffffffffu, pages == 0xffu && ((key0 >= from && key0 + BN - 1 <= last) || !mine));
-          // 64 scores from column c on, -inf where the row does not see the key
-          auto scores = [&](int c, uint32_t(&s)[2][32]) {
+          auto scores = [&](int c, uint32_t(&s)[2][32]) {  // 64 of them from column c on
             tmem_issue_ld32(at + c, s[0]);
             tmem_issue_ld32(at + c + 32, s[1]);
             tmem_wait_ld(s[0]);
             tmem_wait_ld(s[1]);
-            if (!open) {
+          };
+          // (Rolled loops: with 128 scores unrolled the roles' code together does not fit the instruction caches, and the SMs of a
+          // full GPC took 4000 to 5000 clocks for what takes 1400.)
+          float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll 1
+          for (int c = 0; c < BN; c += 64) {
+            uint32_t s[2][32];
+            scores(c, s);
+            if (!open) {  // -inf where the row does not see the key, put back for the second reading (masking twice: 500 clocks a block)
               // bits from .. last of these keys that have a page
               const int lo = min(max(from - key0 - c, 0), 64), hi = min(max(last + 1 - key0 - c, 0), 64);
               const uint64_t seen = (hi == 64 ? ~0ull : (1ull << hi) - 1) & ~(lo == 64 ? ~0ull : (1ull << lo) - 1);
@@ -642,16 +655,10 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int e = 0; e < 32; ++e)
                   if (!(bits & (1u << e))) s[h][e] = 0xff800000u;  // -inf
+                tmem_st32u(at + c + 32 * h, s[h]);
               }
+              tmem_st_wait();
             }
-          };
-          // (Rolled loops: with 128 scores unrolled the roles' code together does not fit the instruction caches, and the SMs of a
-          // full GPC took 4000 to 5000 clocks for what takes 1400.)
-          float mx[2] = {-INFINITY, -INFINITY};
-#pragma unroll 1
-          for (int c = 0; c < BN; c += 64) {
-            uint32_t s[2][32];
-            scores(c, s);
 #pragma unroll
             for (int e = 0; e < 64; ++e) mx[e & 1] = fmaxf(mx[e & 1], __uint_as_float(s[e / 32][e % 32]));
           }
