@@ -3,11 +3,13 @@
 Layout:
   ops/       autograd ops backed by the hand-written sm_100a kernels in csrc/ (engram
              hash/gather/gate/row-grad/Adam, RMSNorm, q/k/v norm + RoPE, GeGLU, softcapped
-             CE, the other objectives over the vocabulary, attention, tcgen05 GEMM), each with a plain PyTorch reference used on CPU
+             CE, the other objectives over the vocabulary, attention, a paged cache with
+             its attention, tcgen05 GEMM), each with a plain PyTorch reference used on CPU
              and as the test oracle
   parallel/  symmetric peer memory over NVLink (CUDA IPC), the row store of the
              row-sharded engram tables, P2P collectives
-  models/    the Gemma-4-style decoder (frozen base) built from the ops above
+  models/    the Gemma-4-style decoder (frozen base) built from the ops above, and generation with
+             it (generate.py)
   utils/     per-phase CUDA-event timers with NVTX ranges (timers.py) and the benchmarks:
              kernel microbenchmarks (kernel_bench), the engram module benchmark (engram_bench),
              the peer-memory all-reduce against NCCL (p2p_bench)

@@ -4,7 +4,7 @@ events (warm-up, synchronize on both sides) and reported against the measured ro
 figures otherwise). Also the workload that the committed ncu summaries in profiles/ capture.
 
   python -m micro_engram_fork_b200.utils.kernel_bench [--case all|gemm|attn_fwd|attn_bwd|gate|ce|qkv|geglu|rows|
-                                                       norms|ce_bwd|nf4|ce_gemm|tp|objectives] [--iters N] [--small]
+                                                       norms|ce_bwd|nf4|ce_gemm|tp|objectives|paged] [--iters N] [--small]
 """
 import argparse
 import json
@@ -417,9 +417,39 @@ def case_objectives(C, dev, it, pk):
     return r
 
 
+def case_paged(C, dev, it, pk):
+    """The paged cache in a sliding layer (window 1024, 32 heads on 16 of 256) and a global one (32 on 4 of 512): 64 answers over 4096
+    tokens each, and a prompt's chunk of 2048 on 6144 before it. Bytes are the keys and values that are seen, read once; flops those of the seen
+    pairs. Every call has a cache of its own, larger than L2 for the answers."""
+    from ..ops import paged as P
+
+    page, r = 64, {}
+    for kind, hq, hk, d, window in (("sliding", 32, 16, 256, 1024), ("global", 32, 4, 512, None)):
+        for name, seqs, length, new in (("64 answers", 64, 4096, 1), ("chunk of 2048", 1, 8192, 2048)):
+            width = length // page
+            k, v = torch.randn(2, seqs * width, hk, page, d, device=dev, dtype=torch.bfloat16)
+            table = torch.randperm(seqs * width, device=dev).int().view(seqs, width)
+            cu = torch.arange(seqs + 1, device=dev, dtype=torch.int32) * new
+            lens = torch.full((seqs,), length, device=dev, dtype=torch.int32)
+            q = torch.randn(seqs * new, hq, d, device=dev, dtype=torch.bfloat16)
+            ms = _time(lambda: P.paged_attention(q, k, v, table, cu, lens, window=window, scale=d ** -0.5, max_q=new), it)
+            label = f"paged_attention {kind}, {name}"
+            if new == 1:
+                r.update(_hbm(label, seqs * min(length, window or length) * hk * d * 4, ms, pk))
+            else:
+                pairs = sum(min(p + 1, window or length) for p in range(length - new, length))
+                tflops = 4 * pairs * hq * d / ms / 1e9
+                r[label] = {"ms": round(ms, 4), "tflops": round(tflops, 1), "frac": round(tflops / pk["bf16_tflops"], 3)}
+            qkv = torch.randn(seqs * new, (hq + 2 * hk) * d, device=dev, dtype=torch.bfloat16)
+            w, freq = torch.ones(d, device=dev), 10000.0 ** (-torch.arange(0, d, 2, device=dev).float() / d)
+            ms = _time(lambda: P.qkv_norm_rope_append(qkv, w, w, freq, k, v, table, cu, lens, hq), it)
+            r.update(_hbm(f"qkv_norm_rope_append {kind}, {name}", qkv.numel() * 4, ms, pk))
+    return r
+
+
 CASES = {"gemm": case_gemm, "attn_fwd": case_attn_fwd, "attn_bwd": case_attn_bwd, "gate": case_gate, "ce": case_ce,
          "qkv": case_qkv, "geglu": case_geglu, "rows": case_rows, "norms": case_norms, "ce_bwd": case_ce_bwd,
-         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp, "objectives": case_objectives}
+         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp, "objectives": case_objectives, "paged": case_paged}
 
 
 def main(argv=None):
