@@ -10,7 +10,7 @@
 // loads, so dim / 16 lanes share a head and a warp works on 512 / dim heads of one token; it keeps them for all tokens of its
 // block, with its heads' weights in registers, and reads the block's table of sines from shared memory.
 //
-// Measured: 8192 new tokens of a sliding layer (32 q, 16 + 16 kv heads of 256; 537 MB) 109 us, 0.75 of the copy rate (half of the issue slots:
+// Measured: 8192 new tokens of a sliding layer (32 q, 16 + 16 kv heads of 256; 537 MB) 102 us, 0.81 of the copy rate (half of the issue slots:
 // 40 operations an element pair with its unpacking and packing). Small calls are the host's: one token 8.2 us, its kernel 3.3.
 #include <algorithm>
 
@@ -20,7 +20,8 @@ namespace me {
 namespace {
 using namespace paged;
 
-constexpr int kThreads = 256, kWarps = 8;
+constexpr int kThreads = 256, kWarps = 8, kResident = 3;  // blocks an SM: 64 to 80 registers
+constexpr float kPrologue = 1.5f;  // (0.7 and 3: the same but for 8192 tokens at dim 512, 125 us with 0.7 and 115 with the others)
 
 // Tokens of a block at most; the table of sines is this many times dim / 2 pairs.
 template <int D>
@@ -140,12 +141,20 @@ __global__ void __launch_bounds__(kThreads) paged_append_kernel(AppendArgs a, in
 template <int D>
 void launch(const AppendArgs& a, int sms, cudaStream_t stream) {
   const int heads = a.q_heads + 2 * a.cache.heads, groups = (heads + 512 / D - 1) / (512 / D);
-  // As many tokens a block as still give every SM four blocks; with fewer blocks than that, the heads are split too.
+  // Tokens a block: its prologue takes about as long as kPrologue tokens, and blocks run in waves of `resident`, so the fewest
+  // (waves x (tokens + prologue)). With fewer blocks than a wave the heads are split too. (Powers of two that left four blocks an SM, which
+  // took a second or third wave for little: 2048 tokens 43 us, 33 now; 1000 of a global layer 41 and 29; 8192 109 and 102.)
+  const int resident = kResident * sms;
   int tb = 1;
-  while (tb < kTokens<D> && (int64_t)a.batch.tokens / (2 * tb) >= 4 * sms) tb *= 2;
+  float least = 1e30f;
+  for (int n = 1; n <= kTokens<D>; ++n) {
+    const int64_t blocks = ((int64_t)a.batch.tokens + n - 1) / n;
+    const float cost = (float)((blocks + resident - 1) / resident) * (n + kPrologue);
+    if (cost < least) least = cost, tb = n;
+  }
   const int blocks = (a.batch.tokens + tb - 1) / tb;
   const int most = (groups + kWarps - 1) / kWarps;
-  const int split = std::min(most, std::max(1, 4 * sms / blocks));
+  const int split = std::min(most, std::max(1, resident / blocks));
   int plog = 0;
   while ((1 << plog) < a.cache.page) ++plog;
   paged_append_kernel<D><<<dim3(blocks, split), kThreads, 0, stream>>>(a, tb, plog);
