@@ -302,3 +302,21 @@ def test_more_refusals():
             paged.paged_attention(b.q, *b.args(), out=room.as_strided((5, 4, 64), strides))
     got = paged.paged_attention(b.q, *b.args(), out=room.as_strided((5, 4, 64), (64, 320, 1)))[0]
     assert torch.equal(got, paged.paged_attention(b.q, *b.args())[0])
+
+
+@pytest.mark.parametrize("hq,hk,d", [(4, 2, 256), (16, 1, 128), (5, 1, 64), (8, 1, 512)])
+@pytest.mark.parametrize("window", [None, 1500])
+def test_long_drafts(hq, hk, d, window):
+    """Up to 16 rows a sequence that go through long caches together, in units that are cut, with single tokens between."""
+    most = 16 // (hq // hk)
+    lens = [(9000, most), (3, 1), (4000, max(most - 1, 1)), (2100, 0), (700, most), (0, most)]
+    batch = oracle.Batch(lens, hq, hk, d, 32, window, BF, DEV, seed=d, before=2, after=1)
+    _attend(batch, most == 1, max_q=most)
+
+
+@pytest.mark.parametrize("hq,hk,d", [(3, 1, 64), (6, 2, 256), (2, 2, 512)])
+def test_append_many(hq, hk, d):
+    """More tokens than a wave has blocks: several a block, a last block that is not full, sequences that end inside one."""
+    for tokens in (451, 1409):
+        batch = oracle.Batch([(5, 301), (77, 1), (0, 0), (9, tokens - 302)], hq, hk, d, 64, None, BF, DEV, seed=d, before=1, after=2)
+        check_append(batch, False, BF, paged.qkv_norm_rope_append)
