@@ -124,19 +124,19 @@ ME_DEVICE uint32_t pack2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&x);
 }
 
-// Zeros for the rows of no sequence.
+// The rows of no sequence: a log-sum-exp of -inf, and zeros (a caller's own output is left as it is).
 template <int D>
 ME_DEVICE void clear_rest(const PagedAttentionArgs& a, int threads) {
-  if (!a.clear_rest) return;
   const PagedBatch& p = a.batch;
   const int head = p.seqs ? min(max(p.cu[0], 0), p.tokens) : p.tokens;
   const int tail = p.seqs ? min(max(p.cu[p.seqs], head), p.tokens) : p.tokens;
   for (int64_t i = (int64_t)blockIdx.x * threads + threadIdx.x; i < (int64_t)(head + p.tokens - tail) * a.q_heads;
        i += (int64_t)gridDim.x * threads) {
     const int h = (int)(i % a.q_heads), n = (int)(i / a.q_heads), t = n < head ? n : n - head + tail;
+    a.lse[(int64_t)h * p.tokens + t] = -INFINITY;
+    if (!a.clear_rest) continue;
     bf16* o = reinterpret_cast<bf16*>(a.o) + t * a.o_token + h * a.o_head;
     for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(o + c) = make_uint4(0, 0, 0, 0);
-    a.lse[(int64_t)h * p.tokens + t] = -INFINITY;
   }
 }
 

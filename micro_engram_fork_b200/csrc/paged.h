@@ -47,7 +47,7 @@ struct PagedAttentionArgs {
   float* lse;            // [q heads, tokens]
   int q_heads, window;   // window 0: none
   float scale;
-  bool clear_rest;       // rows of no sequence: zeros (else left as they are)
+  bool clear_rest;       // rows of no sequence: zeros in o (else left as they are; lse is -inf either way)
   int max_q;             // the longest run of new tokens, as far as the caller knows
 };
 // Bytes of workspace that the call needs (16-byte aligned), and the call; what is wrong, if anything is.

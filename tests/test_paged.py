@@ -276,3 +276,19 @@ def test_a_wait_that_ran_out(monkeypatch):
     with pytest.raises(RuntimeError, match="ran out"):
         paged.check_waits("cuda:3")
     paged.check_waits("cuda:3")
+
+
+def check_lse_of_padding(device, dtype, lens, max_q):
+    """Tokens of no sequence have a log-sum-exp of -inf whether or not the rows' place is the caller's."""
+    batch = oracle.Batch(lens, 4, 2, 64, 16, None, dtype, device, before=2, after=5)
+    want, want_lse = paged.paged_attention(batch.q, *batch.args(), max_q=max_q)
+    out = torch.full_like(batch.q, 9.0)
+    free = [torch.full_like(want_lse, math.nan) for _ in range(8)]  # what a new tensor may lie on
+    del free
+    got, lse = paged.paged_attention(batch.q, *batch.args(), max_q=max_q, out=out)
+    assert torch.equal(lse, want_lse) and bool((lse[:, :2] == -math.inf).all()) and bool((lse[:, -5:] == -math.inf).all())
+    assert torch.equal(got[2:-5], want[2:-5]) and bool((got[:2] == 9).all()) and bool((got[-5:] == 9).all())
+
+
+def test_lse_of_padding():
+    check_lse_of_padding("cpu", F32, [(30, 1), (100, 3)], None)

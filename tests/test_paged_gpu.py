@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import paged_oracle as oracle
+import test_paged
 from micro_engram_fork_b200.ops import paged
 from test_paged import alias_refusals, append_inputs, check_append, check_bad_offsets, check_bad_pages, check_negative_positions, check_wide_numbers, more_refusals, refusals
 
@@ -320,3 +321,9 @@ def test_append_many(hq, hk, d):
     for tokens in (451, 1409):
         batch = oracle.Batch([(5, 301), (77, 1), (0, 0), (9, tokens - 302)], hq, hk, d, 64, None, BF, DEV, seed=d, before=1, after=2)
         check_append(batch, False, BF, paged.qkv_norm_rope_append)
+
+
+@pytest.mark.parametrize("lens,max_q", [([(30, 1), (100, 1)], 1), ([(30, 100), (7, 1)], None), ([(30, 40), (7, 1), (9, 1), (50, 1), (3, 1)], None)])
+def test_lse_of_padding(lens, max_q):
+    """The kernel of few rows, that of chunks, both."""
+    test_paged.check_lse_of_padding(DEV, BF, lens, max_q)
