@@ -37,6 +37,13 @@ from ..ops.linear import dgeglu_linear, geglu_linear, linear, linear_t
 
 
 # ----------------------------------------------------------------------------- config
+def _end_tokens(*given):
+    """All end tokens of ids, lists of ids and Nones, in their order: None, an id, or a list of several."""
+    ids = [t for g in given for t in (g if isinstance(g, (list, tuple)) else [g]) if t is not None]
+    ids = list(dict.fromkeys(ids))
+    return ids if len(ids) > 1 else ids[0] if ids else None
+
+
 @dataclass
 class GemmaConfig:
     vocab_size: int = 262_144
@@ -55,7 +62,7 @@ class GemmaConfig:
     rms_norm_eps: float = 1e-6
     final_logit_softcapping: float | None = 30.0
     pad_token_id: int | None = 0
-    eos_token_id: int | None = 1
+    eos_token_id: int | list | None = 1  # a list where several tokens end an answer
     bos_token_id: int | None = 2
     tie_word_embeddings: bool = True
     hidden_size_per_layer_input: int = 0
@@ -92,18 +99,25 @@ class GemmaConfig:
             top = d
             d = dict(d["text_config"])
             d.setdefault("tie_word_embeddings", top.get("tie_word_embeddings", True))
+            if top.get("eos_token_id") is not None:
+                d["eos_token_id"] = _end_tokens(d.get("eos_token_id"), top["eos_token_id"])
         known = {f for f in cls.__dataclass_fields__ if f != "extra"}
         kw = {k: v for k, v in d.items() if k in known}
-        eos = kw.get("eos_token_id")
-        if isinstance(eos, list):
-            kw["eos_token_id"] = eos[0] if eos else None
+        if "eos_token_id" in kw:
+            kw["eos_token_id"] = _end_tokens(kw["eos_token_id"])
         kw["extra"] = {k: v for k, v in d.items() if k not in known}
         return cls(**kw)
 
     @classmethod
     def from_pretrained(cls, path):
+        """The folder's config.json; the end tokens of its generation_config.json too, where it has one."""
         with open(os.path.join(path, "config.json")) as f:
-            return cls.from_dict(json.load(f))
+            cfg = cls.from_dict(json.load(f))
+        generation = os.path.join(path, "generation_config.json")
+        if os.path.exists(generation):
+            with open(generation) as f:
+                cfg.eos_token_id = _end_tokens(cfg.eos_token_id, json.load(f).get("eos_token_id"))
+        return cfg
 
     def to_dict(self):
         d = {k: getattr(self, k) for k in self.__dataclass_fields__ if k != "extra"}

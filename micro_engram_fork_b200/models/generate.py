@@ -119,8 +119,8 @@ class Generator:
 
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens, temperature=0.0, top_p=1.0, top_k=0, eos=None, generator=None):
-        """The answers to `prompts` (lists of token ids, one a sequence at most), each up to an `eos` token (an id or a set of them,
-        None: the model's) or max_new_tokens. What the sequences held before is forgotten."""
+        """The answers to `prompts` (lists of token ids, one a sequence at most), each up to an `eos` token (an id or several,
+        None: all that the model's configuration has) or max_new_tokens. What the sequences held before is forgotten."""
         if not prompts or len(prompts) > self.sequences or not all(len(p) for p in prompts):
             raise ValueError(f"generate: 1 to {self.sequences} prompts of at least a token are needed")
         longest = max(len(p) for p in prompts)

@@ -203,3 +203,48 @@ def test_wrong_tokens_and_sampling():
     likeliest = gen.next_tokens(h)
     assert torch.equal(gen.next_tokens(h, temperature=1.0, top_p=1e-6), likeliest)
     assert torch.equal(gen.next_tokens(h, temperature=1.0, top_k=1), likeliest)
+
+
+def test_every_end_token_ends_an_answer(tmp_path, monkeypatch, capsys):
+    """Models with several end tokens: config.json's own, those beside its text_config, those of generation_config.json."""
+    from safetensors.torch import save_file
+
+    from micro_engram.tools import infer
+
+    assert G.GemmaConfig.from_dict({"eos_token_id": [1, 106]}).eos_token_id == [1, 106]
+    assert G.GemmaConfig.from_dict({"text_config": {"eos_token_id": 1}, "eos_token_id": [1, 106]}).eos_token_id == [1, 106]
+    assert G.GemmaConfig.from_dict({"text_config": {"hidden_size": 64}, "eos_token_id": [106, 7]}).eos_token_id == [106, 7]
+    for same, ids in ((1, {"eos_token_id": 1}), (1, {"eos_token_id": [1]}), (1, {}), (None, {"eos_token_id": None}), (None, {"eos_token_id": []}),
+                      (1, {"text_config": {"eos_token_id": 1}, "eos_token_id": None}), (1, {"text_config": {}, "eos_token_id": None}), (0, {"eos_token_id": [0, 0]})):
+        assert G.GemmaConfig.from_dict(ids).eos_token_id == same
+    model, _ = small_model(engram=False)
+    model.config.eos_token_id = None
+    gen = Generator(model, 1, 64)
+    answer = gen.generate([[5, 9, 11]], 20)[0]
+    stop, want = answer[0], answer[:1]
+    assert len(answer) == 20
+    never = next(t for t in range(256) if t not in answer)
+    model.config.eos_token_id = [never, stop]
+    assert gen.generate([[5, 9, 11]], 20)[0] == want
+
+    class Tok:
+        def __call__(self, text, return_tensors=None):
+            return type("E", (), {"input_ids": torch.tensor([[5, 9, 11]])})
+
+        def decode(self, ids, skip_special_tokens=False):
+            return " ".join(map(str, ids))
+
+    import transformers
+
+    monkeypatch.setattr(transformers.AutoTokenizer, "from_pretrained", lambda *a, **k: Tok())
+    monkeypatch.setattr(torch.cuda, "is_available", lambda: False)
+    monkeypatch.setattr(infer, "plan_engrams", lambda args: [])
+    save_file({k: v.clone().contiguous() for k, v in model.state_dict().items()}, str(tmp_path / "model.safetensors"))
+    text = {**model.config.to_dict(), "eos_token_id": never}
+    places = [({**text, "eos_token_id": [never, stop]}, None), ({"text_config": text, "eos_token_id": [never, stop]}, None),
+              (text, {"eos_token_id": [never, stop]}), (text, {"eos_token_id": stop})]
+    for conf, generation in places:
+        (tmp_path / "config.json").write_text(json.dumps({**conf, "model_type": "gemma4_text"}))
+        (tmp_path / "generation_config.json").write_text(json.dumps(generation or {}))
+        infer.main(["--model", str(tmp_path), "--prompt", "x", "--max-new-tokens", "20", "--temperature", "0", "--native", "--max-len", "64"])
+        assert list(map(int, capsys.readouterr().out.rsplit("--- output ---\n", 1)[1].split())) == want
