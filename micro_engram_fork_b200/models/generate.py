@@ -17,6 +17,15 @@ from ..ops.linear import linear
 from ..ops.objectives import MAX_TOP, top_logits
 
 
+def draw(p, top_p, u):
+    """[rows, 1]: a rank for each row of falling probabilities p and uniform number u of [0, 1), among those that together have top_p."""
+    p = torch.where(p.cumsum(1) - p < top_p, p, 0.0)
+    upto = p.cumsum(1)
+    last = ((p > 0).sum(1, keepdim=True) - 1).clamp_min(0)  # (a row of NaN: rank 0)
+    # u times the last sum may round up to it, and behind the last kept rank the sums stay the same
+    return (upto <= u * upto[:, -1:]).sum(1, keepdim=True).minimum(last)
+
+
 class PagedCache:
     """Pages of all layers for `sequences` sequences of up to max_len tokens, extended by up to `chunk` tokens a call."""
 
@@ -112,10 +121,7 @@ class Generator:
         k = min(top_k or MAX_TOP, MAX_TOP, z.shape[1])
         values, ids, lse = top_logits(z, k, softcap=cap, temperature=temperature)
         p = torch.exp(values / temperature - lse[:, None])
-        before = p.cumsum(1) - p
-        p = torch.where(before < top_p, p, 0.0)  # (the likeliest always stays)
-        u = torch.rand(p.shape[0], 1, device=p.device, generator=generator) * p.sum(1, keepdim=True)
-        return ids.gather(1, (p.cumsum(1) <= u).sum(1, keepdim=True).clamp_max(k - 1))[:, 0]
+        return ids.gather(1, draw(p, top_p, torch.rand(p.shape[0], 1, device=p.device, generator=generator)))[:, 0]
 
     @torch.no_grad()
     def generate(self, prompts, max_new_tokens, temperature=0.0, top_p=1.0, top_k=0, eos=None, generator=None):

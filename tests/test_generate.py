@@ -248,3 +248,22 @@ def test_every_end_token_ends_an_answer(tmp_path, monkeypatch, capsys):
         (tmp_path / "generation_config.json").write_text(json.dumps(generation or {}))
         infer.main(["--model", str(tmp_path), "--prompt", "x", "--max-new-tokens", "20", "--temperature", "0", "--native", "--max-len", "64"])
         assert list(map(int, capsys.readouterr().out.rsplit("--- output ---\n", 1)[1].split())) == want
+
+
+@pytest.mark.parametrize("top_p", [0.5, 0.9, 1.0])
+def test_draws_stay_among_the_kept(top_p):
+    """The smallest and the largest number that torch.rand gives draw a token that top_p has kept, of any row."""
+    from micro_engram_fork_b200.models.generate import draw
+
+    g = torch.Generator().manual_seed(0)
+    p = torch.softmax(2 * torch.randn(4000, 256, generator=g), 1).sort(1, descending=True).values
+    kept = p.cumsum(1) - p < top_p
+    rows = torch.arange(4000)
+    for u in (0.0, 1 - 2.0 ** -24):
+        rank = draw(p, top_p, torch.full((4000, 1), u))[:, 0]
+        assert bool(kept[rows, rank].all()) and bool((p[rows, rank] > 0).all())
+    assert bool((draw(p, top_p, torch.zeros(4000, 1)) == 0).all())
+    # a certain token and columns of nothing behind it
+    p = torch.tensor([[1.0, 0.0, 0.0]]).expand(2, 3)
+    assert draw(p, top_p, torch.tensor([[0.0], [1 - 2.0 ** -24]])).tolist() == [[0], [0]]
+    assert draw(torch.full((1, 5), math.nan), top_p, torch.tensor([[0.5]])).tolist() == [[0]]  # (an index that exists)
