@@ -29,9 +29,10 @@ CPU tensors run the plain PyTorch forms below, which compute in fp32 (fp64 for f
 Every wait inside the attention kernels is bounded; one that ran out (which no input causes) leaves its results wrong
 and a code on the device: check_waits raises where there is one (it waits for the device, so callers do it where they do anyway).
 
-There is no gradient: a call on tensors that require one is refused while gradients are recorded.
+There is no gradient: a call on tensors that require one is refused while gradients are recorded, and one on tensors with a tangent.
 """
 import torch
+from torch.autograd import forward_ad
 
 from .. import native
 from . import use_native
@@ -44,6 +45,9 @@ DIMS = (64, 128, 256, 512)
 def _no_gradient(what, *tensors):
     if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
         raise ValueError(f"{what} has no gradient: call it under torch.no_grad()")
+    # (without a level there are no tangents, and looking at six tensors would cost a call 3.4 us)
+    if forward_ad._current_level >= 0 and any(forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise ValueError(f"{what} has no gradient: a tensor has a tangent")
 
 
 # ------------------------------------------------------------------------- argument checks of the plain forms

@@ -292,3 +292,27 @@ def check_lse_of_padding(device, dtype, lens, max_q):
 
 def test_lse_of_padding():
     check_lse_of_padding("cpu", F32, [(30, 1), (100, 3)], None)
+
+
+def check_forward_mode(device, dtype):
+    """There is no gradient of either mode: tensors with a tangent are refused, in a dual level and under torch.func."""
+    from torch.autograd import forward_ad
+
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    qkv, q_w, k_w, f = append_inputs(b, False, dtype)
+    calls = [(b.q, lambda t: paged.paged_attention(t, *b.args())), (b.k, lambda t: paged.paged_attention(b.q, t, *b.args()[1:])),
+             (b.q.clone(), lambda t: paged.paged_attention(b.q, *b.args(), out=t)),
+             (qkv, lambda t: paged.qkv_norm_rope_append(t, q_w, k_w, f, *b.args(), 4)),
+             (q_w, lambda t: paged.qkv_norm_rope_append(qkv, t, k_w, f, *b.args(), 4))]
+    for t, call in calls:
+        t = t.nan_to_num(1.0)
+        with forward_ad.dual_level():
+            with pytest.raises(ValueError, match="no gradient"):
+                call(forward_ad.make_dual(t, torch.ones_like(t)))
+            call(t)
+        with pytest.raises(ValueError, match="no gradient"):
+            torch.func.jvp(call, (t,), (torch.ones_like(t),))
+
+
+def test_forward_mode():
+    check_forward_mode("cpu", F32)

@@ -327,3 +327,7 @@ def test_append_many(hq, hk, d):
 def test_lse_of_padding(lens, max_q):
     """The kernel of few rows, that of chunks, both."""
     test_paged.check_lse_of_padding(DEV, BF, lens, max_q)
+
+
+def test_forward_mode():
+    test_paged.check_forward_mode(DEV, BF)
