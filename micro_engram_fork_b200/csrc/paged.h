@@ -57,7 +57,8 @@ const char* launch_paged_attention(const PagedAttentionArgs& a, void* workspace,
 // Its part for sequences with more than `least_rows` rows (new tokens times query heads of a key head): paged_tiles.cu.
 int64_t paged_tiles_workspace(const PagedAttentionArgs& a);
 const char* launch_paged_tiles(const PagedAttentionArgs& a, int least_rows, void* workspace, cudaStream_t stream);
-// The current device's first wait that ran out (a StatusCode, 0: none; waits for the device).
-int paged_status(int* detail);
+// On the current device: blocks in which a wait ran out since the process began, and where the last of them waited. Waits for `stream`, which is not
+// being captured.
+cudaError_t paged_waits(int (&words)[2], cudaStream_t stream);
 
 }  // namespace me

@@ -23,7 +23,7 @@
 //
 // Units (sequence, tile of rows, key head, half of the columns) are dealt to the pairs in turn, the longest of a sequence first. With few of them a
 // sequence's keys are cut into chunks, whose (max, sum, O) a second kernel joins.
-// Every wait is bounded (2 s); a timeout records ME_ERR_TIMEOUT in the status word and the kernel frees tensor memory and returns.
+// Every wait is bounded (2 s); where one runs out the block gives up, frees tensor memory, counts itself in g_waits and returns.
 //
 // Measured: 2048 new tokens over 16048, 32 query heads on 4 of dim 512: 2.29 ms, 880 TFLOP/s of what has to be computed (0.53 of the measured
 // bf16 rate; the tensor cores are 78% busy, a third of it with S a second time). 4096 new tokens under a window of 1024, 32 heads on 16 of dim 256: 195 us,
@@ -83,8 +83,13 @@ struct TilesArgs {
   int plog;
   int least_rows;   // sequences with up to this many rows are others' work
 };
-// The first wait that ran out (ME_ERR_TIMEOUT, where): a device's own word, not an allocation that a captured graph could own.
-__device__ int g_status[2];
+// Blocks in which a wait ran out since the process began, and where the last of them waited: a device's own words, not an allocation that a captured
+// graph could own. Nobody sets them back, so that every caller sees what ran out between two looks of its own.
+__device__ int g_waits[2];
+ME_DEVICE void count_wait(int where) {
+  atomicAdd(&g_waits[0], 1);
+  g_waits[1] = where;
+}
 
 // ------------------------------------------------------------------------------- units of work
 struct UnitsOf {
@@ -342,9 +347,9 @@ __global__ void __launch_bounds__(kThreads, 1)
   const bool leader = rank == 0;
   const int pair = blockIdx.x >> 1;
   const int group = args.group, tokens = args.tokens;
-  int* status = g_status;
+  int* status = reinterpret_cast<int*>(smem + C::BAR_OFF + 632);  // what went wrong first in this block, and where
   if (smem_addr(smem) & 1023) {
-    report(status, ME_ERR_ALIGN, 76);
+    if (threadIdx.x == 0) count_wait(76);
     return;
   }
 
@@ -359,6 +364,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(all_done, 1);
     for (int i = 0; i < 2; ++i) mbar_init(&next_full[i], 1), mbar_init(&next_empty[i], 2 + kSoftWarps + (leader ? 1 : 0));
     *abort = 0;
+    status[0] = status[1] = 0;
     fence_barrier_init();
     prefetch_tmap(&tq);
     prefetch_tmap(&tk);
@@ -785,6 +791,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
   tc_fence_before();
   __syncthreads();
+  if (threadIdx.x == 0 && status[0] != 0) count_wait(status[1]);
+  __syncwarp();
   cluster_sync();  // both SMs are done with every product, copy and remote arrival
   if (warp == 1) {
     tc_fence_after();
@@ -945,14 +953,13 @@ const char* launch(const PagedAttentionArgs& a, int least_rows, void* space, cud
 
 }  // namespace
 
-int paged_status(int* detail) {
-  int word[2] = {0, 0};
-  cudaDeviceSynchronize();  // (streams that do not wait for the default one)
-  cudaMemcpyFromSymbol(word, g_status, sizeof word);
-  const int none[2] = {0, 0};
-  if (word[0] != 0) cudaMemcpyToSymbol(g_status, none, sizeof none);
-  *detail = word[1];
-  return word[0];
+cudaError_t paged_waits(int (&words)[2], cudaStream_t stream) {
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;  // (another thread's capture goes on)
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  cudaError_t e = cudaMemcpyFromSymbolAsync(words, g_waits, sizeof words, 0, cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess) e = cudaStreamSynchronize(stream);
+  cudaThreadExchangeStreamCaptureMode(&mode);
+  return e;
 }
 
 namespace {

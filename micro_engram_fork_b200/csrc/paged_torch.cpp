@@ -1,5 +1,6 @@
 // PyTorch side of the paged cache: argument checks, outputs, workspace, the current stream.
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/CUDAGraphsUtils.cuh>
 #include <c10/cuda/CUDAException.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/types.h>
@@ -184,10 +185,13 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
   return {o, lse};
 }
 
-// (code, where) of the first device wait that ran out in the attention on this device since the last call; (0, 0): none.
+// (blocks, where): blocks of the attention kernels on this device in which a wait ran out since the process began, and where the last of them
+// waited; what the device's current stream has ahead is in it.
 std::vector<int64_t> paged_status(int64_t device) {
   const c10::cuda::CUDAGuard guard((c10::DeviceIndex)device);
-  int detail = 0;
-  const int code = me::paged_status(&detail);
-  return {code, detail};
+  TORCH_CHECK(at::cuda::currentStreamCaptureStatusMayInitCtx() == at::cuda::CaptureStatus::None,
+              "paged_status: it waits for the current stream, which is being captured");
+  int words[2] = {0, 0};
+  C10_CUDA_CHECK(me::paged_waits(words, at::cuda::getCurrentCUDAStream()));
+  return {words[0], words[1]};
 }

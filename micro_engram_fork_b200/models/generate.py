@@ -134,6 +134,7 @@ class Generator:
             raise ValueError(f"generate: a prompt of {longest} and {max_new_tokens} new tokens do not fit the cache's {self.cache.max_len}")
         eos = self.model.config.eos_token_id if eos is None else eos
         stop = set() if eos is None else set(eos) if isinstance(eos, (set, list, tuple)) else {eos}
+        waits = paged.waits_out(self.device)
         self.reset()
         rest = [list(map(int, p)) for p in prompts] + [[]] * (self.sequences - len(prompts))
         last = [None] * len(prompts)  # final hidden state of a prompt's last token
@@ -161,5 +162,5 @@ class Generator:
             if not live or step + 1 == max_new_tokens:
                 break
             hidden = self.extend(new)
-        paged.check_waits(self.device)
+        paged.check_waits(self.device, waits)
         return answers

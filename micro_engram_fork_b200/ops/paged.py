@@ -27,7 +27,8 @@ CPU tensors run the plain PyTorch forms below, which compute in fp32 (fp64 for f
   empty rows a row that sees no key: 0, lse -inf.
 
 Every wait inside the attention kernels is bounded; one that ran out (which no input causes) leaves its results wrong
-and a code on the device: check_waits raises where there is one (it waits for the device, so callers do it where they do anyway).
+and is counted on the device, for good: a caller takes the count (waits_out) before its calls and compares it after them
+(check_waits), whoever else does; another caller's between the two raises as well. Both wait for the current stream.
 
 There is no gradient: a call on tensors that require one is refused while gradients are recorded, and one on tensors with a tangent.
 """
@@ -201,11 +202,22 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         return paged_attention_ref(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(window or 0), float(scale), out)
 
 
-def check_waits(device):
-    """Raises if a bounded wait of the attention kernels ran out on this device since the last look."""
+def _waits(device):
     device = torch.device(device)
     if device.type != "cuda":
-        return
-    code, where = native().paged_status(torch.cuda.current_device() if device.index is None else device.index)
-    if code:
-        raise RuntimeError(f"paged_attention: a wait on the device ran out (code {code}, at {where}); results since the last check are not valid")
+        return 0, 0
+    return native().paged_status(torch.cuda.current_device() if device.index is None else device.index)
+
+
+def waits_out(device):
+    """How often a bounded wait of the attention kernels has run out on this device in this process, up to what its current stream
+    has ahead."""
+    return _waits(device)[0]
+
+
+def check_waits(device, since=0):
+    """Raises if a bounded wait of the attention kernels ran out on this device since waits_out gave `since` (0: in this process)."""
+    count, where = _waits(device)
+    if count != since:
+        raise RuntimeError(f"paged_attention: {count - since} waits on the device ran out (the last at {where}); results since the count was "
+                           f"{since} are not valid")

@@ -267,3 +267,24 @@ def test_draws_stay_among_the_kept(top_p):
     p = torch.tensor([[1.0, 0.0, 0.0]]).expand(2, 3)
     assert draw(p, top_p, torch.tensor([[0.0], [1 - 2.0 ** -24]])).tolist() == [[0], [0]]
     assert draw(torch.full((1, 5), math.nan), top_p, torch.tensor([[0.5]])).tolist() == [[0]]  # (an index that exists)
+
+
+def test_generate_raises_for_its_own_waits(monkeypatch):
+    """Waits that ran out before a call, or that another caller has looked at, change nothing; those within it raise."""
+    from micro_engram_fork_b200.ops import paged
+
+    model, _ = small_model(engram=False)
+    gen = Generator(model, 1, 64)
+    state = {"count": 4, "new": 0}
+
+    def waits(device):
+        state["count"] += state["new"]
+        return state["count"], 71
+
+    monkeypatch.setattr(paged, "_waits", waits)
+    answer = gen.generate([[5, 9]], 3, eos=-1)
+    state["new"] = 1
+    with pytest.raises(RuntimeError, match="ran out"):
+        gen.generate([[5, 9]], 3, eos=-1)
+    state["new"] = 0
+    assert gen.generate([[5, 9]], 3, eos=-1) == answer

@@ -316,3 +316,26 @@ def check_forward_mode(device, dtype):
 
 def test_forward_mode():
     check_forward_mode("cpu", F32)
+
+
+def test_a_wait_that_ran_out_is_every_callers(monkeypatch):
+    """Two callers on a device: the one that looks first takes nothing from the other."""
+    class Native:
+        words = [2, 71]
+
+        def paged_status(self, device):
+            assert device == 1
+            return list(self.words)
+
+    fake = Native()
+    monkeypatch.setattr(paged, "native", lambda: fake)
+    assert paged.waits_out("cpu") == 0
+    first, second = paged.waits_out("cuda:1"), paged.waits_out("cuda:1")
+    paged.check_waits("cuda:1", first)
+    fake.words = [5, 72]
+    for since in (first, second, first):
+        with pytest.raises(RuntimeError, match="3 waits .* ran out .*at 72"):
+            paged.check_waits("cuda:1", since)
+    paged.check_waits("cuda:1", paged.waits_out("cuda:1"))
+    with pytest.raises(RuntimeError):
+        paged.check_waits("cuda:1")

@@ -331,3 +331,25 @@ def test_lse_of_padding(lens, max_q):
 
 def test_forward_mode():
     test_paged.check_forward_mode(DEV, BF)
+
+
+def test_waits_are_counted_beside_a_capture():
+    """Looking at the count in one thread leaves another's capture whole; a stream that is captured is refused."""
+    import threading
+
+    batch = oracle.Batch([(900, 40), (50, 1)], 8, 2, 128, 32, None, BF, DEV)
+    want = [t.clone() for t in paged.paged_attention(batch.q, *batch.args())]
+    seen = []
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = paged.paged_attention(batch.q, *batch.args())
+        look = threading.Thread(target=lambda: (paged.check_waits(DEV), seen.append(paged.waits_out(DEV))))
+        look.start()
+        look.join()
+        with pytest.raises(RuntimeError, match="captured"):
+            paged.waits_out(DEV)
+    assert seen == [0]
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+    with torch.cuda.stream(torch.cuda.Stream()):
+        paged.check_waits(DEV, paged.waits_out(DEV))
