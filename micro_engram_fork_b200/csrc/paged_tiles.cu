@@ -435,10 +435,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (n <= 0) continue;
       const int y0 = u.kv << args.plog;
       // The table's entries for four blocks, a lane for each 16 keys: read four blocks ahead and looked at when they are needed (a look at
-      // once would wait for memory in every block, which held most SMs at 5000 to 6000 clocks a block).
+      // once would wait for memory in every block, which held most SMs at 5000 to 6000 clocks a block). Runs of `box` keys that no new token sees
+      // are none: their pages may be another's by now.
       auto pages_of = [&](int kb) {
-        const int col = (kb * BN + lane * 16) >> args.plog;
-        return col < p.width ? p.table[u.b * p.table_stride + col] : -1;
+        const int key = kb * BN + lane * 16, run = key & ~(box - 1);
+        return run + box > seq.lo && run < seq.hi ? p.table[u.b * p.table_stride + (key >> args.plog)] : -1;  // (seq.hi is within the table's row)
       };
       // 64 keys from `in` of block kb, NC x 64 columns from chunk x on
       auto load64 = [&](uint32_t dst, const CUtensorMap* map, uint32_t bar, int kb, int in, int ids, int x, auto NC) {
@@ -635,7 +636,10 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_after();
         if (any_mine) {  // (rows of nothing: P may be what it is)
           uint32_t pages = 0xff;
-          if (!whole) pages = __ballot_sync(0xffffffffu, lane < 8 && page_at(p, a.cache.pages, u.b, (key0 + (lane & 7) * 16) >> args.plog) >= 0);
+          if (!whole) {
+            const int key = key0 + (lane & 7) * 16;
+            pages = __ballot_sync(0xffffffffu, lane < 8 && key + 15 >= seq.lo && key < seq.hi && page_at(p, a.cache.pages, u.b, key >> args.plog) >= 0);
+          }
           const bool open = __all_sync(0xffffffffu, pages == 0xffu && ((key0 >= from && key0 + BN - 1 <= last) || !mine));
           auto scores = [&](int c, uint32_t(&s)[2][32]) {  // 64 of them from column c on
             tmem_issue_ld32(at + c, s[0]);

@@ -353,3 +353,20 @@ def test_waits_are_counted_beside_a_capture():
     assert all(torch.equal(a, b) for a, b in zip(out, want))
     with torch.cuda.stream(torch.cuda.Stream()):
         paged.check_waits(DEV, paged.waits_out(DEV))
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("lens", [[(300, 1), (400, 1)], [(530, 40)], [(500, 1), (330, 70), (1000, 1), (40, 1), (900, 2)]])
+def test_places_before_the_window(lens, page):
+    """What the table holds for pages that no new token sees (here others' pages) changes nothing, with pages that are none among those seen or not."""
+    for gap in (False, True):
+        batch = oracle.Batch(lens, 4, 2, 64, page, 150, BF, DEV, seed=page)
+        if gap:
+            for b in range(len(lens)):
+                batch.table[b, batch.first[b] + 1] = -1
+        want = paged.paged_attention(batch.q, *batch.args(), window=150)
+        for b, first in enumerate(batch.first):
+            batch.table[b, :first] = batch.table[0, batch.first[0]] if b else batch.k.shape[0] - 1
+            batch.table[b, -1] = 0
+        got = paged.paged_attention(batch.q, *batch.args(), window=150)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and bool(got[0].isfinite().all())
