@@ -148,3 +148,39 @@ def close_append(got, want, size, dtype=torch.bfloat16):
     tol = HALF_STEP[dtype] * want.abs() * 1.01 + size * unit
     bad = ~((got.double() - want).abs() <= tol)
     assert not bool(bad.any()), f"{int(bad.sum())} of {bad.numel()} off, the worst by {float(((got.double() - want).abs() / tol).nan_to_num(1e9).max())} tolerances"
+
+
+def attention_of_pages(batch, scale=1.0):
+    """attention() of a batch whose table may have anything in it: what each token sees is worked out position by position from the table, the
+    lengths and the window. Rows that see nothing: 0 and -inf."""
+    hq, hk, d, page = batch.hq, batch.hk, batch.d, batch.page
+    dev = batch.q.device
+    o = torch.zeros(batch.tokens, hq, d, dtype=torch.float64, device=dev)
+    spread = torch.zeros_like(o)
+    lse = torch.full((hq, batch.tokens), -math.inf, dtype=torch.float64, device=dev)
+    size = torch.zeros(hq, batch.tokens, dtype=torch.float64, device=dev)
+    table, lengths = batch.table.tolist(), batch.seq_lens.tolist()
+    for b, length in enumerate(lengths):
+        s, n = batch.starts[b], batch.starts[b + 1] - batch.starts[b]
+        lo = max(0, length - n - batch.window + 1) if batch.window else 0
+        there = [p for p in range(lo, min(length, len(table[b]) * page)) if 0 <= table[b][p // page] < batch.k.shape[0]]
+        if n == 0 or not there:
+            continue
+        ids = torch.tensor([table[b][p // page] for p in there], device=dev)
+        row = torch.tensor([p % page for p in there], device=dev)
+        pos = torch.tensor(there, device=dev)
+        k, v = (t[ids, :, row].double().transpose(0, 1) for t in (batch.k, batch.v))  # [Hk, keys, D]
+        for i in range(n):
+            p = length - n + i
+            seen = (pos <= p) & (pos > p - batch.window if batch.window else pos <= p)
+            if not bool(seen.any()):
+                continue
+            kk, vv = k[:, seen], v[:, seen]
+            qq = batch.q[s + i].double().view(hk, hq // hk, d)
+            x = scale * torch.matmul(qq, kk.transpose(1, 2))
+            w = torch.softmax(x, -1)
+            o[s + i] = torch.matmul(w, vv).reshape(hq, d)
+            spread[s + i] = torch.matmul(w, vv.abs()).reshape(hq, d)
+            lse[:, s + i] = torch.logsumexp(x, -1).reshape(hq)
+            size[:, s + i] = abs(scale) * torch.matmul(qq.abs(), kk.abs().transpose(1, 2)).amax(-1).reshape(hq)
+    return o, lse, spread, size

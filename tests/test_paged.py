@@ -339,3 +339,33 @@ def test_a_wait_that_ran_out_is_every_callers(monkeypatch):
     paged.check_waits("cuda:1", paged.waits_out("cuda:1"))
     with pytest.raises(RuntimeError):
         paged.check_waits("cuda:1")
+
+
+def with_missing_pages(lens, hq, hk, d, page, window, dtype, device, index=torch.int32):
+    """A batch with numbers that are no pages first, last and between those that its tokens see, a sequence without any page, and a length that passes
+    the table's row (the row's last place has a page, so what a page has past its sequence's end is seen too: all rows are numbers)."""
+    batch = oracle.Batch(lens, hq, hk, d, page, window, dtype, device, seed=page + d, before=1, after=2, index=index)
+    for t in (batch.k, batch.v):
+        t.copy_(torch.randn(t.shape, generator=torch.Generator().manual_seed(d)).to(t))
+    pages, width = batch.k.shape[0], batch.table.shape[1]
+    wrong = [pages, -1, 2 ** 31 - 1, -2 ** 31] + ([2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 63 - 1] if index == torch.int64 else [])
+    for b, (c, n) in enumerate(lens):
+        first, last = batch.first[b], (c + n - 1) // page
+        for i, col in enumerate({0: [first], 1: [last], 2: [(first + last) // 2, (first + last) // 2 + 1], 3: range(first, width), 4: [first, last]}[b % 5]):
+            if col < width:
+                batch.table[b, col] = wrong[(b + i) % len(wrong)]
+    last = len(lens) - 1
+    batch.table[last] = torch.arange(width) % pages
+    batch.seq_lens[last] = width * page + max(1, lens[last][1] // 2)
+    return batch
+
+
+@pytest.mark.parametrize("window", [None, 40])
+def test_missing_pages(window):
+    for index in (torch.int32, torch.int64):
+        batch = with_missing_pages([(60, 20), (100, 3), (90, 30), (20, 5), (33, 1), (50, 20)], 4, 2, 64, 16, window, F64, "cpu", index)
+        got = paged.paged_attention(batch.q, *batch.args(), window=window)
+        oracle.close_attention(got, oracle.attention_of_pages(batch), 64, False, F64)
+    whole = oracle.Batch([(60, 20), (100, 3), (0, 4)], 4, 2, 64, 16, window, F64)
+    for a, b in zip(oracle.attention_of_pages(whole, 0.5), oracle.attention(whole, 0.5)):
+        assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)

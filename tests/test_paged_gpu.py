@@ -370,3 +370,83 @@ def test_places_before_the_window(lens, page):
             batch.table[b, -1] = 0
         got = paged.paged_attention(batch.q, *batch.args(), window=150)
         assert all(torch.equal(x, y) for x, y in zip(got, want)) and bool(got[0].isfinite().all())
+
+
+# Batches that the kernel of few rows takes, that of chunks, and both of them (with 2 rows a token; the last sequence's length passes its table's row).
+MIXES = {"rows": [(60, 3), (100, 1), (90, 4), (20, 5), (33, 1), (50, 2)], "chunks": [(300, 40), (120, 130)],
+         "both": [(300, 30), (100, 1), (500, 2), (20, 5), (133, 1), (40, 1), (50, 20)]}
+
+
+@pytest.mark.parametrize("mix", MIXES)
+@pytest.mark.parametrize("window", [None, 100])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (256, 64), (512, 128), (512, 16), (256, 128)])
+def test_missing_pages(d, page, window, mix):
+    for index in (torch.int32, torch.int64):
+        batch = test_paged.with_missing_pages(MIXES[mix], 4, 2, d, page, window, BF, DEV, index)
+        got = paged.paged_attention(batch.q, *batch.args(), window=window)
+        oracle.close_attention(got, oracle.attention_of_pages(batch), d, mix == "rows")
+    assert bool((got[0][0] == 0).all()) and bool((got[1][:, -2:] == -math.inf).all())
+
+
+@pytest.mark.parametrize("scale", [0.04, 0.3, 2.5])
+@pytest.mark.parametrize("mix", MIXES)
+@pytest.mark.parametrize("d", [64, 256, 512])
+def test_scales(d, mix, scale):
+    batch = oracle.Batch(MIXES[mix], 4, 2, d, 32, 200, BF, DEV, seed=d)
+    _attend(batch, mix == "rows", scale=scale)
+
+
+@pytest.mark.parametrize("group,d", [(17, 64), (17, 512), (24, 256), (40, 128), (64, 64), (65, 256), (100, 512), (128, 64), (128, 256)])
+@pytest.mark.parametrize("lens", [[(5, 1), (300, 1), (64, 1), (0, 1), (1000, 1)], [(200, 9), (37, 1)], [(60, 3), (250, 2), (0, 4), (90, 1), (130, 2)]])
+def test_many_query_heads(lens, group, d):
+    """Up to 128 query heads a key head: tiles of few tokens, rows of a tile that no token has."""
+    for hk in (1, 2):
+        _attend(oracle.Batch(lens, group * hk, hk, d, 16, None, BF, DEV, seed=group, before=1, after=1), False)
+
+
+@pytest.mark.parametrize("d", [64, 256, 512])
+@pytest.mark.parametrize("lens", [[(3000, 40), (5000, 1)], [(2000, 300), (700, 5), (4000, 2)], [(9, 70), (4000, 5), (3000, 1), (20, 17), (100, 1), (8, 1), (5, 2)]])
+def test_max_q_too_low_for_chunks(lens, d):
+    """Longer runs than max_q says: such sequences are not cut, the others are."""
+    for max_q in (5, 9):
+        _attend(oracle.Batch(lens, 8, 2, d, 64, None, BF, DEV, seed=d), False, max_q=max_q)
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("window", [None, 70])
+def test_sixteen_rows_keep_both_terms(d, window):
+    """Drafts of 9 to 16 rows a key head, in units that are cut and whole ones: as near as single tokens."""
+    for hq, hk in ((8, 2), (3, 1)):
+        lens = [(900, 4), (63, 3), (0, 4), (2000, 3), (17, 1), (128, 4)]
+        _attend(oracle.Batch(lens, hq, hk, d, 16, window, BF, DEV, seed=hq), True, max_q=4)
+
+
+@pytest.mark.parametrize("d", [64, 256, 512])
+@pytest.mark.parametrize("lens", [[(400, 40), (90, 130)], [(6000, 40)], [(400, 30), (60, 1), (300, 2), (2000, 1), (7, 1)]])
+def test_values_at_the_edge_in_chunks(lens, d):
+    """Values and keys that are infinite or NaN, at a position that every new token of a sequence sees: they reach that sequence's rows and
+    columns and no others; a score of -inf is a key that is not seen."""
+    for bad in (math.nan, math.inf):
+        batch = oracle.Batch(lens, 4, 2, d, 16, None, BF, DEV, seed=d)
+        clean, clean_lse = paged.paged_attention(batch.q, *batch.args())
+        n = lens[0][1]
+        page = int(batch.table[0, 1])
+        was = float(batch.v[page, 0, 3, 5])
+        batch.v[page, 0, 3, 5] = bad
+        o, lse = paged.paged_attention(batch.q, *batch.args())
+        assert not bool(o[:n, :2, 5].isfinite().any()) and torch.equal(lse, clean_lse)
+        o[:n, :2, 5] = clean[:n, :2, 5]
+        assert torch.equal(o, clean)
+        batch.v[page, 0, 3, 5] = was
+        batch.k[page, 0, 3] = bad
+        batch.q[:n, 0], batch.q[:n, 1] = 1.0, -1.0  # scores of inf, and of -inf
+        o, lse = paged.paged_attention(batch.q, *batch.args())
+        assert not bool(o[:n, 0].isfinite().any()) and torch.equal(o[n:], clean[n:]) and torch.equal(o[:, 2:], clean[:, 2:])
+        assert not bool(lse[0, :n].isfinite().any()) and torch.equal(lse[:, n:], clean_lse[:, n:])
+        if bad == math.inf:
+            k = batch.k.clone()
+            k[page, 0, 3] = 100.0  # a score of -100 d: no share in 32 bits either
+            want = paged.paged_attention(batch.q, k, *batch.args()[1:])
+            assert torch.equal(o[:n, 1], want[0][:n, 1]) and torch.equal(lse[1, :n], want[1][1, :n])
+        else:
+            assert not bool(o[:n, 1].isfinite().any())
