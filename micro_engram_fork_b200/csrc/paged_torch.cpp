@@ -44,6 +44,23 @@ me::PagedCache check_cache(const Tensor& k, const Tensor& v) {
   return {k.data_ptr(), v.data_ptr(), pages == 1 ? whole : k.stride(0), pages == 1 ? whole : v.stride(0), (int)pages, (int)heads, (int)page, (int)dim};
 }
 
+// Whether a page of keys lies over one of values. Pages of each are in order of their addresses.
+bool overlap(const me::PagedCache& c) {
+  const int64_t whole = (int64_t)c.heads * c.page * c.dim;  // elements
+  const int64_t k = reinterpret_cast<intptr_t>(c.k) / 2, v = reinterpret_cast<intptr_t>(c.v) / 2;
+  if (k + (c.pages - 1) * c.k_stride + whole <= v || v + (c.pages - 1) * c.v_stride + whole <= k) return false;
+  if (c.k_stride == c.v_stride) {  // each other's gaps
+    const int64_t by = ((v - k) % c.k_stride + c.k_stride) % c.k_stride;
+    return by < whole || by > c.k_stride - whole;
+  }
+  for (int64_t i = 0, j = 0; i < c.pages && j < c.pages;) {
+    const int64_t by = v + j * c.v_stride - (k + i * c.k_stride);
+    if (by > -whole && by < whole) return true;
+    by > 0 ? ++i : ++j;
+  }
+  return false;
+}
+
 // int32: a number outside its range is no page and no position, and must not come back as another one.
 Tensor narrow(const Tensor& t) { return t.scalar_type() == torch::kInt ? t : t.clamp(-1, INT32_MAX).to(torch::kInt); }
 
@@ -125,6 +142,7 @@ Tensor paged_append(Tensor qkv, Tensor q_w, Tensor k_w, Tensor inv_freq, Tensor 
   a.q_heads = (int)q_heads;
   a.kv_shared = kv_shared;
   a.eps = (float)eps;
+  ME_CHECK_VALUE(!overlap(a.cache), "k_pages and v_pages: they lie over one another, and both are written");
   if (tokens == 0) return q;
   // the kernel writes through the pointers: a graph that has saved the pages learns of it by their versions
   k_pages.unsafeGetTensorImpl()->bump_version();

@@ -62,6 +62,21 @@ def _check_cache(k_pages, v_pages):
         raise ValueError(f"k_pages: a head dimension of 64, 128, 256 or 512 is needed, got {k_pages.shape[3]}")
 
 
+def _overlap(k_pages, v_pages):
+    """Whether a page of keys lies over one of values (pages whose elements are contiguous, as the kernels take them)."""
+    pages, whole, size = len(k_pages), k_pages[0].numel(), k_pages.element_size()
+    k, v = k_pages.data_ptr() // size, v_pages.data_ptr() // size
+    if not (k_pages[0].is_contiguous() and v_pages[0].is_contiguous()):
+        return k == v
+    sk, sv = (whole, whole) if pages == 1 else (k_pages.stride(0), v_pages.stride(0))
+    if k + (pages - 1) * sk + whole <= v or v + (pages - 1) * sv + whole <= k:
+        return False
+    if sk == sv and sk > 0:  # each other's gaps
+        return (v - k) % sk < whole or (v - k) % sk > sk - whole
+    at = sorted([(k + i * sk, 0) for i in range(pages)] + [(v + i * sv, 1) for i in range(pages)])
+    return any(b - a < whole and of != other for (a, of), (b, other) in zip(at, at[1:]))
+
+
 def _check_batch(block_table, cu_seqlens, seq_lens):
     if seq_lens.dim() != 1 or cu_seqlens.dim() != 1 or cu_seqlens.numel() != seq_lens.numel() + 1:
         raise ValueError(f"cu_seqlens, seq_lens: [sequences + 1] and [sequences] are needed, got {tuple(cu_seqlens.shape)} and {tuple(seq_lens.shape)}")
@@ -129,7 +144,7 @@ def qkv_norm_rope_append(qkv, q_w, k_w, inv_freq, k_pages, v_pages, block_table,
     """q [T, Hq, D] of the fused projection's rows qkv [T, (Hq + 2 Hk) D] (or [T, (Hq + Hk) D] with kv_shared: v is
     the raw k); k and v are written into their pages. Each head is normalised (y = x / sqrt(mean x^2 + eps)), q and k take their
     weights [D] and are rotated by position * inv_freq [D / 2] (fp32), v takes neither. All in 32 bits (the angle in 64), rounded
-    once. Two new tokens must not share a place in the cache."""
+    once. Two new tokens must not share a place in the cache, nor pages of keys and of values memory."""
     _no_gradient("qkv_norm_rope_append", qkv, q_w, k_w, inv_freq, k_pages, v_pages)
     args = (qkv, q_w, k_w, inv_freq, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(q_heads), bool(kv_shared), float(eps))
     if use_native(qkv, k_pages):
@@ -143,6 +158,8 @@ def qkv_norm_rope_append(qkv, q_w, k_w, inv_freq, k_pages, v_pages, block_table,
     for t, n, what in ((q_w, d, "q_w"), (k_w, d, "k_w"), (inv_freq, d // 2, "inv_freq")):
         if t.shape != (n,):
             raise ValueError(f"{what}: [{n}] is needed, got {tuple(t.shape)}")
+    if _overlap(k_pages, v_pages):
+        raise ValueError("k_pages and v_pages: they lie over one another, and both are written")
     with torch.no_grad():
         return qkv_norm_rope_append_ref(*args)
 

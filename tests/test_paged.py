@@ -369,3 +369,34 @@ def test_missing_pages(window):
     whole = oracle.Batch([(60, 20), (100, 3), (0, 4)], 4, 2, 64, 16, window, F64)
     for a, b in zip(oracle.attention_of_pages(whole, 0.5), oracle.attention(whole, 0.5)):
         assert torch.allclose(a, b, rtol=1e-12, atol=1e-12)
+
+
+def check_pages_over_one_another(device, dtype):
+    """Appending refuses keys and values in the same memory, and takes them side by side; attention reads them anyhow."""
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    args = append_inputs(b, False, dtype)
+    n, whole = b.k.shape[0], 2 * 16 * 64
+    room = torch.zeros(4 * n * whole, dtype=dtype, device=device)
+
+    def pages(at, stride):
+        return room.as_strided((n, 2, 16, 64), (stride, 16 * 64, 64, 1), at)
+
+    def append(k, v):
+        return paged.qkv_norm_rope_append(*args, k, v, b.table, b.cu, b.seq_lens, 4)
+
+    for k, v in (((0, whole), (0, whole)), ((0, 2 * whole), (whole // 2, 2 * whole)), ((whole, 2 * whole), (8, 2 * whole)), ((0, whole), ((n - 1) * whole, whole)),
+                 ((0, 2 * whole), (whole, 3 * whole)), ((2 * whole, 3 * whole), (0, whole))):
+        for one, two in ((k, v), (v, k)):
+            with pytest.raises(ValueError, match="over one another"):
+                append(pages(*one), pages(*two))
+    want = append(b.k, b.v)
+    for k, v in (((0, 2 * whole), (whole, 2 * whole)), ((0, whole), (n * whole, whole)), ((0, 4 * whole), (2 * whole, 4 * whole)),
+                 ((0, 2 * whole), (2 * (n - 1) * whole + whole, whole))):
+        for one, two in ((k, v), (v, k)):
+            assert torch.equal(append(pages(*one), pages(*two)), want)
+    o, lse = paged.paged_attention(b.q, pages(0, whole), pages(0, whole), b.table, b.cu, b.seq_lens)
+    assert bool(o.isfinite().all())
+
+
+def test_pages_over_one_another():
+    check_pages_over_one_another("cpu", F32)

@@ -450,3 +450,7 @@ def test_values_at_the_edge_in_chunks(lens, d):
             assert torch.equal(o[:n, 1], want[0][:n, 1]) and torch.equal(lse[1, :n], want[1][1, :n])
         else:
             assert not bool(o[:n, 1].isfinite().any())
+
+
+def test_pages_over_one_another():
+    test_paged.check_pages_over_one_another(DEV, BF)
