@@ -165,7 +165,8 @@ std::vector<Tensor> paged_attention(Tensor q, Tensor k_pages, Tensor v_pages, Te
                  " (up to 128 times) are needed, got ", text(q_heads));
   ME_CHECK_VALUE(tokens * q_heads < (1ll << 31), "q: fewer than 2^31 rows (tokens times heads) are needed, got ", shape(q));
   ME_CHECK_VALUE(window >= 0 && window <= INT32_MAX, "window: a positive number or None, got ", text(window));
-  ME_CHECK_VALUE((float)scale > 0 && (float)scale < INFINITY, "scale: a positive number (in 32 bits) is needed");
+  // (the kernels take scores by powers of 2: scale / ln 2 has to be a number in 32 bits)
+  ME_CHECK_VALUE((float)scale > 0 && (float)scale < 0x1p127f, "scale: a positive number (in 32 bits) below 2^127 is needed");
   ME_CHECK_VALUE(max_q >= 0, "max_q: a positive number or None, got ", text(max_q));
   const Batch batch = check_batch(k_pages, table, cu, lens, tokens);
   a.batch = batch.args;

@@ -209,8 +209,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         raise ValueError(f"q: [tokens, heads, {d}] is needed, got {tuple(q.shape)}")
     if q.shape[1] < hk or q.shape[1] % hk or q.shape[1] // hk > 128:
         raise ValueError(f"q: heads a multiple of the pages' {hk} (up to 128 times) are needed, got {q.shape[1]}")
-    if not 0 < float(torch.tensor(scale, dtype=torch.float32)) < float("inf"):
-        raise ValueError(f"scale: a positive number (in 32 bits) is needed, got {scale}")
+    if not 0 < float(torch.tensor(scale, dtype=torch.float32)) < 2.0 ** 127:
+        raise ValueError(f"scale: a positive number (in 32 bits) below 2^127 is needed, got {scale}")
     if out is not None and out.shape != q.shape:
         raise ValueError(f"out: q's shape {tuple(q.shape)} is needed, got {tuple(out.shape)}")
     if out is not None and out.numel() and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():

@@ -400,3 +400,20 @@ def check_pages_over_one_another(device, dtype):
 
 def test_pages_over_one_another():
     check_pages_over_one_another("cpu", F32)
+
+
+def check_largest_scale(device, dtype, lens):
+    """A scale whose 1 / ln 2 fold passes 32 bits is refused; below, equal scores share alike."""
+    b = oracle.Batch(lens, 4, 2, 64, 16, None, dtype, device)
+    for scale in (2.0 ** 127, 3.0e38, 3.4e38):
+        with pytest.raises(ValueError):
+            paged.paged_attention(b.q, *b.args(), scale=scale)
+    b.q.zero_()
+    want = paged.paged_attention(b.q, *b.args())
+    for scale in (1.7e38, 1e-44):
+        got = paged.paged_attention(b.q, *b.args(), scale=scale)
+        assert all(torch.equal(x, y) for x, y in zip(got, want)) and bool(got[0].isfinite().all())
+
+
+def test_largest_scale():
+    check_largest_scale("cpu", F32, [(20, 2), (9, 3)])

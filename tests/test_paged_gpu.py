@@ -454,3 +454,8 @@ def test_values_at_the_edge_in_chunks(lens, d):
 
 def test_pages_over_one_another():
     test_paged.check_pages_over_one_another(DEV, BF)
+
+
+@pytest.mark.parametrize("mix", MIXES)
+def test_largest_scale(mix):
+    test_paged.check_largest_scale(DEV, BF, MIXES[mix])
