@@ -23,7 +23,8 @@
 //
 // Units (sequence, tile of rows, key head, half of the columns) are dealt to the pairs in turn, the longest of a sequence first. With few of them a
 // sequence's keys are cut into chunks, whose (max, sum, O) a second kernel joins.
-// Every wait is bounded (2 s); where one runs out the block gives up, frees tensor memory, counts itself in g_waits and returns.
+// Every wait is bounded: 2 s, 60 s where a whole unit may lie in between (one over 2^31 keys takes up to 40 s; a block that gives up ends these
+// at once). Where one runs out the block gives up, frees tensor memory, counts itself in g_waits and returns.
 //
 // Measured: 2048 new tokens over 16048, 32 query heads on 4 of dim 512: 2.29 ms, 880 TFLOP/s of what has to be computed (0.53 of the measured
 // bf16 rate; the tensor cores are 78% busy, a third of it with S a second time). 4096 new tokens under a window of 1024, 32 heads on 16 of dim 256: 195 us,
@@ -49,6 +50,7 @@ constexpr int kSoftWarps = 4, kFirstSoft = 4, kThreads = (kFirstSoft + kSoftWarp
 constexpr int BM = 128, BN = 128;     // rows an SM, keys a block
 constexpr int kLeastBlocks = 8;       // of a chunk: below, its O costs more to write and join than its keys
 constexpr int kDeals = 4;             // units a pair that cutting aims at
+constexpr uint64_t kUnitLimit = 60000000000ull;
 
 // QR: rows of Q an SM. 64 of them serve calls whose chunks are short (drafts): the product's other 64 rows are then what lies behind,
 // and nobody looks at them; what Q leaves goes to the rings, which such calls need most, for they wait for memory.
@@ -385,15 +387,15 @@ __global__ void __launch_bounds__(kThreads, 1)
   // The `it`-th unit of the pair, by warp 3; false: there is none, or a wait ran out. Whole warps; the numbers are the same in all lanes, and
   // pass a reduction so that they are known to be, and addresses and descriptors that come of them stay in uniform registers.
   auto uniform = [](int x) { return (int)__reduce_or_sync(0xffffffffu, (unsigned)x); };
-  auto wait_u = [&](uint64_t* bar, int parity, int where) {
-    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, status, where, abort));
+  auto wait_u = [&](uint64_t* bar, int parity, int where, uint64_t limit_ns = 2000000000ull) {
+    return __all_sync(0xffffffffu, mbar_try_wait(bar, parity)) || __all_sync(0xffffffffu, mbar_wait(bar, parity, status, where, abort, limit_ns));
   };
   Unit u;
   Keys seq;
   int unit_x = 0;
   bool whole = true;  // every page of the unit's keys is one
   auto take_unit = [&](int it, int where) {
-    if (!wait_u(&next_full[it & 1], (it >> 1) & 1, where)) return false;
+    if (!wait_u(&next_full[it & 1], (it >> 1) & 1, where, kUnitLimit)) return false;
     const int mine = next_unit[(it & 1) * 16 + (lane & 15)];
     __syncwarp();
     if (lane == 0) mbar_arrive(&next_empty[it & 1]);
@@ -599,7 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (key + 15 >= k.lo && key < k.hi) all = all && page_at(p, a.cache.pages, w.b, key >> args.plog) >= 0;
       }
       all = __all_sync(0xffffffffu, all);
-      if (it >= 2 && !wait_u(&next_empty[it & 1], ((it >> 1) - 1) & 1, 80)) break;
+      if (it >= 2 && !wait_u(&next_empty[it & 1], ((it >> 1) - 1) & 1, 80, kUnitLimit)) break;
       int* to = next_unit + (it & 1) * 16;
       if (lane == 0) {
         to[0] = more, to[1] = w.s.first, to[2] = w.s.count, to[3] = w.s.context, to[4] = w.b, to[5] = w.tile, to[6] = w.kv, to[7] = w.half;
