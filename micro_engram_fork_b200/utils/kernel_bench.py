@@ -4,7 +4,7 @@ events (warm-up, synchronize on both sides) and reported against the measured ro
 figures otherwise). Also the workload that the committed ncu summaries in profiles/ capture.
 
   python -m micro_engram_fork_b200.utils.kernel_bench [--case all|gemm|attn_fwd|attn_bwd|gate|ce|qkv|geglu|rows|
-                                                       norms|ce_bwd|nf4|ce_gemm|tp|objectives|paged] [--iters N] [--small]
+                                                       norms|ce_bwd|nf4|ce_gemm|tp|objectives|paged|generate] [--iters N] [--small]
 """
 import argparse
 import json
@@ -447,9 +447,48 @@ def case_paged(C, dev, it, pk):
     return r
 
 
+def case_generate(C, dev, it, pk, layers=12):
+    """Generation with the native decoder as a whole: the benchmark's layers (12 of its 60, random bf16 weights, no engram), 8 prompts of 1000 tokens
+    in chunks of 1024 a sequence, then answers of a token a step, the likeliest (temperature 0), as Generator.generate takes them: wall time with the
+    host's part, the least of three runs. A step's floor is its weights (the output's among them) read once."""
+    import time
+
+    from ..models import gemma as G
+    from ..models.generate import Generator
+
+    cfg = G.config_31b()
+    cfg.num_hidden_layers, cfg.layer_types = layers, cfg.layer_types[:layers]
+    with torch.device("meta"):
+        model = G.GemmaForCausalLM(cfg)
+    model = model.to_empty(device=dev)
+    G.cast_projections_(model, torch.bfloat16)
+    G.init_random_(model)
+    gen = Generator(model.eval(), 8, 1200)
+    g = torch.Generator().manual_seed(0)
+    prompts = torch.randint(3, cfg.vocab_size, (8, 1000), generator=g).tolist()
+
+    def seconds(new):
+        best = float("inf")
+        for _ in range(3):
+            torch.cuda.synchronize()
+            t = time.perf_counter()
+            gen.generate(prompts, new, eos=-1)
+            best = min(best, time.perf_counter() - t)
+        return best
+
+    steps = 64
+    prompt, whole = seconds(1), seconds(1 + steps)
+    step = (whole - prompt) / steps
+    floor = sum(p.numel() * p.element_size() for p in model.parameters()) / (pk["hbm_gbs"] * 1e9)
+    return {f"generate, {layers} layers, 8 prompts of 1000": {"ms": round(prompt * 1e3, 1), "prompt_tokens_per_s": round(8000 / prompt)},
+            f"generate, {layers} layers, 8 answers": {"ms_per_step": round(step * 1e3, 3), "tokens_per_s": round(8 / step),
+                                                      "floor_ms": round(floor * 1e3, 3), "frac": round(floor / step, 3)}}
+
+
 CASES = {"gemm": case_gemm, "attn_fwd": case_attn_fwd, "attn_bwd": case_attn_bwd, "gate": case_gate, "ce": case_ce,
          "qkv": case_qkv, "geglu": case_geglu, "rows": case_rows, "norms": case_norms, "ce_bwd": case_ce_bwd,
-         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp, "objectives": case_objectives, "paged": case_paged}
+         "nf4": case_nf4, "ce_gemm": case_ce_gemm, "tp": case_tp, "objectives": case_objectives, "paged": case_paged,
+         "generate": case_generate}
 
 
 def main(argv=None):
