@@ -16,9 +16,9 @@
 //     what the rounding left, relative error 2^-17), which the idle tensor cores give for nothing: the output is as exact as its own
 //     rounding.
 //
-// Measured, single tokens: 128 sequences of 30 to 9000 tokens in a sliding layer (window 1024, 16 heads of 256; 2.0 GB) 311 us, 0.98 of the copy
-// rate; 64 of 100 to 16000 in a global one (4 heads of 512; 4.5 GB) 755 us, 0.92; one over 131072 (1.07 GB) 196 us, 0.84 (ramp, two partial
-// blocks each piece, the join: 25 us); one sliding sequence (16 MB) 14 us, two launches one after another.
+// Measured, single tokens: 128 sequences of 30 to 9000 tokens in a sliding layer (window 1024, 16 heads of 256; 2.0 GB) 307-324 us, 0.94-1.0 of the copy
+// rate; 64 of 100 to 16000 in a global one (4 heads of 512; 4.5 GB) 745-762 us, 0.91-0.94; one over 131072 (1.07 GB) 196-200 us, 0.82-0.84 (ramp, two partial
+// blocks each piece, the join: 25-30 us); one sliding sequence (16 MB) 14 us, two launches one after another.
 #include <algorithm>
 
 #include "paged.cuh"
@@ -482,12 +482,30 @@ void launch_rows(const PagedAttentionArgs& a, int most_rows, void* workspace, in
   cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, (const RowsArgs)args);
 }
 
-// Which kernel takes which sequence: up to kFewRows rows this file's, more the tensor cores', whose time hardly depends on the rows. 16 rows
-// here | there: dim 256, 64 sequences of 500 to 6000 tokens 239 | 314 us; dim 512 (two passes here) 4 sequences of 500 tokens 26 | 40 us, of
-// 5000 75 | 97, 16 of 5000 253 | 198, 64 of 500 to 6000 652 | 591 (the host does not know the lengths).
+// Which kernel takes which sequence: up to kFewRows rows this file's, more the tensor cores', whose time hardly depends on the rows. 9 to 16 rows a
+// sequence, this kernel | that one, us (500 and 5000 tokens in the cache; every number of sequences from 1 to 64 was measured in powers of 2):
+//   sequences             1                  4                  16                 64
+//   dim 64 (2 heads)      13|19    15|28     13|19    17|28     16|19    25|56     19|29    47|133
+//   dim 128 (3)           12|19    17|29     13|20    21|32     18|21    38|83     25|40    94|197
+//   dim 256 (4)           15|21    21|31     17|21    36|52     23|25    76|83     46|57   217|298
+//   dim 256 (16, window)  17|21    21|26     25|25    35|35     50|57    72|92    129|157  214|281
+//   dim 512 (4)           17|23    33|37     21|24    66|80     39|37   236|193   116|101  830|717
+// Up to dim 256 this kernel is never slower by more than 2%. At dim 512, where it goes through the keys twice, it is from 8 sequences on
+// (8: 27|27 and 133|100); that is not told apart.
 constexpr int kFewRows = 16;
-// With this many rows a sequence on average (or very few sequences) the tensor cores' kernel takes all of them: single tokens among them cost it a
-// little more than they cost this one, and the two launches are saved (19 sequences of 1 to 333 new tokens: 57 us by one kernel, 67 by both).
+// With this many rows a sequence on average, or few sequences, the tensor cores' kernel takes all of them: what single tokens among them cost it more
+// is mostly less than two launches. That kernel for all | both, us:
+//   rows on average                      13 to 27         34 to 66         100 to 160       250 to 410
+//   8 sequences, dim 128                 27|44 (19)       25|41            31|42            31|43
+//   32 sequences, dim 128                35|47 (16)       36|43            39|45            41|59
+//   8 sequences, dim 256, window 1024    105|90  73|85    88|98 105|85     106|112 150|121  100|216
+//   32 sequences, dim 256, window 1024   145|150 148|165  149|170 155|223  163|173 215|215  301|309
+//   8 sequences, dim 512                 97|93 (31)       83|87            111|121 179|150  249|276
+//   32 sequences, dim 512                218|157 (25)     252|219 (54)     291|290          333|396 (206)
+// (two pairs: few long runs second. The rule loses most where one chunk of 300 stands beside seven single tokens at dim 256: 143|78.) A chunk of 40 and one or
+// two single tokens: 23-36|35-53 up to dim 256 with at most 5000 tokens each; at dim 512 27|46 over 500, 113|119 over 5000, 365|347 over 30000. Three
+// single tokens whose max_q is not said take that kernel too: 62|58 us at dim 512 over 5000 (46 with max_q 1, by this kernel alone), 202|163 (147)
+// over 30000. With more than kFewRows query heads a key head `both` has nothing for this file's kernel: 33 against 27 us (31 heads, 32 sequences).
 constexpr int kMeanRows = 32, kFewSequences = 4;
 
 enum Which { kRowsOnly, kTilesOnly, kBoth };

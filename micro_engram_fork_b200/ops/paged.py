@@ -23,8 +23,16 @@ CPU tensors run the plain PyTorch forms below, which compute in fp32 (fp64 for f
              A row that a new token sees and another does not (the chunk's own) must be finite for the other.
   tokens     Tokens of no sequence (before cu_seqlens[0], from cu_seqlens[-1] on) give rows of zeros (lse -inf) and store
              nothing; with `out`, its rows there stay as they were. Sequences without new tokens are left alone. cu_seqlens is
-             taken within [0, tokens]; a token whose position is negative is stored nowhere and sees nothing.
+             taken within [0, tokens]; a token whose position is negative is stored nowhere and sees nothing. cu_seqlens must not fall:
+             tokens that two sequences claim get either's result, or zeros.
   empty rows a row that sees no key: 0, lse -inf.
+
+On a GPU, sums, maxima and outputs in the making are 32-bit. What multiplies the values, exp(score - maximum), is rounded to two bf16 terms
+(relative error 2^-17) by the kernel of single tokens and drafts, and to one (2^-8, as the values have) by that of chunks: errors of o against 64 bits are
+0.0017 and 0.0022 of its mean size, where rounding o alone makes 0.0017. A batch of few sequences, or one of 32 rows (new tokens times query heads a key
+head) a sequence on average, goes through the second one whole, single tokens among them: their last bits depend on what they are batched with.
+The log-sum-exp is that of the unrounded terms either way. A batch of single tokens alone with max_q = 1 always takes the first kernel, up to 16 query
+heads a key head.
 
 Every wait inside the attention kernels is bounded; one that ran out (which no input causes) leaves its results wrong
 and is counted on the device, for good: a caller takes the count (waits_out) before its calls and compares it after them
@@ -194,7 +202,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
     """(o [T, Hq, D], lse [Hq, T] fp32) of q [T, Hq, D]: softmax(scale q . k) v over the keys at positions
     [max(0, p - window + 1), p] of the row's sequence (p: the row's position; window None: all of them). Hq is a multiple of Hk; the
     pages hold the new tokens too (append first). max_q: the longest run of new tokens if the host knows it; with it a batch of
-    single tokens skips what only longer runs need (a longer run than max_q says is still right, and slower). out: where o goes,
+    single tokens skips what only longer runs need, and goes to the kernel that is made for them (a longer run than max_q says is still right, and
+    slower). out: where o goes,
     a tensor of its own."""
     _no_gradient("paged_attention", q, k_pages, v_pages, *(() if out is None else (out,)))
     if window is not None and window < 1 or max_q is not None and max_q < 1:
