@@ -224,6 +224,8 @@ def paged_attention(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, wind
         raise ValueError(f"out: q's shape {tuple(q.shape)} is needed, got {tuple(out.shape)}")
     if out is not None and out.numel() and out.untyped_storage().data_ptr() == q.untyped_storage().data_ptr():
         raise ValueError("out: a tensor of its own is needed, not q's memory")
+    if out is not None and out.numel() and out.untyped_storage().data_ptr() in (k_pages.untyped_storage().data_ptr(), v_pages.untyped_storage().data_ptr()):
+        raise RuntimeError("out: a tensor of its own is needed, not the pages")
     with torch.no_grad():
         return paged_attention_ref(q, k_pages, v_pages, block_table, cu_seqlens, seq_lens, int(window or 0), float(scale), out)
 

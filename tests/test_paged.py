@@ -417,3 +417,15 @@ def check_largest_scale(device, dtype, lens):
 
 def test_largest_scale():
     check_largest_scale("cpu", F32, [(20, 2), (9, 3)])
+
+
+def check_out_is_no_page(device, dtype):
+    """`out` in the cache's memory: sequences are read after others' rows were written."""
+    b = oracle.Batch([(20, 2), (9, 3)], 4, 2, 64, 16, None, dtype, device)
+    for pages in (b.k, b.v):
+        with pytest.raises(RuntimeError, match="not the pages"):
+            paged.paged_attention(b.q, *b.args(), out=pages.view(-1)[:b.q.numel()].view_as(b.q))
+
+
+def test_out_is_no_page():
+    check_out_is_no_page("cpu", F32)

@@ -459,3 +459,7 @@ def test_pages_over_one_another():
 @pytest.mark.parametrize("mix", MIXES)
 def test_largest_scale(mix):
     test_paged.check_largest_scale(DEV, BF, MIXES[mix])
+
+
+def test_out_is_no_page():
+    test_paged.check_out_is_no_page(DEV, BF)
