@@ -23,6 +23,7 @@ into the fused buffers, so loading an HF state dict fills them in place.
 """
 import json
 import os
+import warnings
 from dataclasses import dataclass, field
 
 import torch
@@ -115,8 +116,11 @@ class GemmaConfig:
             cfg = cls.from_dict(json.load(f))
         generation = os.path.join(path, "generation_config.json")
         if os.path.exists(generation):
-            with open(generation) as f:
-                cfg.eos_token_id = _end_tokens(cfg.eos_token_id, json.load(f).get("eos_token_id"))
+            try:
+                with open(generation) as f:
+                    cfg.eos_token_id = _end_tokens(cfg.eos_token_id, json.load(f).get("eos_token_id"))
+            except (ValueError, AttributeError) as e:  # (nothing but generation needs it)
+                warnings.warn(f"{generation} is not read ({e}): answers end with config.json's tokens")
         return cfg
 
     def to_dict(self):

@@ -288,3 +288,12 @@ def test_generate_raises_for_its_own_waits(monkeypatch):
         gen.generate([[5, 9]], 3, eos=-1)
     state["new"] = 0
     assert gen.generate([[5, 9]], 3, eos=-1) == answer
+
+
+@pytest.mark.parametrize("text", ["", "{", "[1, 106]"])
+def test_a_generation_config_that_cannot_be_read(tmp_path, text):
+    """A folder that trains is not refused for it."""
+    (tmp_path / "config.json").write_text(json.dumps({"hidden_size": 64, "eos_token_id": 7}))
+    (tmp_path / "generation_config.json").write_text(text)
+    with pytest.warns(UserWarning, match="generation_config"):
+        assert G.GemmaConfig.from_pretrained(str(tmp_path)).eos_token_id == 7
