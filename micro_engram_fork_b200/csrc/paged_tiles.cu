@@ -28,8 +28,8 @@
 //
 // Measured: 2048 new tokens over 16048, 32 query heads on 4 of dim 512: 2.29 ms, 880 TFLOP/s of what has to be computed (0.53 of the measured
 // bf16 rate; the tensor cores are 78% busy, a third of it with S a second time). 4096 new tokens under a window of 1024, 32 heads on 16 of dim 256: 198 us,
-// 693 TFLOP/s (0.42; 182 us where keys and values are in the L2 cache): a block takes 2950 clocks, of them the softmax 2450 (128 exponentials a thread at 8 clocks a warp's, two
-// readings of the scores, the arrival), the rest the way of P to the products and of the next S back (two S buffers cover one of both); a unit of
+// 693 TFLOP/s (0.42; 182 us where calls on two caches take turns): a block takes 2950 clocks, of them the softmax 2450 (128 exponentials a thread
+// at 8 clocks a warp's, two readings of the scores, the arrival), the rest the way of P to the products and of the next S back (two S buffers cover one of both); a unit of
 // 10 blocks has 7000 clocks between its last softmax and the next unit's first (its last product 1800, O out 4700).
 #include <cudaTypedefs.h>
 
